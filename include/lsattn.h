@@ -37,6 +37,8 @@ extern "C" {
 #define LSATTN_F16 0
 #define LSATTN_BF16 1
 #define LSATTN_F32 2
+/* element type of a KV pool in 8 bits (lsattn_pool_attention): OCP e4m3 with a power-of-two scale per token and head */
+#define LSATTN_E4M3 3
 
 #define LSATTN_MAX_PARTS 16
 #define LSATTN_MAX_KV_CUTS 64 /* cuts of a KV chunk inside one prefill launch (lsattn_prefill_args.kv_cuts) */
@@ -555,6 +557,97 @@ int lsattn_bf16_to_f16_rows(const void* src, int64_t src_stride, void* dst, int6
                             int64_t row_elems, void* stream);
 
 /*
+ * The KV pool held in 8 bits; no counterpart in the reference (its pool is fp16).  A (token, head) row x of head_dim elements
+ * is head_dim e4m3 values q and an exponent byte e + 127 (E8M0): x stands as q * 2^e with e the least integer such that
+ * max |x| <= 448 * 2^e, at least -126, and q = e4m3(x * 2^-e) rounded to nearest even.  Elements that are not finite become NaN and do not
+ * count in the maximum.  pool is [num_slots, num_heads, head_dim] (bytes; the last dimension contiguous, strides multiples of
+ * 16), scales [num_slots, num_heads] bytes with any strides.
+ *
+ * lsattn_kv_scatter_fp8: the rows of src [num_tokens, num_heads, head_dim] (fp16 or bf16, strides in elements, multiples of 8)
+ * quantised into pool[dest_index[i]] and scales[dest_index[i]].  A slot outside [0, num_slots) is skipped; a slot named twice
+ * holds a mixture afterwards.  head_dim 16, 32, 64 or 128.
+ */
+typedef struct lsattn_kv_scatter_fp8_args {
+  const void* src;
+  int64_t src_stride_t, src_stride_h;
+  const void* dest_index;      /* [num_tokens], int32 or int64 (dest_index_is_i64) */
+  int32_t dest_index_is_i64;
+  int32_t dtype;               /* LSATTN_F16 or LSATTN_BF16 (src) */
+  void* pool;
+  int64_t pool_stride_0, pool_stride_1;
+  uint8_t* scales;
+  int64_t scale_stride_0, scale_stride_1;
+  int64_t num_tokens, num_heads, head_dim, num_slots;
+} lsattn_kv_scatter_fp8_args;
+int lsattn_kv_scatter_fp8(const lsattn_kv_scatter_fp8_args* a, void* stream);
+
+/*
+ * lsattn_kv_gather_fp8: contexts back in 16 bits, one request after the other, as lsattn_prefill_step takes them:
+ *   out[b_start_loc[b] + i] = q * 2^e of slot req_to_tokens[b_req_idx[b], b_first[b] + i]   for i < min(b_seq_len[b], max_len_in_batch),
+ * rounded to out's type (exact in its normal range; past fp16's range +-65504).  b_first NULL: 0.  A token whose table entry
+ * or position does not exist is a row of zeros; rows outside [0, out_rows) are not written, no others than those above are.
+ */
+typedef struct lsattn_kv_gather_fp8_args {
+  const void* pool;
+  int64_t pool_stride_0, pool_stride_1;
+  const uint8_t* scales;
+  int64_t scale_stride_0, scale_stride_1;
+  int64_t num_slots;
+  const int32_t* req_to_tokens; /* [num_reqs, max_seq_len] contiguous */
+  int64_t num_reqs, max_seq_len;
+  const int32_t* b_req_idx;     /* [batch] */
+  const int32_t* b_first;       /* [batch] or NULL */
+  const int32_t* b_seq_len;     /* [batch] */
+  const int32_t* b_start_loc;   /* [batch] */
+  int64_t batch, max_len_in_batch;
+  void* out;                    /* [out_rows, num_heads, head_dim], strides in elements, multiples of 8 */
+  int64_t out_stride_t, out_stride_h, out_rows;
+  int32_t dtype;                /* LSATTN_F16 or LSATTN_BF16 (out) */
+  int32_t reserved;
+  int64_t num_heads, head_dim;
+} lsattn_kv_gather_fp8_args;
+int lsattn_kv_gather_fp8(const lsattn_kv_gather_fp8_args* a, void* stream);
+
+/*
+ * Decode attention over a token-indexed pool in 16 or 8 bits, with an optional sliding window and sinks; one new token per
+ * request, whose query sees positions j < n = b_seqlen[b] of its row of the table with j >= n - window or j < sinks:
+ *   o[b, h] = sum_j softmax_j(sm_scale * q[b, h] . k_j) v_j,   lse[b, h] = natural log-sum-exp of the scores
+ * (o = 0, lse = -inf where nothing is seen).  Only rows that are seen are read.  Table entries outside [0, num_slots) count as positions that do not exist,
+ * so do positions past max_seq_len and requests outside [0, num_reqs).
+ * window = 0: none (sinks is not read).  A request's whole context lies in this pool; partials over disjoint keys (windowless
+ * ones of several instances) can be merged by lsattn_lse_merge or lsattn_decode_stage2.
+ * max_len_in_batch only steers the launch.  The partials of launches that cut the contexts need
+ * lsattn_pool_attention_workspace_bytes(...) bytes (0: none; 16-byte aligned, contents irrelevant before and after; calls that overlap in time
+ * need one each).
+ */
+typedef struct lsattn_pool_attention_args {
+  const void* q;                /* [batch, num_q_heads, head_dim] contiguous */
+  const void* k;                /* [num_slots, num_kv_heads, head_dim], the last dimension contiguous */
+  const void* v;
+  int64_t k_stride_0, k_stride_1, v_stride_0, v_stride_1; /* elements; rows 16-byte aligned */
+  const uint8_t* k_scales;      /* [num_slots, num_kv_heads], kv_dtype LSATTN_E4M3 */
+  const uint8_t* v_scales;
+  int64_t ks_stride_0, ks_stride_1, vs_stride_0, vs_stride_1;
+  const int32_t* req_to_tokens; /* [num_reqs, max_seq_len] contiguous */
+  const int32_t* b_req_idx;     /* [batch] */
+  const int32_t* b_seqlen;      /* [batch] */
+  int64_t batch, num_q_heads, num_kv_heads, head_dim; /* head_dim 64 or 128 */
+  int64_t num_slots, num_reqs, max_seq_len, max_len_in_batch;
+  int64_t window, sinks;
+  int32_t dtype;                /* of q: LSATTN_F16 or LSATTN_BF16 */
+  int32_t kv_dtype;             /* as dtype, or LSATTN_E4M3 */
+  float sm_scale;               /* > 0 */
+  int32_t o_dtype;              /* LSATTN_F32, LSATTN_F16 or LSATTN_BF16 */
+  void* o;                      /* [batch, num_q_heads, head_dim] contiguous */
+  float* lse;                   /* [batch, num_q_heads] contiguous */
+  void* workspace;
+  size_t workspace_bytes;
+} lsattn_pool_attention_args;
+size_t lsattn_pool_attention_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                             int64_t max_len_in_batch, int64_t window, int64_t sinks);
+int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* stream);
+
+/*
  * Launch choices that the library otherwise makes from the size of a launch, forced process-wide (tuning, and tests that
  * must reach every kernel shape whatever the size of their inputs).  No counterpart in the reference.  Every field 0 means
  * "the library's choice"; a NULL argument restores that for all of them.  The block is copied; launches made after the
@@ -594,8 +687,8 @@ const char* lsattn_strerror(int code);
  * the counts of lsattn_pool_update_refs also in pinned host memory and, past LSATTN_POOL_REFS_ORDERED entries, not behind the state; 5 = total_kv_rows and kv_cut_even in lsattn_prefill_args,
  * lsattn_prefill_converts_v; 6 = max_kv_len there (a reserved word before), lsattn_prefill_route,
  * lsattn_prefill_cut_count; 7 = o_is_apart in lsattn_decode_stage2_args (a reserved word before); 8 = o_is_apart of 2;
- * 9 = lead_rows in lsattn_decode_stage2_args. */
-#define LSATTN_VERSION 9
+ * 9 = lead_rows in lsattn_decode_stage2_args; 10 = lsattn_kv_scatter_fp8, lsattn_kv_gather_fp8, lsattn_pool_attention. */
+#define LSATTN_VERSION 10
 int lsattn_version(void);
 
 #ifdef __cplusplus

@@ -19,11 +19,12 @@ if not _building:
     from ._lib import set_tuning
     from . import longserve_cuda_kernels
     from .kv_pool import LongServeMemoryManager, LongServeReqManager
-    from .decoding import (longserve_flash_decode_stage1, longserve_flash_decode_stage2,
-                           longserve_token_decode_attention_flash_decoding)
+    from .decoding import (longserve_flash_decode_stage1, longserve_flash_decode_stage2, longserve_fp8_decode_attention,
+                           longserve_token_decode_attention_flash_decoding, longserve_window_decode_attention,
+                           pool_attention_workspace_bytes)
     from .ops import (context_attention_fwd, copy_kv_index_to_req, decoding_stage_migration_receiver_kernel,
                       decoding_stage_migration_sender_kernel, destindex_copy_and_register_kv, destindex_copy_kv,
-                      init_req_to_token_indexes, kv_scatter, lse_merge, pre_copy_and_register_kv, prefill_attention_step,
+                      init_req_to_token_indexes, kv_gather_fp8, kv_scatter, kv_scatter_fp8, lse_merge, pre_copy_and_register_kv, prefill_attention_step,
                       rmsnorm_forward, rotary_emb_fwd, rotary_emb_write_kv, silu_and_mul_fwd)
 
 __all__ = [
@@ -33,5 +34,7 @@ __all__ = [
     "decoding_stage_migration_sender_kernel", "decoding_stage_migration_receiver_kernel",
     "longserve_flash_decode_stage1", "longserve_flash_decode_stage2",
     "longserve_token_decode_attention_flash_decoding", "longserve_cuda_kernels",
+    "kv_scatter_fp8", "kv_gather_fp8", "longserve_fp8_decode_attention", "longserve_window_decode_attention",
+    "pool_attention_workspace_bytes",
     "LongServeMemoryManager", "LongServeReqManager", "set_tuning",
 ]

@@ -15,7 +15,7 @@ import os
 # different compile-time tuning; the default is the in-tree build next to this file.
 LIB_PATH = os.environ.get("LSATTN_LIB_PATH") or os.path.join(os.path.dirname(os.path.abspath(__file__)), "liblsattn.so")
 
-LSATTN_F16, LSATTN_BF16, LSATTN_F32 = 0, 1, 2
+LSATTN_F16, LSATTN_BF16, LSATTN_F32, LSATTN_E4M3 = 0, 1, 2, 3
 LSATTN_MAX_PARTS = 16
 LSATTN_MAX_KV_CUTS = 64
 LSATTN_POOL_REFS_ORDERED = 4096
@@ -96,7 +96,7 @@ TUNING_VALUES = {
     "decode_stage1": {None: 0, "lane": 1, "mfma": 2, "split": 3},
     "decode_listed": {None: 0, "off": 1, "on": 2, "shares": 3},
 }
-LSATTN_VERSION = 9  # of include/lsattn.h, which the argument blocks above mirror
+LSATTN_VERSION = 10  # of include/lsattn.h, which the argument blocks above mirror
 
 
 # every symbol include/lsattn.h declares: name -> (restype, argtypes)
@@ -127,7 +127,40 @@ class RotaryKvWriteArgs(C.Structure):  # mirrors lsattn_rotary_kv_write_args
                 ("batch", _i64), ("max_len_in_batch", _i64), ("register_mode", _i32), ("dest_index_is_i64", _i32)]
 
 
+class KvScatterFp8Args(C.Structure):  # mirrors lsattn_kv_scatter_fp8_args
+    _fields_ = [("src", _vp), ("src_stride_t", _i64), ("src_stride_h", _i64), ("dest_index", _vp),
+                ("dest_index_is_i64", _i32), ("dtype", _i32), ("pool", _vp), ("pool_stride_0", _i64), ("pool_stride_1", _i64),
+                ("scales", _vp), ("scale_stride_0", _i64), ("scale_stride_1", _i64),
+                ("num_tokens", _i64), ("num_heads", _i64), ("head_dim", _i64), ("num_slots", _i64)]
+
+
+class KvGatherFp8Args(C.Structure):  # mirrors lsattn_kv_gather_fp8_args
+    _fields_ = [("pool", _vp), ("pool_stride_0", _i64), ("pool_stride_1", _i64),
+                ("scales", _vp), ("scale_stride_0", _i64), ("scale_stride_1", _i64), ("num_slots", _i64),
+                ("req_to_tokens", _vp), ("num_reqs", _i64), ("max_seq_len", _i64),
+                ("b_req_idx", _vp), ("b_first", _vp), ("b_seq_len", _vp), ("b_start_loc", _vp),
+                ("batch", _i64), ("max_len_in_batch", _i64),
+                ("out", _vp), ("out_stride_t", _i64), ("out_stride_h", _i64), ("out_rows", _i64),
+                ("dtype", _i32), ("reserved", _i32), ("num_heads", _i64), ("head_dim", _i64)]
+
+
+class PoolAttentionArgs(C.Structure):  # mirrors lsattn_pool_attention_args
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp),
+                ("k_stride_0", _i64), ("k_stride_1", _i64), ("v_stride_0", _i64), ("v_stride_1", _i64),
+                ("k_scales", _vp), ("v_scales", _vp),
+                ("ks_stride_0", _i64), ("ks_stride_1", _i64), ("vs_stride_0", _i64), ("vs_stride_1", _i64),
+                ("req_to_tokens", _vp), ("b_req_idx", _vp), ("b_seqlen", _vp),
+                ("batch", _i64), ("num_q_heads", _i64), ("num_kv_heads", _i64), ("head_dim", _i64),
+                ("num_slots", _i64), ("num_reqs", _i64), ("max_seq_len", _i64), ("max_len_in_batch", _i64),
+                ("window", _i64), ("sinks", _i64), ("dtype", _i32), ("kv_dtype", _i32), ("sm_scale", _f32), ("o_dtype", _i32),
+                ("o", _vp), ("lse", _vp), ("workspace", _vp), ("workspace_bytes", C.c_size_t)]
+
+
 EXPORTS = {
+    "lsattn_kv_scatter_fp8": (C.c_int, [C.POINTER(KvScatterFp8Args), _vp]),
+    "lsattn_kv_gather_fp8": (C.c_int, [C.POINTER(KvGatherFp8Args), _vp]),
+    "lsattn_pool_attention": (C.c_int, [C.POINTER(PoolAttentionArgs), _vp]),
+    "lsattn_pool_attention_workspace_bytes": (C.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64, _i64]),
     "lsattn_prefill_step": (C.c_int, [C.POINTER(PrefillArgs), _vp]),
     "lsattn_prefill_step_merge": (C.c_int, [C.POINTER(PrefillArgs), _vp]),
     "lsattn_prefill_step_accumulate": (C.c_int, [C.POINTER(PrefillArgs), _vp]),

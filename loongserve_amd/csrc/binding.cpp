@@ -46,6 +46,10 @@ struct Library {
   decltype(&lsattn_pool_alloc) pool_alloc;
   decltype(&lsattn_pool_update_refs) pool_update_refs;
   decltype(&lsattn_pool_refs_workspace_bytes) pool_refs_workspace_bytes;
+  decltype(&lsattn_kv_scatter_fp8) kv_scatter_fp8;
+  decltype(&lsattn_kv_gather_fp8) kv_gather_fp8;
+  decltype(&lsattn_pool_attention) pool_attention;
+  decltype(&lsattn_pool_attention_workspace_bytes) pool_attention_workspace_bytes;
   decltype(&lsattn_strerror) strerror;
 } lib;
 
@@ -70,6 +74,10 @@ PyObject* bind(PyObject*, PyObject* addresses) {
       {"lsattn_pool_alloc", (void**)&lib.pool_alloc},
       {"lsattn_pool_update_refs", (void**)&lib.pool_update_refs},
       {"lsattn_pool_refs_workspace_bytes", (void**)&lib.pool_refs_workspace_bytes},
+      {"lsattn_kv_scatter_fp8", (void**)&lib.kv_scatter_fp8},
+      {"lsattn_kv_gather_fp8", (void**)&lib.kv_gather_fp8},
+      {"lsattn_pool_attention", (void**)&lib.pool_attention},
+      {"lsattn_pool_attention_workspace_bytes", (void**)&lib.pool_attention_workspace_bytes},
       {"lsattn_strerror", (void**)&lib.strerror},
   };
   for (const auto& e : entries) {
@@ -527,6 +535,121 @@ PyObject* register_tokens(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ------------------------------------------------------------------------------------------------ the pool in 8 bits, windows
+// whether all of these (null: none given) lie on the current device, whose stream takes the launch
+bool here(std::initializer_list<const at::Tensor*> ts) {
+  const auto current = c10::hip::current_device();
+  for (const at::Tensor* t : ts)
+    if (t && t->device().index() != current) return false;
+  return true;
+}
+// an exponent byte per (slot, head)
+bool exponents(const at::Tensor& s, const at::Tensor& pool) {
+  return (is(s, at::kByte) || is(s, at::kFloat8_e8m0fnu)) && s.dim() == 2 && s.size(0) == pool.size(0) && s.size(1) == pool.size(1);
+}
+bool e4m3_rows(const at::Tensor& t) { return is(t, at::kFloat8_e4m3fn) && t.stride(2) == 1; }
+
+// (src, dest_index, pool, scales) -> True or None
+PyObject* kv_scatter_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(4);
+  Args in(args);
+  const at::Tensor &src = in.gpu(3), &index = in.gpu(1), &pool = in.gpu(3), &scales = in.gpu(2);
+  OR_NONE(in.ok && here({&src, &index, &pool, &scales}));
+  OR_NONE(half(src) && src.stride(2) == 1 && e4m3_rows(pool) && exponents(scales, pool) && slots(index, src.size(0)));
+  OR_NONE(src.size(1) == pool.size(1) && src.size(2) == pool.size(2) && src.numel() > 0 && pool.numel() > 0);
+  lsattn_kv_scatter_fp8_args a;
+  std::memset(&a, 0, sizeof a);
+  a.src = src.data_ptr(), a.src_stride_t = src.stride(0), a.src_stride_h = src.stride(1), a.dtype = dtype_of(src);
+  a.dest_index = index.data_ptr(), a.dest_index_is_i64 = is(index, at::kLong);
+  a.pool = pool.data_ptr(), a.pool_stride_0 = pool.stride(0), a.pool_stride_1 = pool.stride(1);
+  a.scales = (uint8_t*)scales.data_ptr(), a.scale_stride_0 = scales.stride(0), a.scale_stride_1 = scales.stride(1);
+  a.num_tokens = src.size(0), a.num_heads = src.size(1), a.head_dim = src.size(2), a.num_slots = pool.size(0);
+  if (const int rc = call(lib.kv_scatter_fp8, &a, stream())) return failed(rc, "lsattn_kv_scatter_fp8");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (pool, scales, table, b_req, b_len, b_start, max_len, out, b_first or None) -> True or None
+PyObject* kv_gather_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(9);
+  Args in(args);
+  const at::Tensor &pool = in.gpu(3), &scales = in.gpu(2), &table = in.gpu(2), &b_req = in.gpu(1), &b_len = in.gpu(1), &b_start = in.gpu(1);
+  const int64_t max_len = in.integer();
+  const at::Tensor& out = in.gpu(3);
+  const at::Tensor* first = in.maybe();
+  OR_NONE(in.ok && here({&pool, &scales, &table, &b_req, &b_len, &b_start, &out, first}));
+  const int64_t B = b_req.size(0);
+  OR_NONE(e4m3_rows(pool) && exponents(scales, pool) && is(table, at::kInt) && table.is_contiguous() && i32(b_req, B) && i32(b_len, B) && i32(b_start, B));
+  OR_NONE(half(out) && out.stride(2) == 1 && out.size(1) == pool.size(1) && out.size(2) == pool.size(2) && max_len >= 0);
+  OR_NONE((!first || (first->dim() == 1 && i32(*first, B))) && B > 0 && max_len > 0 && out.numel() > 0 && pool.numel() > 0);
+  lsattn_kv_gather_fp8_args a;
+  std::memset(&a, 0, sizeof a);
+  a.pool = pool.data_ptr(), a.pool_stride_0 = pool.stride(0), a.pool_stride_1 = pool.stride(1);
+  a.scales = (const uint8_t*)scales.data_ptr(), a.scale_stride_0 = scales.stride(0), a.scale_stride_1 = scales.stride(1);
+  a.num_slots = pool.size(0);
+  a.req_to_tokens = pi32(table), a.num_reqs = table.size(0), a.max_seq_len = table.size(1);
+  a.b_req_idx = pi32(b_req), a.b_first = first ? pi32(*first) : nullptr, a.b_seq_len = pi32(b_len), a.b_start_loc = pi32(b_start);
+  a.batch = B, a.max_len_in_batch = max_len;
+  a.out = out.data_ptr(), a.out_stride_t = out.stride(0), a.out_stride_h = out.stride(1), a.out_rows = out.size(0), a.dtype = dtype_of(out);
+  a.num_heads = pool.size(1), a.head_dim = pool.size(2);
+  if (const int rc = call(lib.kv_gather_fp8, &a, stream())) return failed(rc, "lsattn_kv_gather_fp8");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, table, b_req, b_len, max_len, k, v, k_scales or None, v_scales or None, window, sinks, out or None, lse or None, workspace or None)
+// -> (out, lse) or None
+PyObject* pool_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(14);
+  Args in(args);
+  const at::Tensor &q = in.gpu(3), &table = in.gpu(2), &b_req = in.gpu(1), &b_len = in.gpu(1);
+  const int64_t max_len = in.integer();
+  const at::Tensor &k = in.gpu(3), &v = in.gpu(3);
+  const at::Tensor *ks = in.maybe(), *vs = in.maybe();
+  const int64_t window = in.integer(), sinks = in.integer();
+  PyObject *py_out = args[in.i], *py_lse = args[in.i + 1];
+  const at::Tensor *out_in = in.maybe(), *lse_in = in.maybe(), *ws_in = in.maybe();
+  OR_NONE(in.ok && here({&q, &table, &b_req, &b_len, &k, &v, ks, vs, out_in, lse_in, ws_in}));
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
+  OR_NONE(half(q) && q.is_contiguous() && is(table, at::kInt) && table.is_contiguous() && i32(b_req, B) && i32(b_len, B));
+  OR_NONE(k.sizes() == v.sizes() && k.size(2) == D && k.stride(2) == 1 && v.stride(2) == 1 && k.scalar_type() == v.scalar_type());
+  OR_NONE((D == 128 || D == 64) && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && k.size(0) > 0 && B > 0);
+  const bool k8 = ks != nullptr;
+  OR_NONE(k8 ? vs && is(k, at::kFloat8_e4m3fn) && exponents(*ks, k) && exponents(*vs, v)
+             : !vs && k.scalar_type() == q.scalar_type() && window > 0);
+  OR_NONE(max_len >= 0 && window >= 0 && sinks >= 0);
+  if (out_in) OR_NONE((half(*out_in) || is(*out_in, at::kFloat)) && out_in->is_contiguous() && same_shape(*out_in, q));
+  if (lse_in) OR_NONE(is(*lse_in, at::kFloat) && lse_in->is_contiguous() && lse_in->dim() == 2 && lse_in->size(0) == B && lse_in->size(1) == Hq);
+  lsattn_pool_attention_args a;
+  std::memset(&a, 0, sizeof a);
+  a.workspace_bytes = lib.pool_attention_workspace_bytes(B, Hq, Hkv, D, max_len, window, sinks);
+  OR_NONE(!ws_in || (ws_in->is_contiguous() && ws_in->nbytes() >= a.workspace_bytes));
+  const at::Tensor out = out_in ? *out_in : empty(q.sizes(), q, at::kFloat);
+  const at::Tensor lse = lse_in ? *lse_in : empty({B, Hq}, q, at::kFloat);
+  const at::Tensor ws = ws_in || !a.workspace_bytes ? at::Tensor() : empty({(int64_t)a.workspace_bytes}, q, at::kByte);
+  a.workspace = ws_in ? ws_in->data_ptr() : a.workspace_bytes ? ws.data_ptr() : nullptr;
+  a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
+  a.k_stride_0 = k.stride(0), a.k_stride_1 = k.stride(1), a.v_stride_0 = v.stride(0), a.v_stride_1 = v.stride(1);
+  if (k8) {
+    a.k_scales = (const uint8_t*)ks->data_ptr(), a.v_scales = (const uint8_t*)vs->data_ptr();
+    a.ks_stride_0 = ks->stride(0), a.ks_stride_1 = ks->stride(1), a.vs_stride_0 = vs->stride(0), a.vs_stride_1 = vs->stride(1);
+  }
+  a.req_to_tokens = pi32(table), a.b_req_idx = pi32(b_req), a.b_seqlen = pi32(b_len);
+  a.batch = B, a.num_q_heads = Hq, a.num_kv_heads = Hkv, a.head_dim = D;
+  a.num_slots = k.size(0), a.num_reqs = table.size(0), a.max_seq_len = table.size(1), a.max_len_in_batch = max_len;
+  a.window = window, a.sinks = sinks, a.dtype = dtype_of(q), a.kv_dtype = k8 ? LSATTN_E4M3 : a.dtype;
+  a.sm_scale = (float)(1.0 / std::sqrt((double)D));
+  a.o = out.data_ptr(), a.o_dtype = dtype_of(out), a.lse = (float*)lse.data_ptr();
+  if (const int rc = call(lib.pool_attention, &a, stream())) return failed(rc, "lsattn_pool_attention");
+  PyObject* o1 = out_in ? (Py_INCREF(py_out), py_out) : THPVariable_Wrap(out);
+  PyObject* o2 = lse_in ? (Py_INCREF(py_lse), py_lse) : THPVariable_Wrap(lse);
+  return Py_BuildValue("(NN)", o1, o2);
+  END_HANDLE_TH_ERRORS
+}
+
 // ------------------------------------------------------------------------------------------------ element-wise steps
 bool half_contiguous(const at::Tensor& t) { return is(t, at::kHalf) && t.is_contiguous(); }
 
@@ -735,6 +858,7 @@ PyMethodDef methods[] = {
     ENTRY(context_attention), ENTRY(prefill_partial), ENTRY(token_decode_attention), ENTRY(decode_stage1), ENTRY(decode_stage2),
     ENTRY(kv_scatter), ENTRY(register_decode_tokens), ENTRY(register_tokens), ENTRY(rms_norm), ENTRY(silu_and_mul_inplace),
     ENTRY(rotary_emb), ENTRY(rotary_kv_write), ENTRY(pool_alloc), ENTRY(pool_update_refs),
+    ENTRY(kv_scatter_fp8), ENTRY(kv_gather_fp8), ENTRY(pool_attention),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native argument pass of loongserve_amd's operators.", -1, methods};
 

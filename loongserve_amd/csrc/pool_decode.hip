@@ -1,0 +1,661 @@
+// Decode attention over the token-indexed pool with a sliding window and sinks, and over a pool held in 8 bits (gfx950, wave64).
+//
+// For request b with n tokens and query head h, over the positions j < n with j >= n - window or j < sinks (all, without a window):
+//   s_j = scale * (q_h . k_j),   o = sum_j softmax(s)_j v_j,   LSE = log sum_j exp(s_j),
+// where an e4m3 pool holds k_j and v_j as q * 2^e with one e per token and head.  n_vis visible tokens are numbered 0 .. n_vis - 1, sinks first, and the
+// kernel walks those: a token outside the window costs nothing.
+//
+// What bounds it is HBM: (D + 1) bytes per K and V row of a head in 8 bits, 2 D in 16, against 2 D multiply-adds per query head
+// for each.  Hence a row is read once for up to eight query heads of its KV head, and the vector work beside the matrix pipe is
+// kept below what the memory leaves time for:
+//   * a wave takes blocks of 32 tokens of one KV head.  Lane (g, c) = (lane / 16, lane % 16) loads pieces of K rows c and 16 + c and elements
+//     [c * D / 16, + D / 16) of V rows 4g .. 4g + 3 and 16 + 4g .. 16 + 4g + 3, straight into registers: no LDS tile;
+//   * scores transposed, S^T = K Q^T with 16x16x32 MFMAs: the order of the head's elements along the contraction is whatever
+//     the loads give, the query is read in the same one.  Column c of the product is query head c % 8, so the lane holds the
+//     scores of eight tokens, 4g + r and 16 + 4g + r, of one head: the tokens whose V rows it has;
+//   * O^T += V^T P^T with the V rows turned by byte permutes in registers: P^T goes into the product from the lane that
+//     computed it, and every accumulator of a lane belongs to the head whose maximum and sum it keeps;
+//   * P keeps more than 16 bits although the operands have 16: columns c and c + 8 of the product carry two parts of the same
+//     head's P, high and low, and a second product a third part where the type is bfloat16 (8 bits each).  The parts are
+//     added once, at the end.  bfloat16 where V comes from 8 bits: P times the token's scale has its range;
+//   * the reference of a head's weights is raised only when a score exceeds the maximum it was set by by 8 (log2 units): the accumulators
+//     are seldom rescaled, and no exchange between lanes stands in the common path.
+// Short contexts and windows: the waves of one workgroup share a (request, KV head) and meet in LDS (one launch).  Otherwise the blocks of
+// all requests are dealt to the waves in equal shares, whatever the requests' lengths are (the host does not know them);
+// a wave leaves one partial per request it touches, and a second launch merges them.
+#include "common.hip.h"
+
+namespace lsattn {
+namespace {
+
+struct E4M3 {};  // element tag of the pool
+
+constexpr int kBlock = 32;       // tokens per step of a wave
+constexpr int kHeads = 8;        // query heads per task
+constexpr int64_t kCUs = 256;
+// The reference m of a head's weights is set to the maximum so far less kHead, and raised when a score exceeds it by kLag: weights
+// of up to 2^15 (fp16 ends at 2^16), the largest 2^7 or more, so that the second part of a small fp16 weight does not run out of exponent.
+constexpr float kHead = 7.f, kLag = 15.f;
+
+struct PoolParams {
+  const char* q;
+  const char* k;
+  const char* v;
+  int64_t k_s0, k_s1, v_s0, v_s1;  // bytes
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int64_t ks_s0, ks_s1, vs_s0, vs_s1;
+  const int32_t* table;
+  const int32_t* b_req;
+  const int32_t* b_len;
+  int64_t max_seq_len;
+  int32_t batch, num_reqs, num_slots, hq, hkv, group, sub_groups, tasks;
+  int32_t window, sinks;  // window 0: none
+  float scale_log2;
+  char* o;
+  int32_t o_dtype;
+  float* lse;
+  float* part_o;    // [shares + batch, hq, D]
+  float* part_lse;  // [shares + batch, hq]
+  int32_t shares, min_units;
+  FastDiv by_tasks, by_sub;
+};
+
+__device__ __forceinline__ float xor16(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_ds_swizzle(__builtin_bit_cast(int, v), 0x401F));
+}
+__device__ __forceinline__ float xor32(float v) {
+  const unsigned u = __builtin_bit_cast(unsigned, v);
+  auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+__device__ __forceinline__ float col_max(float v) {
+  v = fmaxf(v, xor16(v));
+  return fmaxf(v, xor32(v));
+}
+__device__ __forceinline__ float col_sum(float v) {
+  v += xor16(v);
+  return v + xor32(v);
+}
+
+template <typename T> __device__ __forceinline__ f32x4 mfma(const u32x4& a, const u32x4& b, const f32x4& c);
+template <> __device__ __forceinline__ f32x4 mfma<F16>(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f32x4 mfma<BF16>(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// two of the four e4m3 values of a word as 16-bit floats (exact)
+template <typename T, bool HI> __device__ __forceinline__ uint32_t widen(uint32_t w);
+template <> __device__ __forceinline__ uint32_t widen<F16, false>(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false)); }
+template <> __device__ __forceinline__ uint32_t widen<F16, true>(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true)); }
+template <> __device__ __forceinline__ uint32_t widen<BF16, false>(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false)); }
+template <> __device__ __forceinline__ uint32_t widen<BF16, true>(uint32_t w) { return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true)); }
+
+// 2^e of an exponent byte (0, which no row written here has, is 2^-127)
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __builtin_bit_cast(float, byte ? byte << 23 : 0x400000u); }
+
+// The parts of eight P values: `hi` lanes give the first, the others the second (fp16: 2^-22 of the value is left out at most).  bfloat16, 8 bits a
+// part: a third comes from the hi lanes in a product of its own, zero from the others; parts are cut off, not rounded, which leaves out 2^-23.
+template <typename T> struct Parts;
+template <> struct Parts<F16> {
+  static constexpr int N = 1;
+  static __device__ __forceinline__ void of(const float (&x)[8], bool hi, u32x4 (&out)[2]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t first = pack2<F16>(x[2 * e], x[2 * e + 1]);
+      float a, b;
+      unpack2<F16>(first, a, b);
+      const uint32_t second = pack2<F16>(x[2 * e] - a, x[2 * e + 1] - b);
+      out[0][e] = hi ? first : second;
+    }
+  }
+};
+template <> struct Parts<BF16> {
+  static constexpr int N = 2;
+  static __device__ __forceinline__ void of(const float (&x)[8], bool hi, u32x4 (&out)[2]) {
+    float first[8], rest[8], third[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      first[e] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[e]) & 0xffff0000u);
+      rest[e] = x[e] - first[e];
+      third[e] = rest[e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[e]) & 0xffff0000u);
+      first[e] = hi ? first[e] : rest[e];
+      third[e] = hi ? third[e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      out[0][e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, first[2 * e + 1]), __builtin_bit_cast(uint32_t, first[2 * e]), 0x07060302u);
+      out[1][e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, third[2 * e + 1]), __builtin_bit_cast(uint32_t, third[2 * e]), 0x07060302u);
+    }
+  }
+};
+
+template <typename KV> struct PvOf { typedef KV type; };
+template <> struct PvOf<E4M3> { typedef BF16 type; };
+
+// visible tokens of a request
+__device__ __forceinline__ int visible(const PoolParams& p, int b, int& len) {
+  len = p.b_len[b];
+  const int req = p.b_req[b];
+  if (len > p.max_seq_len) len = (int)p.max_seq_len;
+  if (len < 0 || req < 0 || req >= p.num_reqs) len = 0;
+  if (!p.window) return len;
+  const int64_t most = (int64_t)p.window + p.sinks;
+  return len < most ? len : (int)most;
+}
+
+// One wave's walk over blocks of visible tokens of one (request, KV head, up to eight query heads).
+template <typename QT, typename KV, int D> struct Walk {
+  typedef typename PvOf<KV>::type PV;
+  static constexpr bool k8 = __is_same(KV, E4M3);
+  static constexpr int KS = D / 32;               // contraction steps of Q K^T
+  static constexpr int EV = D / 16;               // elements of a V row per lane
+  static constexpr int KW = k8 ? D / 16 : D / 8;  // words of a K row per lane (a quarter of the row)
+  static constexpr int VW = k8 ? EV / 4 : EV / 2; // words of a V row per lane
+  static constexpr int ES = k8 ? 1 : 2;           // bytes per element
+
+  const PoolParams& p;
+  const int lane, g, c;
+  int32_t* const slot_lds;   // [32] of this wave
+  float* const scale_lds;    // [64]: K scales (times the softmax scale), V scales
+  u32x4 qf[KS];
+  f32x4 acc[EV];  // acc[j][r] = O[head][EV * (4g + r) + j], of the parts of P in this lane's column
+  float m, l;     // log2-domain maximum of the head; the lane's share of the sum
+
+  __device__ __forceinline__ Walk(const PoolParams& p_, char* lds_wave)
+      : p(p_), lane(threadIdx.x & 63), g(lane >> 4), c(lane & 15), slot_lds((int32_t*)lds_wave), scale_lds((float*)(lds_wave + 128)) {}
+
+  const char *kb, *vb;
+  const uint8_t* sb;  // the lane's column of scales: K for lanes 0 .. 31, V for the others
+  int64_t s_s0;
+  const int32_t* row;
+  int sinks, skip, limit;
+
+  // a task = one KV head and up to eight query heads of its group
+  __device__ __forceinline__ void start(int b, int task, int len, int n_vis) {
+    const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
+    const int h0 = kvh * p.group + sg * kHeads;
+    const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
+    const int h = (c & 7) < nh ? (c & 7) : nh - 1;
+    const char* q = p.q + ((int64_t)b * p.hq + h0 + h) * D * 2;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+      // (the order of the K loads below)
+      const int d = k8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
+      qf[ks] = *(const u32x4*)(q + d * 2);
+    }
+    kb = p.k + kvh * p.k_s1 + 16 * g;
+    vb = p.v + kvh * p.v_s1 + c * EV * ES;
+    if (k8) {
+      sb = lane < 32 ? p.ks + kvh * p.ks_s1 : p.vs + kvh * p.vs_s1;
+      s_s0 = lane < 32 ? p.ks_s0 : p.vs_s0;
+    }
+    row = p.table + (int64_t)p.b_req[b] * p.max_seq_len;
+    sinks = p.window ? p.sinks : 0;
+    skip = len - n_vis;
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < EV; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  // the slot of token `at` + lane % 32 (positions past the end repeat the last one)
+  __device__ __forceinline__ int load_slot(int at) const {
+    int i = at + (lane & 31);
+    i = i < limit ? i : limit - 1;
+    return row[i < sinks ? i : i + skip];
+  }
+
+  u32x4 kr[2][KW / 4];
+  uint32_t vr[8][VW];
+  uint32_t scale_byte;
+  uint32_t there;  // bit i: token i of the block exists
+
+  __device__ __forceinline__ void load_rows(int at, int slot) {
+    const bool ok = at + (lane & 31) < limit && (uint32_t)slot < (uint32_t)p.num_slots;
+    there = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
+    slot = ok ? slot : 0;
+    if (k8) scale_byte = sb[slot * s_s0];
+    slot_lds[lane & 31] = slot;
+    __builtin_amdgcn_wave_barrier();
+    const int k0 = slot_lds[c], k1 = slot_lds[16 + c];
+    int vslot[8];
+    *(u32x4*)vslot = *(const u32x4*)(slot_lds + 4 * g);
+    *(u32x4*)(vslot + 4) = *(const u32x4*)(slot_lds + 16 + 4 * g);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int w = 0; w < KW / 4; w++) {
+      kr[0][w] = __builtin_nontemporal_load((const u32x4*)(kb + k0 * p.k_s0 + 64 * w));
+      kr[1][w] = __builtin_nontemporal_load((const u32x4*)(kb + k1 * p.k_s0 + 64 * w));
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const char* at_v = vb + vslot[i] * p.v_s0;
+      if constexpr (VW == 1) vr[i][0] = __builtin_nontemporal_load((const uint32_t*)at_v);
+      else if constexpr (VW == 2) *(u32x2*)vr[i] = __builtin_nontemporal_load((const u32x2*)at_v);
+      else *(u32x4*)vr[i] = __builtin_nontemporal_load((const u32x4*)at_v);
+    }
+  }
+
+  __device__ __forceinline__ void compute() {
+    // scores of the lane's head with tokens 4g + r (s[0]) and 16 + 4g + r (s[1])
+    f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        u32x4 a;
+        if constexpr (k8) {
+          const uint32_t w0 = kr[t][ks >> 1][2 * (ks & 1)], w1 = kr[t][ks >> 1][2 * (ks & 1) + 1];
+          a = u32x4{widen<QT, false>(w0), widen<QT, true>(w0), widen<QT, false>(w1), widen<QT, true>(w1)};
+        } else {
+          a = kr[t][ks];
+        }
+        s[t] = mfma<QT>(a, qf[ks], s[t]);
+      }
+    float x[8], vscale[8];
+    if constexpr (k8) {
+      scale_lds[lane] = scale_of(scale_byte) * (lane < 32 ? p.scale_log2 : 1.f);
+      __builtin_amdgcn_wave_barrier();
+      f32x4 kf[2], vf[2];
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        kf[t] = *(const f32x4*)(scale_lds + 16 * t + 4 * g);
+        vf[t] = *(const f32x4*)(scale_lds + 32 + 16 * t + 4 * g);
+      }
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = s[e / 4][e % 4] * kf[e / 4][e % 4], vscale[e] = vf[e / 4][e % 4];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = s[e / 4][e % 4] * p.scale_log2;
+    }
+    if (there != 0xffffffffu) {  // (the same for every lane)
+      const uint32_t mine = ((there >> (4 * g)) & 15u) | ((there >> (12 + 4 * g)) & 0xf0u);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const bool ok = (mine >> e) & 1u;
+        x[e] = ok ? x[e] : -INFINITY;
+        if (k8) vscale[e] = ok ? vscale[e] : 0.f;
+#pragma unroll
+        for (int w = 0; w < VW; w++) vr[e][w] = ok ? vr[e][w] : 0u;  // (what lies there may be infinite or NaN)
+      }
+    }
+    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    if (__builtin_amdgcn_ballot_w64(mx > m + kLag) != 0) {
+      const float m_new = fmaxf(m, col_max(mx) - kHead);
+      const float alpha = exp2_diff(m, m_new);
+      l *= alpha;
+#pragma unroll
+      for (int j = 0; j < EV; j++) acc[j] *= alpha;
+      m = m_new;
+    }
+    const float m_safe = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(x[e] - m_safe);
+    l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    if (k8) {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] *= vscale[e];
+    }
+    u32x4 pk[2];
+    Parts<PV>::of(x, c < 8, pk);
+    // V^T operands: element j of the eight tokens
+#pragma unroll
+    for (int w = 0; w < VW; w++) {
+      if constexpr (k8) {
+        u32x4 va[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          const uint32_t lo = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x05010400u);
+          const uint32_t hi = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x07030602u);
+          va[0][t] = widen<PV, false>(lo);
+          va[1][t] = widen<PV, true>(lo);
+          va[2][t] = widen<PV, false>(hi);
+          va[3][t] = widen<PV, true>(hi);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int n = 0; n < Parts<PV>::N; n++) acc[4 * w + j] = mfma<PV>(va[j], pk[n], acc[4 * w + j]);
+      } else {
+        u32x4 va[2];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+          va[0][t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x05040100u);
+          va[1][t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x07060302u);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+          for (int n = 0; n < Parts<PV>::N; n++) acc[2 * w + j] = mfma<PV>(va[j], pk[n], acc[2 * w + j]);
+      }
+    }
+  }
+
+  // visible tokens [from, to) in steps of `step` blocks; the first block exists
+  __device__ __forceinline__ void run(int from, int to, int step) {
+    limit = to;
+    int slot = load_slot(from);
+    for (int at = from; at < to; at += step * kBlock) {
+      load_rows(at, slot);
+      slot = load_slot(at + step * kBlock);
+      compute();
+    }
+  }
+
+  // the parts of P together, and the sum over the head's lanes
+  __device__ __forceinline__ void join() {
+#pragma unroll
+    for (int j = 0; j < EV; j++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) acc[j][r] += dpp_mov<0x128>(acc[j][r]);  // row_ror:8
+    l = col_sum(l);
+  }
+};
+
+__device__ __forceinline__ void store_elem4(char* o, int dtype, int64_t at, const f32x4& v) {
+  if (dtype == LSATTN_F32) *(f32x4*)((float*)o + at) = v;
+  else if (dtype == LSATTN_F16) *(u32x2*)((uint16_t*)o + at) = u32x2{pack2<F16>(v[0], v[1]), pack2<F16>(v[2], v[3])};
+  else *(u32x2*)((uint16_t*)o + at) = u32x2{pack2<BF16>(v[0], v[1]), pack2<BF16>(v[2], v[3])};
+}
+__device__ __forceinline__ float ln_of(float m, float l) { return l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : (l == l ? -INFINITY : l); }
+
+constexpr int kWaveLds = 384;  // bytes of LDS per wave: 32 slots, 64 scales
+
+// One workgroup per (task, request): its NW waves take every NW-th block and meet in LDS.
+template <typename QT, typename KV, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void pool_decode_direct_kernel(PoolParams p) {
+  constexpr int ROW = D + 4;  // floats per head in LDS: O, maximum, sum (and a bank's shift)
+  __shared__ __attribute__((aligned(16))) char lds[NW * kHeads * ROW * 4 > NW * kWaveLds ? NW * kHeads * ROW * 4 : NW * kWaveLds];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int task = blockIdx.x, b = blockIdx.y;
+  const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
+  const int h0 = kvh * p.group + sg * kHeads;
+  const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
+  int len;
+  const int n_vis = visible(p, b, len);
+  Walk<QT, KV, D> w(p, lds + wave * kWaveLds);
+  if (wave * kBlock < n_vis) {
+    w.start(b, task, len, n_vis);
+    w.run(wave * kBlock, n_vis, NW);
+    w.join();
+  } else {
+    w.m = -INFINITY, w.l = 0.f;
+  }
+  __syncthreads();  // (the waves' slots and scales lie where the results go)
+  float* const res = (float*)lds;
+  if (w.c < nh) {
+    float* mine = res + (wave * kHeads + w.c) * ROW;
+    if (wave * kBlock < n_vis) {
+#pragma unroll
+      for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int j = 0; j < D / 16; j += 4)
+          *(f32x4*)(mine + (D / 16) * (4 * w.g + r) + j) = f32x4{w.acc[j][r], w.acc[j + 1][r], w.acc[j + 2][r], w.acc[j + 3][r]};
+    }
+    if (w.g == 0) mine[D] = w.m, mine[D + 1] = w.l;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < nh * (D / 4); i += NW * 64) {
+    const int h = i / (D / 4), d = (i & (D / 4 - 1)) * 4;
+    float M = -INFINITY;
+#pragma unroll
+    for (int v = 0; v < NW; v++) M = fmaxf(M, res[(v * kHeads + h) * ROW + D]);
+    float L = 0.f;
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < NW; v++) {
+      const float* r = res + (v * kHeads + h) * ROW;
+      if (v * kBlock < n_vis) {
+        const float f = exp2_diff(r[D], M);
+        L += r[D + 1] * f;
+        sum += *(const f32x4*)(r + d) * f;
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int64_t at = (int64_t)b * p.hq + h0 + h;
+    store_elem4(p.o, p.o_dtype, at * D + d, sum * inv);
+    if (d == 0) p.lse[at] = ln_of(M, L);
+  }
+}
+
+// How the blocks of all requests are dealt: the units of request b are [first, first + n) of all.  Every wave counts them by itself, 64 requests a step.
+struct Deal {
+  int64_t total;
+  int per_share;
+};
+__device__ __forceinline__ int units_of(const PoolParams& p, int b) {
+  int len;
+  return b < p.batch ? (visible(p, b, len) + kBlock - 1) / kBlock : 0;
+}
+__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
+  return v;
+}
+__device__ __forceinline__ Deal deal(const PoolParams& p) {
+  const int lane = threadIdx.x & 63;
+  int64_t n = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) n += units_of(p, b0 + lane);
+  Deal d;
+  d.total = wave_sum(n);
+  const int64_t per = (d.total + p.shares - 1) / p.shares;
+  d.per_share = (int)(per < p.min_units ? p.min_units : per);
+  return d;
+}
+
+// Four waves per workgroup, each with a share of its own of one task; the tasks of a share are neighbours, on one XCD.
+template <typename QT, typename KV, int D>
+__global__ __launch_bounds__(256) void pool_decode_shares_kernel(PoolParams p) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * kWaveLds];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  // (ids go to the XCDs round-robin; gridDim.x is a multiple of 8)
+  const uint32_t id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+  const uint32_t unit = id * 4 + wave;
+  const int share = (int)div_by(unit, p.by_tasks), task = (int)(unit - (uint32_t)share * p.tasks);
+  if (share >= p.shares) return;
+  const Deal dl = deal(p);
+  int64_t at = (int64_t)share * dl.per_share;
+  const int64_t end = at + dl.per_share < dl.total ? at + dl.per_share : dl.total;
+  if (at >= end) return;
+  // the request of the share's first unit
+  int b = 0;
+  int64_t first = 0;
+  for (int b0 = 0;; b0 += 64) {  // (at < total: found before the batch ends)
+    int64_t incl = units_of(p, b0 + lane);
+    const int64_t mine = incl;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t below = __shfl_up(incl, d, 64);
+      if (lane >= d) incl += below;
+    }
+    const int64_t chunk = __shfl(incl, 63, 64);
+    if (at < first + chunk) {
+      const int l0 = __builtin_ctzll(__builtin_amdgcn_ballot_w64(first + incl > at));
+      b = __builtin_amdgcn_readfirstlane(b0 + l0);
+      first += __shfl(incl - mine, l0, 64);
+      break;
+    }
+    first += chunk;
+  }
+  Walk<QT, KV, D> w(p, lds + wave * kWaveLds);
+  const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
+  const int h0 = kvh * p.group + sg * kHeads;
+  const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
+  for (; at < end && b < p.batch; b++) {
+    int len;
+    const int n_vis = __builtin_amdgcn_readfirstlane(visible(p, b, len));
+    len = __builtin_amdgcn_readfirstlane(len);
+    const int64_t units = (n_vis + kBlock - 1) / kBlock;
+    const int64_t to = first + units < end ? first + units : end;
+    if (to > at) {
+      w.start(b, task, len, n_vis);
+      const int64_t last = (to - first) * kBlock;
+      w.run((int)(at - first) * kBlock, (int)(last < n_vis ? last : n_vis), 1);
+      w.join();
+      if (w.c < nh) {
+        const int64_t r0 = ((int64_t)(share + b) * p.hq + h0 + w.c);
+        const float inv = w.l == 0.f ? 0.f : 1.f / w.l;
+        float* dst = p.part_o + r0 * D;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int j = 0; j < D / 16; j += 4)
+            *(f32x4*)(dst + (D / 16) * (4 * w.g + r) + j) = f32x4{w.acc[j][r], w.acc[j + 1][r], w.acc[j + 2][r], w.acc[j + 3][r]} * inv;
+        if (w.g == 0) p.part_lse[r0] = w.l > 0.f ? w.m + __builtin_amdgcn_logf(w.l) : (w.l == w.l ? -INFINITY : w.l);  // (log2 domain)
+      }
+      at = to;
+    }
+    first += units;
+  }
+}
+
+// o = sum of a request's partials by their log-sum-exps; D / 4 lanes read a row, the rows are dealt to the rest of the workgroup.
+template <int D>
+__global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
+  constexpr int LPR = D / 4, SL = 256 / LPR;
+  __shared__ __attribute__((aligned(16))) float acc[SL][D + 4];
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int lane = threadIdx.x & 63;
+  const Deal dl = deal(p);
+  int64_t first = 0;
+  for (int b0 = 0; b0 < b; b0 += 64) first += b0 + lane < b ? units_of(p, b0 + lane) : 0;
+  first = wave_sum(first);
+  const int64_t units = units_of(p, b);
+  const int s0 = (int)(first / dl.per_share), n = units ? (int)((first + units - 1) / dl.per_share) - s0 + 1 : 0;
+  const int slice = threadIdx.x / LPR, d = (threadIdx.x & (LPR - 1)) * 4;
+  const float* lse = p.part_lse + ((int64_t)(s0 + b) * p.hq + h);
+  const float* row = p.part_o + ((int64_t)(s0 + b) * p.hq + h) * D + d;
+  float M = -INFINITY, L = 0.f;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int i = slice; i < n; i += SL) {
+    const float x = lse[(int64_t)i * p.hq];
+    const f32x4 v = *(const f32x4*)(row + (int64_t)i * p.hq * D);
+    const float m_new = x > M ? x : M;
+    const float f = exp2_diff(M, m_new), w = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - m_new);
+    L = L * f + w;
+    sum = w != 0.f ? sum * f + v * w : sum * f;
+    M = m_new;
+  }
+  *(f32x4*)&acc[slice][d] = sum;
+  if (d == 0) acc[slice][D] = M, acc[slice][D + 1] = L;
+  __syncthreads();
+  if (slice) return;
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < SL; i++) top = fmaxf(top, acc[i][D]);
+  L = 0.f;
+  sum = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < SL; i++) {
+    const float f = exp2_diff(acc[i][D], top);
+    L += acc[i][D + 1] * f;
+    if (f != 0.f) sum += *(const f32x4*)&acc[i][d] * f;
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int64_t at = (int64_t)b * p.hq + h;
+  store_elem4(p.o, p.o_dtype, at * D + d, sum * inv);
+  if (d == 0) p.lse[at] = ln_of(top, L);
+}
+
+constexpr int kDirectWaves = 8;
+constexpr int64_t kDirectTokens = 4096;  // visible tokens of the longest request up to which a workgroup takes a whole (request, KV head)
+constexpr int64_t kShareWaves = 16 * kCUs;
+constexpr int64_t kMinUnits = 2;
+
+int64_t most_visible(int64_t max_len, int64_t window, int64_t sinks) { return window > 0 && window + sinks < max_len ? window + sinks : max_len; }
+int64_t tasks_of(int64_t hq, int64_t hkv) { return hkv * ((hq / hkv + kHeads - 1) / kHeads); }
+bool is_direct(int64_t batch, int64_t tasks, int64_t most) { return most <= kDirectTokens || (batch * tasks >= 2 * kCUs && most <= 2 * kDirectTokens); }
+// shares of a launch that is not direct
+int64_t shares_of(int64_t batch, int64_t tasks, int64_t most) {
+  const int64_t units = batch * ((most + kBlock - 1) / kBlock);
+  const int64_t by_waves = (kShareWaves + tasks - 1) / tasks, by_units = (units + kMinUnits - 1) / kMinUnits;
+  const int64_t n = by_waves < by_units ? by_waves : by_units;
+  return n < 1 ? 1 : n;
+}
+
+template <typename QT, typename KV, int D> void launch(const PoolParams& p, bool direct, hipStream_t st) {
+  if (direct) {
+    LSATTN_LAUNCH_KERNEL((pool_decode_direct_kernel<QT, KV, D, kDirectWaves>), dim3(p.tasks, p.batch), dim3(kDirectWaves * 64), 0, st, p);
+    return;
+  }
+  const int64_t wgs = ((int64_t)p.shares * p.tasks + 3) / 4;
+  LSATTN_LAUNCH_KERNEL((pool_decode_shares_kernel<QT, KV, D>), dim3((unsigned)((wgs + 7) / 8 * 8)), dim3(256), 0, st, p);
+  if (hipPeekAtLastError() != hipSuccess) return;
+  LSATTN_LAUNCH_KERNEL((pool_decode_merge_kernel<D>), dim3(p.hq, p.batch), dim3(256), 0, st, p);
+}
+template <typename QT, typename KV> void launch_d(const PoolParams& p, int64_t d, bool direct, hipStream_t st) {
+  if (d == 128) launch<QT, KV, 128>(p, direct, st);
+  else launch<QT, KV, 64>(p, direct, st);
+}
+
+}  // namespace
+}  // namespace lsattn
+
+using namespace lsattn;
+
+extern "C" size_t lsattn_pool_attention_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                                        int64_t max_len_in_batch, int64_t window, int64_t sinks) {
+  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 || max_len_in_batch <= 0 || window < 0 || sinks < 0)
+    return 0;
+  const int64_t tasks = tasks_of(num_q_heads, num_kv_heads), most = most_visible(max_len_in_batch, window, sinks);
+  if (is_direct(batch, tasks, most)) return 0;
+  return (size_t)((shares_of(batch, tasks, most) + batch) * num_q_heads * (head_dim + 1) * 4);
+}
+
+extern "C" int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* stream) {
+  if (!a || !a->q || !a->k || !a->v || !a->o || !a->lse || !a->req_to_tokens || !a->b_req_idx || !a->b_seqlen) return LSATTN_ERR_INVALID_ARG;
+  if (a->batch < 0 || a->num_q_heads < 1 || a->num_kv_heads < 1 || a->num_slots < 1 || a->num_reqs < 0 || a->max_seq_len < 0 || a->max_len_in_batch < 0 ||
+      a->window < 0 || a->sinks < 0)
+    return LSATTN_ERR_INVALID_ARG;
+  if (a->num_q_heads % a->num_kv_heads || (a->head_dim != 128 && a->head_dim != 64)) return LSATTN_ERR_UNSUPPORTED;
+  if (a->o_dtype != LSATTN_F32 && a->o_dtype != LSATTN_F16 && a->o_dtype != LSATTN_BF16) return LSATTN_ERR_UNSUPPORTED;
+  if ((a->dtype != LSATTN_F16 && a->dtype != LSATTN_BF16) || (a->kv_dtype != a->dtype && a->kv_dtype != LSATTN_E4M3)) return LSATTN_ERR_UNSUPPORTED;
+  const bool k8 = a->kv_dtype == LSATTN_E4M3;
+  const int64_t es = k8 ? 1 : 2;
+  if ((a->k_stride_0 * es) % 16 || (a->k_stride_1 * es) % 16 || (a->v_stride_0 * es) % 16 || (a->v_stride_1 * es) % 16 ||
+      (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->o) & 15))
+    return LSATTN_ERR_INVALID_ARG;
+  if (k8 && (!a->k_scales || !a->v_scales)) return LSATTN_ERR_INVALID_ARG;
+  if (a->batch > 65535 || a->num_q_heads > 65535 || a->max_seq_len > 0x7fffff00 || a->num_slots > 0x7fffffff || a->num_reqs > 0x7fffffff ||
+      a->max_len_in_batch > 0x7fffffff)
+    return LSATTN_ERR_INVALID_ARG;
+  if (!(a->sm_scale > 0.f)) return LSATTN_ERR_INVALID_ARG;
+  if (a->batch == 0) return LSATTN_OK;
+  PoolParams p;
+  p.q = (const char*)a->q, p.k = (const char*)a->k, p.v = (const char*)a->v;
+  p.k_s0 = a->k_stride_0 * es, p.k_s1 = a->k_stride_1 * es, p.v_s0 = a->v_stride_0 * es, p.v_s1 = a->v_stride_1 * es;
+  p.ks = a->k_scales, p.vs = a->v_scales;
+  p.ks_s0 = a->ks_stride_0, p.ks_s1 = a->ks_stride_1, p.vs_s0 = a->vs_stride_0, p.vs_s1 = a->vs_stride_1;
+  p.table = a->req_to_tokens, p.b_req = a->b_req_idx, p.b_len = a->b_seqlen, p.max_seq_len = a->max_seq_len;
+  p.batch = (int32_t)a->batch, p.num_reqs = (int32_t)a->num_reqs, p.num_slots = (int32_t)a->num_slots;
+  p.hq = (int32_t)a->num_q_heads, p.hkv = (int32_t)a->num_kv_heads, p.group = p.hq / p.hkv;
+  p.sub_groups = (p.group + kHeads - 1) / kHeads, p.tasks = p.hkv * p.sub_groups;
+  // (a window that holds every position a table can have is none)
+  p.window = a->window >= a->max_seq_len ? 0 : (int32_t)a->window;
+  p.sinks = a->sinks > a->max_seq_len ? (int32_t)a->max_seq_len : (int32_t)a->sinks;
+  p.scale_log2 = a->sm_scale * kLog2e;
+  p.o = (char*)a->o, p.o_dtype = a->o_dtype, p.lse = a->lse;
+  p.by_tasks = fast_div((uint32_t)p.tasks), p.by_sub = fast_div((uint32_t)p.sub_groups);
+  const int64_t most = most_visible(a->max_len_in_batch, a->window, a->sinks);
+  const bool direct = is_direct(p.batch, p.tasks, most);
+  p.part_o = nullptr, p.part_lse = nullptr, p.shares = 1, p.min_units = (int32_t)kMinUnits;
+  if (!direct) {
+    const int64_t shares = shares_of(p.batch, p.tasks, most), rows = shares + p.batch;
+    if (!a->workspace || a->workspace_bytes < (size_t)(rows * p.hq * (a->head_dim + 1) * 4)) return LSATTN_ERR_WORKSPACE;
+    if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
+    p.shares = (int32_t)shares;
+    p.part_o = (float*)a->workspace, p.part_lse = p.part_o + rows * p.hq * a->head_dim;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (k8) {
+    if (a->dtype == LSATTN_F16) launch_d<F16, E4M3>(p, a->head_dim, direct, st);
+    else launch_d<BF16, E4M3>(p, a->head_dim, direct, st);
+  } else {
+    if (a->dtype == LSATTN_F16) launch_d<F16, F16>(p, a->head_dim, direct, st);
+    else launch_d<BF16, BF16>(p, a->head_dim, direct, st);
+  }
+  return check_launch();
+}

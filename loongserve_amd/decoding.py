@@ -4,10 +4,12 @@ longserve_flash_decoding_stage2.py:53 and longserve_flash_decoding.py:3."""
 from __future__ import annotations
 
 import functools
+from typing import Optional, Tuple
 
 import torch
 
-from . import _native, longserve_cuda_kernels
+from . import _lib, _native, longserve_cuda_kernels
+from .ops import _fp8_pool, _i32vec, _on_current_device
 
 
 # The stage functions called on their own (the master path, longserve_transformer_layer_infer.py:272-281 then :360-367)
@@ -97,3 +99,93 @@ def longserve_token_decode_attention_flash_decoding(q, req_to_token_indexs, b_re
                                           b_req_idx, b_seq_len, max_len_in_batch, o_tensor.view(calcu_shape1), out_logexpsum,
                                           split)
     return o_tensor, out_logexpsum
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# Decode over a pool in 8 bits, and behind a sliding window (lsattn_pool_attention); no reference counterpart.
+def pool_attention_workspace_bytes(batch_size: int, q_head_num: int, kv_head_num: int, head_dim: int, max_len_in_batch: int,
+                                   window: Optional[int] = None, sinks: int = 0) -> int:
+    """Bytes of device memory that the two operators below need for the partials of such a call (0: none)."""
+    return int(_lib.load().lsattn_pool_attention_workspace_bytes(int(batch_size), int(q_head_num), int(kv_head_num), int(head_dim),
+                                                                 int(max_len_in_batch), int(window or 0), int(sinks)))
+
+
+def _pool_attention(q, table, b_req_idx, b_seq_len, max_len_in_batch, cache_k, cache_v, k_scales, v_scales, window, sinks, out, lse, workspace):
+    # (a window of None is 0 to the library; one of 0 would see nothing, not even the token itself)
+    if window is None or window > 0:
+        done = _native.pool_attention(q, table, b_req_idx, b_seq_len, max_len_in_batch, cache_k, cache_v, k_scales, v_scales, window or 0, sinks,
+                                      out, lse, workspace)
+        if done is not None:
+            return done
+    # arguments the native pass does not take: say what is wrong
+    _on_current_device(((q, "q"), (table, "req_to_token_indexs"), (b_req_idx, "b_req_idx"), (b_seq_len, "b_seq_len"), (cache_k, "cache_k"),
+                        (cache_v, "cache_v"), (k_scales, "k_scales"), (v_scales, "v_scales"), (out, "out"), (lse, "o_logexpsum"), (workspace, "workspace")))
+    if q.dtype not in (torch.float16, torch.bfloat16) or q.dim() != 3 or not q.is_contiguous():
+        raise ValueError("q must be a contiguous float16 or bfloat16 [batch, heads, head_dim] tensor")
+    B, Hq, D = q.shape
+    if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous():
+        raise ValueError("req_to_token_indexs must be a contiguous [max_req, max_seq] int32 tensor")
+    _i32vec(b_req_idx, "b_req_idx", B)
+    _i32vec(b_seq_len, "b_seq_len", B)
+    if cache_k.dim() != 3 or cache_k.shape != cache_v.shape or cache_k.shape[2] != D or cache_k.dtype != cache_v.dtype:
+        raise ValueError("cache_k and cache_v must be [slots, kv_heads, head_dim] for q's head_dim, of one type")
+    if cache_k.stride(2) != 1 or cache_v.stride(2) != 1:
+        raise ValueError("cache_k and cache_v must be contiguous in head_dim")
+    if D not in (64, 128):
+        raise ValueError("head_dim must be 64 or 128 (got %d)" % D)
+    if cache_k.shape[1] == 0 or Hq == 0 or Hq % cache_k.shape[1]:
+        raise ValueError("bad head counts: Hq=%d Hkv=%d" % (Hq, cache_k.shape[1]))
+    if k_scales is not None:
+        _fp8_pool(cache_k, k_scales, "cache_k", "k_scales")
+        _fp8_pool(cache_v, v_scales, "cache_v", "v_scales")
+    elif cache_k.dtype != q.dtype:
+        raise ValueError("cache_k and cache_v must have the type of q (a pool in 8 bits: longserve_fp8_decode_attention)")
+    if (window is not None and int(window) < 1) or int(sinks) < 0 or int(max_len_in_batch) < 0:
+        raise ValueError("window must be >= 1 (the token itself), sinks and max_len_in_batch >= 0")
+    if out is not None and (out.dtype not in (torch.float16, torch.bfloat16, torch.float32) or out.shape != q.shape or not out.is_contiguous()):
+        raise ValueError("out must be a contiguous float16, bfloat16 or float32 tensor of q's shape")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (B, Hq) or not lse.is_contiguous()):
+        raise ValueError("o_logexpsum must be a contiguous float32 [batch, heads] tensor")
+    if workspace is not None:
+        need = pool_attention_workspace_bytes(B, Hq, cache_k.shape[1], D, max_len_in_batch, window, sinks)
+        if not workspace.is_contiguous() or workspace.numel() * workspace.element_size() < need:
+            raise ValueError("workspace must be contiguous and hold at least %d bytes (pool_attention_workspace_bytes)" % need)
+    if B == 0:
+        return (torch.empty_like(q, dtype=torch.float32) if out is None else out,
+                torch.empty((0, Hq), dtype=torch.float32, device=q.device) if lse is None else lse)
+    raise ValueError("decode attention: arguments that no kernel takes (an empty pool?)")
+
+
+def longserve_fp8_decode_attention(q: torch.Tensor, req_to_token_indexs: torch.Tensor, b_req_idx: torch.Tensor, b_seq_len: torch.Tensor,
+                                   max_len_in_batch: int, cache_k: torch.Tensor, cache_v: torch.Tensor, k_scales: torch.Tensor,
+                                   v_scales: torch.Tensor, window: Optional[int] = None, sinks: int = 0,
+                                   out: Optional[torch.Tensor] = None, o_logexpsum: Optional[torch.Tensor] = None,
+                                   workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Decode attention of one new token per request over a pool that kv_scatter_fp8 writes: (o, natural log-sum-exp).
+
+    q [batch, q_heads, head_dim] (float16 or bfloat16, head_dim 64 or 128), cache_k / cache_v the K and V heads of the pool
+    (float8_e4m3fn [slots, kv_heads, head_dim], any slot and head strides that keep rows 16-byte aligned), k_scales /
+    v_scales their exponent bytes [slots, kv_heads].  out (None: float32, as longserve_token_decode_attention_flash_decoding
+    returns) may be float32, float16 or bfloat16.  Products and sums are float32-exact in P and V; K and V stand for exactly what the pool holds.
+
+    window: the token sees the last `window` positions of its context (itself among them) and the first `sinks`; None: all.
+    The context of a request lies in this pool as a whole when a window is given; without one, (o, log-sum-exp) of several instances merge by
+    lse_merge.  Requests without tokens get o = 0, -inf.  Entries of the table that name no slot of the pool count as positions that do not exist.
+    max_len_in_batch (a bound of b_seq_len) only sizes the launch and the scratch.  workspace: the caller's scratch
+    (pool_attention_workspace_bytes; else torch allocates it), one for each call that may run at the same time, graphs' replays among them."""
+    if k_scales is None or v_scales is None:
+        raise ValueError("k_scales and v_scales: uint8 [slots, kv_heads]")
+    return _pool_attention(q, req_to_token_indexs, b_req_idx, b_seq_len, max_len_in_batch, cache_k, cache_v, k_scales, v_scales, window, sinks,
+                           out, o_logexpsum, workspace)
+
+
+def longserve_window_decode_attention(q: torch.Tensor, req_to_token_indexs: torch.Tensor, b_req_idx: torch.Tensor, b_seq_len: torch.Tensor,
+                                      max_len_in_batch: int, cache_k: torch.Tensor, cache_v: torch.Tensor, window: int, sinks: int = 0,
+                                      out: Optional[torch.Tensor] = None, o_logexpsum: Optional[torch.Tensor] = None,
+                                      workspace: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """longserve_fp8_decode_attention over the 16-bit pool (cache_k / cache_v of q's type), behind a sliding window: every token sees
+    the last `window` positions of its context (itself among them) and the first `sinks`.  Positions outside cost nothing."""
+    if window is None:
+        raise ValueError("window must be >= 1 (without one: longserve_token_decode_attention_flash_decoding)")
+    return _pool_attention(q, req_to_token_indexs, b_req_idx, b_seq_len, max_len_in_batch, cache_k, cache_v, None, None, window, sinks,
+                           out, o_logexpsum, workspace)

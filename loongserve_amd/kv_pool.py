@@ -79,9 +79,15 @@ class LongServeMemoryManager:
     def _init_buffers(self, size, dtype, head_num, head_dim, layer_num, num_idle_slots=0):
         # K heads then V heads per slot (longserve_mem_manager.py:26)
         self.kv_buffer = torch.empty((layer_num, size + num_idle_slots, 2 * head_num, head_dim), dtype=dtype, device="cuda")
+        # a pool in 8 bits (dtype float8_e4m3fn; not in the reference) has an exponent byte per slot and head beside it, which
+        # kv_scatter_fp8 writes with the rows
+        self.kv_scales = None
+        if dtype == torch.float8_e4m3fn:
+            self.kv_scales = torch.full((layer_num, size + num_idle_slots, 2 * head_num), 127, dtype=torch.uint8, device="cuda")
 
     def _free_buffers(self):
         self.kv_buffer = None
+        self.kv_scales = None
 
     @torch.inference_mode()
     def alloc(self, need_size):

@@ -499,6 +499,79 @@ def kv_scatter(src: torch.Tensor, dest_index: torch.Tensor, pool: torch.Tensor) 
     _lib.check(rc, "lsattn_kv_scatter")
 
 
+def _on_current_device(tensors) -> None:
+    """The launch goes to the current device's stream: a tensor of another GPU is refused."""
+    for t, n in tensors:
+        if t is not None:
+            _dev(t, n)
+            if t.device.index != torch.cuda.current_device():
+                raise ValueError("%s must live on the current device (got %s)" % (n, t.device))
+
+
+def _fp8_pool(pool: torch.Tensor, scales: torch.Tensor, name: str = "pool", scales_name: str = "scales") -> None:
+    if pool.dtype != torch.float8_e4m3fn or pool.dim() != 3 or pool.stride(2) != 1:
+        raise ValueError("%s must be float8_e4m3fn [slots, heads, head_dim], contiguous in head_dim" % name)
+    if scales.dtype not in (torch.uint8, torch.float8_e8m0fnu) or tuple(scales.shape) != tuple(pool.shape[:2]):
+        raise ValueError("%s must be uint8 (or float8_e8m0fnu) [slots, heads] for the slots and heads of %s" % (scales_name, name))
+
+
+def kv_scatter_fp8(src: torch.Tensor, dest_index: torch.Tensor, pool: torch.Tensor, scales: torch.Tensor) -> None:
+    """Quantises rows as they are written: src [tokens, heads, head_dim] (float16 or bfloat16; K heads then V heads, as
+    kv_scatter takes them) into pool[dest_index] (float8_e4m3fn [slots, heads, head_dim]) with one power-of-two scale per
+    token and head in scales[dest_index] (uint8 [slots, heads], exponent + 127; the same bytes as float8_e8m0fnu):
+
+      e = the least integer with max |x| <= 448 * 2^e (at least -126),   pool = e4m3(x * 2^-e),   scales = e + 127.
+
+    x * 2^-e is exact, so a value is off by the rounding to e4m3 alone.  Elements that are not finite become NaN and do not
+    count in the maximum.  dest_index is int32 or, as the allocator returns it, int64; a slot outside the pool is skipped, a
+    slot named twice holds a mixture.  No reference counterpart (its pool is float16)."""
+    if _native.kv_scatter_fp8(src, dest_index, pool, scales):
+        return
+    _on_current_device(((src, "src"), (dest_index, "dest_index"), (pool, "pool"), (scales, "scales")))
+    if src.dtype not in (torch.float16, torch.bfloat16) or src.dim() != 3 or src.stride(2) != 1:
+        raise ValueError("src must be float16 or bfloat16 [tokens, heads, head_dim], contiguous in head_dim")
+    _fp8_pool(pool, scales)
+    if src.shape[1:] != pool.shape[1:]:
+        raise ValueError("src and pool rows must match")
+    if dest_index.dtype not in (torch.int32, torch.int64) or tuple(dest_index.shape) != (src.shape[0],) or not dest_index.is_contiguous():
+        raise ValueError("dest_index must be a contiguous int32 or int64 vector with one slot per token")
+    if src.numel() == 0 or pool.numel() == 0:
+        return  # nothing to write, or nowhere
+    raise ValueError("kv_scatter_fp8: arguments that no kernel takes")
+
+
+def kv_gather_fp8(pool: torch.Tensor, scales: torch.Tensor, req_to_token_indexs: torch.Tensor, b_req_idx: torch.Tensor,
+                  b_seq_len: torch.Tensor, b_start_loc: torch.Tensor, max_len_in_batch: int, out: torch.Tensor,
+                  b_first: Optional[torch.Tensor] = None) -> None:
+    """Reads contexts back from a pool of kv_scatter_fp8, packed one request after the other as the prefill operators take
+    their K/V:
+
+      out[b_start_loc[b] + i] = value of slot req_to_token_indexs[b_req_idx[b], b_first[b] + i]   for i < b_seq_len[b]
+
+    out is float16 or bfloat16 [rows, heads, head_dim]; every value is exact in its normal range (past float16's range
+    +-65504).  b_first (None: 0) starts a request's rows further on in its context.  max_len_in_batch bounds b_seq_len.  A token
+    whose slot is not in the pool (an unused entry of the table) is a row of zeros; rows of out that no request names stay as
+    they were.  The next chunk of a prompt attends to the result through context_attention_fwd or prefill_attention_step."""
+    if _native.kv_gather_fp8(pool, scales, req_to_token_indexs, b_req_idx, b_seq_len, b_start_loc, max_len_in_batch, out, b_first):
+        return
+    _on_current_device(((pool, "pool"), (scales, "scales"), (req_to_token_indexs, "req_to_token_indexs"), (b_req_idx, "b_req_idx"),
+                        (b_seq_len, "b_seq_len"), (b_start_loc, "b_start_loc"), (out, "out"), (b_first, "b_first")))
+    _fp8_pool(pool, scales)
+    if req_to_token_indexs.dtype != torch.int32 or req_to_token_indexs.dim() != 2 or not req_to_token_indexs.is_contiguous():
+        raise ValueError("req_to_token_indexs must be a contiguous [max_req, max_seq] int32 tensor")
+    B = b_req_idx.shape[0]
+    for t, n in ((b_req_idx, "b_req_idx"), (b_seq_len, "b_seq_len"), (b_start_loc, "b_start_loc"), (b_first, "b_first")):
+        if t is not None:
+            _i32vec(t, n, B)
+    if out.dtype not in (torch.float16, torch.bfloat16) or out.dim() != 3 or out.stride(2) != 1 or out.shape[1:] != pool.shape[1:]:
+        raise ValueError("out must be float16 or bfloat16 [rows, heads, head_dim] for the heads and head_dim of pool")
+    if int(max_len_in_batch) < 0:
+        raise ValueError("max_len_in_batch must be >= 0")
+    if B == 0 or int(max_len_in_batch) == 0 or out.numel() == 0:
+        return
+    raise ValueError("kv_gather_fp8: arguments that no kernel takes")
+
+
 def rmsnorm_forward(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:
     """Name and signature of the Triton operator behind the final norm
     (loongserve/models/llama/triton_kernel/rmsnorm.py:41-63, called
