@@ -166,6 +166,14 @@ int lsattn_prefill_step_merge(const lsattn_prefill_args* a, void* stream);
  * from lse = -inf everywhere).  Uses o (F32), lse. */
 int lsattn_prefill_step_accumulate(const lsattn_prefill_args* a, void* stream);
 
+/* A prefill step behind a sliding window with sinks, from the empty state; no counterpart in the reference.  Beside the mask of
+ * lsattn_prefill_step (kv position <= q position) a key counts only if its position is > q position - window or < sinks, in the global
+ * positions of the *_first vectors and sp_peers; the work is that of the tiles that hold such keys.  window >= 1 (1: the position itself), sinks >= 0.
+ * Uses o (o_dtype LSATTN_F32 or dtype) and lse (natural log-sum-exp; NULL: not wanted); rows that see no key get o = 0, lse = -inf.  Partials
+ * over several KV chunks (o in fp32) join by lsattn_lse_merge.  kv_cuts is not taken.  A bfloat16 V is multiplied as fp16 (v_is_f16, or
+ * converted in the kernel): magnitudes past 65504 count as 65504, below 2^-14 they are kept to 2^-24. */
+int lsattn_prefill_window(const lsattn_prefill_args* a, int64_t window, int64_t sinks, void* stream);
+
 /*
  * Merge n normalised partials (O_i fp32 [rows,D] contiguous, LSE_i [rows]) over disjoint key
  * sets: LSE = log sum_i exp(LSE_i), O = sum_i exp(LSE_i-LSE) O_i.  Same recurrence as
@@ -687,7 +695,8 @@ const char* lsattn_strerror(int code);
  * the counts of lsattn_pool_update_refs also in pinned host memory and, past LSATTN_POOL_REFS_ORDERED entries, not behind the state; 5 = total_kv_rows and kv_cut_even in lsattn_prefill_args,
  * lsattn_prefill_converts_v; 6 = max_kv_len there (a reserved word before), lsattn_prefill_route,
  * lsattn_prefill_cut_count; 7 = o_is_apart in lsattn_decode_stage2_args (a reserved word before); 8 = o_is_apart of 2;
- * 9 = lead_rows in lsattn_decode_stage2_args; 10 = lsattn_kv_scatter_fp8, lsattn_kv_gather_fp8, lsattn_pool_attention. */
+ * 9 = lead_rows in lsattn_decode_stage2_args; 10 = lsattn_kv_scatter_fp8, lsattn_kv_gather_fp8, lsattn_pool_attention,
+ * lsattn_prefill_window. */
 #define LSATTN_VERSION 10
 int lsattn_version(void);
 

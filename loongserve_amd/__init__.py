@@ -25,7 +25,7 @@ if not _building:
     from .ops import (context_attention_fwd, copy_kv_index_to_req, decoding_stage_migration_receiver_kernel,
                       decoding_stage_migration_sender_kernel, destindex_copy_and_register_kv, destindex_copy_kv,
                       init_req_to_token_indexes, kv_gather_fp8, kv_scatter, kv_scatter_fp8, lse_merge, pre_copy_and_register_kv, prefill_attention_step,
-                      rmsnorm_forward, rotary_emb_fwd, rotary_emb_write_kv, silu_and_mul_fwd)
+                      rmsnorm_forward, rotary_emb_fwd, rotary_emb_write_kv, silu_and_mul_fwd, window_attention_fwd)
 
 __all__ = [
     "context_attention_fwd", "prefill_attention_step", "lse_merge", "kv_scatter", "init_req_to_token_indexes",
@@ -35,6 +35,6 @@ __all__ = [
     "longserve_flash_decode_stage1", "longserve_flash_decode_stage2",
     "longserve_token_decode_attention_flash_decoding", "longserve_cuda_kernels",
     "kv_scatter_fp8", "kv_gather_fp8", "longserve_fp8_decode_attention", "longserve_window_decode_attention",
-    "pool_attention_workspace_bytes",
+    "pool_attention_workspace_bytes", "window_attention_fwd",
     "LongServeMemoryManager", "LongServeReqManager", "set_tuning",
 ]

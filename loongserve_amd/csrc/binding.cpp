@@ -30,6 +30,7 @@ struct Library {
   decltype(&lsattn_prefill_step) prefill_step;
   decltype(&lsattn_prefill_step_merge) prefill_step_merge;
   decltype(&lsattn_prefill_step_accumulate) prefill_step_accumulate;
+  decltype(&lsattn_prefill_window) prefill_window;
   decltype(&lsattn_prefill_merge_cuts) prefill_merge_cuts;
   decltype(&lsattn_prefill_converts_v) prefill_converts_v;
   decltype(&lsattn_bf16_to_f16_rows) bf16_to_f16_rows;
@@ -58,6 +59,7 @@ PyObject* bind(PyObject*, PyObject* addresses) {
       {"lsattn_prefill_step", (void**)&lib.prefill_step},
       {"lsattn_prefill_step_merge", (void**)&lib.prefill_step_merge},
       {"lsattn_prefill_step_accumulate", (void**)&lib.prefill_step_accumulate},
+      {"lsattn_prefill_window", (void**)&lib.prefill_window},
       {"lsattn_prefill_merge_cuts", (void**)&lib.prefill_merge_cuts},
       {"lsattn_prefill_converts_v", (void**)&lib.prefill_converts_v},
       {"lsattn_bf16_to_f16_rows", (void**)&lib.bf16_to_f16_rows},
@@ -549,6 +551,27 @@ bool exponents(const at::Tensor& s, const at::Tensor& pool) {
 }
 bool e4m3_rows(const at::Tensor& t) { return is(t, at::kFloat8_e4m3fn) && t.stride(2) == 1; }
 
+// (q, k, v, o, six vectors, peers, max_q, window, sinks, lse or None, total_q) -> True or None
+PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(16);
+  Args in(args);
+  const at::Tensor &q = in.gpu(3), &k = in.gpu(3), &v = in.gpu(3), &o = in.gpu(3);
+  OR_NONE(in.ok);
+  Step s;
+  OR_NONE(s.read(in, q, k, v) && same_shape(o, q) && (o.scalar_type() == q.scalar_type() || is(o, at::kFloat)) && s.state(o));
+  const int64_t window = in.integer(), sinks = in.integer();
+  const at::Tensor* lse = in.maybe();
+  s.p.total_q_rows = in.integer();
+  OR_NONE(in.ok && here({&q, &k, &v, &o, s.q_start, s.q_len, lse}) && window >= 1 && sinks >= 0 && s.p.total_q_rows >= 0 && s.p.sp_peers >= 1 && s.p.max_q_len >= 0);
+  if (lse) OR_NONE(is(*lse, at::kFloat) && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == q.size(0) && lse->size(1) == q.size(1));
+  OR_NONE(q.numel() > 0 && k.numel() > 0);
+  s.p.lse = lse ? (float*)lse->data_ptr() : nullptr;
+  if (const int rc = call(lib.prefill_window, &s.p, window, sinks, stream())) return failed(rc, "lsattn_prefill_window");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
 // (src, dest_index, pool, scales) -> True or None
 PyObject* kv_scatter_fp8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
@@ -858,7 +881,7 @@ PyMethodDef methods[] = {
     ENTRY(context_attention), ENTRY(prefill_partial), ENTRY(token_decode_attention), ENTRY(decode_stage1), ENTRY(decode_stage2),
     ENTRY(kv_scatter), ENTRY(register_decode_tokens), ENTRY(register_tokens), ENTRY(rms_norm), ENTRY(silu_and_mul_inplace),
     ENTRY(rotary_emb), ENTRY(rotary_kv_write), ENTRY(pool_alloc), ENTRY(pool_update_refs),
-    ENTRY(kv_scatter_fp8), ENTRY(kv_gather_fp8), ENTRY(pool_attention),
+    ENTRY(window_attention), ENTRY(kv_scatter_fp8), ENTRY(kv_gather_fp8), ENTRY(pool_attention),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native argument pass of loongserve_amd's operators.", -1, methods};
 

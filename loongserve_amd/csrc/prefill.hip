@@ -1403,6 +1403,7 @@ template <typename T, int MODE, bool DV> static int launch_prefill(const lsattn_
   return launch_prefill_shape<T, MODE, DV, false>(a, st);
 }
 
+// mode 3: behind a window, from the empty state, o in fp32 or in q's type, lse optional
 static int validate(const lsattn_prefill_args* a, int mode) {
   if (!a || !a->q || !a->k || !a->v || !a->o) return LSATTN_ERR_INVALID_ARG;
   if (!a->q_b_start_loc || !a->q_b_seq_len || !a->q_first_token_global_idx || !a->kv_b_start_loc || !a->kv_b_seq_len ||
@@ -1429,7 +1430,10 @@ static int validate(const lsattn_prefill_args* a, int mode) {
   // a lane addresses the 64 rows of a K/V tile with a 32-bit byte offset from the tile's first row
   if (a->k_stride_t <= 0 || a->v_stride_t <= 0 || a->k_stride_t > (1 << 24) || a->v_stride_t > (1 << 24)) return LSATTN_ERR_INVALID_ARG;
   if (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->o) & 15) return LSATTN_ERR_INVALID_ARG;
-  if (mode == 0 || mode == 2) {
+  if (mode == 3) {
+    if (a->kv_cuts > 1) return LSATTN_ERR_INVALID_ARG;
+    if (a->o_dtype != LSATTN_F32 && a->o_dtype != a->dtype) return LSATTN_ERR_INVALID_ARG;
+  } else if (mode == 0 || mode == 2) {
     if (!a->lse || a->o_dtype != LSATTN_F32) return LSATTN_ERR_INVALID_ARG;
   } else {
     if (!a->m || !a->l || a->o_dtype != a->dtype) return LSATTN_ERR_INVALID_ARG;
@@ -1466,6 +1470,15 @@ extern "C" int lsattn_prefill_step_accumulate(const lsattn_prefill_args* a, void
   if (a->head_dim != 128 || prefill_short_blocks(a)) return launch_prefill_small(a, 2, (hipStream_t)stream);
   if (a->dtype == LSATTN_F16) return launch_prefill<F16, 2, true>(a, (hipStream_t)stream);
   return a->v_is_f16 ? launch_prefill<BF16, 2, true>(a, (hipStream_t)stream) : launch_prefill<BF16, 2, false>(a, (hipStream_t)stream);
+}
+
+extern "C" int lsattn_prefill_window(const lsattn_prefill_args* a, int64_t window, int64_t sinks, void* stream) {
+  const int rc = validate(a, 3);
+  if (rc != LSATTN_OK) return rc;
+  if (window < 1 || sinks < 0) return LSATTN_ERR_INVALID_ARG;
+  if (a->batch == 0 || a->max_q_len == 0) return LSATTN_OK;
+  // (positions are 31-bit: larger ones change nothing)
+  return launch_prefill_window(a, (int32_t)(window < 0x7fffffff ? window : 0x7fffffff), (int32_t)(sinks < 0x7fffffff ? sinks : 0x7fffffff), (hipStream_t)stream);
 }
 
 extern "C" int lsattn_prefill_route(const lsattn_prefill_args* a) {

@@ -96,6 +96,7 @@ struct SmallParams {
   int64_t ml_st, ml_sh;
   int32_t batch, bunch, turns;  // the grid takes `bunch` requests at a time; whether their places move on by one from tile to tile
   FastDiv d_bunch;
+  int32_t window, sinks;  // (WIN) positions that a query sees up to its own, first positions that every later one sees
 };
 
 constexpr int kWaves = 4;   // waves per workgroup
@@ -140,8 +141,12 @@ template <int D, int WP, bool DV> constexpr int kResident = D == 128 ? (WP == 32
 // KP = 2: two waves share the positions of a wave and take the first and the second 32 keys of every tile (launches of up to a workgroup per CU, whose one
 // wave per SIMD issues an instruction every five cycles or so); their parts are joined in LDS.  A tile takes 0.75 us of a lone workgroup instead of 0.96, the join and the start
 // of twice the waves 1.1.
-template <typename T, int D, int MODE, bool DV, int WP, int KP = 1>
+// WIN: attention behind a sliding window with sinks: the query at position x sees keys at positions y <= x with y > x - window or y < sinks.  The
+// workgroup walks the tiles that hold sinks, then those from its first row's window on; MODE 0, or MODE 3: O in T's type and the LSE,
+// from the empty state.
+template <typename T, int D, int MODE, bool DV, int WP, int KP = 1, bool WIN = false>
 __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void prefill_small_kernel(SmallParams p) {
+  static_assert(WIN ? KP == 1 && (MODE == 0 || MODE == 3) : MODE < 3, "a window knows no state");
   static_assert(KP == 1 || (KP == 2 && WP == 16 && D >= 32), "the parts of a tile of 64 keys, the columns that each of two waves finishes");
   constexpr int NW = kWaves * KP;
   constexpr int QB = WP / 16;               // blocks of 16 positions per wave
@@ -158,9 +163,10 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
   // LDS writes 1 KB in a row); instead the 16-byte chunks of a row are XORed with a function of the row: K so that a
   // column of chunks of sixteen rows, which one read takes, lies in sixteen different sets of four banks, V so that 32 bytes of
   // each of eight rows (half a transposing read) cover the banks once.  Rows sixteen apart share their XOR.
-  // (behind them, for the epilogue that folds into (o, m, l): 256 bytes per wave for the old m and l of its rows)
+  // (behind them, for the epilogue that folds into (o, m, l): 256 bytes per wave for the old m and l of its rows; WIN: 128 for the keys in
+  // front of its rows' windows, which only the steps at a window's edge read)
   constexpr int kStateOff = NS * 2 * TB;
-  constexpr int kJoinOff = kStateOff + (MODE == 1 ? NW * 256 : 0);  // (KP = 2: the waves' maxima and sums)
+  constexpr int kJoinOff = kStateOff + (MODE == 1 ? NW * 256 : WIN ? NW * 128 : 0);  // (KP = 2: the waves' maxima and sums)
   __shared__ __attribute__((aligned(1024))) char lds[kJoinOff + (KP > 1 ? NW * 256 : 0)];
   auto swz_k = [](int row) { return (row / RPB) & (CPR - 1); };
   auto swz_v = [](int row) { return ((row / RPB) & (CPR / 2 - 1)) << 1; };
@@ -194,6 +200,15 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
     const int n = dq >= 0 ? (int)div_by((uint32_t)dq, p.d_peers) + 1 : 0;
     return n > kv_len ? kv_len : n;
   };
+  // (WIN) keys at positions up to x - window; keys that are sinks
+  auto keys_before = [&](int x) -> int {
+    const int64_t d = (int64_t)x - p.window - kf;
+    const int n = d >= 0 ? (int)div_by((uint32_t)d, p.d_peers) + 1 : 0;
+    return n > kv_len ? kv_len : n;
+  };
+  int n_sinks = 0;
+  if (WIN) n_sinks = p.sinks > kf ? (int)div_by((uint32_t)(p.sinks - 1 - kf), p.d_peers) + 1 : 0;
+  if (WIN) n_sinks = __builtin_amdgcn_readfirstlane(n_sinks < kv_len ? n_sinks : kv_len);
   const int lds_base = (int)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
   // The old m and l (MODE 1) are asked for first of all and go straight into LDS: no register is held over the loop, and the epilogue need
   // not go to memory to learn whether a row is still in its start state, whose old o is never read.
@@ -213,6 +228,7 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
   for (int qb = 0; qb < QB; qb++) {
     const int m = m0 + 16 * qb + c;
     cnt[qb] = (m < q_len ? visible_keys(qf + m * P) : 0) - 4 * g;
+    if (WIN && g == 0) *(int*)(lds + kStateOff + wave * 128 + (16 * qb + c) * 4) = keys_before(qf + m * P);
     const char* src = (const char*)p.q + ((q_start + (m < q_len ? m : m_wg)) * p.q_st + (int64_t)h * p.q_sh) * 2;
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) {
@@ -234,6 +250,12 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
   // which nothing reads; its first row sees the fewest keys of the others)
   const int cnt_first = __builtin_amdgcn_readfirstlane(m0 < q_len ? visible_keys(qf + m0 * P) : 0);
   const int cnt_wg = __builtin_amdgcn_readfirstlane(last_seen(m_wg, rows_wg));
+  // (WIN) keys in front of every window of the wave, and in front of the window of its last position
+  int lo_wave = 0, lo_last = 0;
+  if (WIN && m0 < q_len) {
+    lo_wave = __builtin_amdgcn_readfirstlane(keys_before(qf + m0 * P));
+    lo_last = __builtin_amdgcn_readfirstlane(keys_before(qf + (m0 + WP - 1 < q_len ? m0 + WP - 1 : q_len - 1) * P));
+  }
 
   const char* kbase = (const char*)p.k + (kv_start * p.k_st + (int64_t)kvh * p.k_sh) * 2;
   const char* vbase = (const char*)p.v + (kv_start * p.v_st + (int64_t)kvh * p.v_sh) * 2;
@@ -247,9 +269,20 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
   constexpr bool APART = !DV && NS > 2;  // K tiles are requested NS - 1 tiles ahead, V tiles that pass through registers one
   u32x4 vst[NI];
   // K and V of tile t (or one of them)
-  auto request = [&](auto k_tag, auto v_tag, int stage, int t) __attribute__((always_inline)) {
+  // (WIN) the tiles walked: those of the sinks, and from the one on that the window of the workgroup's first position starts in
+  int sink_tiles = 0, tile_skip = 0;
+  if (WIN) {
+    const int first = __builtin_amdgcn_readfirstlane(keys_before(qf + m_wg * P)) / TK;
+    const int seen_sinks = n_sinks < cnt_wg ? n_sinks : cnt_wg;
+    sink_tiles = (seen_sinks + TK - 1) / TK;
+    sink_tiles = sink_tiles < first ? sink_tiles : first;
+    tile_skip = first - sink_tiles;
+  }
+  auto tile_at = [&](int t) __attribute__((always_inline)) { return WIN && t >= sink_tiles ? t + tile_skip : t; };
+  auto request = [&](auto k_tag, auto v_tag, int stage, int walked) __attribute__((always_inline)) {
     constexpr bool K = decltype(k_tag)::value, V = decltype(v_tag)::value;
     if (!stager) return;
+    const int t = tile_at(walked);
     const char* kt = K ? uniform_ptr(kbase + (int64_t)t * TK * k_row) : nullptr;
     const char* vt = V ? uniform_ptr(vbase + (int64_t)t * TK * v_row) : nullptr;
     const int dst = __builtin_amdgcn_readfirstlane(lds_base + stage * 2 * TB + wave * 1024);
@@ -307,7 +340,7 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
     return a;
   };
   const float scale = p.scale_log2;
-  const int nt = (cnt_wg + TK - 1) / TK;  // the same for every wave of the workgroup
+  const int nt = (cnt_wg + TK - 1) / TK - tile_skip;  // the same for every wave of the workgroup
 
   constexpr int VR = LEAN ? 4 : NDB;       // V operands
   u32x4 ka[2][KS];  // K operands of the next 32 keys
@@ -337,11 +370,13 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
       if (t + NS - 1 < nt) request(yes, yes, (S + NS - 1) % NS, t + NS - 1);
     }
     const int k_wave = 32 * kp, b_wave = k_wave * RB;  // (KP = 2) the wave's first key of the tile
-    if (t * TK + k_wave < cnt_wave) load_ka(S * 2 * TB + b_wave);
+    const int tk = tile_at(t) * TK;
+    const bool in_windows = !WIN || tk + TK > lo_wave || tk < n_sinks;
+    if (tk + k_wave < cnt_wave && in_windows) load_ka(S * 2 * TB + b_wave);
 #pragma unroll
     for (int part = 0; part < TK / 32 / KP; part++) {
-      const int k0 = t * TK + k_wave + 32 * part;
-      if (k0 < cnt_wave) {  // (wave-uniform: else none of the wave's rows sees these keys)
+      const int k0 = tk + k_wave + 32 * part;
+      if (k0 < cnt_wave && in_windows) {  // (wave-uniform: else none of the wave's rows sees these keys)
         // S^T = K Q^T: s[qb][kb][j] = score of key k0 + 16 kb + 4 g + j for the lane's query of block qb; a K operand serves all blocks
         // (starting from named zeros: with the zero written into the first product the 128-wide kernel spills 22 registers)
         f32x4 s[QB][2];
@@ -353,7 +388,21 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
           for (int kb = 0; kb < 2; kb++)
 #pragma unroll
             for (int qb = 0; qb < QB; qb++) s[qb][kb] = MfmaS<T>::run(ka[kb][ks], qreg[qb][ks], s[qb][kb]);
-        if (k0 + 32 > cnt_first) {  // (wave-uniform: the wave's first row, which sees the fewest keys, does not see the whole step)
+        if (WIN && (k0 + 32 > cnt_first || k0 < lo_last)) {
+          const int lane_m = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+#pragma unroll
+          for (int qb = 0; qb < QB; qb++) {
+            const int first = k0 + 4 * (lane_m >> 4);
+            const int rel = cnt[qb] - k0, rel_sinks = n_sinks - first;
+            const int rel_lo = *(const int*)(lds + kStateOff + wave * 128 + (16 * qb + (lane_m & 15)) * 4) - first;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+              const int n = 16 * (e / 4) + e % 4;
+              s[qb][e / 4][e % 4] = n < rel && (n >= rel_lo || n < rel_sinks) ? s[qb][e / 4][e % 4] : -INFINITY;
+            }
+          }
+        }
+        if (!WIN && k0 + 32 > cnt_first) {  // (wave-uniform: the wave's first row, which sees the fewest keys, does not see the whole step)
 #pragma unroll
           for (int qb = 0; qb < QB; qb++) {
             const int rel = cnt[qb] - k0;
@@ -447,7 +496,7 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
   // each, a request per row to the L2s, and turned round whole lines of a few rows: 16 x 1024 tokens 32/8 199 -> 190 us in
   // place and 207 -> 201 as fp32, 16 x 512 bf16 72 -> 66 (128-wide heads).  The small launches of 16 positions write directly (turned round, 1 x 100 took 0.4 us more).
   constexpr bool TURNED = MODE != 2 && WP == 32;
-  constexpr int ES = MODE == 1 ? 2 : 4;                // bytes per element of O
+  constexpr int ES = MODE == 1 || MODE == 3 ? 2 : 4;   // bytes per element of O
   constexpr int RBO = D * ES < 256 ? D * ES : 256;     // bytes of a row that are turned round at a time
   constexpr int CO = RBO / 16;                         // 16-byte chunks of them, XORed with a function of the row as the tiles' are
   static_assert(!TURNED || kWaves * WP * RBO <= kStateOff, "the tiles' LDS holds the waves' rows");
@@ -513,8 +562,20 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void pref
 #pragma unroll
           for (int db = 0; db < EDB; db++) *(f32x4*)(orow + 16 * db) = oacc[qb][db] * factor[qb];
         }
-        if (g_e == 0 && kp == 0) p.lse[tok * p.hq + h] = seen ? (m_run[qb] + __builtin_amdgcn_logf(l_tot)) * kLn2 : -INFINITY;
+        if (g_e == 0 && kp == 0 && (!WIN || p.lse)) p.lse[tok * p.hq + h] = seen ? (m_run[qb] + __builtin_amdgcn_logf(l_tot)) * kLn2 : -INFINITY;
       }
+    }
+    if (MODE == 3) {
+      const float f = seen ? fix * (1.f / l_tot) : 0.f;
+      uint16_t* orow = (uint16_t*)p.o + tok * p.o_st + (int64_t)h * p.o_sh + 4 * g_e;
+#pragma unroll
+      for (int db = 0; db < NDB; db++) {
+        const f32x4 x = oacc[qb][db] * f;
+        const u32x2 res = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+        if (TURNED) *(u32x2*)(o_lds + o_chunk(16 * qb + c_e, 2 * db + (g_e >> 1)) + (g_e & 1) * 8) = res;
+        else if (here) *(u32x2*)(orow + 16 * db) = res;
+      }
+      if (here && g_e == 0 && p.lse) p.lse[tok * p.hq + h] = seen ? (m_run[qb] + __builtin_amdgcn_logf(l_tot)) * kLn2 : -INFINITY;
     }
     if (MODE == 1) {
       // the reference's update of (o, m, l); a row in its start state (m = -inf, l = 0) may hold anything in o
@@ -689,7 +750,7 @@ Order order_of(const lsattn_prefill_args* a, int pack_shift) {
   return {bunch, requests_take_turns(a, ids * bunch, tiles)};
 }
 
-template <typename T, int D, int MODE, bool DV, int WP, int KP = 1> int launch_rows(SmallParams p, const lsattn_prefill_args* a, hipStream_t st) {
+template <typename T, int D, int MODE, bool DV, int WP, int KP = 1, bool WIN = false> int launch_rows(SmallParams p, const lsattn_prefill_args* a, hipStream_t st) {
   const int64_t rows_wg = (kWaves * WP) >> p.pack_shift;
   const Order order = WP == 32 ? order_of(a, p.pack_shift) : Order{p.batch, false};
   p.bunch = (int32_t)order.bunch;
@@ -699,7 +760,7 @@ template <typename T, int D, int MODE, bool DV, int WP, int KP = 1> int launch_r
   const unsigned bunches = (unsigned)((a->batch + p.bunch - 1) / p.bunch);
   for (int64_t tiles = (a->max_q_len + rows_wg - 1) / rows_wg; tiles > 0; tiles -= most) {
     p.last_tile = (int32_t)(tiles - 1);
-    LSATTN_LAUNCH_KERNEL((prefill_small_kernel<T, D, MODE, DV, WP, KP>),
+    LSATTN_LAUNCH_KERNEL((prefill_small_kernel<T, D, MODE, DV, WP, KP, WIN>),
                          dim3((unsigned)(p.hkv * p.group), (unsigned)((tiles < most ? tiles : most) * p.bunch), bunches), dim3(kWaves * KP * 64), 0, st, p);
     const int rc = check_launch();
     if (rc != LSATTN_OK) return rc;
@@ -855,9 +916,10 @@ int prefill_small_route(const lsattn_prefill_args* a) {
   return order_of(a, pack).turns ? LSATTN_ROUTE_SMALL_TURNS : LSATTN_ROUTE_SMALL_32;
 }
 
-// One prefill step with head_dim 16, 32 or 64, or a short one with 128 (arguments already validated; epilogue `mode` as in the 128-wide kernel).
-int launch_prefill_small(const lsattn_prefill_args* a, int mode, hipStream_t st) {
-  SmallParams p;
+namespace {
+
+SmallParams params_of(const lsattn_prefill_args* a) {
+  SmallParams p = {};
   p.q = a->q;
   p.k = a->k;
   p.v = a->v;
@@ -892,6 +954,40 @@ int launch_prefill_small(const lsattn_prefill_args* a, int mode, hipStream_t st)
   p.l = a->l;
   p.ml_st = a->ml_stride_t;
   p.ml_sh = a->ml_stride_h;
+  return p;
+}
+
+// A step behind a window: 32 positions per wave, or 16 where those make fewer than three workgroups per CU.
+template <typename T, int D, int MODE, bool DV> int launch_window_rows(const SmallParams& p, const lsattn_prefill_args* a, hipStream_t st) {
+  if (workgroups(a, p.pack_shift, 2) < 3 * kCUs) return launch_rows<T, D, MODE, DV, 16, 1, true>(p, a, st);
+  return launch_rows<T, D, MODE, DV, 32, 1, true>(p, a, st);
+}
+template <typename T, int MODE, bool DV> int launch_window_d(const SmallParams& p, const lsattn_prefill_args* a, hipStream_t st) {
+  switch (a->head_dim) {
+    case 16: return launch_window_rows<T, 16, MODE, DV>(p, a, st);
+    case 32: return launch_window_rows<T, 32, MODE, DV>(p, a, st);
+    case 64: return launch_window_rows<T, 64, MODE, DV>(p, a, st);
+    default: return launch_window_rows<T, 128, MODE, DV>(p, a, st);
+  }
+}
+template <typename T, bool DV> int launch_window(const SmallParams& p, const lsattn_prefill_args* a, hipStream_t st) {
+  return a->o_dtype == LSATTN_F32 ? launch_window_d<T, 0, DV>(p, a, st) : launch_window_d<T, 3, DV>(p, a, st);
+}
+
+}  // namespace
+
+// A step behind a window (arguments already validated; o_dtype F32 or that of q).
+int launch_prefill_window(const lsattn_prefill_args* a, int32_t window, int32_t sinks, hipStream_t st) {
+  if (a->num_q_heads > 65535 || a->batch > 65535) return LSATTN_ERR_INVALID_ARG;
+  SmallParams p = params_of(a);
+  p.window = window, p.sinks = sinks;
+  if (a->dtype == LSATTN_F16) return launch_window<F16, true>(p, a, st);
+  return a->v_is_f16 ? launch_window<BF16, true>(p, a, st) : launch_window<BF16, false>(p, a, st);
+}
+
+// One prefill step with head_dim 16, 32 or 64, or a short one with 128 (arguments already validated; epilogue `mode` as in the 128-wide kernel).
+int launch_prefill_small(const lsattn_prefill_args* a, int mode, hipStream_t st) {
+  const SmallParams p = params_of(a);
   if (a->dtype == LSATTN_F16) return launch_mode<F16, true>(p, a, mode, st);
   return a->v_is_f16 ? launch_mode<BF16, true>(p, a, mode, st) : launch_mode<BF16, false>(p, a, mode, st);
 }

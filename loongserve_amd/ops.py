@@ -447,6 +447,45 @@ def _prefill_attention_step_checked(q, k, v, q_b_start_loc, q_b_seq_len, q_first
     return out, lse
 
 
+def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx,
+                         kv_b_start_loc, kv_b_seq_len, kv_first_token_global_idx,
+                         logical_sp_peers_num: int, max_q_b_seq_len: int, window: int, sinks: int = 0,
+                         lse: Optional[torch.Tensor] = None, total_q_len: Optional[int] = None) -> None:
+    """A prefill step behind a sliding window with sinks, into o and lse; inputs as context_attention_fwd's.  A query sees the
+    keys at positions up to its own that are less than `window` back (its own among them) or among the first `sinks`, in
+    the global positions that the first-token vectors and logical_sp_peers_num give; the time goes by the keys that are
+    seen.  No reference counterpart.
+
+    o has q's type, or is float32 (a partial: with lse, the steps over several KV chunks join by lse_merge); lse, the natural
+    log-sum-exp, float32 [tokens, q_heads], is optional.  Rows that see no key get o = 0, lse = -inf; rows that no
+    request names stay as they were.  A chunk of a longer prompt brings its context in k and v (kv_gather_fp8 reads one back
+    from an 8-bit pool) and the position of its first query in q_first_token_global_idx.  total_q_len: as in
+    context_attention_fwd.  A bfloat16 v is multiplied as float16: magnitudes past 65504 count as 65504.  V rows of keys near
+    a window that a query does not see are multiplied by a weight of zero: they have to be finite (K rows may hold anything)."""
+    if window is not None and _native.window_attention(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx, kv_b_start_loc, kv_b_seq_len,
+                                                       kv_first_token_global_idx, logical_sp_peers_num, max_q_b_seq_len, window, sinks, lse,
+                                                       0 if total_q_len is None else total_q_len):
+        return
+    for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")):
+        _dev(t, n)
+    _on_current_device(((q, "q"), (k, "k"), (v, "v"), (o, "o"), (q_b_start_loc, "q_b_start_loc"), (q_b_seq_len, "q_b_seq_len"), (lse, "lse")))
+    if window is None or int(window) < 1 or int(sinks) < 0:
+        raise ValueError("window must be >= 1 (the position itself), sinks >= 0")
+    if int(logical_sp_peers_num) < 1 or int(max_q_b_seq_len) < 0:
+        raise ValueError("logical_sp_peers_num must be >= 1 and max_q_b_seq_len >= 0")
+    if o.dtype not in (q.dtype, torch.float32):
+        raise ValueError("o must have the dtype of q, or be float32")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != tuple(q.shape[:2]) or not lse.is_contiguous()):
+        raise ValueError("lse must be a contiguous float32 [tokens, q_heads] tensor")
+    _prefill_args(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx, kv_b_start_loc, kv_b_seq_len, kv_first_token_global_idx,
+                  logical_sp_peers_num, max_q_b_seq_len, None, total_q_len=total_q_len, state=None)
+    if q.numel() == 0:
+        return
+    if k.numel() == 0:  # no keys at all: every row that a request names sees none
+        raise ValueError("k and v hold no rows")
+    raise ValueError("window_attention_fwd: arguments that no kernel takes")
+
+
 @torch.inference_mode()
 def lse_merge(parts: Sequence[Tuple[torch.Tensor, torch.Tensor]], out: Optional[torch.Tensor] = None,
               lse: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.float32):
