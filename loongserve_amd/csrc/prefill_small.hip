@@ -145,7 +145,7 @@ template <int D, int WP, bool DV> constexpr int kResident = D == 128 ? (WP == 32
 // workgroup walks the tiles that hold sinks, then those from its first row's window on; MODE 0, or MODE 3: O in T's type and the LSE,
 // from the empty state.
 template <typename T, int D, int MODE, bool DV, int WP, int KP = 1, bool WIN = false>
-__global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV>)) void prefill_small_kernel(SmallParams p) {
+__global__ __launch_bounds__(kWaves * KP * 64, (WIN && D == 128 && WP == 32 ? 2 : kResident<D, WP, DV>)) void prefill_small_kernel(SmallParams p) {
   static_assert(WIN ? KP == 1 && (MODE == 0 || MODE == 3) : MODE < 3, "a window knows no state");
   static_assert(KP == 1 || (KP == 2 && WP == 16 && D >= 32), "the parts of a tile of 64 keys, the columns that each of two waves finishes");
   constexpr int NW = kWaves * KP;
