@@ -173,6 +173,9 @@ int lsattn_prefill_step_accumulate(const lsattn_prefill_args* a, void* stream);
  * over several KV chunks (o in fp32) join by lsattn_lse_merge.  kv_cuts is not taken.  A bfloat16 V is multiplied as fp16 (v_is_f16, or
  * converted in the kernel): magnitudes past 65504 count as 65504, below 2^-14 they are kept to 2^-24. */
 int lsattn_prefill_window(const lsattn_prefill_args* a, int64_t window, int64_t sinks, void* stream);
+/* 1 if that step (v_is_f16 = 0) converts a bfloat16 V on its way at no cost; 0 if the caller should make an fp16 copy of V first, without which the
+ * step runs in a slower shape.  Looks at the numbers in the block alone. */
+int lsattn_prefill_window_converts_v(const lsattn_prefill_args* a, int64_t window);
 
 /*
  * Merge n normalised partials (O_i fp32 [rows,D] contiguous, LSE_i [rows]) over disjoint key
@@ -696,7 +699,7 @@ const char* lsattn_strerror(int code);
  * lsattn_prefill_converts_v; 6 = max_kv_len there (a reserved word before), lsattn_prefill_route,
  * lsattn_prefill_cut_count; 7 = o_is_apart in lsattn_decode_stage2_args (a reserved word before); 8 = o_is_apart of 2;
  * 9 = lead_rows in lsattn_decode_stage2_args; 10 = lsattn_kv_scatter_fp8, lsattn_kv_gather_fp8, lsattn_pool_attention,
- * lsattn_prefill_window. */
+ * lsattn_prefill_window, lsattn_prefill_window_converts_v. */
 #define LSATTN_VERSION 10
 int lsattn_version(void);
 

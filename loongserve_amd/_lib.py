@@ -165,6 +165,7 @@ EXPORTS = {
     "lsattn_prefill_step_merge": (C.c_int, [C.POINTER(PrefillArgs), _vp]),
     "lsattn_prefill_step_accumulate": (C.c_int, [C.POINTER(PrefillArgs), _vp]),
     "lsattn_prefill_window": (C.c_int, [C.POINTER(PrefillArgs), _i64, _i64, _vp]),
+    "lsattn_prefill_window_converts_v": (C.c_int, [C.POINTER(PrefillArgs), _i64]),
     "lsattn_lse_merge": (C.c_int, [C.POINTER(MergeArgs), _vp]),
     "lsattn_prefill_merge_cuts": (C.c_int, [C.POINTER(MergeCutsArgs), _vp]),
     "lsattn_decode_stage1": (C.c_int, [C.POINTER(DecodeStage1Args), _vp]),

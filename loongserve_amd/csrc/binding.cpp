@@ -31,6 +31,7 @@ struct Library {
   decltype(&lsattn_prefill_step_merge) prefill_step_merge;
   decltype(&lsattn_prefill_step_accumulate) prefill_step_accumulate;
   decltype(&lsattn_prefill_window) prefill_window;
+  decltype(&lsattn_prefill_window_converts_v) prefill_window_converts_v;
   decltype(&lsattn_prefill_merge_cuts) prefill_merge_cuts;
   decltype(&lsattn_prefill_converts_v) prefill_converts_v;
   decltype(&lsattn_bf16_to_f16_rows) bf16_to_f16_rows;
@@ -60,6 +61,7 @@ PyObject* bind(PyObject*, PyObject* addresses) {
       {"lsattn_prefill_step_merge", (void**)&lib.prefill_step_merge},
       {"lsattn_prefill_step_accumulate", (void**)&lib.prefill_step_accumulate},
       {"lsattn_prefill_window", (void**)&lib.prefill_window},
+      {"lsattn_prefill_window_converts_v", (void**)&lib.prefill_window_converts_v},
       {"lsattn_prefill_merge_cuts", (void**)&lib.prefill_merge_cuts},
       {"lsattn_prefill_converts_v", (void**)&lib.prefill_converts_v},
       {"lsattn_bf16_to_f16_rows", (void**)&lib.bf16_to_f16_rows},
@@ -551,10 +553,10 @@ bool exponents(const at::Tensor& s, const at::Tensor& pool) {
 }
 bool e4m3_rows(const at::Tensor& t) { return is(t, at::kFloat8_e4m3fn) && t.stride(2) == 1; }
 
-// (q, k, v, o, six vectors, peers, max_q, window, sinks, lse or None, total_q) -> True or None
+// (q, k, v, o, six vectors, peers, max_q, window, sinks, lse or None, total_q, preconvert) -> True or None
 PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  NEED_ARGS(16);
+  NEED_ARGS(17);
   Args in(args);
   const at::Tensor &q = in.gpu(3), &k = in.gpu(3), &v = in.gpu(3), &o = in.gpu(3);
   OR_NONE(in.ok);
@@ -563,11 +565,16 @@ PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const int64_t window = in.integer(), sinks = in.integer();
   const at::Tensor* lse = in.maybe();
   s.p.total_q_rows = in.integer();
+  const bool preconvert = in.integer() != 0;
   OR_NONE(in.ok && here({&q, &k, &v, &o, s.q_start, s.q_len, lse}) && window >= 1 && sinks >= 0 && s.p.total_q_rows >= 0 && s.p.sp_peers >= 1 && s.p.max_q_len >= 0);
   if (lse) OR_NONE(is(*lse, at::kFloat) && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == q.size(0) && lse->size(1) == q.size(1));
   OR_NONE(q.numel() > 0 && k.numel() > 0);
   s.p.lse = lse ? (float*)lse->data_ptr() : nullptr;
-  if (const int rc = call(lib.prefill_window, &s.p, window, sinks, stream())) return failed(rc, "lsattn_prefill_window");
+  void* st = stream();
+  // (a bfloat16 V whose heads lie side by side is rewritten as fp16 in front of a launch that does not convert it itself)
+  if (preconvert && s.p.dtype == LSATTN_BF16 && v.stride(1) == v.size(2) && !lib.prefill_window_converts_v(&s.p, window))
+    if (const int rc = s.convert(st)) return failed(rc, "lsattn_bf16_to_f16_rows");
+  if (const int rc = call(lib.prefill_window, &s.p, window, sinks, st)) return failed(rc, "lsattn_prefill_window");
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }

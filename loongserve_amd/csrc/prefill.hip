@@ -73,6 +73,7 @@ struct PrefillParams {
   int32_t dense, head_bits;  // (cut launches) the grid numbers the units without gaps; log2 of the KV heads
   int32_t spread;    // (cut launches with gaps) how many XCDs further the units of the next (sequence, cut) start
   int32_t cut_mask;  // 0: the cuts of a sequence share its own length, at most kv_cut_len keys each; else all bits: kv_cut_len keys
+  int32_t window, sinks;  // (WIN) positions that a query sees up to its own, first positions that every later one sees
 };
 
 constexpr int BM = 256;   // query rows per workgroup (32 per wave)
@@ -231,17 +232,22 @@ __device__ __forceinline__ void store16_through(float* addr, const f32x4 v) {
   asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1\n\ts_nop 1" : : "v"(addr), "v"(v) : "memory");
 }
 
-template <typename T, int MODE, bool DV, bool SPLIT, bool HALF, bool CUTS>
+// WIN: a step behind a sliding window with sinks (the query at position x sees keys at positions y <= x with y > x - window or y < sinks): the workgroup walks the
+// tiles that hold sinks and those from its first row's window on; masked iterations over the sinks and the windows' starts come in front of the plain ones.  MODE 0, or
+// MODE 3: O in T's type and the LSE, from the empty state.
+template <typename T, int MODE, bool DV, bool SPLIT, bool HALF, bool CUTS, bool WIN = false>
 __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void prefill_kernel(PrefillParams p) {
   static_assert(DV || !SPLIT, "the split variant takes fp16 V tiles only");
   static_assert(!HALF || (DV && !SPLIT), "the four-wave variant takes fp16 V tiles only and is not split");
+  static_assert(WIN ? DV && !SPLIT && !HALF && !CUTS && (MODE == 0 || MODE == 3) : MODE < 3, "a window knows the 256-row shape and no state");
   // (namespace-scope constants: a local one named inside the lambdas below would be captured, and a closure that holds
   // anything but references the optimiser can see through is kept in memory, with every scalar operand it feeds)
   constexpr int RING = kRingOf<HALF>;            // tiles per ring
   constexpr int LDSV = kLdsVOf<HALF>;            // the V ring behind the K ring
-  // (behind the rings, for the epilogue that folds into (o, m, l): a kilobyte per wave for the old m and l of its rows)
+  // (behind the rings, for the epilogue that folds into (o, m, l): a kilobyte per wave for the old m and l of its rows; WIN: 256 bytes per wave for the
+  // keys that its rows see up to their position and those in front of their windows, which only masked iterations read)
   constexpr int kStateOff = 2 * RING * kTileBytes;
-  __shared__ __attribute__((aligned(1024))) char lds[kStateOff + (MODE == 1 ? (HALF ? NWAVE / 2 : NWAVE) * 1024 : 0)];
+  __shared__ __attribute__((aligned(1024))) char lds[kStateOff + (MODE == 1 ? (HALF ? NWAVE / 2 : NWAVE) * 1024 : WIN ? NWAVE * 256 : 0)];
   constexpr int BMW = SPLIT || HALF ? BM / 2 : BM;  // query rows of this workgroup
 
   // Workgroup ids go to the 8 XCDs round-robin.  The (query head, query tile) units of one KV head are dealt to p.slices
@@ -377,7 +383,24 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
     return n > kv_len ? kv_len : n;
   };
   const int m_hi = (m_lo + rows_wg < q_len ? m_lo + rows_wg : q_len) - 1;
-  const int nt = (visible_keys(qf + m_hi * P) + BN - 1) / BN;  // tiles the workgroup walks
+  // (WIN) keys at positions up to x - window; keys that are sinks
+  auto keys_before = [&](int x) -> int {
+    const int64_t d = (int64_t)x - p.window - kf;
+    const int n = (int)div_by((uint32_t)(d > -1 ? d : -1) + (uint32_t)P, p.d_peers);  // (0 for -1: less than a step)
+    return n > kv_len ? kv_len : n;
+  };
+  // (WIN) the tiles walked: those of the sinks, and from the one on that the window of the workgroup's first row starts in
+  int n_sinks = 0, sink_tiles = 0, tile_skip = 0;
+  if constexpr (WIN) {
+    n_sinks = p.sinks > kf ? (int)div_by((uint32_t)(p.sinks - 1 - kf), p.d_peers) + 1 : 0;
+    n_sinks = __builtin_amdgcn_readfirstlane(n_sinks < kv_len ? n_sinks : kv_len);
+    const int seen = visible_keys(qf + m_hi * P), first = keys_before(qf + m_lo * P) / BN;
+    sink_tiles = ((n_sinks < seen ? n_sinks : seen) + BN - 1) / BN;
+    sink_tiles = __builtin_amdgcn_readfirstlane(sink_tiles < first ? sink_tiles : first);
+    tile_skip = __builtin_amdgcn_readfirstlane(first - sink_tiles);
+  }
+  auto tile_at = [&](int t) __attribute__((always_inline)) { return t >= sink_tiles ? t + tile_skip : t; };
+  const int nt = (visible_keys(qf + m_hi * P) + BN - 1) / BN - tile_skip;  // tiles the workgroup walks
 
   const int m_w0 = m_lo + (wrow & ((1 << wph_shift) - 1)) * 32;
 
@@ -412,11 +435,19 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
     // stands between the loads and the tile loads that follow)
     for (int ks = 0; ks < 4; ks++) qreg[qb][ks] = *(const u32x4*)(src + ks * 64);
     cnt[qb] = ok ? visible_keys(qf + m * P) : 0;
+    if constexpr (WIN)
+      if (g == 0) {
+        *(int*)(lds + kStateOff + wave * 256 + (16 * qb + qc) * 4) = cnt[qb];
+        *(int*)(lds + kStateOff + wave * 256 + 128 + (16 * qb + qc) * 4) = keys_before(qf + m * P);
+      }
   }
 
   // keys every row of the wave sees: sub-tiles below this need no mask (rows past the end of the sequence count as rows
   // that see nothing, so a wave that holds some masks everywhere)
   const int cnt_wave = __builtin_amdgcn_readfirstlane(m_w0 + 31 < q_len ? visible_keys(qf + m_w0 * P) : 0);
+  // (WIN) keys in front of the window of the wave's last row: sub-tiles from there on need no mask for it
+  int lo_wave = 0;
+  if constexpr (WIN) lo_wave = __builtin_amdgcn_readfirstlane(keys_before(qf + (m_w0 + 31) * P));
   int koff0 = qc * 256 + ((g ^ swz_k(qc)) << 4);
   int voff0;
   {
@@ -460,7 +491,9 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
   const int last_tile = last_row / BN;
   auto clamped_tile = [&](const char* base, int row_bytes, uint32_t lane_off, int i, int t, const char*& tile, uint32_t& off)
                           __attribute__((always_inline)) {
-    const int tc = __builtin_amdgcn_readfirstlane(t < last_tile ? t : last_tile);
+    int tw = t;
+    if constexpr (WIN) tw = tile_at(t);
+    const int tc = __builtin_amdgcn_readfirstlane(tw < last_tile ? tw : last_tile);
     tile = base + (int64_t)tc * BN * row_bytes;
     // rows of the tile between the lane's row, st_row + 4 i, and the last one of the chunk (the scalar part on its own,
     // so that no further per-lane values are kept across the loop)
@@ -664,7 +697,24 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
       nm[qb] = neg_m[qb];
       if (MASKED) nm[qb] = neg_m[qb] == INFINITY ? 0.f : neg_m[qb];
     }
-    if (MASKED && (i + 1) * SUB > cnt_wave) {  // (wave-uniform: the wave's first row sees the fewest keys)
+    if constexpr (WIN) {
+      if (MASKED && ((i + 1) * SUB > cnt_wave || i * SUB < lo_wave)) {
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++) {
+          int at = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+          asm volatile("" : "+v"(at));  // (worked out here, one row block after the other: no register is held over the loop for it)
+          const int first = i * SUB + ((at >> 4) << 2);
+          const char* const limits = lds + kStateOff + wave * 256 + qb * 64 + (at & 15) * 4;
+          const int rel = *(const int*)limits - first, rel_lo = *(const int*)(limits + 128) - first, rel_sinks = n_sinks - first;
+#pragma unroll
+          for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+              s[kb][qb][r] = (16 * kb + r < rel && (16 * kb + r >= rel_lo || 16 * kb + r < rel_sinks)) ? s[kb][qb][r] : -INFINITY;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    } else if (MASKED && (i + 1) * SUB > cnt_wave) {  // (wave-uniform: the wave's first row sees the fewest keys)
 #pragma unroll
       for (int qb = 0; qb < 2; qb++) {
         const int rel = cnt[qb] - i * SUB - 4 * g;  // keys from the lane's first one of key block 0 to the row's limit
@@ -772,7 +822,15 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
   // tiles they load lie inside the chunk and that every row of the workgroup sees every key of the tile.
   auto request_tiles = [&](auto r_tag, auto masked_tag, int it) __attribute__((always_inline)) {
     constexpr int R = decltype(r_tag)::value;
-    if constexpr (decltype(masked_tag)::value) {
+    // (conditions that do not hang on the tags stand alone: under one that does, the lambda would hold what their branch names)
+    if constexpr (WIN) {
+      if constexpr (decltype(masked_tag)::value) {  // (the running pointers are set where the plain iterations start)
+        load_k_clamped(std::integral_constant<int, (R + KA) & 3>{}, it + KA);
+        load_v_clamped(std::integral_constant<int, (R + VA) & 3>{}, it + VA);
+      } else {
+        load_tiles_fast(r_tag);
+      }
+    } else if constexpr (decltype(masked_tag)::value) {
       // (tiles that lie inside the chunk take the cheaper loads here too; the running pointers advance either way)
       if (it + KA < kv_len / BN) {
         load_tiles_fast(r_tag);
@@ -840,15 +898,17 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
       wait_vmem<4>();
       __builtin_amdgcn_s_barrier();
     } else {
+      int tile = it;
+      if constexpr (WIN) tile = tile_at(it);
       fphase_mfma(std::integral_constant<int, 0>{}, r_tag, std::integral_constant<bool, !MASKED>{});
       __builtin_amdgcn_s_barrier();
       request_tiles(r_tag, masked_tag, it);
-      fphase_softmax(masked_tag, 2 * it);
+      fphase_softmax(masked_tag, 2 * tile);
       __builtin_amdgcn_s_barrier();
       if (DV) wait_vmem<4>();
       fphase_mfma(std::integral_constant<int, 1>{}, r_tag, std::integral_constant<bool, !MASKED>{});
       __builtin_amdgcn_s_barrier();
-      fphase_softmax(masked_tag, 2 * it + 1);
+      fphase_softmax(masked_tag, 2 * tile + 1);
       if (!DV) {
         // everything but this iteration's two K loads has arrived: the registers hold V tile it+2, and K tile it+2
         // (loaded one iteration ago) is complete as well
@@ -888,6 +948,7 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
     // are worked on lie inside the chunk; the loop over them is unrolled over the four ring slots.
     int n_plain = visible_keys(qf + m_lo * P) / BN;
     if (n_plain > kv_len / BN - KA) n_plain = kv_len / BN - KA;
+    const int n_plain_tiles = n_plain;
     if (n_plain > nt) n_plain = nt;
     n_plain = n_plain < 0 ? 0 : (n_plain & ~(kRingOf<HALF> - 1));  // (the loop is unrolled over the ring)
     const int par_off = kp * (SUB * 256);
@@ -913,6 +974,31 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
     vt_run = uniform_ptr(vg + (int64_t)(DV ? VA : 3) * BN * v_row_bytes);
     int it = 0;
     if (wave >= 4) __builtin_amdgcn_s_barrier();
+    if constexpr (WIN) {
+      // Masked iterations up to n_head (sinks, and tiles that lie in front of some row's window), plain ones up to n_plain, masked ones over the
+      // rest.  The rows' sums, which the masked ones keep in l_run lane by lane, go over to the matrix pipe's; the first plain product adds the P of the last
+      // masked step, which is taken out of them beforehand.
+      int n_head = (keys_before(qf + m_hi * P) + BN - 1) / BN - tile_skip;
+      n_head = ((n_head > sink_tiles ? n_head : sink_tiles) + 3) & ~3;
+      const int n_seen = n_plain_tiles - tile_skip;
+      n_plain = n_head + ((n_seen > n_head ? n_seen - n_head : 0) & ~3);
+      for (; it < n_head && it < nt; it += 4) {
+        iteration(std::integral_constant<int, 0>{}, std::true_type{}, it);
+        if (it + 1 < nt) iteration(std::integral_constant<int, 1>{}, std::true_type{}, it + 1);
+        if (it + 2 < nt) iteration(std::integral_constant<int, 2>{}, std::true_type{}, it + 2);
+        if (it + 3 < nt) iteration(std::integral_constant<int, 3>{}, std::true_type{}, it + 3);
+      }
+#pragma unroll
+      for (int qb = 0; qb < 2; qb++) {
+        const float pair = l_run[qb] + lane_xor16(l_run[qb]);
+        const unsigned u = __builtin_bit_cast(unsigned, pair);
+        const auto halves = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const float sum = __builtin_bit_cast(float, (unsigned)halves[0]) + __builtin_bit_cast(float, (unsigned)halves[1]);
+        lacc[qb] = sum - Mfma<F16>::run(ones, pk[qb], f32x4{0.f, 0.f, 0.f, 0.f});
+      }
+      kt_run = uniform_ptr(kg + (int64_t)tile_at(it + KA) * BN * k_row_bytes);
+      vt_run = uniform_ptr(vg + (int64_t)tile_at(it + VA) * BN * v_row_bytes);
+    }
     for (; it < n_plain; it += kRingOf<HALF>) {
       iteration(std::integral_constant<int, 0>{}, std::false_type{}, it);
       iteration(std::integral_constant<int, 1>{}, std::false_type{}, it + 1);
@@ -1017,6 +1103,12 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
   constexpr int NDB = SPLIT ? 4 : 8;
   auto finish = [&](auto db0_tag) __attribute__((always_inline)) {
     constexpr int DB0 = decltype(db0_tag)::value;
+    int col = qc, lane_group = g;
+    if constexpr (WIN) {  // (worked out again and not kept over the loops)
+      int at = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u));
+      asm volatile("" : "+v"(at));
+      col = at & 15, lane_group = at >> 4;
+    }
     if (MODE == 0) {
       // the step's partial from the empty state.  THROUGH (a launch of one or two rounds: every workgroup stores as the launch
       // ends, and what the L2s hold then is written back before the launch counts as done): the stores go through to
@@ -1026,7 +1118,7 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
         constexpr bool THROUGH = decltype(through_tag)::value;
 #pragma unroll
         for (int qb = 0; qb < 2; qb++) {
-          const int m = m_w0 + 16 * qb + qc;
+          const int m = m_w0 + 16 * qb + col;
           const float l_tot = column_sum(l_run[qb]);
           if (m < q_len) {
             const int64_t tok = o_start + m;
@@ -1034,15 +1126,33 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
             float* orow = (float*)p.o + tok * p.o_st + (int64_t)h * p.o_sh;
 #pragma unroll
             for (int i = 0; i < NDB; i++) {
-              if (THROUGH) store16_through(orow + (DB0 + i) * 16 + 4 * g, oacc[DB0 + i][qb] * inv);
-              else *(f32x4*)(orow + (DB0 + i) * 16 + 4 * g) = oacc[DB0 + i][qb] * inv;
+              if (THROUGH) store16_through(orow + (DB0 + i) * 16 + 4 * lane_group, oacc[DB0 + i][qb] * inv);
+              else *(f32x4*)(orow + (DB0 + i) * 16 + 4 * lane_group) = oacc[DB0 + i][qb] * inv;
             }
-            if (g == 0 && DB0 == 0) p.lse[tok * p.hq + h] = l_tot > 0.f ? (m_run[qb] + __builtin_amdgcn_logf(l_tot)) * kLn2 : -INFINITY;
+            if (lane_group == 0 && DB0 == 0 && (!WIN || p.lse)) p.lse[tok * p.hq + h] = l_tot > 0.f ? (m_run[qb] + __builtin_amdgcn_logf(l_tot)) * kLn2 : -INFINITY;
           }
         }
       };
-      if (p.store_through) write_partial(std::true_type{});
+      if (!WIN && p.store_through) write_partial(std::true_type{});
       else write_partial(std::false_type{});
+    }
+    if (MODE == 3) {
+#pragma unroll
+      for (int qb = 0; qb < 2; qb++) {
+        const int m = m_w0 + 16 * qb + col;
+        const float l_tot = column_sum(l_run[qb]);
+        if (m < q_len) {
+          const int64_t tok = o_start + m;
+          const float inv = l_tot > 0.f ? 1.f / l_tot : 0.f;
+          uint16_t* orow = (uint16_t*)p.o + tok * p.o_st + (int64_t)h * p.o_sh;
+#pragma unroll
+          for (int i = 0; i < NDB; i++) {
+            const f32x4 x = oacc[DB0 + i][qb] * inv;
+            *(u32x2*)(orow + (DB0 + i) * 16 + 4 * lane_group) = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+          }
+          if (lane_group == 0 && DB0 == 0 && p.lse) p.lse[tok * p.hq + h] = l_tot > 0.f ? (m_run[qb] + __builtin_amdgcn_logf(l_tot)) * kLn2 : -INFINITY;
+        }
+      }
     }
     if (MODE == 1) {
       // the reference's update of (o, m, l) (RING:171-188).  NB row blocks at a time: all reads of their old o are in
@@ -1183,10 +1293,11 @@ static int pack_shift_for(const lsattn_prefill_args* a, bool split, const Tuning
   return s;
 }
 
-template <typename T, int MODE, bool DV, bool SPLIT, bool HALF, bool CUTS>
-static int launch_prefill_rows(const lsattn_prefill_args* a, bool tile_major, const Tuning& tn, hipStream_t st, bool fold = false) {
+template <typename T, int MODE, bool DV, bool SPLIT, bool HALF, bool CUTS, bool WIN = false>
+static int launch_prefill_rows(const lsattn_prefill_args* a, bool tile_major, const Tuning& tn, hipStream_t st, bool fold = false, int32_t window = 0, int32_t sinks = 0) {
   constexpr int BMW = SPLIT || HALF ? BM / 2 : BM;
   PrefillParams p;
+  p.window = window, p.sinks = sinks;
   p.q = a->q;
   p.k = a->k;
   p.v = a->v;
@@ -1280,7 +1391,7 @@ static int launch_prefill_rows(const lsattn_prefill_args* a, bool tile_major, co
   // (a round: two four-wave workgroups per CU, one of the others.  Two rounds still gain: 16 x 256 tokens 38.0 -> 36.8 us,
   // 1 x 4096 129.0 -> 127.7; six rounds lose 1-3 %, sixteen 5 %.)
   p.store_through = MODE == 0 && wgs_launch <= 2 * (HALF ? 2 * kCUs : kCUs);
-  LSATTN_LAUNCH_KERNEL((prefill_kernel<T, MODE, DV, SPLIT, HALF, CUTS>), dim3((unsigned)wgs_launch), dim3(HALF ? NWAVE * 32 : NWAVE * 64), 0, st, p);
+  LSATTN_LAUNCH_KERNEL((prefill_kernel<T, MODE, DV, SPLIT, HALF, CUTS, WIN>), dim3((unsigned)wgs_launch), dim3(HALF ? NWAVE * 32 : NWAVE * 64), 0, st, p);
   return check_launch();
 }
 
@@ -1472,13 +1583,39 @@ extern "C" int lsattn_prefill_step_accumulate(const lsattn_prefill_args* a, void
   return a->v_is_f16 ? launch_prefill<BF16, 2, true>(a, (hipStream_t)stream) : launch_prefill<BF16, 2, false>(a, (hipStream_t)stream);
 }
 
+// Whether a step behind a window runs in the 256-row shape, by the workgroups it makes
+static bool window_in_256_rows(const lsattn_prefill_args* a, int32_t window) {
+  if (a->head_dim != 128) return false;
+  const Tuning tn = tuning();
+  if (tn.prefill_rows) return tn.prefill_rows == LSATTN_PREFILL_ROWS_256;
+  const int ps = pack_shift_for(a, false, tn);
+  const int64_t wgs = (int64_t)a->batch * (a->num_q_heads >> ps) * ((a->max_q_len + (BM >> ps) - 1) / (BM >> ps));
+  return wgs >= kCUs && window >= 512;
+}
+
+extern "C" int lsattn_prefill_window_converts_v(const lsattn_prefill_args* a, int64_t window) {
+  if (!a || a->dtype != LSATTN_BF16 || a->num_q_heads <= 0 || a->num_kv_heads <= 0 || a->num_q_heads % a->num_kv_heads || a->max_q_len <= 0) return 0;
+  return !window_in_256_rows(a, (int32_t)(window < 0x7fffffff ? window : 0x7fffffff));
+}
+
 extern "C" int lsattn_prefill_window(const lsattn_prefill_args* a, int64_t window, int64_t sinks, void* stream) {
   const int rc = validate(a, 3);
   if (rc != LSATTN_OK) return rc;
   if (window < 1 || sinks < 0) return LSATTN_ERR_INVALID_ARG;
   if (a->batch == 0 || a->max_q_len == 0) return LSATTN_OK;
   // (positions are 31-bit: larger ones change nothing)
-  return launch_prefill_window(a, (int32_t)(window < 0x7fffffff ? window : 0x7fffffff), (int32_t)(sinks < 0x7fffffff ? sinks : 0x7fffffff), (hipStream_t)stream);
+  const int32_t w = (int32_t)(window < 0x7fffffff ? window : 0x7fffffff), s = (int32_t)(sinks < 0x7fffffff ? sinks : 0x7fffffff);
+  hipStream_t st = (hipStream_t)stream;
+  if (window_in_256_rows(a, w)) {
+    const Tuning tn = tuning();
+    if (a->dtype == LSATTN_F16)
+      return a->o_dtype == LSATTN_F32 ? launch_prefill_rows<F16, 0, true, false, false, false, true>(a, false, tn, st, false, w, s)
+                                      : launch_prefill_rows<F16, 3, true, false, false, false, true>(a, false, tn, st, false, w, s);
+    if (a->v_is_f16)
+      return a->o_dtype == LSATTN_F32 ? launch_prefill_rows<BF16, 0, true, false, false, false, true>(a, false, tn, st, false, w, s)
+                                      : launch_prefill_rows<BF16, 3, true, false, false, false, true>(a, false, tn, st, false, w, s);
+  }
+  return launch_prefill_window(a, w, s, st);
 }
 
 extern "C" int lsattn_prefill_route(const lsattn_prefill_args* a) {

@@ -464,7 +464,7 @@ def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_g
     a window that a query does not see are multiplied by a weight of zero: they have to be finite (K rows may hold anything)."""
     if window is not None and _native.window_attention(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx, kv_b_start_loc, kv_b_seq_len,
                                                        kv_first_token_global_idx, logical_sp_peers_num, max_q_b_seq_len, window, sinks, lse,
-                                                       0 if total_q_len is None else total_q_len):
+                                                       0 if total_q_len is None else total_q_len, PRECONVERT_BF16_V):
         return
     for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")):
         _dev(t, n)

@@ -107,11 +107,17 @@ def test_python_operator_refuses():
 
 
 # ------------------------------------------------------------------------------------------------ GPU
+@pytest.fixture(params=[None, "256"])
+def rows(request, tuning):
+    """The library's own shape, and 128-wide heads forced into that of 256 rows, which it keeps for larger launches."""
+    tuning(prefill_rows=request.param)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 128), (3, 3, 128), (4, 1, 64), (2, 2, 32), (6, 3, 16), (7, 1, 128)])
 @pytest.mark.parametrize("window,sinks", [(1, 0), (33, 4), (64, 0), (100, 70), (1 << 40, 3)])
-def test_prompts(lsa, dtype, Hq, Hkv, D, window, sinks):
+def test_prompts(lsa, rows, dtype, Hq, Hkv, D, window, sinks):
     s = Step([(n, 0, n, 0) for n in (1, 130, 0, 64, 301)], Hq, Hkv, D, DT[dtype], seed=Hq)
     s.check(s.run(lsa, window, sinks), window, sinks)
 
@@ -120,7 +126,7 @@ def test_prompts(lsa, dtype, Hq, Hkv, D, window, sinks):
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("D", [128, 64])
 @pytest.mark.parametrize("window,sinks", [(40, 0), (200, 5), (300, 129)])
-def test_chunks_behind_contexts_shorter_and_later_keys_and_no_keys(lsa, dtype, D, window, sinks):
+def test_chunks_behind_contexts_shorter_and_later_keys_and_no_keys(lsa, rows, dtype, D, window, sinks):
     """A chunk at the end of its keys, one whose keys end before its window, one whose keys start behind its first queries, and one without keys."""
     s = Step([(50, 500, 550, 0), (20, 900, 300, 0), (90, 0, 60, 40), (5, 9, 0, 0), (33, 1000, 500, 533), (3, 5, -4, 0)], 4, 2, D, DT[dtype], seed=4)
     s.check(s.run(lsa, window, sinks), window, sinks)
@@ -131,7 +137,7 @@ def test_chunks_behind_contexts_shorter_and_later_keys_and_no_keys(lsa, dtype, D
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("Hq,Hkv,D,lens", [(32, 8, 128, [700, 333, 900]), (32, 32, 128, [400, 400]), (32, 4, 64, [900, 1000])])
-def test_launches_that_fill_the_chip(lsa, dtype, Hq, Hkv, D, lens):
+def test_launches_that_fill_the_chip(lsa, rows, dtype, Hq, Hkv, D, lens):
     """Many workgroups: 32 positions per wave."""
     s = Step([(n, 0, n, 0) for n in lens] * (8 if D == 128 else 5), Hq, Hkv, D, DT[dtype], seed=6)
     s.seqs, keep = s.seqs, s.seqs
@@ -150,7 +156,7 @@ def test_launches_that_fill_the_chip(lsa, dtype, Hq, Hkv, D, lens):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", list(DT))
-def test_a_ring_of_striped_chunks_joins_to_the_whole(lsa, dtype):
+def test_a_ring_of_striped_chunks_joins_to_the_whole(lsa, rows, dtype):
     """Three instances hold every third token; the partials of one instance's queries over the three chunks merge to the step over all keys."""
     n, P, W, S = 300, 3, 70, 8
     q, kv = _rows((n, 4, 128), 1, DT[dtype]), _rows((n, 4, 128), 2, DT[dtype])
@@ -175,7 +181,20 @@ def test_a_ring_of_striped_chunks_joins_to_the_whole(lsa, dtype):
 
 
 @pytest.mark.gpu
-def test_far_positions(lsa):
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("Hq,Hkv,window,sinks,seqs", [(4, 1, 900, 70, [(1200, 0, 1200, 0), (300, 2000, 2300, 0)]), (2, 2, 1500, 3, [(2100, 0, 2100, 0)]),
+                                                      (1, 1, 640, 0, [(500, 1000, 1500, 0), (260, 700, 600, 100)]), (8, 1, 1100, 200, [(70, 3000, 3070, 0)])])
+def test_windows_of_many_tiles(lsa, rows, dtype, Hq, Hkv, window, sinks, seqs):
+    """Windows long enough for iterations without masks between those of the sinks, of the windows' starts and of the diagonal."""
+    s = Step(seqs, Hq, Hkv, 128, DT[dtype], seed=10)
+    # (scores that grow along the keys: the maximum is raised in every part of the walk)
+    s.kv[:, :Hkv] *= torch.linspace(0.2, 3.0, s.kv.shape[0])[:, None, None].to(DT[dtype])
+    s.check(s.run(lsa, window, sinks), window, sinks)
+    s.check(s.run(lsa, window, sinks, o_dtype=torch.float32), window, sinks)
+
+
+@pytest.mark.gpu
+def test_far_positions(lsa, rows):
     """Positions close to 2^31, and a window wider than they are."""
     top = 2 ** 31 - 700
     s = Step([(40, top + 300, 340, top)], 4, 2, 128, torch.float16, seed=7)
@@ -230,7 +249,7 @@ def test_refusals_on_the_gpu(lsa):
 
 
 @pytest.mark.gpu
-def test_scores_of_keys_that_are_not_seen_do_not_matter(lsa):
+def test_scores_of_keys_that_are_not_seen_do_not_matter(lsa, rows):
     """Infinities and NaN in K rows that no query sees, inside tiles that are walked."""
     s = Step([(300, 0, 300, 0)], 4, 2, 128, torch.float16, seed=9)
     ks = s.k_start[0]
