@@ -130,9 +130,11 @@ __device__ __forceinline__ const char* uniform_ptr(const char* ptr) {
 // A launch's shape by head size and positions per wave: keys per LDS tile, tiles in LDS (requested one fewer ahead), workgroups per CU.
 // 128-wide heads, 32 positions per wave: three stages of 32 keys (48 KB) and at most 168 registers (158; 168 where V is bfloat16), so that three
 // workgroups fit a CU.
-template <int D, int WP> constexpr int kTileOf = D == 128 && WP == 32 ? 32 : 64;
-template <int D, int WP> constexpr int kStagesOf = D == 128 && WP == 32 ? 3 : 2;
-template <int D, int WP, bool DV> constexpr int kResident = D == 128 ? (WP == 32 ? 3 : 2) : WP == 32 && D == 64 && !DV ? 3 : 4;
+// Behind a window (WIN) the compiler's registers do not fit those 168 (22 to 38 spills, 3.07 ms for 32768 tokens behind 4096 + 16, 32/8 heads; 2.30 with two workgroups per CU): two stages
+// of 64 keys there, operands and addresses in registers of their own (4096 tokens behind 1024, 32/32: 591 -> 642 TFLOP/s).
+template <int D, int WP, bool WIN> constexpr int kTileOf = D == 128 && WP == 32 && !WIN ? 32 : 64;
+template <int D, int WP, bool WIN> constexpr int kStagesOf = D == 128 && WP == 32 && !WIN ? 3 : 2;
+template <int D, int WP, bool DV, bool WIN> constexpr int kResident = D == 128 ? (WP == 32 && !WIN ? 3 : 2) : WP == 32 && D == 64 && !DV ? 3 : 4;
 
 // DV: the V tiles are fp16 in memory and go straight into LDS as the K tiles do; otherwise (bfloat16 V) they pass through
 // registers and are converted on the way.  WP: query positions per wave, 16 or 32.  (Products of 32 x 32 x 16, which take a tenth fewer
@@ -145,14 +147,14 @@ template <int D, int WP, bool DV> constexpr int kResident = D == 128 ? (WP == 32
 // workgroup walks the tiles that hold sinks, then those from its first row's window on; MODE 0, or MODE 3: O in T's type and the LSE,
 // from the empty state.
 template <typename T, int D, int MODE, bool DV, int WP, int KP = 1, bool WIN = false>
-__global__ __launch_bounds__(kWaves * KP * 64, (WIN && D == 128 && WP == 32 ? 2 : kResident<D, WP, DV>)) void prefill_small_kernel(SmallParams p) {
+__global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV, WIN>)) void prefill_small_kernel(SmallParams p) {
   static_assert(WIN ? KP == 1 && (MODE == 0 || MODE == 3) : MODE < 3, "a window knows no state");
   static_assert(KP == 1 || (KP == 2 && WP == 16 && D >= 32), "the parts of a tile of 64 keys, the columns that each of two waves finishes");
   constexpr int NW = kWaves * KP;
   constexpr int QB = WP / 16;               // blocks of 16 positions per wave
   constexpr int KS = D >= 32 ? D / 32 : 1;  // contraction steps of Q K^T (32 elements each; D = 16 fills half of one)
   constexpr int NDB = D / 16;               // 16-wide blocks of the head
-  constexpr int TK = kTileOf<D, WP>, NS = kStagesOf<D, WP>;
+  constexpr int TK = kTileOf<D, WP, WIN>, NS = kStagesOf<D, WP, WIN>;
   constexpr int CPR = D / 8;                // 16-byte chunks per K or V row
   constexpr int RB = D * 2;                 // bytes per row in LDS
   constexpr int TB = TK * RB;               // bytes per tile
@@ -316,7 +318,7 @@ __global__ __launch_bounds__(kWaves * KP * 64, (WIN && D == 128 && WP == 32 ? 2 
   // whose scores the lane holds
   // (the contraction step and the block are bits of the chunk number that g and the lane leave free, so they are XORed into the address:
   // in registers of their own, or, where none are to spare (LEAN), next to each read)
-  constexpr bool LEAN = D == 128 && WP == 32;
+  constexpr bool LEAN = D == 128 && WP == 32 && !WIN;
   constexpr bool LEAN_V = LEAN || (D == 64 && WP == 32);
   constexpr int NKA = LEAN ? 1 : KS, NVA = LEAN_V ? 1 : NDB;
   int kaddr[NKA], vaddr[NVA];
