@@ -8,8 +8,9 @@
 // What bounds it is HBM: (D + 1) bytes per K and V row of a head in 8 bits, 2 D in 16, against 2 D multiply-adds per query head
 // for each.  Hence a row is read once for up to eight query heads of its KV head, and the vector work beside the matrix pipe is
 // kept below what the memory leaves time for:
-//   * a wave takes blocks of 32 tokens of one KV head.  Lane (g, c) = (lane / 16, lane % 16) loads pieces of K rows c and 16 + c and elements
-//     [c * D / 16, + D / 16) of V rows 4g .. 4g + 3 and 16 + 4g .. 16 + 4g + 3, straight into registers: no LDS tile;
+//   * a wave takes blocks of 32 tokens of one KV head.  Every load instruction takes whole rows (a row in two instructions of half a row each reads
+//     a sixth slower): lane (g, c) = (lane / 16, lane % 16) has elements [c * D / 16, + D / 16) of V rows 4g .. 4g + 3 and 16 + 4g .. 16 + 4g + 3;
+//     K rows are turned round in the wave's own LDS, from pieces of 16 bytes to the operands of the products;
 //   * scores transposed, S^T = K Q^T with 16x16x32 MFMAs: the order of the head's elements along the contraction is whatever
 //     the loads give, the query is read in the same one.  Column c of the product is query head c % 8, so the lane holds the
 //     scores of eight tokens, 4g + r and 16 + 4g + r, of one head: the tokens whose V rows it has;
@@ -17,7 +18,9 @@
 //     computed it, and every accumulator of a lane belongs to the head whose maximum and sum it keeps;
 //   * P keeps more than 16 bits although the operands have 16: columns c and c + 8 of the product carry two parts of the same
 //     head's P, high and low, and a second product a third part where the type is bfloat16 (8 bits each).  The parts are
-//     added once, at the end.  bfloat16 where V comes from 8 bits: P times the token's scale has its range;
+//     added once, at the end;
+//   * the scale of a token's V row goes into its weight: 2^(s + e) multiplies the e4m3 values as they are, and the reference that the weights are
+//     taken relative to follows the maximum of s + e, so that they fit fp16 whatever the scales are; the sum takes them times 2^-e;
 //   * the reference of a head's weights is raised only when a score exceeds the maximum it was set by by 8 (log2 units): the accumulators
 //     are seldom rescaled, and no exchange between lanes stands in the common path.
 // Short contexts and windows: the waves of one workgroup share a (request, KV head) and meet in LDS (one launch).  Otherwise the blocks of
@@ -31,6 +34,11 @@ namespace {
 struct E4M3 {};  // element tag of the pool
 
 constexpr int kBlock = 32;       // tokens per step of a wave
+// LDS of a wave: the byte offsets of a block's K rows and of its V rows, the factors of its scores, the exponents of its V rows, 2^-exponent, and what
+// is left of exponents below kLeast
+constexpr int kVOff = 256, kKScale = 512, kVExp = 640, kVInv = 768, kVRest = 896, kKRows = 1024;  // (and the K rows of a block)
+template <typename KV, int D> constexpr int kWaveLds = kKRows + kBlock * D * (__is_same(KV, E4M3) ? 1 : 2);
+constexpr int kLeast = -80;      // a V row's exponent counts as this in the weights if it is less (2^80 times a weight stays a float)
 constexpr int kHeads = 8;        // query heads per task
 constexpr int64_t kCUs = 256;
 // The reference m of a head's weights is set to the maximum so far less kHead, and raised when a score exceeds it by kLag: weights
@@ -73,6 +81,12 @@ __device__ __forceinline__ float col_max(float v) {
   v = fmaxf(v, xor16(v));
   return fmaxf(v, xor32(v));
 }
+// (one instruction: from fmaxf the compiler makes three, which quiet signalling NaNs first)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 __device__ __forceinline__ float col_sum(float v) {
   v += xor16(v);
   return v + xor32(v);
@@ -105,35 +119,37 @@ template <> struct Parts<F16> {
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const uint32_t first = pack2<F16>(x[2 * e], x[2 * e + 1]);
-      float a, b;
-      unpack2<F16>(first, a, b);
-      const uint32_t second = pack2<F16>(x[2 * e] - a, x[2 * e + 1] - b);
+      float a, b;  // x less its first part
+      asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(a) : "v"(first), "v"(x[2 * e]));
+      asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(b) : "v"(first), "v"(x[2 * e + 1]));
+      const uint32_t second = pack2<F16>(a, b);
       out[0][e] = hi ? first : second;
     }
   }
 };
 template <> struct Parts<BF16> {
   static constexpr int N = 2;
+  static __device__ __forceinline__ float cut(float v) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u); }
+  static __device__ __forceinline__ uint32_t upper(float lo, float hi) { return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u); }
   static __device__ __forceinline__ void of(const float (&x)[8], bool hi, u32x4 (&out)[2]) {
-    float first[8], rest[8], third[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      first[e] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[e]) & 0xffff0000u);
-      rest[e] = x[e] - first[e];
-      third[e] = rest[e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, rest[e]) & 0xffff0000u);
-      first[e] = hi ? first[e] : rest[e];
-      third[e] = hi ? third[e] : 0.f;
-    }
+    const uint32_t mine = hi ? 0xffffffffu : 0u;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      out[0][e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, first[2 * e + 1]), __builtin_bit_cast(uint32_t, first[2 * e]), 0x07060302u);
-      out[1][e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, third[2 * e + 1]), __builtin_bit_cast(uint32_t, third[2 * e]), 0x07060302u);
+      float rest[2], third[2], first[2];
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        rest[k] = x[2 * e + k] - cut(x[2 * e + k]);
+        third[k] = rest[k] - cut(rest[k]);
+        first[k] = hi ? x[2 * e + k] : rest[k];
+      }
+      out[0][e] = upper(first[0], first[1]);
+      out[1][e] = upper(third[0], third[1]) & mine;
     }
   }
 };
 
 template <typename KV> struct PvOf { typedef KV type; };
-template <> struct PvOf<E4M3> { typedef BF16 type; };
+template <> struct PvOf<E4M3> { typedef F16 type; };
 
 // visible tokens of a request
 __device__ __forceinline__ int visible(const PoolParams& p, int b, int& len) {
@@ -152,24 +168,25 @@ template <typename QT, typename KV, int D> struct Walk {
   static constexpr bool k8 = __is_same(KV, E4M3);
   static constexpr int KS = D / 32;               // contraction steps of Q K^T
   static constexpr int EV = D / 16;               // elements of a V row per lane
-  static constexpr int KW = k8 ? D / 16 : D / 8;  // words of a K row per lane (a quarter of the row)
+  static constexpr int CPR = k8 ? D / 16 : D / 8; // 16-byte pieces of a K row
+  static constexpr int RPI = 64 / CPR;            // K rows per load instruction
+  static constexpr int KI = kBlock / RPI;         // and instructions for a block
   static constexpr int VW = k8 ? EV / 4 : EV / 2; // words of a V row per lane
   static constexpr int ES = k8 ? 1 : 2;           // bytes per element
 
   const PoolParams& p;
   const int lane, g, c;
-  int32_t* const slot_lds;   // [32] of this wave
-  float* const scale_lds;    // [64]: K scales (times the softmax scale), V scales
+  char* const lds;
   u32x4 qf[KS];
   f32x4 acc[EV];  // acc[j][r] = O[head][EV * (4g + r) + j], of the parts of P in this lane's column
   float m, l;     // log2-domain maximum of the head; the lane's share of the sum
 
   __device__ __forceinline__ Walk(const PoolParams& p_, char* lds_wave)
-      : p(p_), lane(threadIdx.x & 63), g(lane >> 4), c(lane & 15), slot_lds((int32_t*)lds_wave), scale_lds((float*)(lds_wave + 128)) {}
+      : p(p_), lane(threadIdx.x & 63), g(lane >> 4), c(lane & 15), lds(lds_wave) {}
 
   const char *kb, *vb;
   const uint8_t* sb;  // the lane's column of scales: K for lanes 0 .. 31, V for the others
-  int64_t s_s0;
+  uint32_t s_s0, row_s0;  // and the bytes from one slot to the next there, and in the rows
   const int32_t* row;
   int sinks, skip, limit;
 
@@ -186,12 +203,13 @@ template <typename QT, typename KV, int D> struct Walk {
       const int d = k8 ? 64 * (ks >> 1) + 16 * g + 8 * (ks & 1) : 32 * ks + 8 * g;
       qf[ks] = *(const u32x4*)(q + d * 2);
     }
-    kb = p.k + kvh * p.k_s1 + 16 * g;
+    kb = p.k + kvh * p.k_s1 + 16 * (lane & (CPR - 1));
     vb = p.v + kvh * p.v_s1 + c * EV * ES;
     if (k8) {
       sb = lane < 32 ? p.ks + kvh * p.ks_s1 : p.vs + kvh * p.vs_s1;
-      s_s0 = lane < 32 ? p.ks_s0 : p.vs_s0;
+      s_s0 = (uint32_t)(lane < 32 ? p.ks_s0 : p.vs_s0);
     }
+    row_s0 = (uint32_t)(lane < 32 ? p.k_s0 : p.v_s0);
     row = p.table + (int64_t)p.b_req[b] * p.max_seq_len;
     sinks = p.window ? p.sinks : 0;
     skip = len - n_vis;
@@ -207,82 +225,110 @@ template <typename QT, typename KV, int D> struct Walk {
     return row[i < sinks ? i : i + skip];
   }
 
-  u32x4 kr[2][KW / 4];
-  uint32_t vr[8][VW];
-  uint32_t scale_byte;
-  uint32_t there;  // bit i: token i of the block exists
+  struct Rows {  // a block's K and V in flight
+    u32x4 k[KI];
+    uint32_t v[8][VW];
+    uint32_t scale_byte;
+    uint32_t there;  // bit i: token i of the block exists
+  };
 
-  __device__ __forceinline__ void load_rows(int at, int slot) {
+  // the rows of the block at `at`, whose slots the lanes have in `slot`; `next`: where the block after it starts, whose slots are asked for in front
+  __device__ __forceinline__ void load_rows(Rows& r, int at, int& slot_of, int next) {
+    int slot = slot_of;
+    slot_of = load_slot(next);
     const bool ok = at + (lane & 31) < limit && (uint32_t)slot < (uint32_t)p.num_slots;
-    there = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
+    r.there = (uint32_t)__builtin_amdgcn_ballot_w64(ok);
     slot = ok ? slot : 0;
-    if (k8) scale_byte = sb[slot * s_s0];
-    slot_lds[lane & 31] = slot;
+    if (k8) r.scale_byte = sb[(uint64_t)(uint32_t)slot * s_s0];
+    *(uint64_t*)(lds + lane * 8) = (uint64_t)(uint32_t)slot * row_s0;
     __builtin_amdgcn_wave_barrier();
-    const int k0 = slot_lds[c], k1 = slot_lds[16 + c];
-    int vslot[8];
-    *(u32x4*)vslot = *(const u32x4*)(slot_lds + 4 * g);
-    *(u32x4*)(vslot + 4) = *(const u32x4*)(slot_lds + 16 + 4 * g);
-    __builtin_amdgcn_wave_barrier();
+    uint64_t koff[KI], voff[8];
 #pragma unroll
-    for (int w = 0; w < KW / 4; w++) {
-      kr[0][w] = __builtin_nontemporal_load((const u32x4*)(kb + k0 * p.k_s0 + 64 * w));
-      kr[1][w] = __builtin_nontemporal_load((const u32x4*)(kb + k1 * p.k_s0 + 64 * w));
+    for (int i = 0; i < KI; i++) koff[i] = *(const uint64_t*)(lds + (RPI * i + lane / CPR) * 8);
+#pragma unroll
+    for (int i = 0; i < 4; i++) *(u32x4*)(voff + 2 * i) = *(const u32x4*)(lds + kVOff + (i >> 1) * 128 + 32 * g + (i & 1) * 16);
+    __builtin_amdgcn_wave_barrier();
+    // (the empty statements keep each 64-bit address next to its load instead of ten of them live at once)
+#pragma unroll
+    for (int i = 0; i < KI; i++) {
+      asm volatile("" : "+v"(koff[i]));
+      r.k[i] = __builtin_nontemporal_load((const u32x4*)(kb + koff[i]));
     }
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const char* at_v = vb + vslot[i] * p.v_s0;
-      if constexpr (VW == 1) vr[i][0] = __builtin_nontemporal_load((const uint32_t*)at_v);
-      else if constexpr (VW == 2) *(u32x2*)vr[i] = __builtin_nontemporal_load((const u32x2*)at_v);
-      else *(u32x4*)vr[i] = __builtin_nontemporal_load((const u32x4*)at_v);
+      asm volatile("" : "+v"(voff[i]));
+      const char* at_v = vb + voff[i];
+      if constexpr (VW == 1) r.v[i][0] = __builtin_nontemporal_load((const uint32_t*)at_v);
+      else if constexpr (VW == 2) *(u32x2*)r.v[i] = __builtin_nontemporal_load((const u32x2*)at_v);
+      else *(u32x4*)r.v[i] = __builtin_nontemporal_load((const u32x4*)at_v);
     }
   }
 
-  __device__ __forceinline__ void compute() {
+  __device__ __forceinline__ void compute(Rows& rows) {
+    // the K rows through LDS: pieces XORed with the row, so that neither side meets in the banks
+    char* const k_lds = lds + kKRows;
+#pragma unroll
+    for (int i = 0; i < KI; i++) {
+      const int row = RPI * i + lane / CPR;
+      *(u32x4*)(k_lds + row * (CPR * 16) + (((lane & (CPR - 1)) ^ (row & (CPR - 1))) << 4)) = rows.k[i];
+    }
+    __builtin_amdgcn_wave_barrier();
     // scores of the lane's head with tokens 4g + r (s[0]) and 16 + 4g + r (s[1])
     f32x4 s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    constexpr int PIECES = CPR / 4;  // pieces of a row per lane, the contraction's 16 (8 bits) or 8 elements each
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++)
+    for (int w = 0; w < PIECES; w++)
 #pragma unroll
       for (int t = 0; t < 2; t++) {
-        u32x4 a;
+        const u32x4 k = *(const u32x4*)(k_lds + (16 * t + c) * (CPR * 16) + (((4 * w + g) ^ (c & (CPR - 1))) << 4));
         if constexpr (k8) {
-          const uint32_t w0 = kr[t][ks >> 1][2 * (ks & 1)], w1 = kr[t][ks >> 1][2 * (ks & 1) + 1];
-          a = u32x4{widen<QT, false>(w0), widen<QT, true>(w0), widen<QT, false>(w1), widen<QT, true>(w1)};
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            const u32x4 a = u32x4{widen<QT, false>(k[2 * n]), widen<QT, true>(k[2 * n]), widen<QT, false>(k[2 * n + 1]), widen<QT, true>(k[2 * n + 1])};
+            s[t] = mfma<QT>(a, qf[2 * w + n], s[t]);
+          }
         } else {
-          a = kr[t][ks];
+          s[t] = mfma<QT>(k, qf[w], s[t]);
         }
-        s[t] = mfma<QT>(a, qf[ks], s[t]);
+        if (t) __builtin_amdgcn_sched_barrier(0);
       }
-    float x[8], vscale[8];
+    __builtin_amdgcn_wave_barrier();
+    // x: the score in log2 units, plus the exponent of the token's V row
+    float x[8];
+    bool tiny = false;
     if constexpr (k8) {
-      scale_lds[lane] = scale_of(scale_byte) * (lane < 32 ? p.scale_log2 : 1.f);
+      const int e = (int)rows.scale_byte - 127;
+      tiny = __builtin_amdgcn_ballot_w64(lane >= 32 && e < kLeast) != 0;
+      const int kept = e < kLeast ? kLeast : e;
+      *(float*)(lds + kKScale + lane * 4) = lane < 32 ? scale_of(rows.scale_byte) * p.scale_log2 : (float)kept;
+      if (lane >= 32) {
+        *(float*)(lds + kVInv - 128 + lane * 4) = __builtin_bit_cast(float, (uint32_t)(127 - kept) << 23);
+        if (tiny) *(float*)(lds + kVRest - 128 + lane * 4) = __builtin_amdgcn_exp2f((float)(e - kept));
+      }
       __builtin_amdgcn_wave_barrier();
       f32x4 kf[2], vf[2];
 #pragma unroll
       for (int t = 0; t < 2; t++) {
-        kf[t] = *(const f32x4*)(scale_lds + 16 * t + 4 * g);
-        vf[t] = *(const f32x4*)(scale_lds + 32 + 16 * t + 4 * g);
+        kf[t] = *(const f32x4*)(lds + kKScale + 64 * t + 16 * g);
+        vf[t] = *(const f32x4*)(lds + kVExp + 64 * t + 16 * g);
       }
-      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = s[e / 4][e % 4] * kf[e / 4][e % 4], vscale[e] = vf[e / 4][e % 4];
+      for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(s[e / 4][e % 4], kf[e / 4][e % 4], vf[e / 4][e % 4]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) x[e] = s[e / 4][e % 4] * p.scale_log2;
     }
-    if (there != 0xffffffffu) {  // (the same for every lane)
-      const uint32_t mine = ((there >> (4 * g)) & 15u) | ((there >> (12 + 4 * g)) & 0xf0u);
+    if (rows.there != 0xffffffffu) {  // (the same for every lane)
+      const uint32_t mine = ((rows.there >> (4 * g)) & 15u) | ((rows.there >> (12 + 4 * g)) & 0xf0u);
 #pragma unroll
       for (int e = 0; e < 8; e++) {
         const bool ok = (mine >> e) & 1u;
         x[e] = ok ? x[e] : -INFINITY;
-        if (k8) vscale[e] = ok ? vscale[e] : 0.f;
 #pragma unroll
-        for (int w = 0; w < VW; w++) vr[e][w] = ok ? vr[e][w] : 0u;  // (what lies there may be infinite or NaN)
+        for (int w = 0; w < VW; w++) rows.v[e][w] = ok ? rows.v[e][w] : 0u;  // (what lies there may be infinite or NaN)
       }
     }
-    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+    const float mx = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
     if (__builtin_amdgcn_ballot_w64(mx > m + kLag) != 0) {
       const float m_new = fmaxf(m, col_max(mx) - kHead);
       const float alpha = exp2_diff(m, m_new);
@@ -294,13 +340,25 @@ template <typename QT, typename KV, int D> struct Walk {
     const float m_safe = m == -INFINITY ? 0.f : m;
 #pragma unroll
     for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(x[e] - m_safe);
-    l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-    if (k8) {
+    if constexpr (k8) {
+      f32x4 inv[2];
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] *= vscale[e];
+      for (int t = 0; t < 2; t++) inv[t] = *(const f32x4*)(lds + kVInv + 64 * t + 16 * g);
+      float even = 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; e++) even = __builtin_fmaf(x[e], inv[0][e], even), l = __builtin_fmaf(x[4 + e], inv[1][e], l);
+      l += even;
+      if (tiny) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= *(const float*)(lds + kVRest + 64 * (e / 4) + 16 * g + 4 * (e % 4));
+      }
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     }
     u32x4 pk[2];
     Parts<PV>::of(x, c < 8, pk);
+    __builtin_amdgcn_sched_barrier(0);
     // V^T operands: element j of the eight tokens
 #pragma unroll
     for (int w = 0; w < VW; w++) {
@@ -308,8 +366,8 @@ template <typename QT, typename KV, int D> struct Walk {
         u32x4 va[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-          const uint32_t lo = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x05010400u);
-          const uint32_t hi = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x07030602u);
+          const uint32_t lo = __builtin_amdgcn_perm(rows.v[2 * t + 1][w], rows.v[2 * t][w], 0x05010400u);
+          const uint32_t hi = __builtin_amdgcn_perm(rows.v[2 * t + 1][w], rows.v[2 * t][w], 0x07030602u);
           va[0][t] = widen<PV, false>(lo);
           va[1][t] = widen<PV, true>(lo);
           va[2][t] = widen<PV, false>(hi);
@@ -319,29 +377,39 @@ template <typename QT, typename KV, int D> struct Walk {
         for (int j = 0; j < 4; j++)
 #pragma unroll
           for (int n = 0; n < Parts<PV>::N; n++) acc[4 * w + j] = mfma<PV>(va[j], pk[n], acc[4 * w + j]);
+        __builtin_amdgcn_sched_barrier(0);
       } else {
         u32x4 va[2];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-          va[0][t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x05040100u);
-          va[1][t] = __builtin_amdgcn_perm(vr[2 * t + 1][w], vr[2 * t][w], 0x07060302u);
+          va[0][t] = __builtin_amdgcn_perm(rows.v[2 * t + 1][w], rows.v[2 * t][w], 0x05040100u);
+          va[1][t] = __builtin_amdgcn_perm(rows.v[2 * t + 1][w], rows.v[2 * t][w], 0x07060302u);
         }
 #pragma unroll
         for (int j = 0; j < 2; j++)
 #pragma unroll
           for (int n = 0; n < Parts<PV>::N; n++) acc[2 * w + j] = mfma<PV>(va[j], pk[n], acc[2 * w + j]);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
 
-  // visible tokens [from, to) in steps of `step` blocks; the first block exists
+  // Visible tokens [from, to) in steps of `step` blocks; the first block exists.  The next block's rows are in flight while one is worked on (a lone
+  // wave otherwise spends 2 us on a block, nearly all of it waiting), and the slots of the one after it.
   __device__ __forceinline__ void run(int from, int to, int step) {
     limit = to;
+    step *= kBlock;
+    Rows a, b;
     int slot = load_slot(from);
-    for (int at = from; at < to; at += step * kBlock) {
-      load_rows(at, slot);
-      slot = load_slot(at + step * kBlock);
-      compute();
+    load_rows(a, from, slot, from + step);
+    // (loads without a condition around them: behind one the compiler would wait for all of them.  Past the end they repeat the last rows)
+    for (int at = from; at < to; at += 2 * step) {
+      load_rows(b, at + step, slot, at + 2 * step);
+      __builtin_amdgcn_sched_barrier(0);
+      compute(a);
+      load_rows(a, at + 2 * step, slot, at + 3 * step);
+      __builtin_amdgcn_sched_barrier(0);
+      if (at + step < to) compute(b);
     }
   }
 
@@ -362,13 +430,13 @@ __device__ __forceinline__ void store_elem4(char* o, int dtype, int64_t at, cons
 }
 __device__ __forceinline__ float ln_of(float m, float l) { return l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : (l == l ? -INFINITY : l); }
 
-constexpr int kWaveLds = 384;  // bytes of LDS per wave: 32 slots, 64 scales
+
 
 // One workgroup per (task, request): its NW waves take every NW-th block and meet in LDS.
 template <typename QT, typename KV, int D, int NW>
 __global__ __launch_bounds__(NW * 64) void pool_decode_direct_kernel(PoolParams p) {
   constexpr int ROW = D + 4;  // floats per head in LDS: O, maximum, sum (and a bank's shift)
-  __shared__ __attribute__((aligned(16))) char lds[NW * kHeads * ROW * 4 > NW * kWaveLds ? NW * kHeads * ROW * 4 : NW * kWaveLds];
+  __shared__ __attribute__((aligned(16))) char lds[NW * (kHeads * ROW * 4 > kWaveLds<KV, D> ? kHeads * ROW * 4 : kWaveLds<KV, D>)];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int task = blockIdx.x, b = blockIdx.y;
   const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
@@ -376,7 +444,7 @@ __global__ __launch_bounds__(NW * 64) void pool_decode_direct_kernel(PoolParams 
   const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
   int len;
   const int n_vis = visible(p, b, len);
-  Walk<QT, KV, D> w(p, lds + wave * kWaveLds);
+  Walk<QT, KV, D> w(p, lds + wave * kWaveLds<KV, D>);
   if (wave * kBlock < n_vis) {
     w.start(b, task, len, n_vis);
     w.run(wave * kBlock, n_vis, NW);
@@ -448,8 +516,8 @@ __device__ __forceinline__ Deal deal(const PoolParams& p) {
 
 // Four waves per workgroup, each with a share of its own of one task; the tasks of a share are neighbours, on one XCD.
 template <typename QT, typename KV, int D>
-__global__ __launch_bounds__(256) void pool_decode_shares_kernel(PoolParams p) {
-  __shared__ __attribute__((aligned(16))) char lds[4 * kWaveLds];
+__global__ __launch_bounds__(256, (D == 128 && !__is_same(KV, E4M3) ? 2 : 3)) void pool_decode_shares_kernel(PoolParams p) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * kWaveLds<KV, D>];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   // (ids go to the XCDs round-robin; gridDim.x is a multiple of 8)
   const uint32_t id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
@@ -480,7 +548,7 @@ __global__ __launch_bounds__(256) void pool_decode_shares_kernel(PoolParams p) {
     }
     first += chunk;
   }
-  Walk<QT, KV, D> w(p, lds + wave * kWaveLds);
+  Walk<QT, KV, D> w(p, lds + wave * kWaveLds<KV, D>);
   const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
   const int h0 = kvh * p.group + sg * kHeads;
   const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
@@ -512,66 +580,77 @@ __global__ __launch_bounds__(256) void pool_decode_shares_kernel(PoolParams p) {
   }
 }
 
-// o = sum of a request's partials by their log-sum-exps; D / 4 lanes read a row, the rows are dealt to the rest of the workgroup.
+// o = sum of a request's partials by their log-sum-exps: first the weights of all of them, by all threads, into LDS, then the rows, whose loads wait for nothing.
+// D / 4 lanes read a row, the rows are dealt to the rest of the workgroup.
+constexpr int kMaxShares = 12 * (int)kCUs;
 template <int D>
 __global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
   constexpr int LPR = D / 4, SL = 256 / LPR;
-  __shared__ __attribute__((aligned(16))) float acc[SL][D + 4];
+  __shared__ __attribute__((aligned(16))) float acc[SL][D];
+  __shared__ float weight[kMaxShares], part[8];
   const int h = blockIdx.x, b = blockIdx.y;
-  const int lane = threadIdx.x & 63;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Deal dl = deal(p);
   int64_t first = 0;
   for (int b0 = 0; b0 < b; b0 += 64) first += b0 + lane < b ? units_of(p, b0 + lane) : 0;
   first = wave_sum(first);
   const int64_t units = units_of(p, b);
   const int s0 = (int)(first / dl.per_share), n = units ? (int)((first + units - 1) / dl.per_share) - s0 + 1 : 0;
-  const int slice = threadIdx.x / LPR, d = (threadIdx.x & (LPR - 1)) * 4;
   const float* lse = p.part_lse + ((int64_t)(s0 + b) * p.hq + h);
-  const float* row = p.part_o + ((int64_t)(s0 + b) * p.hq + h) * D + d;
-  float M = -INFINITY, L = 0.f;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int i = slice; i < n; i += SL) {
+  float M = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += 256) {
     const float x = lse[(int64_t)i * p.hq];
+    weight[i] = x;
+    M = fmaxf(M, x);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  if (lane == 0) part[wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+  float L = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const float w = exp2_diff(weight[i], M);  // (NaN stays NaN)
+    weight[i] = w;
+    L += w;
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) L += __shfl_xor(L, d, 64);
+  if (lane == 0) part[4 + wave] = L;
+  __syncthreads();
+  L = (part[4] + part[5]) + (part[6] + part[7]);
+  const int slice = threadIdx.x / LPR, d = (threadIdx.x & (LPR - 1)) * 4;
+  const float* row = p.part_o + ((int64_t)(s0 + b) * p.hq + h) * D + d;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int i = slice; i < n; i += SL) {
     const f32x4 v = *(const f32x4*)(row + (int64_t)i * p.hq * D);
-    const float m_new = x > M ? x : M;
-    const float f = exp2_diff(M, m_new), w = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - m_new);
-    L = L * f + w;
-    sum = w != 0.f ? sum * f + v * w : sum * f;
-    M = m_new;
+    sum += v * weight[i];  // (every row is finite unless the result is not)
   }
   *(f32x4*)&acc[slice][d] = sum;
-  if (d == 0) acc[slice][D] = M, acc[slice][D + 1] = L;
   __syncthreads();
   if (slice) return;
-  float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < SL; i++) top = fmaxf(top, acc[i][D]);
-  L = 0.f;
-  sum = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < SL; i++) {
-    const float f = exp2_diff(acc[i][D], top);
-    L += acc[i][D + 1] * f;
-    if (f != 0.f) sum += *(const f32x4*)&acc[i][d] * f;
-  }
+  for (int i = 1; i < SL; i++) sum += *(const f32x4*)&acc[i][d];
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int64_t at = (int64_t)b * p.hq + h;
   store_elem4(p.o, p.o_dtype, at * D + d, sum * inv);
-  if (d == 0) p.lse[at] = ln_of(top, L);
+  if (d == 0) p.lse[at] = ln_of(M, L);
 }
 
 constexpr int kDirectWaves = 8;
-constexpr int64_t kDirectTokens = 4096;  // visible tokens of the longest request up to which a workgroup takes a whole (request, KV head)
-constexpr int64_t kShareWaves = 16 * kCUs;
+constexpr int64_t kDirectTokens = 1024;  // visible tokens of the longest request up to which a workgroup takes a whole (request, KV head)
+// Waves that a launch of shares deals to: those that are on the chip at once (registers), so that none starts late
+int64_t share_waves(bool k8, int64_t head_dim) { return (head_dim == 128 && !k8 ? 8 : 12) * kCUs; }
 constexpr int64_t kMinUnits = 2;
 
 int64_t most_visible(int64_t max_len, int64_t window, int64_t sinks) { return window > 0 && window + sinks < max_len ? window + sinks : max_len; }
 int64_t tasks_of(int64_t hq, int64_t hkv) { return hkv * ((hq / hkv + kHeads - 1) / kHeads); }
-bool is_direct(int64_t batch, int64_t tasks, int64_t most) { return most <= kDirectTokens || (batch * tasks >= 2 * kCUs && most <= 2 * kDirectTokens); }
+bool is_direct(int64_t batch, int64_t tasks, int64_t most) { return most <= kDirectTokens || (batch * tasks >= kCUs && most <= 2 * kDirectTokens); }
 // shares of a launch that is not direct
-int64_t shares_of(int64_t batch, int64_t tasks, int64_t most) {
+int64_t shares_of(int64_t waves, int64_t batch, int64_t tasks, int64_t most) {
   const int64_t units = batch * ((most + kBlock - 1) / kBlock);
-  const int64_t by_waves = (kShareWaves + tasks - 1) / tasks, by_units = (units + kMinUnits - 1) / kMinUnits;
+  const int64_t by_waves = waves / tasks, by_units = (units + kMinUnits - 1) / kMinUnits;
   const int64_t n = by_waves < by_units ? by_waves : by_units;
   return n < 1 ? 1 : n;
 }
@@ -602,7 +681,7 @@ extern "C" size_t lsattn_pool_attention_workspace_bytes(int64_t batch, int64_t n
     return 0;
   const int64_t tasks = tasks_of(num_q_heads, num_kv_heads), most = most_visible(max_len_in_batch, window, sinks);
   if (is_direct(batch, tasks, most)) return 0;
-  return (size_t)((shares_of(batch, tasks, most) + batch) * num_q_heads * (head_dim + 1) * 4);
+  return (size_t)((shares_of(share_waves(true, head_dim), batch, tasks, most) + batch) * num_q_heads * (head_dim + 1) * 4);
 }
 
 extern "C" int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* stream) {
@@ -619,6 +698,10 @@ extern "C" int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* 
       (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->o) & 15))
     return LSATTN_ERR_INVALID_ARG;
   if (k8 && (!a->k_scales || !a->v_scales)) return LSATTN_ERR_INVALID_ARG;
+  // (offsets are a slot times a stride of 32 bits)
+  auto slot_stride = [](int64_t bytes) { return bytes >= 0 && bytes <= 0x7fffffff; };
+  if (!slot_stride(a->k_stride_0 * es) || !slot_stride(a->v_stride_0 * es) || (k8 && (!slot_stride(a->ks_stride_0) || !slot_stride(a->vs_stride_0))))
+    return LSATTN_ERR_INVALID_ARG;
   if (a->batch > 65535 || a->num_q_heads > 65535 || a->max_seq_len > 0x7fffff00 || a->num_slots > 0x7fffffff || a->num_reqs > 0x7fffffff ||
       a->max_len_in_batch > 0x7fffffff)
     return LSATTN_ERR_INVALID_ARG;
@@ -643,7 +726,7 @@ extern "C" int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* 
   const bool direct = is_direct(p.batch, p.tasks, most);
   p.part_o = nullptr, p.part_lse = nullptr, p.shares = 1, p.min_units = (int32_t)kMinUnits;
   if (!direct) {
-    const int64_t shares = shares_of(p.batch, p.tasks, most), rows = shares + p.batch;
+    const int64_t shares = shares_of(share_waves(k8, a->head_dim), p.batch, p.tasks, most), rows = shares + p.batch;
     if (!a->workspace || a->workspace_bytes < (size_t)(rows * p.hq * (a->head_dim + 1) * 4)) return LSATTN_ERR_WORKSPACE;
     if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
     p.shares = (int32_t)shares;
