@@ -66,7 +66,7 @@ struct PoolParams {
   float* part_o;    // [shares + batch, hq, D]
   float* part_lse;  // [shares + batch, hq]
   int32_t shares, min_units;
-  FastDiv by_tasks, by_sub;
+  FastDiv by_tasks, by_sub, by_shares;
 };
 
 __device__ __forceinline__ float xor16(float v) {
@@ -152,9 +152,9 @@ template <typename KV> struct PvOf { typedef KV type; };
 template <> struct PvOf<E4M3> { typedef F16 type; };
 
 // visible tokens of a request
-__device__ __forceinline__ int visible(const PoolParams& p, int b, int& len) {
+__device__ __forceinline__ int visible(const PoolParams& p, int b, int& len, int& req) {
   len = p.b_len[b];
-  const int req = p.b_req[b];
+  req = p.b_req[b];
   if (len > p.max_seq_len) len = (int)p.max_seq_len;
   if (len < 0 || req < 0 || req >= p.num_reqs) len = 0;
   if (!p.window) return len;
@@ -191,7 +191,7 @@ template <typename QT, typename KV, int D> struct Walk {
   int sinks, skip, limit;
 
   // a task = one KV head and up to eight query heads of its group
-  __device__ __forceinline__ void start(int b, int task, int len, int n_vis) {
+  __device__ __forceinline__ void start(int b, int req, int task, int len, int n_vis) {
     const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
     const int h0 = kvh * p.group + sg * kHeads;
     const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
@@ -210,7 +210,7 @@ template <typename QT, typename KV, int D> struct Walk {
       s_s0 = (uint32_t)(lane < 32 ? p.ks_s0 : p.vs_s0);
     }
     row_s0 = (uint32_t)(lane < 32 ? p.k_s0 : p.v_s0);
-    row = p.table + (int64_t)p.b_req[b] * p.max_seq_len;
+    row = p.table + (int64_t)req * p.max_seq_len;
     sinks = p.window ? p.sinks : 0;
     skip = len - n_vis;
     m = -INFINITY, l = 0.f;
@@ -248,7 +248,8 @@ template <typename QT, typename KV, int D> struct Walk {
 #pragma unroll
     for (int i = 0; i < 4; i++) *(u32x4*)(voff + 2 * i) = *(const u32x4*)(lds + kVOff + (i >> 1) * 128 + 32 * g + (i & 1) * 16);
     __builtin_amdgcn_wave_barrier();
-    // (the empty statements keep each 64-bit address next to its load instead of ten of them live at once)
+    // Rows are read once and loaded so (nontemporal): on a pool that no cache holds yet a fifth to a quarter faster in 16 bits (64 requests behind a window of 4096,
+    // 1.1 GB: 185 us, 235 without), 6 - 30 % in 8.  (the empty statements keep each 64-bit address next to its load instead of ten of them live at once)
 #pragma unroll
     for (int i = 0; i < KI; i++) {
       asm volatile("" : "+v"(koff[i]));
@@ -430,11 +431,10 @@ __device__ __forceinline__ void store_elem4(char* o, int dtype, int64_t at, cons
 }
 __device__ __forceinline__ float ln_of(float m, float l) { return l > 0.f ? (m + __builtin_amdgcn_logf(l)) * kLn2 : (l == l ? -INFINITY : l); }
 
-
-
-// One workgroup per (task, request): its NW waves take every NW-th block and meet in LDS.
+// One workgroup per (task, request): its NW waves take every NW-th block and meet in LDS.  Four of them, so that two or three workgroups fill a CU (8 bits, 256
+// requests of 512 tokens, 277 MB: 73 us, 86 with eight waves; a lone request of 512 as well, 8.4 and 9.9).
 template <typename QT, typename KV, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void pool_decode_direct_kernel(PoolParams p) {
+__global__ __launch_bounds__(NW * 64, (D == 128 && !__is_same(KV, E4M3) ? 2 : 3)) void pool_decode_direct_kernel(PoolParams p) {
   constexpr int ROW = D + 4;  // floats per head in LDS: O, maximum, sum (and a bank's shift)
   __shared__ __attribute__((aligned(16))) char lds[NW * (kHeads * ROW * 4 > kWaveLds<KV, D> ? kHeads * ROW * 4 : kWaveLds<KV, D>)];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -442,11 +442,11 @@ __global__ __launch_bounds__(NW * 64) void pool_decode_direct_kernel(PoolParams 
   const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
   const int h0 = kvh * p.group + sg * kHeads;
   const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
-  int len;
-  const int n_vis = visible(p, b, len);
+  int len, req;
+  const int n_vis = visible(p, b, len, req);
   Walk<QT, KV, D> w(p, lds + wave * kWaveLds<KV, D>);
   if (wave * kBlock < n_vis) {
-    w.start(b, task, len, n_vis);
+    w.start(b, req, task, len, n_vis);
     w.run(wave * kBlock, n_vis, NW);
     w.join();
   } else {
@@ -489,79 +489,70 @@ __global__ __launch_bounds__(NW * 64) void pool_decode_direct_kernel(PoolParams 
   }
 }
 
-// How the blocks of all requests are dealt: the units of request b are [first, first + n) of all.  Every wave counts them by itself, 64 requests a step.
-struct Deal {
-  int64_t total;
-  int per_share;
-};
-__device__ __forceinline__ int units_of(const PoolParams& p, int b) {
-  int len;
-  return b < p.batch ? (visible(p, b, len) + kBlock - 1) / kBlock : 0;
-}
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+// How the blocks of all requests are dealt: numbered request by request, per_share to a share.  Every wave counts them by itself, 64 requests at a
+// time, of which a lane has one each; up to 64 requests are one look at their lengths.
+struct Requests {
+  int first_request, len, req, n_vis, units, up_to;  // up_to: units of the 64 up to the lane's request
+  __device__ __forceinline__ void look(const PoolParams& p, int b0) {
+    const int lane = threadIdx.x & 63;
+    first_request = b0;
+    n_vis = 0;
+    if (b0 + lane < p.batch) n_vis = visible(p, b0 + lane, len, req);
+    units = (n_vis + kBlock - 1) / kBlock;
+    up_to = units;
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-  return v;
-}
-__device__ __forceinline__ Deal deal(const PoolParams& p) {
-  const int lane = threadIdx.x & 63;
-  int64_t n = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) n += units_of(p, b0 + lane);
-  Deal d;
-  d.total = wave_sum(n);
-  const int64_t per = (d.total + p.shares - 1) / p.shares;
-  d.per_share = (int)(per < p.min_units ? p.min_units : per);
-  return d;
+    for (int d = 1; d < 64; d <<= 1) {
+      const int below = __shfl_up(up_to, d, 64);
+      if (lane >= d) up_to += below;
+    }
+  }
+  __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(up_to, 63); }
+};
+__device__ __forceinline__ int per_share_of(const PoolParams& p, int total) {
+  const int per = (int)div_by((uint32_t)(total + p.shares - 1), p.by_shares);
+  return per < p.min_units ? p.min_units : per;
 }
 
 // Four waves per workgroup, each with a share of its own of one task; the tasks of a share are neighbours, on one XCD.
 template <typename QT, typename KV, int D>
 __global__ __launch_bounds__(256, (D == 128 && !__is_same(KV, E4M3) ? 2 : 3)) void pool_decode_shares_kernel(PoolParams p) {
   __shared__ __attribute__((aligned(16))) char lds[4 * kWaveLds<KV, D>];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (ids go to the XCDs round-robin; gridDim.x is a multiple of 8)
   const uint32_t id = (blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3);
   const uint32_t unit = id * 4 + wave;
   const int share = (int)div_by(unit, p.by_tasks), task = (int)(unit - (uint32_t)share * p.tasks);
   if (share >= p.shares) return;
-  const Deal dl = deal(p);
-  int64_t at = (int64_t)share * dl.per_share;
-  const int64_t end = at + dl.per_share < dl.total ? at + dl.per_share : dl.total;
-  if (at >= end) return;
-  // the request of the share's first unit
-  int b = 0;
-  int64_t first = 0;
-  for (int b0 = 0;; b0 += 64) {  // (at < total: found before the batch ends)
-    int64_t incl = units_of(p, b0 + lane);
-    const int64_t mine = incl;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t below = __shfl_up(incl, d, 64);
-      if (lane >= d) incl += below;
-    }
-    const int64_t chunk = __shfl(incl, 63, 64);
-    if (at < first + chunk) {
-      const int l0 = __builtin_ctzll(__builtin_amdgcn_ballot_w64(first + incl > at));
-      b = __builtin_amdgcn_readfirstlane(b0 + l0);
-      first += __shfl(incl - mine, l0, 64);
-      break;
-    }
-    first += chunk;
+  Requests rs;
+  rs.look(p, 0);
+  int total = rs.all();
+  if (p.batch > 64) {
+    for (int b0 = 64; b0 < p.batch; b0 += 64) rs.look(p, b0), total += rs.all();
+    rs.look(p, 0);
   }
+  const int per_share = per_share_of(p, total);
+  int at = share * per_share;  // (up to shares - 1 more than there are units)
+  const int end = total - at < per_share ? total : at + per_share;
+  if (at >= end) return;
+  // the request of the share's first unit (at < total: found before the batch ends)
+  int first = 0;
+  while (at >= first + rs.all()) {
+    first += rs.all();
+    rs.look(p, rs.first_request + 64);
+  }
+  int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(first + rs.up_to > at));
+  first += __builtin_amdgcn_readlane(rs.up_to, l) - __builtin_amdgcn_readlane(rs.units, l);
   Walk<QT, KV, D> w(p, lds + wave * kWaveLds<KV, D>);
   const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
   const int h0 = kvh * p.group + sg * kHeads;
   const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
-  for (; at < end && b < p.batch; b++) {
-    int len;
-    const int n_vis = __builtin_amdgcn_readfirstlane(visible(p, b, len));
-    len = __builtin_amdgcn_readfirstlane(len);
-    const int64_t units = (n_vis + kBlock - 1) / kBlock;
-    const int64_t to = first + units < end ? first + units : end;
+  for (;;) {
+    const int b = rs.first_request + l, units = __builtin_amdgcn_readlane(rs.units, l), n_vis = __builtin_amdgcn_readlane(rs.n_vis, l);
+    const int to = end - first < units ? end : first + units;
     if (to > at) {
-      w.start(b, task, len, n_vis);
-      const int64_t last = (to - first) * kBlock;
-      w.run((int)(at - first) * kBlock, (int)(last < n_vis ? last : n_vis), 1);
+      w.start(b, __builtin_amdgcn_readlane(rs.req, l), task, __builtin_amdgcn_readlane(rs.len, l), n_vis);
+      const int last = (to - first) * kBlock;
+      w.run((at - first) * kBlock, last < n_vis ? last : n_vis, 1);
       w.join();
       if (w.c < nh) {
         const int64_t r0 = ((int64_t)(share + b) * p.hq + h0 + w.c);
@@ -576,26 +567,35 @@ __global__ __launch_bounds__(256, (D == 128 && !__is_same(KV, E4M3) ? 2 : 3)) vo
       }
       at = to;
     }
+    if (at >= end) return;
     first += units;
+    if (++l == 64) rs.look(p, rs.first_request + 64), l = 0;
   }
 }
 
 // o = sum of a request's partials by their log-sum-exps: first the weights of all of them, by all threads, into LDS, then the rows, whose loads wait for nothing.
-// D / 4 lanes read a row, the rows are dealt to the rest of the workgroup.
+// W lanes read W * 4 elements of a row, the rows are dealt to the rest of the workgroup; D / 4 / W workgroups share a head (few requests: a lone workgroup draws 350
+// rows in 9 us).
 constexpr int kMaxShares = 12 * (int)kCUs;
-template <int D>
+template <int D, int W>
 __global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
-  constexpr int LPR = D / 4, SL = 256 / LPR;
-  __shared__ __attribute__((aligned(16))) float acc[SL][D];
+  constexpr int SL = 256 / W;
+  __shared__ __attribute__((aligned(16))) float acc[SL][W * 4];
   __shared__ float weight[kMaxShares], part[8];
   const int h = blockIdx.x, b = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const Deal dl = deal(p);
-  int64_t first = 0;
-  for (int b0 = 0; b0 < b; b0 += 64) first += b0 + lane < b ? units_of(p, b0 + lane) : 0;
-  first = wave_sum(first);
-  const int64_t units = units_of(p, b);
-  const int s0 = (int)(first / dl.per_share), n = units ? (int)((first + units - 1) / dl.per_share) - s0 + 1 : 0;
+  Requests rs;
+  int total = 0, first = 0, units = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    rs.look(p, b0);
+    if (b >= b0 && b < b0 + 64) {
+      units = __builtin_amdgcn_readlane(rs.units, b - b0);
+      first = total + __builtin_amdgcn_readlane(rs.up_to, b - b0) - units;
+    }
+    total += rs.all();
+  }
+  const uint32_t per_share = (uint32_t)per_share_of(p, total);
+  const int s0 = (int)((uint32_t)first / per_share), n = units ? (int)((uint32_t)(first + units - 1) / per_share) - s0 + 1 : 0;
   const float* lse = p.part_lse + ((int64_t)(s0 + b) * p.hq + h);
   float M = -INFINITY;
   for (int i = threadIdx.x; i < n; i += 256) {
@@ -619,8 +619,8 @@ __global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
   if (lane == 0) part[4 + wave] = L;
   __syncthreads();
   L = (part[4] + part[5]) + (part[6] + part[7]);
-  const int slice = threadIdx.x / LPR, d = (threadIdx.x & (LPR - 1)) * 4;
-  const float* row = p.part_o + ((int64_t)(s0 + b) * p.hq + h) * D + d;
+  const int slice = threadIdx.x / W, d = (threadIdx.x & (W - 1)) * 4, d0 = (int)blockIdx.z * W * 4;
+  const float* row = p.part_o + ((int64_t)(s0 + b) * p.hq + h) * D + d0 + d;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 8
   for (int i = slice; i < n; i += SL) {
@@ -630,23 +630,28 @@ __global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
   *(f32x4*)&acc[slice][d] = sum;
   __syncthreads();
   if (slice) return;
-#pragma unroll
+#pragma unroll 8
   for (int i = 1; i < SL; i++) sum += *(const f32x4*)&acc[i][d];
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int64_t at = (int64_t)b * p.hq + h;
-  store_elem4(p.o, p.o_dtype, at * D + d, sum * inv);
-  if (d == 0) p.lse[at] = ln_of(M, L);
+  store_elem4(p.o, p.o_dtype, at * D + d0 + d, sum * inv);
+  if (d0 + d == 0) p.lse[at] = ln_of(M, L);
 }
 
-constexpr int kDirectWaves = 8;
-constexpr int64_t kDirectTokens = 1024;  // visible tokens of the longest request up to which a workgroup takes a whole (request, KV head)
+constexpr int kDirectWaves = 4;
+// A workgroup takes a whole (request, KV head) where the longest request's visible tokens are few for the workgroups there are: 32 / 8 heads of 128, cold, against
+// shares: 1 request of 512 tokens 8.4 us (12.6), of 1024 14.1 (12.8); 16 of 1024 14.9 (20.2); 32 of 2048 34 (48); 16 of 2048 35 (34).
+constexpr int64_t kDirectTokens = 512;
 // Waves that a launch of shares deals to: those that are on the chip at once (registers), so that none starts late
 int64_t share_waves(bool k8, int64_t head_dim) { return (head_dim == 128 && !k8 ? 8 : 12) * kCUs; }
 constexpr int64_t kMinUnits = 2;
 
 int64_t most_visible(int64_t max_len, int64_t window, int64_t sinks) { return window > 0 && window + sinks < max_len ? window + sinks : max_len; }
 int64_t tasks_of(int64_t hq, int64_t hkv) { return hkv * ((hq / hkv + kHeads - 1) / kHeads); }
-bool is_direct(int64_t batch, int64_t tasks, int64_t most) { return most <= kDirectTokens || (batch * tasks >= kCUs && most <= 2 * kDirectTokens); }
+bool is_direct(int64_t batch, int64_t tasks, int64_t most) {
+  const int64_t wgs = batch * tasks;
+  return most <= kDirectTokens * (wgs >= kCUs ? 4 : wgs >= kCUs / 4 ? 2 : 1);
+}
 // shares of a launch that is not direct
 int64_t shares_of(int64_t waves, int64_t batch, int64_t tasks, int64_t most) {
   const int64_t units = batch * ((most + kBlock - 1) / kBlock);
@@ -663,7 +668,8 @@ template <typename QT, typename KV, int D> void launch(const PoolParams& p, bool
   const int64_t wgs = ((int64_t)p.shares * p.tasks + 3) / 4;
   LSATTN_LAUNCH_KERNEL((pool_decode_shares_kernel<QT, KV, D>), dim3((unsigned)((wgs + 7) / 8 * 8)), dim3(256), 0, st, p);
   if (hipPeekAtLastError() != hipSuccess) return;
-  LSATTN_LAUNCH_KERNEL((pool_decode_merge_kernel<D>), dim3(p.hq, p.batch), dim3(256), 0, st, p);
+  if ((int64_t)p.hq * p.batch <= kCUs / 2) LSATTN_LAUNCH_KERNEL((pool_decode_merge_kernel<D, 8>), dim3(p.hq, p.batch, D / 32), dim3(256), 0, st, p);
+  else LSATTN_LAUNCH_KERNEL((pool_decode_merge_kernel<D, D / 4>), dim3(p.hq, p.batch), dim3(256), 0, st, p);
 }
 template <typename QT, typename KV> void launch_d(const PoolParams& p, int64_t d, bool direct, hipStream_t st) {
   if (d == 128) launch<QT, KV, 128>(p, direct, st);
@@ -702,7 +708,7 @@ extern "C" int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* 
   auto slot_stride = [](int64_t bytes) { return bytes >= 0 && bytes <= 0x7fffffff; };
   if (!slot_stride(a->k_stride_0 * es) || !slot_stride(a->v_stride_0 * es) || (k8 && (!slot_stride(a->ks_stride_0) || !slot_stride(a->vs_stride_0))))
     return LSATTN_ERR_INVALID_ARG;
-  if (a->batch > 65535 || a->num_q_heads > 65535 || a->max_seq_len > 0x7fffff00 || a->num_slots > 0x7fffffff || a->num_reqs > 0x7fffffff ||
+  if (a->batch > 65535 || a->num_q_heads > 65535 || a->max_seq_len > 0x7fff0000 || a->num_slots > 0x7fffffff || a->num_reqs > 0x7fffffff ||
       a->max_len_in_batch > 0x7fffffff)
     return LSATTN_ERR_INVALID_ARG;
   if (!(a->sm_scale > 0.f)) return LSATTN_ERR_INVALID_ARG;
@@ -724,12 +730,13 @@ extern "C" int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* 
   p.by_tasks = fast_div((uint32_t)p.tasks), p.by_sub = fast_div((uint32_t)p.sub_groups);
   const int64_t most = most_visible(a->max_len_in_batch, a->window, a->sinks);
   const bool direct = is_direct(p.batch, p.tasks, most);
-  p.part_o = nullptr, p.part_lse = nullptr, p.shares = 1, p.min_units = (int32_t)kMinUnits;
+  p.part_o = nullptr, p.part_lse = nullptr, p.shares = 1, p.by_shares = fast_div(1), p.min_units = (int32_t)kMinUnits;
   if (!direct) {
     const int64_t shares = shares_of(share_waves(k8, a->head_dim), p.batch, p.tasks, most), rows = shares + p.batch;
     if (!a->workspace || a->workspace_bytes < (size_t)(rows * p.hq * (a->head_dim + 1) * 4)) return LSATTN_ERR_WORKSPACE;
     if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
-    p.shares = (int32_t)shares;
+    p.shares = (int32_t)shares, p.by_shares = fast_div((uint32_t)shares);
+    if (a->batch * ((a->max_seq_len + kBlock - 1) / kBlock) > kMaxUnits - kMaxShares) return LSATTN_ERR_INVALID_ARG;  // (blocks are numbered with 31 bits)
     p.part_o = (float*)a->workspace, p.part_lse = p.part_o + rows * p.hq * a->head_dim;
   }
   hipStream_t st = (hipStream_t)stream;
