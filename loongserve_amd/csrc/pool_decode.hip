@@ -641,7 +641,6 @@ __global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
 constexpr int kDirectWaves = 4;
 // A workgroup takes a whole (request, KV head) where the longest request's visible tokens are few for the workgroups there are: 32 / 8 heads of 128, cold, against
 // shares: 1 request of 512 tokens 8.4 us (12.6), of 1024 14.1 (12.8); 16 of 1024 14.9 (20.2); 32 of 2048 34 (48); 16 of 2048 35 (34).
-constexpr int64_t kDirectTokens = 512;
 // Waves that a launch of shares deals to: those that are on the chip at once (registers), so that none starts late
 int64_t share_waves(bool k8, int64_t head_dim) { return (head_dim == 128 && !k8 ? 8 : 12) * kCUs; }
 constexpr int64_t kMinUnits = 2;
@@ -650,7 +649,7 @@ int64_t most_visible(int64_t max_len, int64_t window, int64_t sinks) { return wi
 int64_t tasks_of(int64_t hq, int64_t hkv) { return hkv * ((hq / hkv + kHeads - 1) / kHeads); }
 bool is_direct(int64_t batch, int64_t tasks, int64_t most) {
   const int64_t wgs = batch * tasks;
-  return most <= kDirectTokens * (wgs >= kCUs ? 4 : wgs >= kCUs / 4 ? 2 : 1);
+  return most <= (wgs >= kCUs ? 2048 : wgs >= kCUs / 4 ? 1024 : 768);
 }
 // shares of a launch that is not direct
 int64_t shares_of(int64_t waves, int64_t batch, int64_t tasks, int64_t most) {

@@ -459,12 +459,12 @@ def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_g
     o has q's type, or is float32 (a partial: with lse, the steps over several KV chunks join by lse_merge); lse, the natural
     log-sum-exp, float32 [tokens, q_heads], is optional.  Rows that see no key get o = 0, lse = -inf; rows that no
     request names stay as they were.  A chunk of a longer prompt brings its context in k and v (kv_gather_fp8 reads one back
-    from an 8-bit pool) and the position of its first query in q_first_token_global_idx.  total_q_len: as in
-    context_attention_fwd.  A bfloat16 v is multiplied as float16: magnitudes past 65504 count as 65504.  V rows of keys near
+    from an 8-bit pool) and the position of its first query in q_first_token_global_idx.  Requests share no
+    rows of q: total_q_len, an upper bound of all their lengths together, is q's rows unless given.  A bfloat16 v is multiplied as float16: magnitudes past 65504 count as 65504.  V rows of keys near
     a window that a query does not see are multiplied by a weight of zero: they have to be finite (K rows may hold anything)."""
     if window is not None and _native.window_attention(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx, kv_b_start_loc, kv_b_seq_len,
                                                        kv_first_token_global_idx, logical_sp_peers_num, max_q_b_seq_len, window, sinks, lse,
-                                                       0 if total_q_len is None else total_q_len, PRECONVERT_BF16_V):
+                                                       q.shape[0] if total_q_len is None else total_q_len, PRECONVERT_BF16_V):
         return
     for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")):
         _dev(t, n)
