@@ -148,7 +148,7 @@ template <int D, int WP, bool DV, bool WIN> constexpr int kResident = D == 128 ?
 // from the empty state.
 template <typename T, int D, int MODE, bool DV, int WP, int KP = 1, bool WIN = false>
 __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV, WIN>)) void prefill_small_kernel(SmallParams p) {
-  static_assert(WIN ? KP == 1 && (MODE == 0 || MODE == 3) : MODE < 3, "a window knows no state");
+  static_assert(WIN ? MODE == 0 || MODE == 3 : MODE < 3, "a window knows no state");
   static_assert(KP == 1 || (KP == 2 && WP == 16 && D >= 32), "the parts of a tile of 64 keys, the columns that each of two waves finishes");
   constexpr int NW = kWaves * KP;
   constexpr int QB = WP / 16;               // blocks of 16 positions per wave
@@ -569,15 +569,15 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV, WIN>)) void
     }
     if (MODE == 3) {
       const float f = seen ? fix * (1.f / l_tot) : 0.f;
-      uint16_t* orow = (uint16_t*)p.o + tok * p.o_st + (int64_t)h * p.o_sh + 4 * g_e;
+      uint16_t* orow = (uint16_t*)p.o + tok * p.o_st + (int64_t)h * p.o_sh + col0 + 4 * g_e;
 #pragma unroll
-      for (int db = 0; db < NDB; db++) {
+      for (int db = 0; db < EDB; db++) {
         const f32x4 x = oacc[qb][db] * f;
         const u32x2 res = u32x2{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
         if (TURNED) *(u32x2*)(o_lds + o_chunk(16 * qb + c_e, 2 * db + (g_e >> 1)) + (g_e & 1) * 8) = res;
         else if (here) *(u32x2*)(orow + 16 * db) = res;
       }
-      if (here && g_e == 0 && p.lse) p.lse[tok * p.hq + h] = seen ? (m_run[qb] + __builtin_amdgcn_logf(l_tot)) * kLn2 : -INFINITY;
+      if (here && g_e == 0 && kp == 0 && p.lse) p.lse[tok * p.hq + h] = seen ? (m_run[qb] + __builtin_amdgcn_logf(l_tot)) * kLn2 : -INFINITY;
     }
     if (MODE == 1) {
       // the reference's update of (o, m, l); a row in its start state (m = -inf, l = 0) may hold anything in o
@@ -964,8 +964,21 @@ SmallParams params_of(const lsattn_prefill_args* a) {
 }
 
 // A step behind a window: 32 positions per wave, or 16 where those make fewer than three workgroups per CU.
+// Two waves share a wave's positions behind a window as well, up to a workgroup per CU: microseconds, one wave each | two; 128-wide heads: 100 tokens 32/8
+// behind 64 6.5 | 6.8, 300 behind 256 10.4 | 10.0, 1024 8/1 behind 512 16.3 | 15.0, 2048 behind 1024 25.2 | 22.5, bf16 28.8 | 25.2; 64-wide 19.6 | 18.0;
+// but 777 tokens 32/8 (1.5 workgroups per CU) behind 512 18.1 | 19.2, 1024 18.8 | 25.3.
+bool two_waves_share_window(const lsattn_prefill_args* a, int pack_shift, int64_t window) {
+  int64_t keys = a->total_kv_rows / a->batch;
+  if (a->total_kv_rows <= 0) keys = window;
+  if (keys < a->max_q_len) keys = a->max_q_len;
+  return workgroups(a, pack_shift, 1) <= kCUs && (keys < window ? keys : window) >= 256;
+}
 template <typename T, int D, int MODE, bool DV> int launch_window_rows(const SmallParams& p, const lsattn_prefill_args* a, hipStream_t st) {
-  if (workgroups(a, p.pack_shift, 2) < 3 * kCUs) return launch_rows<T, D, MODE, DV, 16, 1, true>(p, a, st);
+  if (workgroups(a, p.pack_shift, 2) < 3 * kCUs) {
+    if constexpr (D >= 64)
+      if (two_waves_share_window(a, p.pack_shift, p.window)) return launch_rows<T, D, MODE, DV, 16, 2, true>(p, a, st);
+    return launch_rows<T, D, MODE, DV, 16, 1, true>(p, a, st);
+  }
   return launch_rows<T, D, MODE, DV, 32, 1, true>(p, a, st);
 }
 template <typename T, int MODE, bool DV> int launch_window_d(const SmallParams& p, const lsattn_prefill_args* a, hipStream_t st) {

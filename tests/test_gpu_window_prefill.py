@@ -262,3 +262,17 @@ def test_scores_of_keys_that_are_not_seen_do_not_matter(lsa, rows):
     late.kv[ks + 2:ks + 151, 1] = math.nan
     got = late.run(lsa, 50, 2)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("window,sinks", [(256, 0), (300, 70), (1 << 40, 0)])
+def test_waves_that_share_positions(lsa, dtype, D, window, sinks):
+    """Launches of a workgroup per CU and less, two waves to a wave's positions: rows whose keys all lie in one wave's part, rows of none, a window that
+    starts inside a part, lengths of zero and one."""
+    s = Step([(301, 0, 301, 0), (1, 0, 1, 0), (0, 0, 0, 0), (17, 0, 17, 0), (40, 610, 650, 0), (33, 5, 20, 20), (9, 900, 400, 0)], 6, 2, D, DT[dtype], seed=12)
+    s.kv[:, :2] *= torch.linspace(0.2, 3.0, s.kv.shape[0])[:, None, None].to(DT[dtype])
+    s.check(s.run(lsa, window, sinks), window, sinks)
+    s.check(s.run(lsa, window, sinks, o_dtype=torch.float32), window, sinks)
+    s.check(s.run(lsa, window, sinks, lse=False), window, sinks)
