@@ -80,7 +80,7 @@ struct Read8Params {
   int64_t pool_s0, pool_s1;
   const uint8_t* scales;
   int64_t sc_s0, sc_s1;
-  int64_t num_slots, num_reqs, max_seq_len, out_rows;
+  int64_t num_slots, num_reqs, max_seq_len, out_rows, max_len;
   const int32_t* req_to_tokens;
   const int32_t* b_req_idx;
   const int32_t* b_first;
@@ -105,7 +105,8 @@ template <typename T, int D>
 __global__ __launch_bounds__(256) void kv_gather_fp8_kernel(Read8Params p) {
   constexpr uint32_t LPR = D / 16;
   const int64_t b = blockIdx.y;
-  const int32_t len = p.b_seq_len[b], first = p.b_first ? p.b_first[b] : 0, req = p.b_req_idx[b];
+  const int64_t len = p.b_seq_len[b] < p.max_len ? p.b_seq_len[b] : p.max_len;
+  const int32_t first = p.b_first ? p.b_first[b] : 0, req = p.b_req_idx[b];
   const int64_t start = p.b_start_loc[b];
   const uint32_t rw = div_by(threadIdx.x, p.by_parts);
   // a workgroup takes rows_per_wg whole rows at a time where these have at most 256 pieces; longer rows take several steps
@@ -208,7 +209,7 @@ extern "C" int lsattn_kv_gather_fp8(const lsattn_kv_gather_fp8_args* a, void* st
   Read8Params p;
   p.pool = (const char*)a->pool, p.pool_s0 = a->pool_stride_0, p.pool_s1 = a->pool_stride_1;
   p.scales = a->scales, p.sc_s0 = a->scale_stride_0, p.sc_s1 = a->scale_stride_1;
-  p.num_slots = a->num_slots, p.num_reqs = a->num_reqs, p.max_seq_len = a->max_seq_len, p.out_rows = a->out_rows;
+  p.num_slots = a->num_slots, p.num_reqs = a->num_reqs, p.max_seq_len = a->max_seq_len, p.out_rows = a->out_rows, p.max_len = a->max_len_in_batch;
   p.req_to_tokens = a->req_to_tokens, p.b_req_idx = a->b_req_idx, p.b_first = a->b_first, p.b_seq_len = a->b_seq_len;
   p.b_start_loc = a->b_start_loc;
   p.out = (char*)a->out, p.out_st = a->out_stride_t * 2, p.out_sh = a->out_stride_h * 2;

@@ -223,6 +223,19 @@ def test_read_back_of_values_past_fp16_and_outside_the_buffers(lsa):
     assert (big[0] == 5).all() and big[1, 0, 0] == 65536 and big[3, 0, 0] == 65536
 
 
+@pytest.mark.gpu
+def test_read_back_stops_at_the_longest_length_given(lsa):
+    """A request longer than the bound: the rows behind it stay as they were, also those that the last workgroup could reach."""
+    for H, D in ((1, 16), (3, 64), (40, 128)):
+        pool, sc = torch.zeros(40, H, D, device="cuda").to(F8), torch.full((40, H), 127, dtype=torch.uint8, device="cuda")
+        out = torch.full((40, H, D), 5.0, dtype=torch.float16, device="cuda")
+        i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        lsa.kv_gather_fp8(pool, sc, torch.arange(40, dtype=torch.int32, device="cuda").view(1, 40), i(0, 0), i(30, 2), i(0, 20), 7, out)
+        want = torch.full((40, H, D), 5.0, dtype=torch.float16)
+        want[:7] = want[20:22] = 0
+        assert torch.equal(out.cpu(), want)
+
+
 # ------------------------------------------------------------------------------------------------ decode
 KINDS = {"f16": (torch.float16, None), "bf16": (torch.bfloat16, None), "e4m3-f16": (torch.float16, F8), "e4m3-bf16": (torch.bfloat16, F8)}
 
