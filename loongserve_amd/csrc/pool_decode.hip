@@ -645,7 +645,7 @@ constexpr int kDirectWaves = 4;
 int64_t share_waves(bool k8, int64_t head_dim) { return (head_dim == 128 && !k8 ? 8 : 12) * kCUs; }
 constexpr int64_t kMinUnits = 2;
 
-int64_t most_visible(int64_t max_len, int64_t window, int64_t sinks) { return window > 0 && window + sinks < max_len ? window + sinks : max_len; }
+int64_t most_visible(int64_t max_len, int64_t window, int64_t sinks) { return window > 0 && window < max_len && sinks < max_len - window ? window + sinks : max_len; }
 int64_t tasks_of(int64_t hq, int64_t hkv) { return hkv * ((hq / hkv + kHeads - 1) / kHeads); }
 bool is_direct(int64_t batch, int64_t tasks, int64_t most) {
   const int64_t wgs = batch * tasks;
@@ -682,7 +682,8 @@ using namespace lsattn;
 
 extern "C" size_t lsattn_pool_attention_workspace_bytes(int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
                                                         int64_t max_len_in_batch, int64_t window, int64_t sinks) {
-  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 || max_len_in_batch <= 0 || window < 0 || sinks < 0)
+  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || head_dim <= 0 || max_len_in_batch <= 0 || window < 0 || sinks < 0 ||
+      batch > 65535 || num_q_heads > 65535 || max_len_in_batch > 0x7fffffff)  // (as the launch refuses)
     return 0;
   const int64_t tasks = tasks_of(num_q_heads, num_kv_heads), most = most_visible(max_len_in_batch, window, sinks);
   if (is_direct(batch, tasks, most)) return 0;

@@ -112,6 +112,7 @@ def test_library_refuses_what_it_cannot_run():
     assert attend(batch=2, max_len_in_batch=1 << 20) == -4  # (partials, and no workspace)
     size = lib.lsattn_pool_attention_workspace_bytes
     assert size(2, 4, 2, 128, 1 << 20, 0, 0) > 0 and size(2, 4, 2, 128, 1 << 20, 512, 4) == 0 and size(0, 4, 2, 128, 9, 0, 0) == 0
+    assert size(2, 4, 2, 128, 1 << 20, 2 ** 63 - 1, 9) == size(2, 4, 2, 128, 1 << 20, 9, 2 ** 63 - 1) == size(2, 4, 2, 128, 1 << 20, 0, 0)
 
 
 def test_python_operators_refuse_cpu_tensors():
@@ -343,6 +344,14 @@ def test_decode_outputs_in_16_bits_given_buffers_and_workspace(lsa, kind, lens):
     if need:
         with pytest.raises(ValueError, match="workspace"):
             c.run(lsa, workspace=ws[:need // 4 - 1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[70, 31], [9000]])
+def test_windows_as_wide_as_integers_go(lsa, lens):
+    c = Case("f16", len(lens), 4, 2, 128, lens, seed=8)
+    for window, sinks in ((2 ** 63 - 1, 5), (2 ** 63 - 1, 2 ** 63 - 1), (9, 2 ** 63 - 1), (2 ** 31 - 1, 2 ** 31 - 1)):
+        c.check(c.run(lsa, window, sinks))
 
 
 @pytest.mark.gpu
