@@ -187,7 +187,7 @@ at::Tensor empty(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType s
 // q, k, v, six int32 vectors, peers, max_q_len: the arguments both prefill operators share
 struct Step {
   lsattn_prefill_args p;
-  const at::Tensor *q, *k, *v, *q_start, *q_len;
+  const at::Tensor *q, *k, *v, *q_start, *q_len, *vectors[6];
   at::Tensor v16;  // the fp16 copy of a bfloat16 V, alive until the launches are out
 
   bool read(Args& in, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_) {
@@ -203,6 +203,7 @@ struct Step {
     for (auto t : w)
       if (!i32(*t, B)) return false;
     q_start = w[0], q_len = w[1];
+    std::copy(w, w + 6, vectors);
     std::memset(&p, 0, sizeof p);
     p.q = q->data_ptr(), p.k = k->data_ptr(), p.v = v->data_ptr();
     p.q_stride_t = q->stride(0), p.q_stride_h = q->stride(1);
@@ -566,7 +567,7 @@ PyObject* window_attention(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const at::Tensor* lse = in.maybe();
   s.p.total_q_rows = in.integer();
   const bool preconvert = in.integer() != 0;
-  OR_NONE(in.ok && here({&q, &k, &v, &o, s.q_start, s.q_len, lse}) && window >= 1 && sinks >= 0 && s.p.total_q_rows >= 0 && s.p.sp_peers >= 1 && s.p.max_q_len >= 0);
+  OR_NONE(in.ok && here({&q, &k, &v, &o, s.vectors[0], s.vectors[1], s.vectors[2], s.vectors[3], s.vectors[4], s.vectors[5], lse}) && window >= 1 && sinks >= 0 && s.p.total_q_rows >= 0 && s.p.sp_peers >= 1 && s.p.max_q_len >= 0);
   if (lse) OR_NONE(is(*lse, at::kFloat) && lse->is_contiguous() && lse->dim() == 2 && lse->size(0) == q.size(0) && lse->size(1) == q.size(1));
   OR_NONE(q.numel() > 0 && k.numel() > 0);
   s.p.lse = lse ? (float*)lse->data_ptr() : nullptr;

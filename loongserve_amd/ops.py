@@ -468,7 +468,9 @@ def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_g
         return
     for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")):
         _dev(t, n)
-    _on_current_device(((q, "q"), (k, "k"), (v, "v"), (o, "o"), (q_b_start_loc, "q_b_start_loc"), (q_b_seq_len, "q_b_seq_len"), (lse, "lse")))
+    _on_current_device(((q, "q"), (k, "k"), (v, "v"), (o, "o"), (q_b_start_loc, "q_b_start_loc"), (q_b_seq_len, "q_b_seq_len"),
+                        (q_first_token_global_idx, "q_first_token_global_idx"), (kv_b_start_loc, "kv_b_start_loc"), (kv_b_seq_len, "kv_b_seq_len"),
+                        (kv_first_token_global_idx, "kv_first_token_global_idx"), (lse, "lse")))
     if window is None or int(window) < 1 or int(sinks) < 0:
         raise ValueError("window must be >= 1 (the position itself), sinks >= 0")
     if int(logical_sp_peers_num) < 1 or int(max_q_b_seq_len) < 0:
