@@ -187,7 +187,7 @@ at::Tensor empty(at::IntArrayRef sizes, const at::Tensor& like, at::ScalarType s
 // q, k, v, six int32 vectors, peers, max_q_len: the arguments both prefill operators share
 struct Step {
   lsattn_prefill_args p;
-  const at::Tensor *q, *k, *v, *q_start, *q_len, *vectors[6];
+  const at::Tensor *q, *k, *v, *vectors[6];
   at::Tensor v16;  // the fp16 copy of a bfloat16 V, alive until the launches are out
 
   bool read(Args& in, const at::Tensor& q_, const at::Tensor& k_, const at::Tensor& v_) {
@@ -202,7 +202,6 @@ struct Step {
     if (q->stride(2) != 1 || k->stride(2) != 1 || v->stride(2) != 1) return false;
     for (auto t : w)
       if (!i32(*t, B)) return false;
-    q_start = w[0], q_len = w[1];
     std::copy(w, w + 6, vectors);
     std::memset(&p, 0, sizeof p);
     p.q = q->data_ptr(), p.k = k->data_ptr(), p.v = v->data_ptr();
