@@ -1584,11 +1584,9 @@ extern "C" int lsattn_prefill_step_accumulate(const lsattn_prefill_args* a, void
 }
 
 // Whether a step behind a window runs in the 256-row shape: the more keys a workgroup walks the better it does (fewer reads of a key, more of its time
-// in iterations without a mask), and packed heads leave a workgroup fewer positions, so fewer keys that only some of its rows see.  Where the workgroups with eight
-// heads side by side just fill the chip, the other shape's smaller ones end later.  Measured (microseconds, this shape | the short prompts' kernel; fp16, 4 sinks):
+// in iterations without a mask), and packed heads leave a workgroup fewer positions, so fewer keys that only some of its rows see.  Measured (microseconds, this shape | the short prompts' kernel; fp16, 4 sinks):
 //   32768 tokens 32/8, windows of 512, 1024, 2048: 536 | 424, 798 | 666, 1235 | 1146; 8192 tokens, 4096: 416 | 403 (bf16 415 | 424); 8/1 32768, 4096: 521 | 532 (510 | 561);
 //   65536, 8192: 7313 | 7936; 32/32 32768, 2048: 1472 | 1260, 8192: 3788 | 4090, 8192 tokens, 4096: 469 | 424; 16 x 1024 32/8 254 | 182
-//   one round: 8192 tokens 8/1, 512 and 2048: 34.5 | 37.7, 80 | 90; but 2048 tokens 32/8, 1024: 51.8 | 45.6; 7 x 1500 8/1, 512, a little more than a round: 62 | 45
 // bfloat16 adds the copy of V here and a conversion per tile there, which moves none of these far.
 static bool window_in_256_rows(const lsattn_prefill_args* a, int32_t window) {
   if (a->head_dim != 128) return false;
@@ -1596,11 +1594,10 @@ static bool window_in_256_rows(const lsattn_prefill_args* a, int32_t window) {
   if (tn.prefill_rows) return tn.prefill_rows == LSATTN_PREFILL_ROWS_256;
   const int ps = pack_shift_for(a, false, tn);
   const int64_t wgs = (int64_t)a->batch * (a->num_q_heads >> ps) * ((a->max_q_len + (BM >> ps) - 1) / (BM >> ps));
-  const bool one_round = wgs >= kCUs - kCUs / 8 && wgs <= kCUs && ps > 2;
-  if (wgs < kCUs && !one_round) return false;
+  if (wgs < kCUs) return false;
   int64_t keys = window / (a->sp_peers > 1 ? a->sp_peers : 1);  // (the window's on this rank, at most what a request has in the mean)
   if (a->total_kv_rows > 0 && a->total_kv_rows / a->batch < keys) keys = a->total_kv_rows / a->batch;
-  return keys >= (one_round ? 512 : ps ? 4096 : 8192);
+  return keys >= (ps ? 4096 : 8192);
 }
 
 extern "C" int lsattn_prefill_window_converts_v(const lsattn_prefill_args* a, int64_t window) {

@@ -761,8 +761,8 @@ template <typename T, int D, int MODE, bool DV, int WP, int KP = 1, bool WIN = f
   const int64_t rows_wg = (kWaves * WP) >> p.pack_shift;
   Order order = WP == 32 ? order_of(a, p.pack_shift) : Order{p.batch, false};
   // Behind a window a request's tiles are all alike but the first ones and read K/V of their own, and a ragged batch goes one request after the other: that
-  // leaves no ids without work among those of the longest.  Windows of 1024, microseconds, in turn | the order above: 6 x 700..4000 32/8 226 | 279, 64/8
-  // 445 | 556, 5 x 700..7400 32/8 553 | 749, 24 x 50..1500 8/1 80 | 119; 32/32 within 3 %; 5 x 2000..6200 8/1 116 | 108.  Equal lengths: 8 x 4096 8/1 184 | 170.
+  // leaves no ids without work among those of the longest.  Windows of 1024, microseconds, in turn | the order above: 6 x 700..4000 32/8 190 | 228, 8/1
+  // 61 | 73, 64-wide 32/8 110 | 124, 5 x 700..7400 32/8 471 | 625, 24 x 50..1500 8/1 61 | 70; 32/32 and 64/8 within 3 %; 5 x 2000..6200 8/1 95 | 91, 4 x 300..1200 32/8 38 | 33.
   if (WIN && WP == 32 && ragged(a)) order = Order{1, false};
   p.bunch = (int32_t)order.bunch;
   p.d_bunch = fast_div((uint32_t)p.bunch);
@@ -969,9 +969,9 @@ SmallParams params_of(const lsattn_prefill_args* a) {
 }
 
 // A step behind a window: 32 positions per wave, or 16 where those make fewer than three workgroups per CU.
-// Two waves share a wave's positions behind a window as well, up to a workgroup per CU: microseconds, one wave each | two; 128-wide heads: 100 tokens 32/8
-// behind 64 6.5 | 6.8, 300 behind 256 10.4 | 10.0, 1024 8/1 behind 512 16.3 | 15.0, 2048 behind 1024 25.2 | 22.5, bf16 28.8 | 25.2; 64-wide 19.6 | 18.0;
-// but 777 tokens 32/8 (1.5 workgroups per CU) behind 512 18.1 | 19.2, 1024 18.8 | 25.3.
+// Two waves share a wave's positions behind a window as well, up to a workgroup per CU: microseconds, one wave each | two; 128-wide heads: 300 tokens
+// 32/8 behind 256 9.6 | 9.2, 1024 8/1 behind 512 14.8 | 13.0, 2048 behind 1024 22.6 | 19.2, bf16 25.9 | 21.7; 64-wide 17.2 | 15.1; with the maxima raised as often as elsewhere 100
+// tokens behind 64 were 6.5 | 6.8, and past a workgroup per CU (777 tokens 32/8) behind 512 18.1 | 19.2, 1024 behind 512 18.8 | 25.3.
 bool two_waves_share_window(const lsattn_prefill_args* a, int pack_shift, int64_t window) {
   int64_t keys = a->total_kv_rows / a->batch;
   if (a->total_kv_rows <= 0) keys = window;
@@ -979,7 +979,9 @@ bool two_waves_share_window(const lsattn_prefill_args* a, int pack_shift, int64_
   return workgroups(a, pack_shift, 1) <= kCUs && (keys < window ? keys : window) >= 256;
 }
 template <typename T, int D, int MODE, bool DV> int launch_window_rows(const SmallParams& p, const lsattn_prefill_args* a, hipStream_t st) {
-  if (workgroups(a, p.pack_shift, 2) < 3 * kCUs) {
+  // (128-wide heads fit two workgroups of 32 positions per wave on a CU; 32/8, microseconds, 16 | 32: 1300 tokens behind 512 and 1024 21.8 | 23.1, 25.1 | 33.4;
+  // 1500 26.9 | 23.9, 30.1 | 34.0; 1800 31.4 | 28.7, 40.2 | 35.3; 2300 38.5 | 31.4, 49.7 | 44.6; 8192 8/1 behind 1024 55.9 | 45.1; 64-wide 2300 28.4 | 32.4)
+  if (2 * workgroups(a, p.pack_shift, 2) < (D == 128 ? 3 : 6) * kCUs) {
     if constexpr (D >= 64)
       if (two_waves_share_window(a, p.pack_shift, p.window)) return launch_rows<T, D, MODE, DV, 16, 2, true>(p, a, st);
     return launch_rows<T, D, MODE, DV, 16, 1, true>(p, a, st);
