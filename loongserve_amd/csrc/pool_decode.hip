@@ -26,6 +26,8 @@
 // Short contexts and windows: the waves of one workgroup share a (request, KV head) and meet in LDS (one launch).  Otherwise the blocks of
 // all requests are dealt to the waves in equal shares, whatever the requests' lengths are (the host does not know them);
 // a wave leaves one partial per request it touches, and a second launch merges them.
+// Measured (32 / 8 heads of 128): 64 requests of 4096 .. 32768 tokens in 8 bits 420 us (5.75 TB/s; the loads alone 399), 96 behind a window of 16-bit rows 232
+// (6.15 TB/s); one request of 2047 tokens 10.8, of 131072 71.
 #include "common.hip.h"
 
 namespace lsattn {

@@ -477,3 +477,47 @@ def test_a_layer_over_the_8_bit_pool(lsa):
     again = lsa.longserve_fp8_decode_attention(qd, req.req_to_token_indexs, r, i(n), n, pool[:, :Hkv], pool[:, Hkv:], sc[:, :Hkv], sc[:, Hkv:], window=64, sinks=4)
     assert all(torch.equal(x, y) for x, y in zip(again, got))
     assert mem.kv_scales is not None and lsa.LongServeMemoryManager(8, torch.float16, 1, 16, 1).kv_scales is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", list(KINDS))
+@pytest.mark.parametrize("lens", [[0, 0, 0], [0, 0, 1]])
+def test_batches_without_tokens(lsa, kind, lens):
+    """Padded batches, in both launch forms (the bound only steers)."""
+    c = Case(kind, 3, 8, 2, 128, lens, seed=9)
+    for max_len in (0, 64, 1 << 17):
+        got = c.run(lsa, max_len=max_len)
+        c.check(got)
+        assert not got[0][:2].any() and (got[1][:2] == -math.inf).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [300, 9000])
+def test_slots_past_four_gigabytes(lsa, n):
+    """A pool whose last slots lie more than 2^32 bytes (8 bits) and 2^33 bytes (16 bits) behind its first."""
+    Hkv, D, slots = 8, 128, (1 << 21) + 12000  # 2 KB a slot in 8 bits
+    x = _rows((n, 2 * Hkv, D), 3, torch.float16)
+    where = (slots - 1 - torch.randperm(n, generator=torch.Generator().manual_seed(1))).to(torch.int32)
+    table = where.view(1, n).cuda()
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = _rows((1, 16, D), 4, torch.float16)
+    pool, sc = torch.empty(slots, 2 * Hkv, D, dtype=F8, device="cuda"), torch.empty(slots, 2 * Hkv, dtype=torch.uint8, device="cuda")
+    lsa.kv_scatter_fp8(x.cuda(), where.cuda(), pool, sc)
+    want, e = orc.quantise(x)
+    value = want * torch.pow(2.0, (e - 127).double())[..., None]
+    out = torch.empty(n, 2 * Hkv, D, dtype=torch.float16, device="cuda")
+    lsa.kv_gather_fp8(pool, sc, table, i(0), i(n), i(0), n, out)
+    assert torch.equal(out.cpu().double(), value.to(torch.float16).double())
+    near = torch.zeros(1, n, dtype=torch.int32)
+    near[0] = torch.arange(n)
+    for k8 in (True, False):
+        if k8:
+            got = lsa.longserve_fp8_decode_attention(q.cuda(), table, i(0), i(n), n, pool[:, :Hkv], pool[:, Hkv:], sc[:, :Hkv], sc[:, Hkv:])
+        else:
+            del pool
+            pool = torch.empty(slots, 2 * Hkv, D, dtype=torch.float16, device="cuda")
+            lsa.kv_scatter(x.cuda(), where.cuda(), pool)
+            got = lsa.longserve_window_decode_attention(q.cuda(), table, i(0), i(n), n, pool[:, :Hkv], pool[:, Hkv:], n, 0)
+        rows = value if k8 else x.double()
+        o, lse, tol_o, tol_l = orc.decode(q, rows[:, :Hkv], rows[:, Hkv:], near, torch.zeros(1, dtype=torch.int32), torch.tensor([n], dtype=torch.int32), None, 0)
+        assert ((got[0].cpu().double() - o).abs() <= tol_o + 1e-30).all() and ((got[1].cpu().double() - lse).abs() <= tol_l).all()
