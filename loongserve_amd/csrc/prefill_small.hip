@@ -131,7 +131,8 @@ __device__ __forceinline__ const char* uniform_ptr(const char* ptr) {
 // 128-wide heads, 32 positions per wave: three stages of 32 keys (48 KB) and at most 168 registers (158; 168 where V is bfloat16), so that three
 // workgroups fit a CU.
 // Behind a window (WIN) the compiler's registers do not fit those 168 (22 to 38 spills, 3.07 ms for 32768 tokens behind 4096 + 16, 32/8 heads; 2.30 with two workgroups per CU): two stages
-// of 64 keys there, operands and addresses in registers of their own (4096 tokens behind 1024, 32/32: 591 -> 642 TFLOP/s).
+// of 64 keys there, operands and addresses in registers of their own (4096 tokens behind 1024, 32/32: 591 -> 642 TFLOP/s; these figures
+// before the maxima had headroom, with it 725).
 template <int D, int WP, bool WIN> constexpr int kTileOf = D == 128 && WP == 32 && !WIN ? 32 : 64;
 template <int D, int WP, bool WIN> constexpr int kStagesOf = D == 128 && WP == 32 && !WIN ? 3 : 2;
 template <int D, int WP, bool DV, bool WIN> constexpr int kResident = D == 128 ? (WP == 32 && !WIN ? 3 : 2) : WP == 32 && D == 64 && !DV ? 3 : 4;
