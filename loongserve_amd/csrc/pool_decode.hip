@@ -26,8 +26,8 @@
 // Short contexts and windows: the waves of one workgroup share a (request, KV head) and meet in LDS (one launch).  Otherwise the blocks of
 // all requests are dealt to the waves in equal shares, whatever the requests' lengths are (the host does not know them);
 // a wave leaves one partial per request it touches, and a second launch merges them.
-// Measured (32 / 8 heads of 128): 64 requests of 4096 .. 32768 tokens in 8 bits 420 us (5.75 TB/s; the loads alone 399), 96 behind a window of 16-bit rows 232
-// (6.15 TB/s); one request of 2047 tokens 10.8, of 131072 71.
+// Measured (32 / 8 heads of 128): 64 requests of 4096 .. 32768 tokens in 8 bits 408 us (5.9 TB/s), 96 behind a window of 16-bit rows 231 (6.2 TB/s); one request of 2047
+// tokens 10.5, of 131072 55.
 #include "common.hip.h"
 
 namespace lsattn {
@@ -517,7 +517,7 @@ __device__ __forceinline__ int per_share_of(const PoolParams& p, int total) {
 
 // Four waves per workgroup, each with a share of its own of one task; the tasks of a share are neighbours, on one XCD.
 template <typename QT, typename KV, int D>
-__global__ __launch_bounds__(256, (D == 128 && !__is_same(KV, E4M3) ? 2 : 3)) void pool_decode_shares_kernel(PoolParams p) {
+__global__ __launch_bounds__(256, 2) void pool_decode_shares_kernel(PoolParams p) {
   __shared__ __attribute__((aligned(16))) char lds[4 * kWaveLds<KV, D>];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // (ids go to the XCDs round-robin; gridDim.x is a multiple of 8)
@@ -578,7 +578,7 @@ __global__ __launch_bounds__(256, (D == 128 && !__is_same(KV, E4M3) ? 2 : 3)) vo
 // o = sum of a request's partials by their log-sum-exps: first the weights of all of them, by all threads, into LDS, then the rows, whose loads wait for nothing.
 // W lanes read W * 4 elements of a row, the rows are dealt to the rest of the workgroup; D / 4 / W workgroups share a head (few requests: a lone workgroup draws 350
 // rows in 9 us).
-constexpr int kMaxShares = 12 * (int)kCUs;
+constexpr int kMaxShares = 4 * (int)kCUs;  // (kShareWaves)
 template <int D, int W>
 __global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
   constexpr int SL = 256 / W;
@@ -641,10 +641,13 @@ __global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
 }
 
 constexpr int kDirectWaves = 4;
-// A workgroup takes a whole (request, KV head) where the longest request's visible tokens are few for the workgroups there are: 32 / 8 heads of 128, cold, against
-// shares: 1 request of 512 tokens 8.4 us (12.6), of 1024 14.1 (12.8); 16 of 1024 14.9 (20.2); 32 of 2048 34 (48); 16 of 2048 35 (34).
-// Waves that a launch of shares deals to: those that are on the chip at once (registers), so that none starts late
-int64_t share_waves(bool k8, int64_t head_dim) { return (head_dim == 128 && !k8 ? 8 : 12) * kCUs; }
+// A workgroup takes a whole (request, KV head) where the longest request's visible tokens are few for the workgroups there are: 8 bits, 32 / 8 heads of 128, cold, against
+// shares (microseconds): 1 request of 512 tokens 8.4 (11.8), of 768 11.8 (11.5), of 1024 13.3 (11.6); 16 of 1024 15.6 (14.7), 32 of 1024 19.3 (23.1), of 2048 35.1 (34.7), 16 of
+// 2048 28.9 (21.9); 256 of 512 73 (89); 8 / 1 heads 64 of 1024 12.2 (15.1), 256 of 2048 31.8 (45.6); 32 / 32 32 of 2048 126 (113).
+// Waves that a launch of shares deals to: one per SIMD.  More leave shorter shares, whose starts and partials cost more than the loads in flight bring (microseconds, cold;
+// 4 | 8 in 16 bits, 12 in 8, of a CU's waves): 8 bits 1 request of 32768 27 | 36, 32 of 8192 116 | 131, 64 of 4096 .. 32768 469 | 482, 64-wide 84 | 96; 16 bits 8 behind
+// 8192 33.1 | 34.8, 128 678 | 689.  Numbers that leave the SIMDs of a CU with unequal counts lose a fifth: 3 134, 5 154, 6 139 for the 32.
+constexpr int64_t kShareWaves = 4 * kCUs;
 constexpr int64_t kMinUnits = 2;
 
 int64_t most_visible(int64_t max_len, int64_t window, int64_t sinks) { return window > 0 && window < max_len && sinks < max_len - window ? window + sinks : max_len; }
@@ -654,9 +657,9 @@ bool is_direct(int64_t batch, int64_t tasks, int64_t most) {
   return most <= (wgs >= kCUs ? 2048 : wgs >= kCUs / 4 ? 1024 : 768);
 }
 // shares of a launch that is not direct
-int64_t shares_of(int64_t waves, int64_t batch, int64_t tasks, int64_t most) {
+int64_t shares_of(int64_t batch, int64_t tasks, int64_t most) {
   const int64_t units = batch * ((most + kBlock - 1) / kBlock);
-  const int64_t by_waves = waves / tasks, by_units = (units + kMinUnits - 1) / kMinUnits;
+  const int64_t by_waves = kShareWaves / tasks, by_units = (units + kMinUnits - 1) / kMinUnits;
   const int64_t n = by_waves < by_units ? by_waves : by_units;
   return n < 1 ? 1 : n;
 }
@@ -689,7 +692,7 @@ extern "C" size_t lsattn_pool_attention_workspace_bytes(int64_t batch, int64_t n
     return 0;
   const int64_t tasks = tasks_of(num_q_heads, num_kv_heads), most = most_visible(max_len_in_batch, window, sinks);
   if (is_direct(batch, tasks, most)) return 0;
-  return (size_t)((shares_of(share_waves(true, head_dim), batch, tasks, most) + batch) * num_q_heads * (head_dim + 1) * 4);
+  return (size_t)((shares_of(batch, tasks, most) + batch) * num_q_heads * (head_dim + 1) * 4);
 }
 
 extern "C" int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* stream) {
@@ -734,7 +737,7 @@ extern "C" int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* 
   const bool direct = is_direct(p.batch, p.tasks, most);
   p.part_o = nullptr, p.part_lse = nullptr, p.shares = 1, p.by_shares = fast_div(1), p.min_units = (int32_t)kMinUnits;
   if (!direct) {
-    const int64_t shares = shares_of(share_waves(k8, a->head_dim), p.batch, p.tasks, most), rows = shares + p.batch;
+    const int64_t shares = shares_of(p.batch, p.tasks, most), rows = shares + p.batch;
     if (!a->workspace || a->workspace_bytes < (size_t)(rows * p.hq * (a->head_dim + 1) * 4)) return LSATTN_ERR_WORKSPACE;
     if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
     p.shares = (int32_t)shares, p.by_shares = fast_div((uint32_t)shares);
