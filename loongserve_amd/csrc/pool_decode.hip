@@ -300,10 +300,12 @@ template <typename QT, typename KV, int D> struct Walk {
     float x[8];
     bool tiny = false;
     if constexpr (k8) {
-      const int e = (int)rows.scale_byte - 127;
+      // (a position that does not exist has the factor 1: what lies in the slot that was read in its place may be any byte)
+      const uint32_t byte = (rows.there >> (lane & 31)) & 1u ? rows.scale_byte : 127u;
+      const int e = (int)byte - 127;
       tiny = __builtin_amdgcn_ballot_w64(lane >= 32 && e < kLeast) != 0;
       const int kept = e < kLeast ? kLeast : e;
-      *(float*)(lds + kKScale + lane * 4) = lane < 32 ? scale_of(rows.scale_byte) * p.scale_log2 : (float)kept;
+      *(float*)(lds + kKScale + lane * 4) = lane < 32 ? scale_of(byte) * p.scale_log2 : (float)kept;
       if (lane >= 32) {
         *(float*)(lds + kVInv - 128 + lane * 4) = __builtin_bit_cast(float, (uint32_t)(127 - kept) << 23);
         if (tiny) *(float*)(lds + kVRest - 128 + lane * 4) = __builtin_amdgcn_exp2f((float)(e - kept));
