@@ -20,8 +20,10 @@
 //     head's P, high and low, and a second product a third part where the type is bfloat16 (8 bits each).  The parts are
 //     added once, at the end;
 //   * the scale of a token's V row goes into its weight: 2^(s + e) multiplies the e4m3 values as they are, and the reference that the weights are
-//     taken relative to follows the maximum of s + e, so that they fit fp16 whatever the scales are; the sum takes them times 2^-e;
-//   * the reference of a head's weights is raised only when a score exceeds the maximum it was set by by 8 (log2 units): the accumulators
+//     taken relative to follows the maximum of s + e, so that they fit fp16 whatever the scales are.  The sum takes 2^s, relative to a reference that
+//     follows the maximum of s: drawn from the weights instead it would lose a token whose s + e lies far below the largest (a V row of zeros beside one
+//     of 2^61).  Both references are whole numbers, so 2^(their difference) is exact;
+//   * the references are raised only when a score exceeds the maximum they were set by (by 8 log2 units, the sum's by 80): the accumulators
 //     are seldom rescaled, and no exchange between lanes stands in the common path.
 // Short contexts and windows: the waves of one workgroup share a (request, KV head) and meet in LDS (one launch).  Otherwise the blocks of
 // all requests are dealt to the waves in equal shares, whatever the requests' lengths are (the host does not know them);
@@ -36,16 +38,17 @@ namespace {
 struct E4M3 {};  // element tag of the pool
 
 constexpr int kBlock = 32;       // tokens per step of a wave
-// LDS of a wave: the byte offsets of a block's K rows and of its V rows, the factors of its scores, the exponents of its V rows, 2^-exponent, and what
-// is left of exponents below kLeast
-constexpr int kVOff = 256, kKScale = 512, kVExp = 640, kVInv = 768, kVRest = 896, kKRows = 1024;  // (and the K rows of a block)
+// LDS of a wave: the byte offsets of a block's K rows and of its V rows, the factors of its scores, the exponents of its V rows
+constexpr int kVOff = 256, kKScale = 512, kVExp = 640, kKRows = 768;  // (and the K rows of a block)
 template <typename KV, int D> constexpr int kWaveLds = kKRows + kBlock * D * (__is_same(KV, E4M3) ? 1 : 2);
-constexpr int kLeast = -80;      // a V row's exponent counts as this in the weights if it is less (2^80 times a weight stays a float)
 constexpr int kHeads = 8;        // query heads per task
 constexpr int64_t kCUs = 256;
 // The reference m of a head's weights is set to the maximum so far less kHead, and raised when a score exceeds it by kLag: weights
 // of up to 2^15 (fp16 ends at 2^16), the largest 2^7 or more, so that the second part of a small fp16 weight does not run out of exponent.
 constexpr float kHead = 7.f, kLag = 15.f;
+// 8 bits: both references start here (finite, so that the scores of a block whose positions do not exist, -inf, leave them alone), and the sum's is raised where
+// eight of its terms come to this (2^80 times 2^31 tokens stays a float, and so does what lies 2^-40 below the largest).
+constexpr float kStart = -0x1p100f, kSumLimit = 0x1p80f;
 
 struct PoolParams {
   const char* q;
@@ -182,6 +185,7 @@ template <typename QT, typename KV, int D> struct Walk {
   u32x4 qf[KS];
   f32x4 acc[EV];  // acc[j][r] = O[head][EV * (4g + r) + j], of the parts of P in this lane's column
   float m, l;     // log2-domain maximum of the head; the lane's share of the sum
+  float ml;       // (8 bits) what the sum is relative to
 
   __device__ __forceinline__ Walk(const PoolParams& p_, char* lds_wave)
       : p(p_), lane(threadIdx.x & 63), g(lane >> 4), c(lane & 15), lds(lds_wave) {}
@@ -215,7 +219,7 @@ template <typename QT, typename KV, int D> struct Walk {
     row = p.table + (int64_t)req * p.max_seq_len;
     sinks = p.window ? p.sinks : 0;
     skip = len - n_vis;
-    m = -INFINITY, l = 0.f;
+    m = k8 ? kStart : -INFINITY, ml = kStart, l = 0.f;
 #pragma unroll
     for (int j = 0; j < EV; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -296,29 +300,22 @@ template <typename QT, typename KV, int D> struct Walk {
         if (t) __builtin_amdgcn_sched_barrier(0);
       }
     __builtin_amdgcn_wave_barrier();
-    // x: the score in log2 units, plus the exponent of the token's V row
-    float x[8];
-    bool tiny = false;
+    float x[8];  // the score in log2 units
+    f32x4 ve[2];  // (8 bits) the exponent of the token's V row
     if constexpr (k8) {
-      // (a position that does not exist has the factor 1: what lies in the slot that was read in its place may be any byte)
+      // (a position that does not exist has the exponent 0: what lies in the slot that was read in its place may be any byte)
       const uint32_t byte = (rows.there >> (lane & 31)) & 1u ? rows.scale_byte : 127u;
-      const int e = (int)byte - 127;
-      tiny = __builtin_amdgcn_ballot_w64(lane >= 32 && e < kLeast) != 0;
-      const int kept = e < kLeast ? kLeast : e;
-      *(float*)(lds + kKScale + lane * 4) = lane < 32 ? scale_of(byte) * p.scale_log2 : (float)kept;
-      if (lane >= 32) {
-        *(float*)(lds + kVInv - 128 + lane * 4) = __builtin_bit_cast(float, (uint32_t)(127 - kept) << 23);
-        if (tiny) *(float*)(lds + kVRest - 128 + lane * 4) = __builtin_amdgcn_exp2f((float)(e - kept));
-      }
+      *(float*)(lds + kKScale + lane * 4) = lane < 32 ? scale_of(byte) * p.scale_log2 : (float)((int)byte - 127);
       __builtin_amdgcn_wave_barrier();
-      f32x4 kf[2], vf[2];
+      f32x4 kf[2];
 #pragma unroll
       for (int t = 0; t < 2; t++) {
         kf[t] = *(const f32x4*)(lds + kKScale + 64 * t + 16 * g);
-        vf[t] = *(const f32x4*)(lds + kVExp + 64 * t + 16 * g);
+        ve[t] = *(const f32x4*)(lds + kVExp + 64 * t + 16 * g);
       }
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(s[e / 4][e % 4], kf[e / 4][e % 4], vf[e / 4][e % 4]);
+      for (int e = 0; e < 8; e++) x[e] = s[e / 4][e % 4] * kf[e / 4][e % 4];
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e++) x[e] = s[e / 4][e % 4] * p.scale_log2;
@@ -333,32 +330,45 @@ template <typename QT, typename KV, int D> struct Walk {
         for (int w = 0; w < VW; w++) rows.v[e][w] = ok ? rows.v[e][w] : 0u;  // (what lies there may be infinite or NaN)
       }
     }
-    const float mx = max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), fmaxf(x[6], x[7]));
-    if (__builtin_amdgcn_ballot_w64(mx > m + kLag) != 0) {
-      const float m_new = fmaxf(m, col_max(mx) - kHead);
-      const float alpha = exp2_diff(m, m_new);
-      l *= alpha;
-#pragma unroll
-      for (int j = 0; j < EV; j++) acc[j] *= alpha;
-      m = m_new;
-    }
-    const float m_safe = m == -INFINITY ? 0.f : m;
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(x[e] - m_safe);
+    auto largest = [](const float (&v)[8]) __attribute__((always_inline)) { return max3(max3(v[0], v[1], v[2]), max3(v[3], v[4], v[5]), fmaxf(v[6], v[7])); };
     if constexpr (k8) {
-      f32x4 inv[2];
+      // the arguments of the weights, s + e - m (e - m is exact, and so they are rounded where they are small), and the sum's terms, 2^(s - ml)
+      float y[8], part;
+      auto relative = [&]() __attribute__((always_inline)) {
+        float w[8];
 #pragma unroll
-      for (int t = 0; t < 2; t++) inv[t] = *(const f32x4*)(lds + kVInv + 64 * t + 16 * g);
-      float even = 0.f;
+        for (int e = 0; e < 8; e++) y[e] = x[e] + (ve[e / 4][e % 4] - m), w[e] = __builtin_amdgcn_exp2f(x[e] - ml);
+        part = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+      };
+      relative();
+      if (__builtin_amdgcn_ballot_w64(largest(y) > kLag || !(part < kSumLimit)) != 0) {
+        float with_e[8];
 #pragma unroll
-      for (int e = 0; e < 4; e++) even = __builtin_fmaf(x[e], inv[0][e], even), l = __builtin_fmaf(x[4 + e], inv[1][e], l);
-      l += even;
-      if (tiny) {
+        for (int e = 0; e < 8; e++) with_e[e] = x[e] + ve[e / 4][e % 4];
+        const float m_new = fmaxf(m, floorf(col_max(largest(with_e))) - kHead), ml_new = fmaxf(ml, floorf(col_max(largest(x))));
+        const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+        l *= __builtin_amdgcn_exp2f(ml - ml_new);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] *= *(const float*)(lds + kVRest + 64 * (e / 4) + 16 * g + 4 * (e % 4));
+        for (int j = 0; j < EV; j++) acc[j] *= alpha;
+        m = m_new, ml = ml_new;
+        relative();
       }
-      __builtin_amdgcn_wave_barrier();
+      l += part;
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(y[e]);
     } else {
+      const float mx = largest(x);
+      if (__builtin_amdgcn_ballot_w64(mx > m + kLag) != 0) {
+        const float m_new = fmaxf(m, col_max(mx) - kHead);
+        const float alpha = exp2_diff(m, m_new);
+        l *= alpha;
+#pragma unroll
+        for (int j = 0; j < EV; j++) acc[j] *= alpha;
+        m = m_new;
+      }
+      const float m_safe = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = __builtin_amdgcn_exp2f(x[e] - m_safe);
       l += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
     }
     u32x4 pk[2];
@@ -418,13 +428,23 @@ template <typename QT, typename KV, int D> struct Walk {
     }
   }
 
-  // the parts of P together, and the sum over the head's lanes
+  // the parts of P together, and the sum over the head's lanes.  8 bits: O as the mean, m the log-sum-exp, a sum of 1 (0: nothing seen)
   __device__ __forceinline__ void join() {
 #pragma unroll
     for (int j = 0; j < EV; j++)
 #pragma unroll
       for (int r = 0; r < 4; r++) acc[j][r] += dpp_mov<0x128>(acc[j][r]);  // row_ror:8
     l = col_sum(l);
+    if constexpr (k8) {
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int up = l > 0.f ? (int)(m - ml) : 0;  // (whole numbers; the difference of the two may pass what a float's exponent takes)
+#pragma unroll
+      for (int j = 0; j < EV; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[j][r] = __builtin_amdgcn_ldexpf(acc[j][r] * inv, up);
+      m = l > 0.f ? ml + __builtin_amdgcn_logf(l) : -INFINITY;
+      l = l > 0.f ? 1.f : l;
+    }
   }
 };
 

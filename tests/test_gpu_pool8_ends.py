@@ -1,7 +1,10 @@
 """Decode over the 8-bit pool where its exponents are at their ends: slots that nobody wrote, V rows of zeros, very small and very large ones."""
+import math
+
 import pytest
 import torch
 
+from oracle import pool8_oracle as orc
 from tests.test_gpu_pool8 import Case
 
 K8 = ["e4m3-f16", "e4m3-bf16"]
@@ -35,3 +38,102 @@ def test_exponents_of_slots_that_are_not_seen_do_not_matter(lsa, kind, lens, hol
     for max_len in (None, 1 << 17):
         c.check(c.run(lsa, max_len=max_len))
         c.check(c.run(lsa, 50, 3, max_len=max_len), 50, 3)
+
+
+def _rows_at(exponents, D, seed):
+    """(bytes of e4m3 values, exponent bytes, float64 values) of rows [tokens, heads] with the largest element in (224, 448] * 2^e; e = None: zeros."""
+    g = torch.Generator().manual_seed(seed)
+    T, H = len(exponents), len(exponents[0])
+    x = torch.randn(T, H, D, generator=g, dtype=torch.float64)
+    q = orc.round_e4m3(x / x.abs().amax(-1, keepdim=True) * 440)
+    e = torch.tensor([[-126 if y is None else y for y in row] for row in exponents])
+    q[torch.tensor([[y is None for y in row] for row in exponents])] = 0
+    return q.float().to(torch.float8_e4m3fn), (e + 127).to(torch.uint8), q * torch.pow(2.0, e.double())[..., None], e
+
+
+class Ends:
+    """One request whose V rows have the exponents given (per token and KV head), K ordinary; `lift` names tokens whose scores lie that many
+    nats above (or below) what the others have."""
+
+    def __init__(self, dtype, exponents, lift=(), Hq=8, Hkv=2, D=128, seed=0):
+        T = len(exponents)
+        g = torch.Generator().manual_seed(seed)
+        base = torch.randn(Hkv, D, generator=g, dtype=torch.float64)
+        self.q = (base.repeat_interleave(Hq // Hkv, 0) + 0.1 * torch.randn(Hq, D, generator=g, dtype=torch.float64))[None].to(dtype)
+        k = torch.randn(T, Hkv, D, generator=g, dtype=torch.float64)
+        for t, nats in lift:
+            k[t] = base * (nats * math.sqrt(D) / (base * base).sum(-1, keepdim=True))
+        kq, ke = orc.quantise(k)
+        v8, vb, v, self.e = _rows_at(exponents, D, seed + 1)
+        self.k, self.v, self.T, self.Hkv, self.Hq, self.D = kq * torch.pow(2.0, (ke - 127).double())[..., None], v, T, Hkv, Hq, D
+        order = torch.randperm(T + 3, generator=g)[:T]
+        pool = torch.full((T + 3, 2 * Hkv, D), 0x7F, dtype=torch.uint8)
+        scales = torch.full((T + 3, 2 * Hkv), 255, dtype=torch.uint8)
+        pool[order] = torch.cat([kq.float().to(torch.float8_e4m3fn).view(torch.uint8), v8.view(torch.uint8)], 1)
+        scales[order] = torch.cat([ke.to(torch.uint8), vb], 1)
+        self.pool, self.scales, self.table = pool.cuda().view(torch.float8_e4m3fn), scales.cuda(), order.to(torch.int32)[None].cuda()
+
+    def check(self, lsa, max_len=None):
+        T, h, D = self.T, self.Hkv, self.D
+        i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        o, l = lsa.longserve_fp8_decode_attention(self.q.cuda(), self.table, i(0), i(T), T if max_len is None else max_len, self.pool[:, :h], self.pool[:, h:],
+                                                  self.scales[:, :h], self.scales[:, h:])
+        G = self.Hq // h
+        q, k, v = self.q[0].double(), self.k.repeat_interleave(G, 1), self.v.repeat_interleave(G, 1)
+        s = torch.einsum("hd,nhd->hn", q, k) / math.sqrt(D)
+        size = torch.einsum("hd,nhd->hn", q.abs(), k.abs()).amax(-1) / math.sqrt(D)
+        lse = torch.logsumexp(s, -1)
+        p = torch.exp(s - lse[:, None])
+        want, mean = torch.einsum("hn,nhd->hd", p, v), torch.einsum("hn,nhd->hd", p, v.abs())
+        # float32 (eps = 2^-24, half a step): a score is a sum of D products, twice (numerator and sum); up to 30 eps for each exponential, whose argument is
+        # up to some 24 where the weight counts, its division and the parts of the weight (2^-22 = 4 eps); sums in blocks of 32 tokens.  A weight is kept to
+        # 2^-25 beside a largest one of 2^7 at least, and stands for e4m3 values of up to 448 * 2^e.  Results below 2^-126 may be flushed.
+        eps = 2.0 ** -24
+        rel = 2 * ((D + 8) * eps * size + 30 * eps + (T / 32 + 40) * eps)
+        top = (p * torch.pow(2.0, self.e.double()).repeat_interleave(G, 1).T).amax(-1)
+        tol = rel[:, None] * mean + (T * 2.0 ** -32 * 448 * top)[:, None] + 2.0 ** -126
+        got = o[0].cpu().double()
+        assert torch.isfinite(got).all()
+        assert ((got - want).abs() <= tol).all(), ((got - want).abs() / tol).max()
+        assert ((l[0].cpu().double() - lse).abs() <= rel + 8 * eps * lse.abs()).all(), (l[0].cpu().double() - lse).abs().max()
+
+
+def _ends(name, T):
+    """Exponents of T tokens, and tokens with scores of their own."""
+    r = torch.Generator().manual_seed(5)
+    pick = lambda *v: [[v[int(x)] for x in row] for row in torch.randint(0, len(v), (T, 2), generator=r)]  # noqa: E731
+    if name == "a zero row takes the weight":
+        return [[None, None]] + pick(-7, -8)[1:], [(0, 15.0)]
+    if name == "zero rows":
+        return pick(None), []
+    if name == "zero rows beside ordinary ones":
+        return pick(None, -7, -8), []
+    if name == "very small rows beside ordinary ones":
+        return pick(-100, -7), [(T // 2, 12.0)]
+    if name == "zero rows beside 2^61 and more":
+        return pick(None, 54, 61), []
+    if name == "small rows that take the weight beside the largest there are":
+        return pick(-110, -100)[:-1] + [[118, 118]], [(T - 1, -60.0), (0, 5.0)]
+    if name == "the largest there are":
+        return pick(112, 118), []
+    if name == "the smallest there are":
+        return pick(-126, -124), []
+    if name == "all sizes":
+        return pick(None, -126, -100, -80, -60, -30, 0, 30, 60, 90, 110), []
+    assert name == "growing from the smallest to the largest"
+    return [[-126 + 240 * t // T, 114 - 240 * t // T] for t in range(T)], []
+
+
+NAMES = ["a zero row takes the weight", "zero rows", "zero rows beside ordinary ones", "very small rows beside ordinary ones", "zero rows beside 2^61 and more",
+         "small rows that take the weight beside the largest there are", "the largest there are", "the smallest there are", "all sizes",
+         "growing from the smallest to the largest"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("T,max_len", [(333, None), (333, 1 << 17), (4100, None)])
+def test_v_rows_of_any_exponents(lsa, dtype, name, T, max_len):
+    """Both launch forms, exponents from -126 to 118."""
+    exponents, lift = _ends(name, T)
+    Ends(dtype, exponents, lift, seed=T).check(lsa, max_len)
