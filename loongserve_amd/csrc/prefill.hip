@@ -85,6 +85,10 @@ constexpr int64_t kTileMajorBelowWorkgroups = 2048;  // 256-row workgroups in a 
 constexpr int64_t kListedFromWorkgroups = 4096;  // launches from which a caller's bound on the rows of all requests may shrink the grid
 constexpr int kListedMaxBatch = 4096;            // (every workgroup walks the batch's lengths once)
 constexpr float kLazyRescale = 8.f;  // log2 units the running max may lag before O is rescaled
+// (behind a window) P uses fp16's whole range: a raise leaves a row's largest at 2^kWinHead, the next one comes where one would exceed 2^kWinLag.  So weights
+// down to 2^-23 of the largest keep 11 bits (a first key that outweighs thousands of others needs them), and raises are few: 32768 tokens
+// 32/8 behind 4096 1865 us, 2065 with maxima as they were seen and a plain step's P up to 2, although the largest P takes four instructions more to find.
+constexpr float kWinHead = 9.f, kWinLag = 15.f;
 
 template <typename T> struct Mfma;
 template <> struct Mfma<F16> {
@@ -773,8 +777,20 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
       // Every key counts here, so no maxima are needed to tell whether the running ones still hold: some P is 2 or more
       // (also infinite, as for the first keys a row sees, when m is still -inf) exactly if bit 14 of one of the packed
       // fp16 values, the top bit of its exponent, is set.  Six instructions instead of the eleven of the maxima.
-      const uint32_t any = (pk[0][0] | pk[0][1] | pk[0][2]) | (pk[0][3] | pk[1][0] | pk[1][1]) | (pk[1][2] | pk[1][3]);
-      over = (any & 0x40004000u) != 0;
+      if constexpr (WIN) {
+        // (P of up to 2^15: the largest as a whole number, exponent and mantissa, and 0x800 above 2^15 is bit 15 of its half)
+        auto halves = [&](int qb, int e) __attribute__((always_inline)) {
+          const uint32_t word = pk[qb][e];  // (a copy: the cast of a vector's element takes its first one)
+          return __builtin_bit_cast(u16x2, word);
+        };
+        u16x2 most = halves(0, 0);
+#pragma unroll
+        for (int e = 1; e < 8; e++) most = __builtin_elementwise_max(most, halves(e / 4, e % 4));
+        over = ((__builtin_bit_cast(uint32_t, most) + 0x08000800u) & 0x80008000u) != 0;
+      } else {
+        const uint32_t any = (pk[0][0] | pk[0][1] | pk[0][2]) | (pk[0][3] | pk[1][0] | pk[1][1]) | (pk[1][2] | pk[1][3]);
+        over = (any & 0x40004000u) != 0;
+      }
     }
     if (__builtin_expect(__builtin_amdgcn_ballot_w64(over) != 0, 0)) {
       // rare: some score is above the lazy threshold (always so for the first key a row sees); raise the running maxima
@@ -788,11 +804,12 @@ __global__ __launch_bounds__(HALF ? NWAVE * 32 : NWAVE * 64, HALF ? 2 : 1) void 
       }
 #pragma unroll
       for (int qb = 0; qb < 2; qb++) {
-        const float m_new = fminf(neg_m[qb], -column_max(mx[qb]) * scale);  // -max(m, mx*scale)
+        const float top = column_max(mx[qb]);
+        const float m_new = fminf(neg_m[qb], WIN ? kWinHead - top * scale : -top * scale);  // -max(m, mx*scale (- kWinHead))
         // (a block of rows that still has seen no key keeps neg_m = +inf: no inf - inf)
         const float al = (MASKED && m_new == neg_m[qb]) ? 1.f : __builtin_amdgcn_exp2f(m_new - neg_m[qb]);
         neg_m[qb] = m_new;
-        thr_raw[qb] = (kLazyRescale - m_new) * inv_scale;
+        thr_raw[qb] = ((WIN ? kWinLag : kLazyRescale) - m_new) * inv_scale;
         if (MASKED) l_run[qb] *= al;
         else lacc[qb] *= al;
 #pragma unroll

@@ -100,6 +100,7 @@ struct SmallParams {
 };
 
 constexpr int kWaves = 4;   // waves per workgroup
+constexpr float kWinHead = 9.f;
 constexpr uint32_t kOnes = 0x3C003C00u;  // two ones in fp16
 constexpr int64_t kCUs = 256;
 constexpr int64_t kL2Bytes = 32 << 20;    // of the eight L2s together
@@ -413,12 +414,13 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV, WIN>)) void
             for (int e = 0; e < 8; e++) s[qb][e / 4][e % 4] = 16 * (e / 4) + e % 4 < rel ? s[qb][e / 4][e % 4] : -INFINITY;
           }
         }
-        // Behind a window, where a row's keys are few, every raise counts (250 vector instructions, where a step takes 140): the maxima are set 3 above what was
-        // seen, so that P is at most 1/8 then and a row is raised again only by a score 4 above (log2 units).  What fp16 loses for it are the bits of weights
-        // below 2^-11 of the largest, each off by at most 2^-22 of that.  32768 tokens 32/8 behind 1024 751 -> 661 us (2 above: 670, 4: 657), 64-wide heads 222 -> 186.
         // P = exp2(S * scale - m) with the running maxima as they are; they are raised, and the step done again, only if some
         // P comes out as 2 or more (or as inf or NaN, as for a row that has seen no key yet: m = -inf), which is bit 14 of
         // its fp16 form.  No exchange between lanes, no chain through the maximum in the common case.
+        // WIN: every raise counts where a row's keys are few (250 vector instructions, where a step takes 140), so P uses fp16's whole range: a raise leaves
+        // the largest P at 2^kWinHead, the next one comes when a lane's eight P add up to 2^15 (or to inf or NaN).  So weights down to
+        // 2^-(14 + kWinHead) of the largest keep 11 bits, which a first key that outweighs thousands of others needs.  32768 tokens 32/8 behind 1024 678 us
+        // (kWinHead 7: 670, 11: 687; the maxima as they were seen and P up to 2, as without a window: a seventh more), 64-wide heads 376 (371, 386).
         u32x4 pk[QB];  // P^T as B operands: the lane's eight keys are contraction slots 8 g .. 8 g + 7, the order the V^T operand uses
         float ps[QB];
         auto compute_p = [&](int qb, float neg_m) __attribute__((always_inline)) {
@@ -430,18 +432,21 @@ __global__ __launch_bounds__(kWaves * KP * 64, (kResident<D, WP, DV, WIN>)) void
           for (int e = 0; e < 4; e++) pk[qb][e] = pack2<F16>(pv[2 * e], pv[2 * e + 1]);
         };
         uint32_t any = 0;
+        bool over = false;
 #pragma unroll
         for (int qb = 0; qb < QB; qb++) {
           compute_p(qb, -m_run[qb]);
-          any |= (pk[qb][0] | pk[qb][1]) | (pk[qb][2] | pk[qb][3]);
+          if (WIN) over |= !(ps[qb] < 32768.f);
+          else any |= (pk[qb][0] | pk[qb][1]) | (pk[qb][2] | pk[qb][3]);
         }
-        if (__builtin_expect(__builtin_amdgcn_ballot_w64((any & 0x40004000u) != 0) != 0, 0)) {
+        if (!WIN) over = (any & 0x40004000u) != 0;
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(over) != 0, 0)) {
 #pragma unroll
           for (int qb = 0; qb < QB; qb++) {
             const float mx = fmaxf(fmaxf(fmaxf(s[qb][0][0], s[qb][0][1]), fmaxf(s[qb][0][2], s[qb][0][3])),
                                    fmaxf(fmaxf(s[qb][1][0], s[qb][1][1]), fmaxf(s[qb][1][2], s[qb][1][3])));
             float top = col_max(mx) * scale;  // (the scale is positive)
-            if constexpr (WIN) top += 3.f;
+            if constexpr (WIN) top -= kWinHead;
             const float m_new = fmaxf(m_run[qb], top);
             const float alpha = exp2_diff(m_run[qb], m_new);
             l_run[qb] *= alpha;

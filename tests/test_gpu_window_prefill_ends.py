@@ -1,0 +1,30 @@
+"""The prefill step behind a window at its ends: one key that outweighs thousands, no keys at all, every request of a full launch."""
+import math
+
+import pytest
+import torch
+
+from oracle import pool8_oracle as orc
+from tests.test_gpu_window_prefill import DT, Step, rows  # noqa: F401 (a fixture: both shapes of 128-wide heads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("Hq,Hkv,D,q_len", [(4, 2, 128, 40), (2, 2, 64, 33), (2, 1, 32, 20), (3, 3, 16, 17), (32, 32, 128, 1200)])
+def test_a_first_key_that_outweighs_the_others(lsa, rows, dtype, Hq, Hkv, D, q_len):
+    """A sink whose score lies 20 to 22 binary orders above those of 4000 others, which are alike: their weights keep 11 bits each (the oracle's
+    tolerance), whatever share of a row they make up.  V is 0 at the sink, so that nothing hides them."""
+    n = 4000 + q_len
+    for bits in (20.03, 22.03):
+        s = Step([(q_len, 4000, n, 0)], Hq, Hkv, D, DT[dtype], seed=31)
+        ks = s.k_start[0]
+        s.q.zero_(), s.kv[ks:ks + n, :Hkv].zero_()
+        s.q[..., 0] = 16.0
+        s.kv[ks, :Hkv, 0] = bits * math.log(2) * math.sqrt(D) / 16.0
+        s.kv[ks, Hkv:] = 0
+        s.kv[ks + 1:ks + n, Hkv:] = s.kv[ks + 1:ks + n, Hkv:].abs() + 0.5
+        got = s.run(lsa, 5000, 1, o_dtype=torch.float32)
+        q0, m = s.q_start[0], min(q_len, 64)  # (float64 over the first rows)
+        want, lse, tol_o, tol_l = orc.prefill(s.q[q0:q0 + m], s.kv[ks:ks + n, :Hkv], s.kv[ks:ks + n, Hkv:], m, 4000, n, 0, 1, 5000, 1)
+        assert ((got[0][q0:q0 + m].cpu().double() - want).abs() <= tol_o).all(), ((got[0][q0:q0 + m].cpu().double() - want).abs() / tol_o).max()
+        assert ((got[1][q0:q0 + m].cpu().double() - lse).abs() <= tol_l).all()
