@@ -172,7 +172,7 @@ int lsattn_prefill_step_accumulate(const lsattn_prefill_args* a, void* stream);
  * Uses o (o_dtype LSATTN_F32 or dtype) and lse (natural log-sum-exp; NULL: not wanted); rows that see no key get o = 0, lse = -inf.  Partials
  * over several KV chunks (o in fp32) join by lsattn_lse_merge.  kv_cuts is not taken.  A bfloat16 V is multiplied as fp16 (v_is_f16, or
  * converted in the kernel): magnitudes past 65504 count as 65504, below 2^-14 they are cut to multiples of 2^-24.  A row's weights are rounded to fp16
- * (11 bits down to 2^-23 of the row's largest) for the product with V, whatever o's type is; the log-sum-exp is that of the unrounded ones. */
+ * (11 bits down to 2^-23 of the row's largest) for the product with V, whatever o's type is. */
 int lsattn_prefill_window(const lsattn_prefill_args* a, int64_t window, int64_t sinks, void* stream);
 /* 1 if that step (v_is_f16 = 0) converts a bfloat16 V on its way at no cost; 0 if the caller should make an fp16 copy of V first, without which the
  * step runs in a slower shape.  Looks at the numbers in the block alone. */

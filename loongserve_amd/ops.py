@@ -457,7 +457,7 @@ def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_g
     seen.  No reference counterpart.
 
     o has q's type, or is float32 (a partial: with lse, the steps over several KV chunks join by lse_merge); lse, the natural
-    log-sum-exp, float32 [tokens, q_heads], is optional.  Rows that see no key get o = 0, lse = -inf; rows that no
+    log-sum-exp, float32 [tokens, q_heads], is optional.  Rows that see no key get o = 0, lse = -inf (all of them where k and v have no rows); rows that no
     request names stay as they were.  A chunk of a longer prompt brings its context in k and v (kv_gather_fp8 reads one back
     from an 8-bit pool) and the position of its first query in q_first_token_global_idx.  Requests share no
     rows of q: total_q_len, an upper bound of all their lengths together, is q's rows unless given.  A bfloat16 v is multiplied as float16: magnitudes past 65504 count as 65504.  V rows of keys near
@@ -483,8 +483,11 @@ def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_g
                   logical_sp_peers_num, max_q_b_seq_len, None, total_q_len=total_q_len, state=None)
     if q.numel() == 0:
         return
-    if k.numel() == 0:  # no keys at all: every row that a request names sees none
-        raise ValueError("k and v hold no rows")
+    if k.shape[0] == 0:  # no keys at all: every row that a request names sees none
+        nothing, none = k.new_zeros((1, *k.shape[1:])), torch.zeros_like(kv_b_seq_len)
+        window_attention_fwd(q, nothing, nothing, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx, none, none, kv_first_token_global_idx,
+                             logical_sp_peers_num, max_q_b_seq_len, window, sinks, lse=lse, total_q_len=total_q_len)
+        return
     raise ValueError("window_attention_fwd: arguments that no kernel takes")
 
 

@@ -28,3 +28,27 @@ def test_a_first_key_that_outweighs_the_others(lsa, rows, dtype, Hq, Hkv, D, q_l
         want, lse, tol_o, tol_l = orc.prefill(s.q[q0:q0 + m], s.kv[ks:ks + n, :Hkv], s.kv[ks:ks + n, Hkv:], m, 4000, n, 0, 1, 5000, 1)
         assert ((got[0][q0:q0 + m].cpu().double() - want).abs() <= tol_o).all(), ((got[0][q0:q0 + m].cpu().double() - want).abs() / tol_o).max()
         assert ((got[1][q0:q0 + m].cpu().double() - lse).abs() <= tol_l).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [16, 64, 128])
+@pytest.mark.parametrize("o_dtype", [None, torch.float32])
+def test_no_keys_at_all(lsa, rows, dtype, D, o_dtype):
+    """K and V without rows, as an instance of a ring has them whose part of a prompt is empty: the empty partial, on the rows that requests name."""
+    s = Step([(70, 9, 0, 0), (0, 0, 0, 0), (3, 500, 0, 0)], 4, 2, D, DT[dtype], seed=33)
+    none = s.kv[:0].cuda()
+    s.check(s.run(lsa, 20, 2, o_dtype=o_dtype, kv=none), 20, 2)
+    s.check(s.run(lsa, 20, 2, o_dtype=o_dtype, kv=none, lse=False, total_q_len=73), 20, 2)
+    with pytest.raises(ValueError, match="window"):
+        s.run(lsa, 0, 2, kv=none)
+
+
+@pytest.mark.gpu
+def test_an_empty_partial_joins(lsa):
+    s = Step([(40, 60, 100, 0)], 4, 2, 128, torch.float16, seed=34)
+    o, l = s.run(lsa, 50, 3, o_dtype=torch.float32)
+    o0, l0 = s.run(lsa, 50, 3, o_dtype=torch.float32, kv=s.kv[:0].cuda())
+    q0 = s.q_start[0]
+    got = lsa.lse_merge([(o0[q0:].contiguous(), l0[q0:].contiguous()), (o[q0:].contiguous(), l[q0:].contiguous())])
+    assert torch.equal(got[0], o[q0:]) and torch.equal(got[1], l[q0:])
