@@ -4,12 +4,13 @@ longserve_flash_decoding_stage2.py:53 and longserve_flash_decoding.py:3."""
 from __future__ import annotations
 
 import functools
+from operator import index as as_int
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib, _native, longserve_cuda_kernels
-from .ops import _fp8_pool, _i32vec, _on_current_device
+from .ops import _fp8_pool, _i32vec, _on_current_device, _other_ints
 
 
 # The stage functions called on their own (the master path, longserve_transformer_layer_infer.py:272-281 then :360-367)
@@ -117,6 +118,10 @@ def _pool_attention(q, table, b_req_idx, b_seq_len, max_len_in_batch, cache_k, c
                                       out, lse, workspace)
         if done is not None:
             return done
+    numbers = (max_len_in_batch, window, sinks)
+    if _other_ints(*numbers):
+        max_len, window, sinks = (None if x is None else as_int(x) for x in numbers)
+        return _pool_attention(q, table, b_req_idx, b_seq_len, max_len, cache_k, cache_v, k_scales, v_scales, window, sinks, out, lse, workspace)
     # arguments the native pass does not take: say what is wrong
     _on_current_device(((q, "q"), (table, "req_to_token_indexs"), (b_req_idx, "b_req_idx"), (b_seq_len, "b_seq_len"), (cache_k, "cache_k"),
                         (cache_v, "cache_v"), (k_scales, "k_scales"), (v_scales, "v_scales"), (out, "out"), (lse, "o_logexpsum"), (workspace, "workspace")))

@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+from operator import index as as_int
 from typing import List, Optional, Sequence, Tuple
 
 import torch
@@ -447,6 +448,11 @@ def _prefill_attention_step_checked(q, k, v, q_b_start_loc, q_b_seq_len, q_first
     return out, lse
 
 
+def _other_ints(*values) -> bool:
+    """Whether some of these (None: not given) are integers of another kind than Python's, such as numpy's, which the native pass leaves to its caller."""
+    return any(x is not None and not isinstance(x, int) for x in values)
+
+
 def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx,
                          kv_b_start_loc, kv_b_seq_len, kv_first_token_global_idx,
                          logical_sp_peers_num: int, max_q_b_seq_len: int, window: int, sinks: int = 0,
@@ -466,6 +472,11 @@ def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_g
                                                        kv_first_token_global_idx, logical_sp_peers_num, max_q_b_seq_len, window, sinks, lse,
                                                        q.shape[0] if total_q_len is None else total_q_len, PRECONVERT_BF16_V):
         return
+    numbers = (logical_sp_peers_num, max_q_b_seq_len, window, sinks, total_q_len)
+    if _other_ints(*numbers):
+        peers, max_q, window, sinks, total = (None if x is None else as_int(x) for x in numbers)
+        return window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx, kv_b_start_loc, kv_b_seq_len,
+                                    kv_first_token_global_idx, peers, max_q, window, sinks, lse=lse, total_q_len=total)
     for t, n in ((q, "q"), (k, "k"), (v, "v"), (o, "o")):
         _dev(t, n)
     _on_current_device(((q, "q"), (k, "k"), (v, "v"), (o, "o"), (q_b_start_loc, "q_b_start_loc"), (q_b_seq_len, "q_b_seq_len"),
@@ -598,6 +609,8 @@ def kv_gather_fp8(pool: torch.Tensor, scales: torch.Tensor, req_to_token_indexs:
     they were.  The next chunk of a prompt attends to the result through context_attention_fwd or prefill_attention_step."""
     if _native.kv_gather_fp8(pool, scales, req_to_token_indexs, b_req_idx, b_seq_len, b_start_loc, max_len_in_batch, out, b_first):
         return
+    if _other_ints(max_len_in_batch):
+        return kv_gather_fp8(pool, scales, req_to_token_indexs, b_req_idx, b_seq_len, b_start_loc, as_int(max_len_in_batch), out, b_first)
     _on_current_device(((pool, "pool"), (scales, "scales"), (req_to_token_indexs, "req_to_token_indexs"), (b_req_idx, "b_req_idx"),
                         (b_seq_len, "b_seq_len"), (b_start_loc, "b_start_loc"), (out, "out"), (b_first, "b_first")))
     _fp8_pool(pool, scales)

@@ -1,6 +1,7 @@
 """Decode over the 8-bit pool where its exponents are at their ends: slots that nobody wrote, V rows of zeros, very small and very large ones."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -137,3 +138,22 @@ def test_v_rows_of_any_exponents(lsa, dtype, name, T, max_len):
     """Both launch forms, exponents from -126 to 118."""
     exponents, lift = _ends(name, T)
     Ends(dtype, exponents, lift, seed=T).check(lsa, max_len)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f16", "e4m3-f16"])
+def test_lengths_and_windows_as_numpy_integers(lsa, kind):
+    """What a scheduler that keeps its lengths in numpy passes."""
+    c = Case(kind, 2, 8, 2, 128, [70, 31], seed=24)
+    for window, sinks in ((50, 3), (None, 0)):
+        got = c.run(lsa, window if window is None else np.int64(window), np.int32(sinks), max_len=np.int64(70))
+        c.check(got, window, sinks)
+    if c.k8:
+        i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        a = (c.pool, c.scales, c.table.cuda(), c.req.cuda(), c.len.cuda(), i(0, 70))
+        outs = [torch.zeros(101, 4, 128, dtype=torch.float16, device="cuda") for _ in range(2)]
+        lsa.kv_gather_fp8(*a, 70, outs[0])
+        lsa.kv_gather_fp8(*a, np.int64(70), outs[1])
+        assert torch.equal(*outs) and outs[0].any()
+    with pytest.raises(ValueError, match="window"):
+        c.run(lsa, np.int64(0), 2)

@@ -1,11 +1,12 @@
 """The prefill step behind a window at its ends: one key that outweighs thousands, no keys at all, every request of a full launch."""
 import math
 
+import numpy as np
 import pytest
 import torch
 
 from oracle import pool8_oracle as orc
-from tests.test_gpu_window_prefill import DT, Step, rows  # noqa: F401 (a fixture: both shapes of 128-wide heads)
+from tests.test_gpu_window_prefill import DT, Step, _vec, rows  # noqa: F401 (a fixture: both shapes of 128-wide heads)
 
 
 @pytest.mark.gpu
@@ -52,3 +53,22 @@ def test_an_empty_partial_joins(lsa):
     q0 = s.q_start[0]
     got = lsa.lse_merge([(o0[q0:].contiguous(), l0[q0:].contiguous()), (o[q0:].contiguous(), l[q0:].contiguous())])
     assert torch.equal(got[0], o[q0:]) and torch.equal(got[1], l[q0:])
+
+
+@pytest.mark.gpu
+def test_lengths_and_windows_as_numpy_integers(lsa):
+    """What a scheduler that keeps its lengths in numpy passes."""
+    s = Step([(40, 60, 100, 0), (9, 0, 9, 0)], 4, 2, 128, torch.float16, seed=35)
+    n = np.int64
+    for total in (None, n(49)):
+        got = s.run(lsa, n(50), np.int32(3), total_q_len=total)
+        s.check(got, 50, 3)
+    o = torch.zeros(s.q.shape, dtype=torch.float16, device="cuda")
+    q, kv, v = s.q.cuda(), s.kv.cuda(), [_vec(s.q_start), _vec([40, 9]), _vec([60, 0]), _vec(s.k_start), _vec([100, 9]), _vec([0, 0])]
+    lsa.window_attention_fwd(q, kv[:, :2], kv[:, 2:], o, *v, n(1), n(40), n(50), n(3))
+    q0 = s.q_start[0]
+    assert torch.equal(o[q0:q0 + 40], got[0][q0:q0 + 40])
+    with pytest.raises(ValueError, match="window"):
+        s.run(lsa, n(0), 2)
+    with pytest.raises(TypeError):
+        s.run(lsa, 4.5, 2)
