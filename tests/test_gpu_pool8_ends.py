@@ -157,3 +157,27 @@ def test_lengths_and_windows_as_numpy_integers(lsa, kind):
         assert torch.equal(*outs) and outs[0].any()
     with pytest.raises(ValueError, match="window"):
         c.run(lsa, np.int64(0), 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", K8)
+@pytest.mark.parametrize("lens", [[300, 31], [9000]])
+def test_exponents_as_e8m0(lsa, kind, lens):
+    """The exponent bytes as a float8_e8m0fnu tensor: written, read back and attended over as the same bytes of uint8 are."""
+    c = Case(kind, len(lens), 8, 2, 128, lens, seed=23)
+    e8 = torch.float8_e8m0fnu
+    want = c.run(lsa)
+    c.scales = c.scales.view(e8)
+    got = c.run(lsa)
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
+    x = torch.randn(7, 4, 128, generator=torch.Generator().manual_seed(1)).to(c.dtype).cuda()
+    idx = torch.arange(7, device="cuda")
+    outs = []
+    for t in (torch.uint8, e8):
+        pool, sc = torch.zeros(9, 4, 128, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn), torch.zeros(9, 4, dtype=torch.uint8, device="cuda")
+        lsa.kv_scatter_fp8(x, idx, pool, sc.view(t))
+        out = torch.zeros(7, 4, 128, dtype=c.dtype, device="cuda")
+        i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+        lsa.kv_gather_fp8(pool, sc.view(t), idx.int().view(1, 7), i(0), i(7), i(0), 7, out)
+        outs.append((pool.view(torch.uint8), sc, out))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import pool8_oracle as orc
-from tests.test_gpu_window_prefill import DT, Step, _vec, rows  # noqa: F401 (a fixture: both shapes of 128-wide heads)
+from tests.test_gpu_window_prefill import DT, Step, _rows, _vec, rows  # noqa: F401 (a fixture: both shapes of 128-wide heads)
 
 
 @pytest.mark.gpu
@@ -72,3 +72,69 @@ def test_lengths_and_windows_as_numpy_integers(lsa):
         s.run(lsa, n(0), 2)
     with pytest.raises(TypeError):
         s.run(lsa, 4.5, 2)
+
+
+def _step64(q, k, v, qp, kp, window, sinks):
+    """(o, lse, mean of |v|, largest sum of a score's magnitudes) in float64 on the GPU: queries at positions qp, keys at kp."""
+    G = q.shape[1] // k.shape[1]
+    qd, kd, vd = (t.cuda().double().transpose(0, 1).contiguous() for t in (q, k, v))  # [heads, rows, D]
+    kd, vd = kd.repeat_interleave(G, 0), vd.repeat_interleave(G, 0)
+    qp, kp = qp.cuda()[:, None], kp.cuda()[None]
+    unseen = ~((kp <= qp) & ((kp > qp - window) | (kp < sinks)))
+    kt = kd.transpose(1, 2).contiguous()
+    s = (torch.matmul(qd, kt) / math.sqrt(q.shape[2])).masked_fill(unseen, -math.inf)
+    size = (torch.matmul(qd.abs(), kt.abs()) / math.sqrt(q.shape[2])).masked_fill(unseen, 0.0).amax(-1)
+    lse = torch.logsumexp(s, -1)
+    p = torch.exp(s - lse[..., None])
+    o, mean = torch.matmul(p, vd), torch.matmul(p, vd.abs()).amax(-1)
+    return o.transpose(0, 1).cpu(), lse.T.cpu(), mean.T.cpu()[..., None], size.T.cpu()[..., None]
+
+
+EPS = 2.0 ** -24
+
+
+def _rel(D, n, size):
+    """As in the oracle: float32 sums of D products and of n weights in blocks of 32, twice."""
+    return 2 * ((D + 8) * EPS * size + 8 * EPS + (n / 32 + 40) * EPS)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("Hq,Hkv,D,lens", [(32, 8, 128, [700, 333, 900]), (32, 32, 128, [400, 400]), (32, 4, 64, [900, 1000])])
+def test_every_request_of_a_launch_that_fills_the_chip(lsa, rows, dtype, Hq, Hkv, D, lens):
+    """Many workgroups, 32 positions per wave, the requests in bunches or one after the other: all of them against float64."""
+    s = Step([(n, 0, n, 0) for n in lens] * (8 if D == 128 else 5), Hq, Hkv, D, DT[dtype], seed=36)
+    half = 2.0 ** -11 if s.dtype == torch.float16 else 2.0 ** -8
+    for window, sinks in ((128, 4), (250, 0)):
+        got = [t.cpu().double() for t in s.run(lsa, window, sinks)]
+        for (n, _, _, _), qs, ks in zip(s.seqs, s.q_start, s.k_start):
+            kv = s.kv[ks:ks + n]
+            o, lse, mean, size = _step64(s.q[qs:qs + n], kv[:, :Hkv], kv[:, Hkv:], torch.arange(n), torch.arange(n), window, sinks)
+            rel = _rel(D, n, size)
+            tol = (rel + 2.0 ** -11) * mean
+            assert ((got[0][qs:qs + n] - o).abs() <= tol + half * (o.abs() + tol) + 2.0 ** -24).all()
+            assert ((got[1][qs:qs + n] - lse).abs() <= rel[..., 0] + 8 * EPS * lse.abs()).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("n,P,W,S", [(300, 3, 70, 8), (1000, 2, 333, 0), (500, 4, 1, 5)])
+def test_striped_chunks_join_row_by_row(lsa, rows, dtype, n, P, W, S):
+    """P instances hold every P-th token; one instance's partials over all chunks, merged, against the step over all keys, each row by its own bound: a
+    partial's weight is exp of its log-sum-exp, off by a partial's tolerance in the numerator and in the sum."""
+    q, kv = _rows((n, 4, 128), 1, DT[dtype]), _rows((n, 4, 128), 2, DT[dtype])
+    for mine in range(P):
+        qs = q[mine::P].contiguous()
+        o, lse, mean, size = _step64(qs, kv[:, :2], kv[:, 2:], torch.arange(mine, n, P), torch.arange(n), W, S)
+        parts = []
+        for r in range(P):
+            rows_r = kv[r::P].contiguous().cuda()
+            po, pl = torch.empty(qs.shape, device="cuda"), torch.empty(qs.shape[:2], device="cuda")
+            lsa.window_attention_fwd(qs.cuda(), rows_r[:, :2], rows_r[:, 2:], po, _vec([0]), _vec([len(qs)]), _vec([mine]), _vec([0]), _vec([len(rows_r)]),
+                                     _vec([r]), P, len(qs), W, S, lse=pl)
+            parts.append((po, pl))
+        got = [t.cpu().double() for t in lsa.lse_merge(parts)]
+        rel = _rel(128, n, size)
+        of_a_part = rel + 8 * EPS * (size + math.log(n)) + 16 * EPS
+        assert ((got[0] - o).abs() <= (rel + 2.0 ** -11 + 2 * of_a_part) * mean + 2.0 ** -24).all()
+        assert ((got[1] - lse).abs() <= of_a_part[..., 0]).all()
