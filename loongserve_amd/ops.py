@@ -536,6 +536,9 @@ def kv_scatter(src: torch.Tensor, dest_index: torch.Tensor, pool: torch.Tensor) 
 
     Semantics of destindex_copy_kv
     (loongserve/common/basemodel/triton_kernel/destindex_copy_kv.py:31-51).
+
+    Rows are moved as bytes: of a pool in 8 bits (kv_scatter_fp8) the exponents of the same slots have to be moved by a call of their own,
+    with src and pool as [rows, heads] of uint8, where the heads are a multiple of 16; else by indexing (scales[new] = scales[old]).
     """
     if _native.kv_scatter(src, dest_index, pool):
         return
@@ -819,7 +822,10 @@ def destindex_copy_and_register_kv(batch_size: int, new_kv_cache_len: torch.Tens
     the slots in the request table.
 
     Signature and semantics of destindex_copy_and_register_kv
-    (loongserve/models/llama/triton_kernel/copy_and_register_kv.py:119-170)."""
+    (loongserve/models/llama/triton_kernel/copy_and_register_kv.py:119-170).
+
+    Rows are moved as bytes: of a pool in 8 bits (kv_scatter_fp8) the exponents of the same slots have to be moved by a call of their own:
+    kv and total_kv_cache as [rows, heads] of uint8 (heads a multiple of 16), should_register_kv False."""
     B = int(batch_size)
     if B == 0:
         return
@@ -883,7 +889,10 @@ def _migration_args(buf, req_to_token_indexes, kv_cache, request_ids, num_tokens
 def decoding_stage_migration_sender_kernel(send_buf, req_to_token_indexes, mem_state, kv_cache, request_ids, num_tokens, b_seq_len) -> None:
     """Gather the last num_tokens[b] tokens of every request from every layer of kv_cache into send_buf and mark their
     slots free.  Signature of decoding_stage_migration_sender_kernel
-    (loongserve/models/llama/triton_kernel/decoding_stage_migration.py:70-98)."""
+    (loongserve/models/llama/triton_kernel/decoding_stage_migration.py:70-98).
+
+    Rows are moved as bytes: of a pool in 8 bits (kv_scatter_fp8) the exponents of the same slots have to be moved by a call of their own,
+    send_buf and kv_cache as [layers, rows, heads, 1] of uint8 (kv_scales[..., None]; heads a multiple of 16)."""
     if request_ids.shape[0] == 0:
         return
     _i32vec(mem_state, "mem_state")
@@ -896,7 +905,8 @@ def decoding_stage_migration_sender_kernel(send_buf, req_to_token_indexes, mem_s
 def decoding_stage_migration_receiver_kernel(recv_buf, req_to_token_indexes, kv_cache, alloc_mem, request_ids, num_tokens, b_seq_len) -> None:
     """Store recv_buf into the freshly allocated slots of every layer of kv_cache and append the slots to the request
     table.  Signature of decoding_stage_migration_receiver_kernel
-    (loongserve/models/llama/triton_kernel/decoding_stage_migration.py:159-183)."""
+    (loongserve/models/llama/triton_kernel/decoding_stage_migration.py:159-183).  The exponents of a pool in 8 bits are received
+    by a call of their own, as the sender sends them."""
     if request_ids.shape[0] == 0:
         return
     alloc_mem = _slots(alloc_mem, "alloc_mem")

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import pool8_oracle as orc
-from tests.test_gpu_pool8 import Case
+from tests.test_gpu_pool8 import PAD, Case
 
 K8 = ["e4m3-f16", "e4m3-bf16"]
 
@@ -181,3 +181,53 @@ def test_exponents_as_e8m0(lsa, kind, lens):
         lsa.kv_gather_fp8(pool, sc.view(t), idx.int().view(1, 7), i(0), i(7), i(0), 7, out)
         outs.append((pool.view(torch.uint8), sc, out))
     assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [70, 3001])
+def test_rows_move_with_their_exponents(lsa, n):
+    """The decoding-stage migration, the context migration and kv_scatter on a pool in 8 bits: rows and, in a second call, exponents; decode gives
+    the same bits from the new slots."""
+    L, H, Hq, D, slots = 2, 8, 16, 128, 4000
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    g = torch.Generator().manual_seed(n)
+    rows = torch.randn(L, n, 2 * H, D, generator=g) * torch.exp(3 * torch.randn(L, n, 2 * H, 1, generator=g))
+    mem, there = (lsa.LongServeMemoryManager(slots, torch.float8_e4m3fn, H, D, L) for _ in range(2))
+    at = torch.randperm(slots, generator=g)[:n].cuda()
+    for layer in range(L):
+        lsa.kv_scatter_fp8(rows[layer].half().cuda(), at, mem.kv_buffer[layer], mem.kv_scales[layer])
+    q = torch.randn(1, Hq, D, generator=g).half().cuda()
+    table = torch.full((3, n + 7), PAD, dtype=torch.int32, device="cuda")
+    table[1, :n] = at.int()
+
+    def decode(pool, scales, t):
+        return lsa.longserve_fp8_decode_attention(q, t, i(1), i(n), n, pool[:, :H], pool[:, H:], scales[:, :H], scales[:, H:])
+    want = [decode(mem.kv_buffer[layer], mem.kv_scales[layer], table) for layer in range(L)]
+
+    def same(pool, scales, t):
+        for layer in range(L):
+            # (as bits: a row past fp16 is infinite, so NaN in the pool)
+            assert all(torch.equal(x.view(torch.int32), y.view(torch.int32)) for x, y in zip(decode(pool[layer], scales[layer], t), want[layer]))
+    # the decoding-stage migration of the whole context
+    to = torch.randperm(slots, generator=g)[:n].to(torch.int32).cuda()
+    state, new = torch.ones(slots, dtype=torch.int32, device="cuda"), torch.full_like(table, PAD)
+    for src, dst in ((mem.kv_buffer, there.kv_buffer), (mem.kv_scales[..., None], there.kv_scales[..., None])):
+        buf = torch.zeros((L, n, *src.shape[2:]), dtype=torch.uint8, device="cuda").view(src.dtype)
+        lsa.decoding_stage_migration_sender_kernel(buf, table, state, src, i(1), i(n), i(n))
+        lsa.decoding_stage_migration_receiver_kernel(buf, new, dst, to, i(1), i(n), i(0))
+    assert torch.equal(new[1, :n], to) and int((state == 0).sum()) == n
+    same(there.kv_buffer, there.kv_scales, new)
+    # packed rows copied into their slots and registered; and row by row, from one slot to another
+    for how in ("register", "scatter"):
+        pool, scales = torch.zeros_like(there.kv_buffer.view(torch.uint8)), torch.zeros_like(there.kv_scales)
+        new = torch.full_like(table, PAD)
+        for layer in range(L):
+            for k, (src, dst) in enumerate(((mem.kv_buffer.view(torch.uint8)[layer], pool[layer]), (mem.kv_scales[layer], scales[layer]))):
+                if how == "register":
+                    lsa.destindex_copy_and_register_kv(1, i(n), i(0), i(n), torch.tensor([n], device="cuda"), src[at].contiguous(), i(0), i(0), to, dst, new, i(1),
+                                                       0, n, layer == 0 and k == 0)
+                else:
+                    lsa.kv_scatter(src[at].contiguous(), to, dst)
+        if how == "scatter":
+            new[1, :n] = to
+        same(pool.view(torch.float8_e4m3fn), scales, new)
