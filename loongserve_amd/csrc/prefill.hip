@@ -1602,9 +1602,12 @@ extern "C" int lsattn_prefill_step_accumulate(const lsattn_prefill_args* a, void
 
 // Whether a step behind a window runs in the 256-row shape: the more keys a workgroup walks the better it does (fewer reads of a key, more of its time
 // in iterations without a mask), and packed heads leave a workgroup fewer positions, so fewer keys that only some of its rows see.  Measured (microseconds, this shape | the short prompts' kernel; fp16, 4 sinks):
-//   32768 tokens 32/8, windows of 512, 1024, 2048: 536 | 424, 798 | 666, 1235 | 1146; 8192 tokens, 4096: 416 | 403 (bf16 415 | 424); 8/1 32768, 4096: 521 | 532 (510 | 561);
-//   65536, 8192: 7313 | 7936; 32/32 32768, 2048: 1472 | 1260, 8192: 3788 | 4090, 8192 tokens, 4096: 469 | 424; 16 x 1024 32/8 254 | 182
-// bfloat16 adds the copy of V here and a conversion per tile there, which moves none of these far.
+//   four or eight heads packed: 32768 tokens 32/8, windows of 512, 1024, 1536, 2048, 4096: 477 | 414, 682 | 660, 888 | 902, 1086 | 1135, 1850 | 2010 (bf16 692 | 697, 1079 | 1199 behind 1024 and 2048);
+//   8192 tokens, 2048, 4096: 263 | 256, 379 | 403 (bf16 263 | 271, 371 | 429); 8/1 32768, 1024, 2048, 4096: 170 | 169, 273 | 292, 477 | 527; 16384 16/2, 2048: 275 | 280; 16 x 1024, 2048, 8 x 4096 32/8 behind 1024, 2048,
+//   2048: 208 | 182, 624 | 617, 874 | 897; ragged, 2000 tokens in the mean, 2048: 264 | 254
+//   others: 32/32 32768, 2048, 4096, 8192: 1324 | 1260, 2170 | 2233, 3643 | 4024 (bf16 1351 | 1327, 2180 | 2358, 3612 | 4258), 8192 tokens, 2048, 4096: 296 | 276, 431 | 425 (bf16 446 | 450);
+//   16384 tokens 28/4, 2048, 4096: 533 | 489, 812 | 830; 16/8 (two packed): 290 | 280, 480 | 480
+// bfloat16 adds the copy of V here and a conversion per tile there.
 static bool window_in_256_rows(const lsattn_prefill_args* a, int32_t window) {
   if (a->head_dim != 128) return false;
   const Tuning tn = tuning();
@@ -1614,7 +1617,7 @@ static bool window_in_256_rows(const lsattn_prefill_args* a, int32_t window) {
   if (wgs < kCUs) return false;
   int64_t keys = window / (a->sp_peers > 1 ? a->sp_peers : 1);  // (the window's on this rank, at most what a request has in the mean)
   if (a->total_kv_rows > 0 && a->total_kv_rows / a->batch < keys) keys = a->total_kv_rows / a->batch;
-  return keys >= (ps ? 4096 : 8192);
+  return keys >= (ps >= 2 ? 2048 : 4096);
 }
 
 extern "C" int lsattn_prefill_window_converts_v(const lsattn_prefill_args* a, int64_t window) {

@@ -132,8 +132,8 @@ __device__ __forceinline__ const char* uniform_ptr(const char* ptr) {
 // 128-wide heads, 32 positions per wave: three stages of 32 keys (48 KB) and at most 168 registers (158; 168 where V is bfloat16), so that three
 // workgroups fit a CU.
 // Behind a window (WIN) the compiler's registers do not fit those 168 (22 to 38 spills, 3.07 ms for 32768 tokens behind 4096 + 16, 32/8 heads; 2.30 with two workgroups per CU): two stages
-// of 64 keys there, operands and addresses in registers of their own (4096 tokens behind 1024, 32/32: 591 -> 642 TFLOP/s; these figures
-// before the maxima had headroom, with it 725).
+// of 64 keys there, operands and addresses in registers of their own (4096 tokens behind 1024, 32/32: 591 -> 642 TFLOP/s).  (Figures of the
+// time, when maxima were raised more often; 2.0 ms now.)
 template <int D, int WP, bool WIN> constexpr int kTileOf = D == 128 && WP == 32 && !WIN ? 32 : 64;
 template <int D, int WP, bool WIN> constexpr int kStagesOf = D == 128 && WP == 32 && !WIN ? 3 : 2;
 template <int D, int WP, bool DV, bool WIN> constexpr int kResident = D == 128 ? (WP == 32 && !WIN ? 3 : 2) : WP == 32 && D == 64 && !DV ? 3 : 4;
@@ -767,8 +767,8 @@ template <typename T, int D, int MODE, bool DV, int WP, int KP = 1, bool WIN = f
   const int64_t rows_wg = (kWaves * WP) >> p.pack_shift;
   Order order = WP == 32 ? order_of(a, p.pack_shift) : Order{p.batch, false};
   // Behind a window a request's tiles are all alike but the first ones and read K/V of their own, and a ragged batch goes one request after the other: that
-  // leaves no ids without work among those of the longest.  Windows of 1024, microseconds, in turn | the order above: 6 x 700..4000 32/8 190 | 228, 8/1
-  // 61 | 73, 64-wide 32/8 110 | 124, 5 x 700..7400 32/8 471 | 625, 24 x 50..1500 8/1 61 | 70; 32/32 and 64/8 within 3 %; 5 x 2000..6200 8/1 95 | 91, 4 x 300..1200 32/8 38 | 33.
+  // leaves no ids without work among those of the longest.  Windows of 1024, microseconds, in turn | the order above: 6 x 700..4000 32/8 189 | 225, 8/1
+  // 61 | 75, 64-wide 32/8 110 | 122, 32/32 226 | 221, 5 x 700..7400 32/8 327 | 327, 24 x 50..1500 8/1 64 | 61, 5 x 2000..6200 8/1 101 | 98, 4 x 300..1200 32/8 39 | 37.
   if (WIN && WP == 32 && ragged(a)) order = Order{1, false};
   p.bunch = (int32_t)order.bunch;
   p.d_bunch = fast_div((uint32_t)p.bunch);
@@ -974,10 +974,10 @@ SmallParams params_of(const lsattn_prefill_args* a) {
   return p;
 }
 
-// A step behind a window: 32 positions per wave, or 16 where those make fewer than three workgroups per CU.
+// A step behind a window: 32 positions per wave, or 16 where those make fewer than one and a half workgroups per CU (128-wide heads), three (the others).
 // Two waves share a wave's positions behind a window as well, up to a workgroup per CU: microseconds, one wave each | two; 128-wide heads: 300 tokens
-// 32/8 behind 256 9.6 | 9.2, 1024 8/1 behind 512 14.8 | 13.0, 2048 behind 1024 22.6 | 19.2, bf16 25.9 | 21.7; 64-wide 17.2 | 15.1; with the maxima raised as often as elsewhere 100
-// tokens behind 64 were 6.5 | 6.8, and past a workgroup per CU (777 tokens 32/8) behind 512 18.1 | 19.2, 1024 behind 512 18.8 | 25.3.
+// 32/8 behind 256 9.7 | 9.1, 1024 8/1 behind 512 14.2 | 12.7, 2048 behind 1024 22.0 | 18.7, bf16 25.5 | 21.4; 64-wide 16.4 | 14.7; 100 tokens behind 64 6.4 | 6.5, and past a
+// workgroup per CU (777 tokens 32/8) behind 512 16.1 | 16.8, 1024 behind 512 17.1 | 21.4.
 bool two_waves_share_window(const lsattn_prefill_args* a, int pack_shift, int64_t window) {
   int64_t keys = a->total_kv_rows / a->batch;
   if (a->total_kv_rows <= 0) keys = window;
@@ -985,8 +985,8 @@ bool two_waves_share_window(const lsattn_prefill_args* a, int pack_shift, int64_
   return workgroups(a, pack_shift, 1) <= kCUs && (keys < window ? keys : window) >= 256;
 }
 template <typename T, int D, int MODE, bool DV> int launch_window_rows(const SmallParams& p, const lsattn_prefill_args* a, hipStream_t st) {
-  // (128-wide heads fit two workgroups of 32 positions per wave on a CU; 32/8, microseconds, 16 | 32: 1300 tokens behind 512 and 1024 21.8 | 23.1, 25.1 | 33.4;
-  // 1500 26.9 | 23.9, 30.1 | 34.0; 1800 31.4 | 28.7, 40.2 | 35.3; 2300 38.5 | 31.4, 49.7 | 44.6; 8192 8/1 behind 1024 55.9 | 45.1; 64-wide 2300 28.4 | 32.4)
+  // (128-wide heads fit two workgroups of 32 positions per wave on a CU; 32/8, microseconds, 16 | 32: 1300 tokens behind 512 and 1024 23.6 | 23.3, 25.2 | 32.7;
+  // 1500 26.7 | 23.2, 30.3 | 33.5; 1800 30.9 | 27.8, 40.9 | 34.7; 2300 37.5 | 31.5, 50.0 | 44.6; 8192 8/1 behind 1024 55.5 | 44.2; 64-wide behind 1024 2300 28.6 | 31.5, 4000 49.7 | 45.6)
   if (2 * workgroups(a, p.pack_shift, 2) < (D == 128 ? 3 : 6) * kCUs) {
     if constexpr (D >= 64)
       if (two_waves_share_window(a, p.pack_shift, p.window)) return launch_rows<T, D, MODE, DV, 16, 2, true>(p, a, st);
