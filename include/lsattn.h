@@ -624,9 +624,9 @@ int lsattn_kv_gather_fp8(const lsattn_kv_gather_fp8_args* a, void* stream);
  * Decode attention over a token-indexed pool in 16 or 8 bits, with an optional sliding window and sinks; one new token per
  * request, whose query sees positions j < n = b_seqlen[b] of its row of the table with j >= n - window or j < sinks:
  *   o[b, h] = sum_j softmax_j(sm_scale * q[b, h] . k_j) v_j,   lse[b, h] = natural log-sum-exp of the scores
- * (o = 0, lse = -inf where nothing is seen).  Rows and exponents that are not seen do not matter, whatever bytes lie
- * there (slot 0 is read where a position does not exist, and dropped).  Table entries outside [0, num_slots) count as positions that do not exist,
- * so do positions past max_seq_len and requests outside [0, num_reqs).
+ * (o = 0, lse = -inf where nothing is seen).  Exponent bytes of rows that are seen are as lsattn_kv_scatter_fp8 writes them (1 .. 247); rows and
+ * exponents that are not seen do not matter, whatever bytes lie there (slot 0 is read where a position does not exist, and dropped).  Table entries
+ * outside [0, num_slots) count as positions that do not exist, so do positions past max_seq_len and requests outside [0, num_reqs).
  * window = 0: none (sinks is not read).  A request's whole context lies in this pool; partials over disjoint keys (windowless
  * ones of several instances) can be merged by lsattn_lse_merge or lsattn_decode_stage2.
  * max_len_in_batch only steers the launch.  The partials of launches that cut the contexts need

@@ -29,7 +29,7 @@
 // all requests are dealt to the waves in equal shares, whatever the requests' lengths are (the host does not know them);
 // a wave leaves one partial per request it touches, and a second launch merges them.
 // Measured (32 / 8 heads of 128): 64 requests of 4096 .. 32768 tokens in 8 bits 408 us (5.9 TB/s), 96 behind a window of 16-bit rows 231 (6.2 TB/s); one request of 2047
-// tokens 10.5, of 131072 55.
+// tokens 10.7, of 131072 55.
 #include "common.hip.h"
 
 namespace lsattn {
@@ -663,12 +663,19 @@ __global__ __launch_bounds__(256) void pool_decode_merge_kernel(PoolParams p) {
 }
 
 constexpr int kDirectWaves = 4;
-// A workgroup takes a whole (request, KV head) where the longest request's visible tokens are few for the workgroups there are: 8 bits, 32 / 8 heads of 128, cold, against
-// shares (microseconds): 1 request of 512 tokens 8.4 (11.8), of 768 11.8 (11.5), of 1024 13.3 (11.6); 16 of 1024 15.6 (14.7), 32 of 1024 19.3 (23.1), of 2048 35.1 (34.7), 16 of
-// 2048 28.9 (21.9); 256 of 512 73 (89); 8 / 1 heads 64 of 1024 12.2 (15.1), 256 of 2048 31.8 (45.6); 32 / 32 32 of 2048 126 (113).
+// A workgroup takes a whole (request, KV head) where the longest request's visible tokens are few for the workgroups there are.  Microseconds on a cold pool, a workgroup | shares,
+// heads of 128, 8 bits (16 bits):
+//   32/8: 1 request of 512 tokens 9.2 | 11.5 (11.0 | 13.1), 768 11.5 | 11.7 (13.6 | 13.1), 1024 13.8 | 11.9 (16.8 | 13.2); 16 of 768 13.4 | 15.5 (17.4 | 19.3), 1024 16.8 | 16.4 (21.4 | 21.2),
+//   2048 30.3 | 23.5 (36.9 | 31.3); 32 of 512 13.6 | 18.4 (16.5 | 21.8), 1024 20.8 | 23.4 (27.5 | 32.4), 2048 36.3 | 36.4 (49.8 | 53.4); 64 of 2048 66.4 | 62.6 (94.4 | 96.8); 256 of 512
+//   75.4 | 91.6 (105.7 | 124.1), 2048 259 | 244 (371 | 377)
+//   8/1: 16 of 1024 13.7 | 13.4 (15.1 | 14.1); 256 of 1024 20.1 | 31.9 (29.0 | 41.9), 2048 34.2 | 46.2 (52.2 | 64.9)
+//   32/32: 1 of 768 13.3 | 13.6 (14.2 | 13.5), 1024 15.5 | 13.9 (17.5 | 14.2); 32 of 1024 66.7 | 61.8 (92.1 | 93.5), 2048 127 | 113 (179 | 175); 64/4: 32 of 1024 19.3 | 23.8 (28.9 | 29.9),
+//   2048 32.7 | 33.0 (52.2 | 46.1)
+// Length and workgroups alone do not tell all of it: in 8 bits this rule takes the slower form for 2048 tokens of 64 and more requests (6 %) and of
+// 32 with 32/32 heads (12 %; 1024 tokens 8 %), in 16 bits for 32 of 2048 with 64/4 (13 %).
 // Waves that a launch of shares deals to: one per SIMD.  More leave shorter shares, whose starts and partials cost more than the loads in flight bring (microseconds, cold;
-// 4 | 8 in 16 bits, 12 in 8, of a CU's waves): 8 bits 1 request of 32768 27 | 36, 32 of 8192 116 | 131, 64 of 4096 .. 32768 469 | 482, 64-wide 84 | 96; 16 bits 8 behind
-// 8192 33.1 | 34.8, 128 678 | 689.  Numbers that leave the SIMDs of a CU with unequal counts lose a fifth: 3 134, 5 154, 6 139 for the 32.
+// 4 | 8 of a CU's waves): 8 bits 1 request of 32768 24.0 | 25.3, 32 of 8192 112 | 115, 64 of 4096 .. 32768 465 | 465, 32 of 8192 64-wide 86 | 94; 16 bits 8 behind
+// 8192 52.4 | 55.2, 128 681 | 688.  Numbers that leave the SIMDs of a CU with unequal counts lose a fifth: 3 134, 5 154, 6 139 for the 32 when 4 took 116.
 constexpr int64_t kShareWaves = 4 * kCUs;
 constexpr int64_t kMinUnits = 2;
 

@@ -466,7 +466,8 @@ def window_attention_fwd(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_g
     log-sum-exp, float32 [tokens, q_heads], is optional.  Rows that see no key get o = 0, lse = -inf (all of them where k and v have no rows); rows that no
     request names stay as they were.  A chunk of a longer prompt brings its context in k and v (kv_gather_fp8 reads one back
     from an 8-bit pool) and the position of its first query in q_first_token_global_idx.  Requests share no
-    rows of q: total_q_len, an upper bound of all their lengths together, is q's rows unless given.  A bfloat16 v is multiplied as float16: magnitudes past 65504 count as 65504.  V rows of keys near
+    rows of q: total_q_len, an upper bound of all their lengths together, is q's rows unless given.  A row's weights are rounded to float16 for the product with v, whatever o's type is (11 bits down to
+    2^-23 of the row's largest), and a bfloat16 v is multiplied as float16: magnitudes past 65504 count as 65504, below 2^-14 they are cut to multiples of 2^-24.  V rows of keys near
     a window that a query does not see are multiplied by a weight of zero: they have to be finite (K rows may hold anything)."""
     if window is not None and _native.window_attention(q, k, v, o, q_b_start_loc, q_b_seq_len, q_first_token_global_idx, kv_b_start_loc, kv_b_seq_len,
                                                        kv_first_token_global_idx, logical_sp_peers_num, max_q_b_seq_len, window, sinks, lse,
