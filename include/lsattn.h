@@ -596,7 +596,7 @@ int lsattn_kv_scatter_fp8(const lsattn_kv_scatter_fp8_args* a, void* stream);
 /*
  * lsattn_kv_gather_fp8: contexts back in 16 bits, one request after the other, as lsattn_prefill_step takes them:
  *   out[b_start_loc[b] + i] = q * 2^e of slot req_to_tokens[b_req_idx[b], b_first[b] + i]   for i < min(b_seq_len[b], max_len_in_batch),
- * rounded to out's type (exact in its normal range; past fp16's range +-65504).  b_first NULL: 0.  A token whose table entry
+ * rounded to out's type (exact in its normal range; past its range its largest value, +-65504 for fp16).  b_first NULL: 0.  A token whose table entry
  * or position does not exist is a row of zeros; rows outside [0, out_rows) are not written, no others than those above are.
  */
 typedef struct lsattn_kv_gather_fp8_args {

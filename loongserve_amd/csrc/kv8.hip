@@ -93,13 +93,19 @@ struct Read8Params {
   FastDiv by_parts;
 };
 
-// 2^e times an e4m3 value as 16 bits: one rounding (none in the normal range of the type).  What lies past fp16's range (a row
-// whose maximum rounded up to 65536) becomes +-65504, NaN stays.
+// 2^e times an e4m3 value as 16 bits: one rounding (none in the normal range of the type).  What lies past the type's range (a row
+// whose maximum rounded up to 65536, or to 2^128) becomes its largest value, NaN stays.
 template <typename T> __device__ __forceinline__ uint32_t pack2_in_range(float a, float b) { return pack2<T>(a, b); }
 template <> __device__ __forceinline__ uint32_t pack2_in_range<F16>(float a, float b) {
   a = fabsf(a) > 65504.f ? copysignf(65504.f, a) : a;
   b = fabsf(b) > 65504.f ? copysignf(65504.f, b) : b;
   return pack2<F16>(a, b);
+}
+// (bfloat16: infinities of a pair as the largest value)
+__device__ __forceinline__ uint32_t finite_bf16(uint32_t w) {
+  if ((w & 0x7fffu) == 0x7f80u) w -= 1;
+  if ((w & 0x7fff0000u) == 0x7f800000u) w -= 0x10000u;
+  return w;
 }
 
 template <typename T, int D>
@@ -129,6 +135,11 @@ __global__ __launch_bounds__(256) void kv_gather_fp8_kernel(Read8Params p) {
         const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], true);
         r[2 * k] = pack2_in_range<T>(lo[0] * scale, lo[1] * scale);
         r[2 * k + 1] = pack2_in_range<T>(hi[0] * scale, hi[1] * scale);
+      }
+      // (only rows of the largest exponent hold such; a look at every value costs 5 %)
+      if (!__is_same(T, F16) && __builtin_amdgcn_ballot_w64(byte >= 247) != 0) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) r[k] = finite_bf16(r[k]);
       }
       o0 = u32x4{r[0], r[1], r[2], r[3]};
       o1 = u32x4{r[4], r[5], r[6], r[7]};

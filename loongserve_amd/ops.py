@@ -607,8 +607,8 @@ def kv_gather_fp8(pool: torch.Tensor, scales: torch.Tensor, req_to_token_indexs:
 
       out[b_start_loc[b] + i] = value of slot req_to_token_indexs[b_req_idx[b], b_first[b] + i]   for i < b_seq_len[b]
 
-    out is float16 or bfloat16 [rows, heads, head_dim]; every value is exact in its normal range (past float16's range
-    +-65504).  b_first (None: 0) starts a request's rows further on in its context.  max_len_in_batch bounds b_seq_len.  A token
+    out is float16 or bfloat16 [rows, heads, head_dim]; every value is exact in its normal range (past its range the
+    type's largest value, +-65504 for float16).  b_first (None: 0) starts a request's rows further on in its context.  max_len_in_batch bounds b_seq_len.  A token
     whose slot is not in the pool (an unused entry of the table) is a row of zeros; rows of out that no request names stay as
     they were.  The next chunk of a prompt attends to the result through context_attention_fwd or prefill_attention_step."""
     if _native.kv_gather_fp8(pool, scales, req_to_token_indexs, b_req_idx, b_seq_len, b_start_loc, max_len_in_batch, out, b_first):

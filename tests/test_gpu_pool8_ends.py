@@ -231,3 +231,49 @@ def test_rows_move_with_their_exponents(lsa, n):
         if how == "scatter":
             new[1, :n] = to
         same(pool.view(torch.float8_e4m3fn), scales, new)
+
+
+@pytest.mark.gpu
+def test_rows_at_the_ends_of_bfloat16(lsa):
+    """Subnormal rows, the largest finite ones, and both in one row: bits and exponents as defined; read back as the value, to bfloat16's last bit."""
+    D = 128
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(12, 2, D, generator=g, dtype=torch.float64)
+    x = (x / x.abs().amax(-1, keepdim=True)).clamp(-1, 1)
+    for t, top in enumerate([2.0 ** -133, 2.0 ** -130, 2.0 ** -127, 2.0 ** -126, 2.0 ** -118, 448 * 2.0 ** -126, 449 * 2.0 ** -126, 2.0 ** -100, 2.0 ** 100, 2.0 ** 127,
+                             3.38e38, 3.3895313892515355e38]):
+        x[t] *= top
+    src = x.to(torch.bfloat16)
+    src[-1, 0, 0], src[-1, 1, 1], src[-2, 0, :4] = 3.3895313892515355e38, -3.3895313892515355e38, torch.tensor([2.0 ** -133, -2.0 ** -130, 1.0, 0.0]).to(torch.bfloat16)
+    pool = torch.zeros(12, 2, D, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    sc = torch.zeros(12, 2, dtype=torch.uint8, device="cuda")
+    lsa.kv_scatter_fp8(src.cuda(), torch.arange(12, device="cuda"), pool, sc)
+    q, e = orc.quantise(src)
+    assert torch.equal(pool.cpu().double(), q) and torch.equal(sc.cpu().long(), e)
+    assert int(e.min()) == 1 and int(e.max()) == 247
+    out = torch.zeros(12, 2, D, dtype=torch.bfloat16, device="cuda")
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    lsa.kv_gather_fp8(pool, sc, torch.arange(12, dtype=torch.int32, device="cuda").view(1, 12), i(0), i(12), i(0), 12, out)
+    value = q * torch.pow(2.0, (e - 127).double())[..., None]
+    want = value.clamp(-3.3895313892515355e38, 3.3895313892515355e38).to(torch.bfloat16).double()
+    assert (value.abs() > 3.39e38).any()  # (the largest ones round up to 2^128 as they are written, and come back as the largest bfloat16)
+    assert ((out.cpu().double() - want).abs() <= 2.0 ** -133 * (value.abs() < 2.0 ** -126)).all()  # (a step of the subnormal ones)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["f16", "e4m3-bf16"])
+def test_two_calls_at_once(lsa, kind):
+    """Two streams, each with launches of its own that cut the contexts (scratch of their own from the allocator)."""
+    cases = [Case(kind, 2, 8, 2, 128, lens, seed=s) for s, lens in ((40, [9000, 77]), (41, [5000, 8000]))]
+    want = [[t.clone() for t in c.run(lsa)] for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for c, st, g in zip(cases, streams, got):
+            with torch.cuda.stream(st):
+                g.append(c.run(lsa))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for r in g:
+            assert torch.equal(r[0], w[0]) and torch.equal(r[1], w[1])
