@@ -138,3 +138,56 @@ def test_striped_chunks_join_row_by_row(lsa, rows, dtype, n, P, W, S):
         of_a_part = rel + 8 * EPS * (size + math.log(n)) + 16 * EPS
         assert ((got[0] - o).abs() <= (rel + 2.0 ** -11 + 2 * of_a_part) * mean + 2.0 ** -24).all()
         assert ((got[1] - lse).abs() <= of_a_part[..., 0]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [32, 64, 128])
+@pytest.mark.parametrize("o_dtype", [None, torch.float32])
+@pytest.mark.parametrize("lens", [[130, 301], [1700, 900]])
+def test_outputs_and_queries_inside_wider_rows(lsa, rows, dtype, D, o_dtype, lens):
+    """q and o as slices of wider rows and heads: the same bits as packed, nothing written beside them."""
+    Hq, Hkv = 16, 4
+    s = Step([(n, 0, n, 0) for n in lens], Hq, Hkv, D, DT[dtype], seed=41)
+    want = s.run(lsa, 90, 3, o_dtype=o_dtype)
+    n = s.q.shape[0]
+    wide_q = torch.full((n, Hq + 5, D + 16), 3.0, dtype=s.dtype, device="cuda")
+    wide_q[:, 2:2 + Hq, 8:8 + D] = s.q.cuda()
+    wide_o = torch.full((n, Hq + 3, D + 8), 7.0, dtype=o_dtype or s.dtype, device="cuda")
+    o, l = wide_o[:, 1:1 + Hq, 8:], torch.full((n, Hq), 7.0, device="cuda")
+    col = lambda i: _vec([t[i] for t in s.seqs])  # noqa: E731
+    kv = s.kv.cuda()
+    lsa.window_attention_fwd(wide_q[:, 2:2 + Hq, 8:8 + D], kv[:, :Hkv], kv[:, Hkv:], o, _vec(s.q_start), col(0), col(1), _vec(s.k_start), col(2), col(3), 1, max(lens), 90, 3,
+                             lse=l)
+    assert torch.equal(o, want[0]) and torch.equal(l, want[1])
+    wide_o[:, 1:1 + Hq, 8:] = 7.0
+    assert (wide_o == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_padded_batch_of_many_requests(lsa, rows, D):
+    """Three hundred requests, most of them without rows."""
+    r = torch.Generator().manual_seed(42)
+    lens = [int(torch.randint(1, 90, (1,), generator=r)) if i % 7 == 3 else 0 for i in range(300)]
+    s = Step([(n, i % 40, n + i % 40, 0) if n else (0, 0, i % 5, 0) for i, n in enumerate(lens)], 4, 2, D, torch.float16, seed=43)
+    s.check(s.run(lsa, 33, 4), 33, 4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(DT))
+def test_rows_past_four_gigabytes(lsa, rows, dtype):
+    """K/V rows more than 2^33 bytes, q and o rows more than 2^32 bytes behind the first."""
+    Hq, Hkv, D, nq, nk, n = 32, 8, 128, 600000, 2200000, 333
+    q, kv = (torch.empty(m, h, D, dtype=DT[dtype], device="cuda") for m, h in ((nq, Hq), (nk, 2 * Hkv)))
+    o, l = torch.full((nq, Hq, D), 7.0, dtype=DT[dtype], device="cuda"), torch.full((nq, Hq), 7.0, device="cuda")
+    qs, kvs = _rows((n, Hq, D), 5, DT[dtype]), _rows((n, 2 * Hkv, D), 6, DT[dtype])
+    q[nq - n:], kv[nk - n:] = qs.cuda(), kvs.cuda()
+    lsa.window_attention_fwd(q, kv[:, :Hkv], kv[:, Hkv:], o, _vec([nq - n]), _vec([n]), _vec([0]), _vec([nk - n]), _vec([n]), _vec([0]), 1, n, 100, 2, lse=l)
+    want, lse, mean, size = _step64(qs, kvs[:, :Hkv], kvs[:, Hkv:], torch.arange(n), torch.arange(n), 100, 2)
+    rel = _rel(D, n, size)
+    tol = (rel + 2.0 ** -11) * mean
+    half = 2.0 ** -11 if dtype == "f16" else 2.0 ** -8
+    assert ((o[nq - n:].cpu().double() - want).abs() <= tol + half * (want.abs() + tol) + 2.0 ** -24).all()
+    assert ((l[nq - n:].cpu().double() - lse).abs() <= rel[..., 0] + 8 * EPS * lse.abs()).all()
+    assert (o[:nq - n:997] == 7).all() and (o[nq - n - 400:nq - n] == 7).all() and (l[:nq - n] == 7).all()
