@@ -469,7 +469,7 @@ def run(state):
             s["m"].fill_(-math.inf)
             s["l"].zero_()
             lsa.shared_prefix_attention_fwd(s["q"], s["pool"][:, :hkv], s["pool"][:, hkv:], s["o"], s["g_start"], s["g_size"], s["table"], s["g_req"],
-                                            s["g_prefix"], s["longest_rows"], s["longest_prefix"], s["m"], s["l"], total_q_len=s["q"].shape[0])
+                                            s["g_prefix"], s["longest_rows"], s["longest_prefix"], s["m"], s["l"])
             return s["o"], torch.log2(s["l"]).add_(s["m"]).mul_(math.log(2.0))
         if c["kind"] == "fork":
             if not c["copies"]:
