@@ -661,6 +661,150 @@ size_t lsattn_pool_attention_workspace_bytes(int64_t batch, int64_t num_q_heads,
 int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* stream);
 
 /*
+ * Decode attention for requests that share the first tokens of their contexts; one new token per request.  Group g are the requests
+ * g_start_loc[g] .. + g_size[g] - 1 of the batch; the first g_prefix_len[g] positions of each are the slots that row g_req_idx[g] of the table
+ * names there (the members' own rows are not read so far), positions behind them are those of the request's own row:
+ *   o[b, h] = sum_j softmax_j(sm_scale * q[b, h] . k_j) v_j  over the b_seqlen[b] positions j,   lse[b, h] = natural log-sum-exp of the scores
+ * (o = 0, lse = -inf where there is none).  A prefix's rows are read once for 128 query rows of the group.  Groups stand in ascending order of their requests; a
+ * request that two groups name belongs to the first of them, one that no group names, or that is shorter than its group's prefix, shares nothing: its
+ * own row of the table has all its positions.  Table entries outside [0, num_slots) count as positions that do not exist, so do positions past max_seq_len
+ * and rows outside [0, num_reqs).  P is held in the type of V (bfloat16: in two parts) and O divided by the sum of the weights so rounded.
+ * max_prefix_len bounds g_prefix_len: of a longer prefix the first max_prefix_len positions are shared.  max_own_len (a bound of the positions behind the prefix) only
+ * steers the launch.
+ * Workspace: lsattn_shared_decode_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant before and after; calls that overlap in time need one each.
+ * No counterpart in the reference.
+ */
+typedef struct lsattn_shared_decode_args {
+  const void* q;                /* [batch, num_q_heads, head_dim] contiguous */
+  const void* k;                /* [num_slots, num_kv_heads, head_dim], the last dimension contiguous */
+  const void* v;
+  int64_t k_stride_0, k_stride_1, v_stride_0, v_stride_1; /* elements; rows 16-byte aligned */
+  const int32_t* req_to_tokens; /* [num_reqs, max_seq_len] contiguous */
+  const int32_t* b_req_idx;     /* [batch] */
+  const int32_t* b_seqlen;      /* [batch], prefixes included */
+  const int32_t* g_start_loc;   /* [num_groups] */
+  const int32_t* g_size;        /* [num_groups] */
+  const int32_t* g_req_idx;     /* [num_groups] */
+  const int32_t* g_prefix_len;  /* [num_groups] */
+  int64_t batch, num_groups, num_q_heads, num_kv_heads, head_dim; /* head_dim 64 or 128 */
+  int64_t num_slots, num_reqs, max_seq_len, max_prefix_len, max_own_len;
+  int32_t dtype;                /* of q, k and v: LSATTN_F16 or LSATTN_BF16 */
+  int32_t o_dtype;              /* LSATTN_F32, LSATTN_F16 or LSATTN_BF16 */
+  float sm_scale;               /* > 0 */
+  int32_t reserved;
+  void* o;                      /* [batch, num_q_heads, head_dim] contiguous */
+  float* lse;                   /* [batch, num_q_heads] contiguous */
+  void* workspace;
+  size_t workspace_bytes;
+} lsattn_shared_decode_args;
+size_t lsattn_shared_decode_workspace_bytes(int64_t batch, int64_t num_groups, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                            int64_t max_prefix_len, int64_t max_own_len);
+int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* stream);
+
+/*
+ * The prompts' step over the same prefixes: rows g_start_loc[g] .. + g_size[g] - 1 of q (tokens of any requests of the group, none of which is
+ * masked from the prefix) against the first g_prefix_len[g] positions of row g_req_idx[g] of the table, folded in place into (o, m, l) as
+ * lsattn_prefill_step_merge folds a step (ring_context_flashattention_nopad.py:171-188); the requests' own chunks are further steps of that kind, in any order.  Rows of no
+ * group, and rows that see no key, stay as they are.  Groups and table entries as in lsattn_shared_decode; prefixes longer than max_prefix_len are cut there.
+ * max_group_rows bounds g_size (rows past it may stay uncomputed).  Few rows are taken against the pool's rows where they lie; for many the prefix is laid out once
+ * in the workspace for the prefill kernel (a bfloat16 V as fp16, values beyond its range as +-65504).  Workspace as above, by
+ * lsattn_shared_prefill_workspace_bytes.
+ */
+typedef struct lsattn_shared_prefill_args {
+  const void* q;                /* [rows, num_q_heads, head_dim], strides in elements, multiples of 8 */
+  int64_t q_stride_t, q_stride_h;
+  const void* k;                /* as in lsattn_shared_decode_args */
+  const void* v;
+  int64_t k_stride_0, k_stride_1, v_stride_0, v_stride_1;
+  const int32_t* req_to_tokens;
+  const int32_t* g_start_loc;
+  const int32_t* g_size;
+  const int32_t* g_req_idx;
+  const int32_t* g_prefix_len;
+  int64_t rows, num_groups, num_q_heads, num_kv_heads, head_dim;
+  int64_t num_slots, num_reqs, max_seq_len, max_prefix_len, max_group_rows;
+  int32_t dtype;                /* of q, k, v and o: LSATTN_F16 or LSATTN_BF16 */
+  float sm_scale;
+  void* o;                      /* [rows, num_q_heads, head_dim], strides in elements, multiples of 8 */
+  int64_t o_stride_t, o_stride_h;
+  float* m;                     /* [rows, num_q_heads] */
+  float* l;
+  int64_t ml_stride_t, ml_stride_h;
+  void* workspace;
+  size_t workspace_bytes;
+} lsattn_shared_prefill_args;
+size_t lsattn_shared_prefill_workspace_bytes(int64_t rows, int64_t num_groups, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                             int64_t max_prefix_len);
+int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* stream);
+
+/*
+ * New requests over another's tokens, the same slots: for i < n and pos < b_seq_len[i]
+ *   req_to_tokens[dst_req_idx[i], pos] = slot = req_to_tokens[src_req_idx[i], pos],   mem_state[slot] += 1   (a slot outside the pool is not counted).
+ * Destination rows are distinct and no source of the call.  Forks of one request cost one addition per token where they stand next to each other.
+ * max_len_in_batch bounds b_seq_len: positions past it are left out.  No counterpart in the reference, nor have the four entry points below.
+ */
+int lsattn_fork_requests(int32_t* req_to_tokens, int64_t num_reqs, int64_t max_seq_len, const int32_t* src_req_idx, const int32_t* dst_req_idx,
+                         const int32_t* b_seq_len, int64_t n, int64_t max_len_in_batch, int32_t* mem_state, int64_t pool_size, void* stream);
+
+/* The rows of a pool in all layers: [num_layers, num_slots, row_bytes], and of an 8-bit pool the exponent bytes beside them (scales NULL: none). */
+typedef struct lsattn_pool_rows {
+  void* rows;                                     /* 16-byte aligned; row_bytes and strides multiples of 16 */
+  int64_t layer_stride_bytes, slot_stride_bytes, row_bytes;
+  int64_t num_layers, num_slots;
+  void* scales;
+  int64_t scale_layer_stride_bytes, scale_slot_stride_bytes, scale_bytes;
+} lsattn_pool_rows;
+
+/*
+ * New requests over copies of another's tokens: for i < n and pos < b_seq_len[i], in every layer
+ *   row[slot] = row[req_to_tokens[src_req_idx[i], pos]],   req_to_tokens[dst_req_idx[i], pos] = slot = mem_index[b_start_loc[i] + pos].
+ * The slots come from the allocator: distinct, and none of a source's.  Slots outside the pool and places past num_index are left out.
+ */
+typedef struct lsattn_copy_requests_args {
+  int32_t* req_to_tokens;       /* [num_reqs, max_seq_len] contiguous */
+  int64_t num_reqs, max_seq_len;
+  const int32_t* src_req_idx;   /* [n] */
+  const int32_t* dst_req_idx;   /* [n] */
+  const int32_t* b_seq_len;     /* [n] */
+  const int32_t* b_start_loc;   /* [n] */
+  int64_t n, max_len_in_batch;
+  const int64_t* mem_index;     /* [num_index] */
+  int64_t num_index;
+} lsattn_copy_requests_args;
+int lsattn_copy_requests(const lsattn_copy_requests_args* a, const lsattn_pool_rows* rows, void* stream);
+
+/*
+ * One reference less on the slot of every token of the requests: mem_state[req_to_tokens[b_req_idx[i], pos]] -= 1 for i < n, pos < b_seq_len[i], a slot that several of
+ * them name as often as they do (lsattn_pool_update_refs counts it once, as the reference does).  counts[0]: slots that became free; counts[1]: tokens whose entry
+ * names no slot of the pool, or one that was free already (its count stays 0).  counts is device memory or pinned host memory, written last.  The table stays as it is.
+ * Workspace: lsattn_release_workspace_bytes(n, max_len_in_batch) bytes (0: none).
+ */
+size_t lsattn_release_workspace_bytes(int64_t n, int64_t max_len_in_batch);
+int lsattn_release_requests(const int32_t* req_to_tokens, int64_t num_reqs, int64_t max_seq_len, const int32_t* b_req_idx, const int32_t* b_seq_len, int64_t n,
+                            int64_t max_len_in_batch, int32_t* mem_state, int64_t pool_size, int64_t* counts, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Slots in use to the front of the pool: with U of them, the k-th free slot below U takes the k-th used slot from U on, its row in every layer, its exponents and its
+ * count; the old slot is free then.  remap[slot] = where a used slot is now, -1 for a free one.  The first b_seq_len[i] entries of the rows b_req_idx[i] of the table, i < n (of
+ * distinct rows), follow, entries that name no used slot stay.  rows->rows NULL (num_layers 0): counts, table and remap alone.  Nothing is read back: how much moves only the
+ * device knows.  Workspace: lsattn_compact_workspace_bytes(pool_size) bytes, 16-byte aligned.
+ */
+typedef struct lsattn_compact_args {
+  int32_t* mem_state;           /* [pool_size] */
+  int64_t pool_size;
+  int32_t* remap;               /* [pool_size] */
+  int32_t* req_to_tokens;       /* [num_reqs, max_seq_len] contiguous */
+  int64_t num_reqs, max_seq_len;
+  const int32_t* b_req_idx;     /* [n] */
+  const int32_t* b_seq_len;     /* [n] */
+  int64_t n, max_len_in_batch;
+  void* workspace;
+  size_t workspace_bytes;
+} lsattn_compact_args;
+size_t lsattn_compact_workspace_bytes(int64_t pool_size);
+int lsattn_compact_pool(const lsattn_compact_args* a, const lsattn_pool_rows* rows, void* stream);
+
+/*
  * Launch choices that the library otherwise makes from the size of a launch, forced process-wide (tuning, and tests that
  * must reach every kernel shape whatever the size of their inputs).  No counterpart in the reference.  Every field 0 means
  * "the library's choice"; a NULL argument restores that for all of them.  The block is copied; launches made after the
@@ -701,8 +845,9 @@ const char* lsattn_strerror(int code);
  * lsattn_prefill_converts_v; 6 = max_kv_len there (a reserved word before), lsattn_prefill_route,
  * lsattn_prefill_cut_count; 7 = o_is_apart in lsattn_decode_stage2_args (a reserved word before); 8 = o_is_apart of 2;
  * 9 = lead_rows in lsattn_decode_stage2_args; 10 = lsattn_kv_scatter_fp8, lsattn_kv_gather_fp8, lsattn_pool_attention,
- * lsattn_prefill_window, lsattn_prefill_window_converts_v. */
-#define LSATTN_VERSION 10
+ * lsattn_prefill_window, lsattn_prefill_window_converts_v; 11 = lsattn_shared_decode, lsattn_shared_prefill, lsattn_fork_requests, lsattn_copy_requests,
+ * lsattn_release_requests, lsattn_compact_pool. */
+#define LSATTN_VERSION 11
 int lsattn_version(void);
 
 #ifdef __cplusplus

@@ -26,6 +26,8 @@ if not _building:
                       decoding_stage_migration_sender_kernel, destindex_copy_and_register_kv, destindex_copy_kv,
                       init_req_to_token_indexes, kv_gather_fp8, kv_scatter, kv_scatter_fp8, lse_merge, pre_copy_and_register_kv, prefill_attention_step,
                       rmsnorm_forward, rotary_emb_fwd, rotary_emb_write_kv, silu_and_mul_fwd, window_attention_fwd)
+    from .sharing import (compact_pool, compact_workspace_bytes, copy_requests, fork_requests, longserve_shared_prefix_decode_attention,
+                          release_requests, shared_prefix_attention_fwd, shared_prefix_attention_workspace_bytes, shared_prefix_decode_workspace_bytes)
 
 __all__ = [
     "context_attention_fwd", "prefill_attention_step", "lse_merge", "kv_scatter", "init_req_to_token_indexes",
@@ -36,5 +38,7 @@ __all__ = [
     "longserve_token_decode_attention_flash_decoding", "longserve_cuda_kernels",
     "kv_scatter_fp8", "kv_gather_fp8", "longserve_fp8_decode_attention", "longserve_window_decode_attention",
     "pool_attention_workspace_bytes", "window_attention_fwd",
+    "longserve_shared_prefix_decode_attention", "shared_prefix_decode_workspace_bytes", "shared_prefix_attention_fwd",
+    "shared_prefix_attention_workspace_bytes", "fork_requests", "copy_requests", "release_requests", "compact_pool", "compact_workspace_bytes",
     "LongServeMemoryManager", "LongServeReqManager", "set_tuning",
 ]

@@ -96,7 +96,7 @@ TUNING_VALUES = {
     "decode_stage1": {None: 0, "lane": 1, "mfma": 2, "split": 3},
     "decode_listed": {None: 0, "off": 1, "on": 2, "shares": 3},
 }
-LSATTN_VERSION = 10  # of include/lsattn.h, which the argument blocks above mirror
+LSATTN_VERSION = 11  # of include/lsattn.h, which the argument blocks above mirror
 
 
 # every symbol include/lsattn.h declares: name -> (restype, argtypes)
@@ -156,7 +156,56 @@ class PoolAttentionArgs(C.Structure):  # mirrors lsattn_pool_attention_args
                 ("o", _vp), ("lse", _vp), ("workspace", _vp), ("workspace_bytes", C.c_size_t)]
 
 
+class SharedDecodeArgs(C.Structure):  # mirrors lsattn_shared_decode_args
+    _fields_ = [("q", _vp), ("k", _vp), ("v", _vp),
+                ("k_stride_0", _i64), ("k_stride_1", _i64), ("v_stride_0", _i64), ("v_stride_1", _i64),
+                ("req_to_tokens", _vp), ("b_req_idx", _vp), ("b_seqlen", _vp),
+                ("g_start_loc", _vp), ("g_size", _vp), ("g_req_idx", _vp), ("g_prefix_len", _vp),
+                ("batch", _i64), ("num_groups", _i64), ("num_q_heads", _i64), ("num_kv_heads", _i64), ("head_dim", _i64),
+                ("num_slots", _i64), ("num_reqs", _i64), ("max_seq_len", _i64), ("max_prefix_len", _i64), ("max_own_len", _i64),
+                ("dtype", _i32), ("o_dtype", _i32), ("sm_scale", _f32), ("reserved", _i32),
+                ("o", _vp), ("lse", _vp), ("workspace", _vp), ("workspace_bytes", C.c_size_t)]
+
+
+class SharedPrefillArgs(C.Structure):  # mirrors lsattn_shared_prefill_args
+    _fields_ = [("q", _vp), ("q_stride_t", _i64), ("q_stride_h", _i64), ("k", _vp), ("v", _vp),
+                ("k_stride_0", _i64), ("k_stride_1", _i64), ("v_stride_0", _i64), ("v_stride_1", _i64),
+                ("req_to_tokens", _vp), ("g_start_loc", _vp), ("g_size", _vp), ("g_req_idx", _vp), ("g_prefix_len", _vp),
+                ("rows", _i64), ("num_groups", _i64), ("num_q_heads", _i64), ("num_kv_heads", _i64), ("head_dim", _i64),
+                ("num_slots", _i64), ("num_reqs", _i64), ("max_seq_len", _i64), ("max_prefix_len", _i64), ("max_group_rows", _i64),
+                ("dtype", _i32), ("sm_scale", _f32),
+                ("o", _vp), ("o_stride_t", _i64), ("o_stride_h", _i64), ("m", _vp), ("l", _vp), ("ml_stride_t", _i64), ("ml_stride_h", _i64),
+                ("workspace", _vp), ("workspace_bytes", C.c_size_t)]
+
+
+class PoolRows(C.Structure):  # mirrors lsattn_pool_rows
+    _fields_ = [("rows", _vp), ("layer_stride_bytes", _i64), ("slot_stride_bytes", _i64), ("row_bytes", _i64),
+                ("num_layers", _i64), ("num_slots", _i64),
+                ("scales", _vp), ("scale_layer_stride_bytes", _i64), ("scale_slot_stride_bytes", _i64), ("scale_bytes", _i64)]
+
+
+class CopyRequestsArgs(C.Structure):  # mirrors lsattn_copy_requests_args
+    _fields_ = [("req_to_tokens", _vp), ("num_reqs", _i64), ("max_seq_len", _i64),
+                ("src_req_idx", _vp), ("dst_req_idx", _vp), ("b_seq_len", _vp), ("b_start_loc", _vp),
+                ("n", _i64), ("max_len_in_batch", _i64), ("mem_index", _vp), ("num_index", _i64)]
+
+
+class CompactArgs(C.Structure):  # mirrors lsattn_compact_args
+    _fields_ = [("mem_state", _vp), ("pool_size", _i64), ("remap", _vp), ("req_to_tokens", _vp), ("num_reqs", _i64), ("max_seq_len", _i64),
+                ("b_req_idx", _vp), ("b_seq_len", _vp), ("n", _i64), ("max_len_in_batch", _i64), ("workspace", _vp), ("workspace_bytes", C.c_size_t)]
+
+
 EXPORTS = {
+    "lsattn_shared_decode": (C.c_int, [C.POINTER(SharedDecodeArgs), _vp]),
+    "lsattn_shared_decode_workspace_bytes": (C.c_size_t, [_i64] * 7),
+    "lsattn_shared_prefill": (C.c_int, [C.POINTER(SharedPrefillArgs), _vp]),
+    "lsattn_shared_prefill_workspace_bytes": (C.c_size_t, [_i64] * 6),
+    "lsattn_fork_requests": (C.c_int, [_vp, _i64, _i64, _vp, _vp, _vp, _i64, _i64, _vp, _i64, _vp]),
+    "lsattn_copy_requests": (C.c_int, [C.POINTER(CopyRequestsArgs), C.POINTER(PoolRows), _vp]),
+    "lsattn_release_requests": (C.c_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _vp, _i64, _vp, _vp, C.c_size_t, _vp]),
+    "lsattn_release_workspace_bytes": (C.c_size_t, [_i64, _i64]),
+    "lsattn_compact_pool": (C.c_int, [C.POINTER(CompactArgs), C.POINTER(PoolRows), _vp]),
+    "lsattn_compact_workspace_bytes": (C.c_size_t, [_i64]),
     "lsattn_kv_scatter_fp8": (C.c_int, [C.POINTER(KvScatterFp8Args), _vp]),
     "lsattn_kv_gather_fp8": (C.c_int, [C.POINTER(KvGatherFp8Args), _vp]),
     "lsattn_pool_attention": (C.c_int, [C.POINTER(PoolAttentionArgs), _vp]),

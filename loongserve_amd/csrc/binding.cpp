@@ -52,6 +52,16 @@ struct Library {
   decltype(&lsattn_kv_gather_fp8) kv_gather_fp8;
   decltype(&lsattn_pool_attention) pool_attention;
   decltype(&lsattn_pool_attention_workspace_bytes) pool_attention_workspace_bytes;
+  decltype(&lsattn_shared_decode) shared_decode;
+  decltype(&lsattn_shared_decode_workspace_bytes) shared_decode_workspace_bytes;
+  decltype(&lsattn_shared_prefill) shared_prefill;
+  decltype(&lsattn_shared_prefill_workspace_bytes) shared_prefill_workspace_bytes;
+  decltype(&lsattn_fork_requests) fork_requests;
+  decltype(&lsattn_copy_requests) copy_requests;
+  decltype(&lsattn_release_requests) release_requests;
+  decltype(&lsattn_release_workspace_bytes) release_workspace_bytes;
+  decltype(&lsattn_compact_pool) compact_pool;
+  decltype(&lsattn_compact_workspace_bytes) compact_workspace_bytes;
   decltype(&lsattn_strerror) strerror;
 } lib;
 
@@ -82,6 +92,16 @@ PyObject* bind(PyObject*, PyObject* addresses) {
       {"lsattn_kv_gather_fp8", (void**)&lib.kv_gather_fp8},
       {"lsattn_pool_attention", (void**)&lib.pool_attention},
       {"lsattn_pool_attention_workspace_bytes", (void**)&lib.pool_attention_workspace_bytes},
+      {"lsattn_shared_decode", (void**)&lib.shared_decode},
+      {"lsattn_shared_decode_workspace_bytes", (void**)&lib.shared_decode_workspace_bytes},
+      {"lsattn_shared_prefill", (void**)&lib.shared_prefill},
+      {"lsattn_shared_prefill_workspace_bytes", (void**)&lib.shared_prefill_workspace_bytes},
+      {"lsattn_fork_requests", (void**)&lib.fork_requests},
+      {"lsattn_copy_requests", (void**)&lib.copy_requests},
+      {"lsattn_release_requests", (void**)&lib.release_requests},
+      {"lsattn_release_workspace_bytes", (void**)&lib.release_workspace_bytes},
+      {"lsattn_compact_pool", (void**)&lib.compact_pool},
+      {"lsattn_compact_workspace_bytes", (void**)&lib.compact_workspace_bytes},
       {"lsattn_strerror", (void**)&lib.strerror},
   };
   for (const auto& e : entries) {
@@ -838,6 +858,29 @@ class Cells {
   }
 };
 
+// The two counts of a launch as a pair.  Past a few milliseconds of looking (much work queued before this call), or where the launch has to have ended, the thread waits
+// on the stream.
+PyObject* told(Cells& cells, const c10::hip::HIPStream& st, bool ended, const char* what) {
+  int64_t counted, outside;
+  {
+    NoGil others_run;
+    if (ended) st.synchronize();
+    const volatile int64_t* c = cells.words;
+    const auto until = std::chrono::steady_clock::now() + std::chrono::milliseconds(4);
+    while (c[0] < 0 || c[1] < 0) {
+      for (int i = 0; i < 64 && (c[0] < 0 || c[1] < 0); i++) __builtin_ia32_pause();
+      if (std::chrono::steady_clock::now() > until) {
+        st.synchronize();
+        break;
+      }
+    }
+    counted = c[0], outside = c[1];
+  }
+  if (counted < 0 || outside < 0) return PyErr_Format(PyExc_RuntimeError, "%s: the launch left no counts", what);
+  cells.give_back();
+  return Py_BuildValue("LL", (long long)counted, (long long)outside);
+}
+
 // (state int32, index int64, delta, workspace for lists of up to LSATTN_POOL_REFS_ORDERED entries) -> (counted, outside).  Waits for the
 // two counts, which the kernel writes to host memory: the caller needs them at once, and a copy of eight bytes behind a
 // synchronisation takes three times as long as looking for them.  Past a few milliseconds of looking (much work queued before this
@@ -859,26 +902,215 @@ PyObject* pool_update_refs(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (const int rc = call_pool(lib.pool_update_refs, (int32_t*)state.data_ptr(), state.size(0), n ? (const int64_t*)index.data_ptr() : nullptr, n, (int)delta,
                                           (int64_t*)cells.words, ws.data_ptr(), ws.nbytes(), st.stream()))
     return failed(rc, "lsattn_pool_update_refs");
-  int64_t counted, outside;
-  {
-    NoGil others_run;
-    // Up to 4096 entries the counts are written behind the state; of a longer list (two launches) they may be there before
-    // it: the caller, who may go on to another stream, waits for the launch.
-    if (!ordered) st.synchronize();
-    const volatile int64_t* c = cells.words;
-    const auto until = std::chrono::steady_clock::now() + std::chrono::milliseconds(4);
-    while (c[0] < 0 || c[1] < 0) {
-      for (int i = 0; i < 64 && (c[0] < 0 || c[1] < 0); i++) __builtin_ia32_pause();
-      if (std::chrono::steady_clock::now() > until) {
-        st.synchronize();
-        break;
-      }
-    }
-    counted = c[0], outside = c[1];
+  // Up to 4096 entries the counts are written behind the state; of a longer list (two launches) they may be there before
+  // it: the caller, who may go on to another stream, waits for the launch.
+  return told(cells, st, !ordered, "pool_update_refs");
+  END_HANDLE_TH_ERRORS
+}
+
+// ------------------------------------------------------------------------------------------------ requests that share tokens
+struct GroupVectors {
+  const at::Tensor &start, &size, &req, &prefix;
+  explicit GroupVectors(Args& in) : start(in.gpu(1)), size(in.gpu(1)), req(in.gpu(1)), prefix(in.gpu(1)) {}
+  bool ok() const {
+    const int64_t n = start.size(0);
+    return i32(start, n) && i32(size, n) && i32(req, n) && i32(prefix, n);
   }
-  if (counted < 0 || outside < 0) return PyErr_Format(PyExc_RuntimeError, "pool_update_refs: the launch left no counts");
-  cells.give_back();
-  return Py_BuildValue("LL", (long long)counted, (long long)outside);
+  template <typename A> void put(A& a) const {
+    a.num_groups = start.size(0);
+    a.g_start_loc = pi32(start), a.g_size = pi32(size), a.g_req_idx = pi32(req), a.g_prefix_len = pi32(prefix);
+  }
+};
+
+// (q, table, b_req, b_len, k, v, g_start, g_size, g_req, g_prefix, max_prefix, max_own, out or None, lse or None, workspace or None) -> (out, lse) or None
+PyObject* shared_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(15);
+  Args in(args);
+  const at::Tensor &q = in.gpu(3), &table = in.gpu(2), &b_req = in.gpu(1), &b_len = in.gpu(1), &k = in.gpu(3), &v = in.gpu(3);
+  const GroupVectors g(in);
+  const int64_t max_prefix = in.integer(), max_own = in.integer();
+  PyObject *py_out = args[in.i], *py_lse = args[in.i + 1];
+  const at::Tensor *out_in = in.maybe(), *lse_in = in.maybe(), *ws_in = in.maybe();
+  OR_NONE(in.ok && here({&q, &table, &b_req, &b_len, &k, &v, &g.start, &g.size, &g.req, &g.prefix, out_in, lse_in, ws_in}));
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1);
+  OR_NONE(half(q) && q.is_contiguous() && is(table, at::kInt) && table.is_contiguous() && i32(b_req, B) && i32(b_len, B) && g.ok());
+  OR_NONE(k.sizes() == v.sizes() && k.size(2) == D && k.stride(2) == 1 && v.stride(2) == 1 && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type());
+  OR_NONE((D == 128 || D == 64) && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && k.size(0) > 0 && B > 0 && max_prefix >= 0 && max_own >= 0);
+  if (out_in) OR_NONE((half(*out_in) || is(*out_in, at::kFloat)) && out_in->is_contiguous() && same_shape(*out_in, q));
+  if (lse_in) OR_NONE(is(*lse_in, at::kFloat) && lse_in->is_contiguous() && lse_in->dim() == 2 && lse_in->size(0) == B && lse_in->size(1) == Hq);
+  lsattn_shared_decode_args a;
+  std::memset(&a, 0, sizeof a);
+  g.put(a);
+  a.workspace_bytes = lib.shared_decode_workspace_bytes(B, a.num_groups, Hq, Hkv, D, max_prefix, max_own);
+  OR_NONE(!ws_in || (ws_in->is_contiguous() && ws_in->nbytes() >= a.workspace_bytes));
+  const at::Tensor out = out_in ? *out_in : empty(q.sizes(), q, q.scalar_type());
+  const at::Tensor lse = lse_in ? *lse_in : empty({B, Hq}, q, at::kFloat);
+  const at::Tensor ws = ws_in ? *ws_in : empty({(int64_t)a.workspace_bytes}, q, at::kByte);
+  a.workspace = ws.data_ptr();
+  a.q = q.data_ptr(), a.k = k.data_ptr(), a.v = v.data_ptr();
+  a.k_stride_0 = k.stride(0), a.k_stride_1 = k.stride(1), a.v_stride_0 = v.stride(0), a.v_stride_1 = v.stride(1);
+  a.req_to_tokens = pi32(table), a.b_req_idx = pi32(b_req), a.b_seqlen = pi32(b_len);
+  a.batch = B, a.num_q_heads = Hq, a.num_kv_heads = Hkv, a.head_dim = D;
+  a.num_slots = k.size(0), a.num_reqs = table.size(0), a.max_seq_len = table.size(1), a.max_prefix_len = max_prefix, a.max_own_len = max_own;
+  a.dtype = dtype_of(q), a.sm_scale = (float)(1.0 / std::sqrt((double)D));
+  a.o = out.data_ptr(), a.o_dtype = dtype_of(out), a.lse = (float*)lse.data_ptr();
+  if (const int rc = call(lib.shared_decode, &a, stream())) return failed(rc, "lsattn_shared_decode");
+  PyObject* o1 = out_in ? (Py_INCREF(py_out), py_out) : THPVariable_Wrap(out);
+  PyObject* o2 = lse_in ? (Py_INCREF(py_lse), py_lse) : THPVariable_Wrap(lse);
+  return Py_BuildValue("(NN)", o1, o2);
+  END_HANDLE_TH_ERRORS
+}
+
+// (q, k, v, o, g_start, g_size, table, g_req, g_prefix, max_rows, max_prefix, m, l, rows, workspace or None) -> True or None
+PyObject* shared_prefill(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(14);
+  Args in(args);
+  const at::Tensor &q = in.gpu(3), &k = in.gpu(3), &v = in.gpu(3), &o = in.gpu(3), &g_start = in.gpu(1), &g_size = in.gpu(1), &table = in.gpu(2), &g_req = in.gpu(1),
+                   &g_prefix = in.gpu(1);
+  const int64_t max_rows = in.integer(), max_prefix = in.integer();
+  const at::Tensor &m = in.gpu(2), &l = in.gpu(2);
+  const at::Tensor* ws_in = in.maybe();
+  OR_NONE(in.ok && here({&q, &k, &v, &o, &g_start, &g_size, &table, &g_req, &g_prefix, &m, &l, ws_in}));
+  const int64_t T = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k.size(1), G = g_start.size(0);
+  OR_NONE(half(q) && q.stride(2) == 1 && o.scalar_type() == q.scalar_type() && same_shape(o, q) && o.stride(2) == 1);
+  OR_NONE(is(table, at::kInt) && table.is_contiguous() && i32(g_start, G) && i32(g_size, G) && i32(g_req, G) && i32(g_prefix, G));
+  OR_NONE(k.sizes() == v.sizes() && k.size(2) == D && k.stride(2) == 1 && v.stride(2) == 1 && k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type());
+  OR_NONE((D == 128 || D == 64) && Hkv > 0 && Hq > 0 && Hq % Hkv == 0 && k.size(0) > 0 && T > 0 && G > 0 && max_rows > 0 && max_prefix > 0);
+  OR_NONE(is(m, at::kFloat) && is(l, at::kFloat) && m.size(0) == T && m.size(1) == Hq && m.sizes() == l.sizes() && m.strides() == l.strides());
+  lsattn_shared_prefill_args a;
+  std::memset(&a, 0, sizeof a);
+  a.num_groups = G;
+  a.workspace_bytes = lib.shared_prefill_workspace_bytes(T, G, Hq, Hkv, D, max_prefix);
+  OR_NONE(!ws_in || (ws_in->is_contiguous() && ws_in->nbytes() >= a.workspace_bytes));
+  const at::Tensor ws = ws_in ? *ws_in : empty({(int64_t)a.workspace_bytes}, q, at::kByte);
+  a.workspace = ws.data_ptr();
+  a.q = q.data_ptr(), a.q_stride_t = q.stride(0), a.q_stride_h = q.stride(1);
+  a.k = k.data_ptr(), a.v = v.data_ptr();
+  a.k_stride_0 = k.stride(0), a.k_stride_1 = k.stride(1), a.v_stride_0 = v.stride(0), a.v_stride_1 = v.stride(1);
+  a.req_to_tokens = pi32(table), a.g_start_loc = pi32(g_start), a.g_size = pi32(g_size), a.g_req_idx = pi32(g_req), a.g_prefix_len = pi32(g_prefix);
+  a.rows = T, a.num_q_heads = Hq, a.num_kv_heads = Hkv, a.head_dim = D;
+  a.num_slots = k.size(0), a.num_reqs = table.size(0), a.max_seq_len = table.size(1), a.max_prefix_len = max_prefix, a.max_group_rows = max_rows;
+  a.dtype = dtype_of(q), a.sm_scale = (float)(1.0 / std::sqrt((double)D));
+  a.o = o.data_ptr(), a.o_stride_t = o.stride(0), a.o_stride_h = o.stride(1);
+  a.m = (float*)m.data_ptr(), a.l = (float*)l.data_ptr(), a.ml_stride_t = m.stride(0), a.ml_stride_h = m.stride(1);
+  if (const int rc = call(lib.shared_prefill, &a, stream())) return failed(rc, "lsattn_shared_prefill");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (table, src, dst, len, max_len, state) -> True or None
+PyObject* fork_requests(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(6);
+  Args in(args);
+  const at::Tensor &table = in.gpu(2), &src = in.gpu(1), &dst = in.gpu(1), &len = in.gpu(1);
+  const int64_t max_len = in.integer();
+  const at::Tensor& state = in.gpu(1);
+  OR_NONE(in.ok && here({&table, &src, &dst, &len, &state}));
+  const int64_t n = src.size(0);
+  OR_NONE(is(table, at::kInt) && table.is_contiguous() && i32(src, n) && i32(dst, n) && i32(len, n) && i32(state, state.size(0)) && max_len > 0 && n > 0);
+  OR_NONE(table.numel() > 0 && state.numel() > 0);
+  if (const int rc = call(lib.fork_requests, (int32_t*)table.data_ptr(), table.size(0), table.size(1), pi32(src), pi32(dst), pi32(len), n, max_len,
+                          (int32_t*)state.data_ptr(), state.size(0), stream()))
+    return failed(rc, "lsattn_fork_requests");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// the rows of a pool [layers, slots, heads, head_dim] and the exponents [layers, slots, heads] beside an 8-bit one
+bool pool_rows(const at::Tensor& kv, const at::Tensor* scales, lsattn_pool_rows& r) {
+  std::memset(&r, 0, sizeof r);
+  const int64_t es = kv.element_size(), D = kv.size(3);
+  if (!kv.numel() || kv.stride(3) != 1 || kv.stride(2) != D) return false;
+  r.rows = kv.data_ptr(), r.layer_stride_bytes = kv.stride(0) * es, r.slot_stride_bytes = kv.stride(1) * es, r.row_bytes = kv.size(2) * D * es;
+  r.num_layers = kv.size(0), r.num_slots = kv.size(1);
+  if ((r.scales = scales ? scales->data_ptr() : nullptr)) {
+    if (scales->element_size() != 1 || scales->dim() != 3 || scales->sizes() != kv.sizes().slice(0, 3) || scales->stride(2) != 1) return false;
+    r.scale_layer_stride_bytes = scales->stride(0), r.scale_slot_stride_bytes = scales->stride(1), r.scale_bytes = scales->size(2);
+  }
+  return (scales != nullptr) == is(kv, at::kFloat8_e4m3fn);
+}
+
+// (table, src, dst, len, start, max_len, index, kv, scales or None) -> True or None
+PyObject* copy_requests(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(9);
+  Args in(args);
+  const at::Tensor &table = in.gpu(2), &src = in.gpu(1), &dst = in.gpu(1), &len = in.gpu(1), &start = in.gpu(1);
+  const int64_t max_len = in.integer();
+  const at::Tensor &index = in.gpu(1), &kv = in.gpu(4);
+  const at::Tensor* scales = in.maybe();
+  OR_NONE(in.ok && here({&table, &src, &dst, &len, &start, &index, &kv, scales}));
+  const int64_t n = src.size(0);
+  OR_NONE(is(table, at::kInt) && table.is_contiguous() && i32(src, n) && i32(dst, n) && i32(len, n) && i32(start, n) && max_len > 0 && n > 0 && table.numel() > 0);
+  OR_NONE(is(index, at::kLong) && index.is_contiguous() && index.numel() > 0);
+  lsattn_pool_rows r;
+  OR_NONE(pool_rows(kv, scales, r));
+  lsattn_copy_requests_args a;
+  std::memset(&a, 0, sizeof a);
+  a.req_to_tokens = (int32_t*)table.data_ptr(), a.num_reqs = table.size(0), a.max_seq_len = table.size(1);
+  a.src_req_idx = pi32(src), a.dst_req_idx = pi32(dst), a.b_seq_len = pi32(len), a.b_start_loc = pi32(start), a.n = n, a.max_len_in_batch = max_len;
+  a.mem_index = (const int64_t*)index.data_ptr(), a.num_index = index.numel();
+  if (const int rc = call(lib.copy_requests, &a, &r, stream())) return failed(rc, "lsattn_copy_requests");
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+// (table, req, len, max_len, state) -> (freed, wrong) or None.  Waits for the counts as pool_update_refs does.
+PyObject* release_requests(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(5);
+  Args in(args);
+  const at::Tensor &table = in.gpu(2), &req = in.gpu(1), &len = in.gpu(1);
+  const int64_t max_len = in.integer();
+  const at::Tensor& state = in.gpu(1);
+  OR_NONE(in.ok && here({&table, &req, &len, &state}));
+  const int64_t n = req.size(0);
+  OR_NONE(is(table, at::kInt) && table.is_contiguous() && i32(req, n) && i32(len, n) && i32(state, state.size(0)) && max_len > 0 && n > 0);
+  OR_NONE(table.numel() > 0 && state.numel() > 0);
+  const int64_t most = std::min(max_len, table.size(1));
+  const int64_t bytes = (int64_t)lib.release_workspace_bytes(n, most);
+  const at::Tensor ws = bytes ? empty({bytes}, state, at::kByte) : at::Tensor();
+  Cells cells;
+  const auto st = c10::hip::getCurrentHIPStream();
+  if (const int rc = call(lib.release_requests, pi32(table), table.size(0), table.size(1), pi32(req), pi32(len), n, most, (int32_t*)state.data_ptr(), state.size(0),
+                          (int64_t*)cells.words, bytes ? ws.data_ptr() : nullptr, (size_t)bytes, st.stream()))
+    return failed(rc, "lsattn_release_requests");
+  return told(cells, st, false, "release_requests");
+  END_HANDLE_TH_ERRORS
+}
+
+// (state, kv or None, table, req, len, max_len, scales or None, remap) -> True or None
+PyObject* compact_pool(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  NEED_ARGS(9);
+  Args in(args);
+  const at::Tensor& state = in.gpu(1);
+  const at::Tensor& kv = in.gpu(4);
+  const at::Tensor &table = in.gpu(2), &req = in.gpu(1), &len = in.gpu(1);
+  const int64_t max_len = in.integer();
+  const at::Tensor* scales = in.maybe();
+  const at::Tensor& remap = in.gpu(1);
+  const at::Tensor* ws_in = in.maybe();
+  OR_NONE(in.ok && here({&state, &kv, &table, &req, &len, scales, &remap, ws_in}));
+  const int64_t n = req.size(0), size = state.size(0);
+  OR_NONE(i32(state, size) && i32(remap, size) && is(table, at::kInt) && table.is_contiguous() && i32(req, n) && i32(len, n) && max_len >= 0 && size > 0);
+  lsattn_pool_rows r;
+  OR_NONE(kv.size(1) >= size && pool_rows(kv, scales, r));
+  lsattn_compact_args a;
+  std::memset(&a, 0, sizeof a);
+  a.workspace_bytes = lib.compact_workspace_bytes(size);
+  OR_NONE(!ws_in || (ws_in->is_contiguous() && ws_in->nbytes() >= a.workspace_bytes));
+  const at::Tensor ws = ws_in ? *ws_in : empty({(int64_t)a.workspace_bytes}, state, at::kByte);
+  a.mem_state = (int32_t*)state.data_ptr(), a.pool_size = size, a.remap = (int32_t*)remap.data_ptr();
+  a.n = table.numel() ? n : 0;
+  if (a.n) a.req_to_tokens = (int32_t*)table.data_ptr(), a.b_req_idx = pi32(req), a.b_seq_len = pi32(len);
+  a.num_reqs = table.size(0), a.max_seq_len = table.size(1), a.max_len_in_batch = max_len;
+  a.workspace = ws.data_ptr();
+  if (const int rc = call(lib.compact_pool, &a, &r, stream())) return failed(rc, "lsattn_compact_pool");
+  Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
 
@@ -889,6 +1121,7 @@ PyMethodDef methods[] = {
     ENTRY(kv_scatter), ENTRY(register_decode_tokens), ENTRY(register_tokens), ENTRY(rms_norm), ENTRY(silu_and_mul_inplace),
     ENTRY(rotary_emb), ENTRY(rotary_kv_write), ENTRY(pool_alloc), ENTRY(pool_update_refs),
     ENTRY(window_attention), ENTRY(kv_scatter_fp8), ENTRY(kv_gather_fp8), ENTRY(pool_attention),
+    ENTRY(shared_decode), ENTRY(shared_prefill), ENTRY(fork_requests), ENTRY(copy_requests), ENTRY(release_requests), ENTRY(compact_pool),
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Native argument pass of loongserve_amd's operators.", -1, methods};
 

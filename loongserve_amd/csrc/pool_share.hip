@@ -1,0 +1,439 @@
+// Requests that share pool slots, and the moving of slots (gfx950): new requests over the slots of another or over copies of them, the release of
+// requests' tokens, and compaction.  No counterpart in the reference, whose slots have reference counts too (loongserve/common/longserve_mem_manager.py:61-88) but whose
+// lists count a slot that is named twice once, so that requests that share tokens cannot be freed together.
+//
+// All of it is whole numbers and rows as bytes.  What bounds it: rows, HBM (a row read and written once per layer); the rest, launch latency and a
+// few MB of tables and counts.  Counts change by integer atomics, whose order does not change a result.
+#include "common.hip.h"
+
+namespace lsattn {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int64_t kCUs = 256;
+
+// ------------------------------------------------------------------------------------------------ fork
+struct ForkParams {
+  int32_t* table;
+  int64_t max_seq_len;
+  int32_t most;  // positions that the call takes of a request: max_len_in_batch, at most max_seq_len
+  const int32_t* src;
+  const int32_t* dst;
+  const int32_t* len;
+  int32_t n, num_reqs;
+  int32_t* state;
+  int32_t size;
+};
+__device__ __forceinline__ int fork_len(const ForkParams& p, int i) {
+  const int n = p.len[i];
+  return p.src[i] < 0 || p.src[i] >= p.num_reqs || p.dst[i] < 0 || p.dst[i] >= p.num_reqs ? 0 : n < p.most ? n : p.most;
+}
+// A thread has a position of a fork.  Forks of one request that stand next to each other count as one addition per token, made by the first of them: many samples of one
+// question would otherwise queue at the same words.
+__global__ __launch_bounds__(kThreads) void fork_share_kernel(ForkParams p) {
+  const int i = blockIdx.y, pos = (int)(blockIdx.x * kThreads + threadIdx.x), lane = threadIdx.x & 63;
+  const int src = p.src[i], mine = fork_len(p, i);
+  int slot = -1;
+  const bool valid_src = src >= 0 && src < p.num_reqs;
+  const bool leads = i == 0 || p.src[i - 1] != src;
+  if (pos < mine) {
+    slot = p.table[(int64_t)src * p.max_seq_len + pos];
+    p.table[(int64_t)p.dst[i] * p.max_seq_len + pos] = slot;
+  }
+  if (!leads || !valid_src) return;
+  int refs = 0;
+  for (int k0 = i; k0 < p.n; k0 += 64) {  // the run's lengths, one per lane
+    const int k = k0 + lane;
+    const bool same = k < p.n && p.src[k] == src;
+    const int len = same ? fork_len(p, k) : 0;
+    const uint64_t ends = __builtin_amdgcn_ballot_w64(!same);
+    const int run = ends ? __builtin_ctzll(ends) : 64;
+    for (int j = 0; j < run; j++) refs += __builtin_amdgcn_readlane(len, j) > pos;
+    if (run < 64) break;
+  }
+  if (refs == 0) return;
+  if (slot < 0 && pos >= mine && pos < p.most) slot = p.table[(int64_t)src * p.max_seq_len + pos];  // (a longer fork behind the first)
+  if ((uint32_t)slot < (uint32_t)p.size) atomicAdd(p.state + slot, refs);
+}
+
+// ------------------------------------------------------------------------------------------------ rows
+struct RowsParams {
+  char* rows;  // [layers, slots, row]
+  int64_t layer_stride, slot_stride;  // bytes
+  int32_t pieces, lanes_shift;        // pieces of a row; log2 of the lanes that take one
+  int32_t num_slots;
+};
+// `row_of(i, src, dst)`: the slots of the workgroup's row i, false if it has none.
+template <typename Piece, int ROWS, typename F> __device__ __forceinline__ void move_rows(const RowsParams& p, int layer, F row_of) {
+  const int lanes = 1 << p.lanes_shift, sub = threadIdx.x & (lanes - 1);
+  char* const base = p.rows + layer * p.layer_stride;
+  for (int i = threadIdx.x >> p.lanes_shift; i < ROWS; i += kThreads >> p.lanes_shift) {
+    int src, dst;
+    if (!row_of(i, src, dst)) continue;
+    const Piece* from = (const Piece*)(base + (int64_t)src * p.slot_stride);
+    Piece* to = (Piece*)(base + (int64_t)dst * p.slot_stride);
+#pragma unroll 4
+    for (int x = sub; x < p.pieces; x += lanes) to[x] = from[x];
+  }
+}
+
+struct CopyParams {
+  ForkParams f;
+  RowsParams r;
+  const int64_t* index;
+  const int32_t* start;
+  int64_t num_index;
+  int32_t registers;  // whether this launch writes the table
+};
+constexpr int kCopyRows = 16;
+// grid (positions, forks, layers)
+template <typename Piece> __global__ __launch_bounds__(kThreads) void fork_copy_kernel(CopyParams p) {
+  const int i = blockIdx.y, pos0 = (int)blockIdx.x * kCopyRows, len = fork_len(p.f, i);
+  if (pos0 >= len) return;
+  const int32_t* const src_row = p.f.table + (int64_t)p.f.src[i] * p.f.max_seq_len;
+  const int64_t start = p.start[i];
+  auto target = [&](int pos) -> int {  // the slot of a position, -1 if there is none
+    const int64_t at = start + pos;
+    const int64_t d = pos < len && at >= 0 && at < p.num_index ? p.index[at] : -1;
+    return d >= 0 && d < p.r.num_slots ? (int)d : -1;
+  };
+  if (p.registers && blockIdx.z == 0 && threadIdx.x < kCopyRows) {
+    const int d = target(pos0 + threadIdx.x);
+    if (d >= 0) p.f.table[(int64_t)p.f.dst[i] * p.f.max_seq_len + pos0 + threadIdx.x] = d;
+  }
+  move_rows<Piece, kCopyRows>(p.r, blockIdx.z, [&](int k, int& src, int& dst) {
+    if (pos0 + k >= len) return false;
+    src = src_row[pos0 + k];
+    dst = target(pos0 + k);
+    return dst >= 0 && (uint32_t)src < (uint32_t)p.r.num_slots;
+  });
+}
+
+// ------------------------------------------------------------------------------------------------ release
+struct ReleaseParams {
+  const int32_t* table;
+  int64_t max_seq_len;
+  int32_t most;  // as ForkParams::most
+  const int32_t* req;
+  const int32_t* len;
+  int32_t n, num_reqs;
+  int32_t* state;
+  int32_t size;
+  int32_t blocks;  // of kThreads positions per request
+  int32_t* sums;   // (freed, wrong) of every workgroup
+  int64_t* cells;
+};
+// One reference less on the slot of a position.  A count that is zero stays there (taken back: it never rises above what it was, so of any number of threads
+// one sees it end), and counts as wrong, as does an entry that names no slot.
+__device__ __forceinline__ void release_one(const ReleaseParams& p, int i, int pos, int& freed, int& wrong) {
+  const int req = p.req[i];
+  const bool known = req >= 0 && req < p.num_reqs;
+  int len = p.len[i];
+  len = len < p.most ? len : p.most;
+  if (pos >= len) return;
+  const int slot = known ? p.table[(int64_t)req * p.max_seq_len + pos] : -1;
+  if ((uint32_t)slot >= (uint32_t)p.size) {
+    wrong++;
+    return;
+  }
+  const int old = atomicSub(p.state + slot, 1);
+  if (old == 1) freed++;
+  if (old <= 0) {
+    atomicAdd(p.state + slot, 1);
+    wrong++;
+  }
+}
+template <int THREADS> __device__ __forceinline__ void sum_group(int& a, int& b) {
+  __shared__ int sh[2][THREADS / 64];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) a += __shfl_xor(a, d, 64), b += __shfl_xor(b, d, 64);
+  if ((threadIdx.x & 63) == 0) sh[0][threadIdx.x >> 6] = a, sh[1][threadIdx.x >> 6] = b;
+  __syncthreads();
+  a = b = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; w++) a += sh[0][w], b += sh[1][w];
+}
+// behind the counts themselves: who sees the cells filled sees the states of this call (they may lie in host memory)
+__device__ __forceinline__ void tell(int64_t* cells, int64_t freed, int64_t wrong) {
+  __threadfence_system();
+  __hip_atomic_store(cells, freed, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
+  __hip_atomic_store(cells + 1, wrong, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_SYSTEM);
+}
+__global__ __launch_bounds__(kThreads) void release_kernel(ReleaseParams p) {
+  int freed = 0, wrong = 0;
+  release_one(p, blockIdx.y, (int)(blockIdx.x * kThreads + threadIdx.x), freed, wrong);
+  sum_group<kThreads>(freed, wrong);
+  if (threadIdx.x == 0) {
+    int32_t* s = p.sums + 2 * ((int64_t)blockIdx.y * p.blocks + blockIdx.x);
+    s[0] = freed, s[1] = wrong;
+  }
+}
+__global__ __launch_bounds__(1024) void release_sum_kernel(ReleaseParams p) {
+  __shared__ int64_t sh[2][16];
+  int64_t a = 0, b = 0;
+  for (int64_t i = threadIdx.x; i < (int64_t)p.n * p.blocks; i += 1024) a += p.sums[2 * i], b += p.sums[2 * i + 1];
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) a += __shfl_xor(a, d, 64), b += __shfl_xor(b, d, 64);
+  if ((threadIdx.x & 63) == 0) sh[0][threadIdx.x >> 6] = a, sh[1][threadIdx.x >> 6] = b;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int w = 1; w < 16; w++) a += sh[0][w], b += sh[1][w];
+  tell(p.cells, a, b);
+}
+// Few tokens: one workgroup takes all of them and tells the counts itself.
+constexpr int64_t kOneGroupTokens = 4096;
+__global__ __launch_bounds__(1024) void release_one_group_kernel(ReleaseParams p, int max_len) {
+  int freed = 0, wrong = 0;
+  for (int i = threadIdx.x; i < p.n * max_len; i += 1024) release_one(p, i / max_len, i % max_len, freed, wrong);
+  __threadfence_system();
+  sum_group<1024>(freed, wrong);
+  if (threadIdx.x == 0) tell(p.cells, freed, wrong);
+}
+
+// ------------------------------------------------------------------------------------------------ compact
+// With U slots in use, the k-th free slot below U takes the k-th used slot from U on: as few moves as there are, and what moves keeps its order.
+constexpr int kPlanThreads = 1024, kPlanSlots = kPlanThreads * 4;
+struct CompactParams {
+  int32_t* state;
+  int32_t size, blocks;
+  int32_t* used;    // [blocks] slots in use
+  int32_t* header;  // [0] moves
+  int32_t* hole;    // [size / 2 + 1]
+  int32_t* source;
+  int32_t* code;    // [size]: the new slot; -1 free; -2 - k: the k-th move's source
+  int32_t* remap;
+  int32_t* table;
+  int64_t max_seq_len;
+  const int32_t* req;
+  const int32_t* len;
+  int32_t n, num_reqs;
+  RowsParams r;
+  int32_t move_wgs, table_blocks, layers, most;
+};
+__device__ __forceinline__ void load_states(const CompactParams& p, int64_t at, int (&s)[4]) {  // (past the end: free)
+#pragma unroll
+  for (int e = 0; e < 4; e++) s[e] = at + e < p.size ? p.state[at + e] : 0;
+}
+__device__ __forceinline__ int count_group(int mine, int* sh) {  // over the workgroup
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d, 64);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mine;
+  __syncthreads();
+  int all = 0;
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; w++) all += sh[w];
+  return all;
+}
+__global__ __launch_bounds__(kPlanThreads) void compact_count_kernel(CompactParams p) {
+  __shared__ int sh[kPlanThreads / 64];
+  int s[4];
+  load_states(p, (int64_t)blockIdx.x * kPlanSlots + 4 * threadIdx.x, s);
+  const int all = count_group((s[0] != 0) + (s[1] != 0) + (s[2] != 0) + (s[3] != 0), sh);
+  if (threadIdx.x == 0) p.used[blockIdx.x] = all;
+}
+__global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParams p) {
+  __shared__ int sh[kPlanThreads / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t at = (int64_t)blockIdx.x * kPlanSlots + 4 * threadIdx.x;
+  int s[4];
+  load_states(p, at, s);
+  int before = 0, all = 0;
+  for (int b = threadIdx.x; b < p.blocks; b += kPlanThreads) {
+    const int n = p.used[b];
+    before += b < (int)blockIdx.x ? n : 0;
+    all += n;
+  }
+  before = count_group(before, sh), all = count_group(all, sh);
+  // slots in use in front of slot `all`
+  const int border = all / kPlanSlots;
+  int front = 0;
+  for (int b = threadIdx.x; b < border; b += kPlanThreads) front += p.used[b];
+  int t[4];
+  const int64_t bat = (int64_t)border * kPlanSlots + 4 * threadIdx.x;
+  load_states(p, bat, t);
+#pragma unroll
+  for (int e = 0; e < 4; e++) front += bat + e < all && t[e] != 0;
+  front = count_group(front, sh);
+  if (blockIdx.x == 0 && threadIdx.x == 0) p.header[0] = all - front;
+  // ranks
+  const int mine = (s[0] != 0) + (s[1] != 0) + (s[2] != 0) + (s[3] != 0);
+  int up_to = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int below = __shfl_up(up_to, d, 64);
+    if (lane >= d) up_to += below;
+  }
+  __syncthreads();
+  if (lane == 63) sh[wave] = up_to;
+  __syncthreads();
+  int rank = before + up_to - mine;  // used slots in front of the thread's first one
+#pragma unroll
+  for (int w = 0; w < kPlanThreads / 64; w++) rank += w < wave ? sh[w] : 0;
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const int64_t slot = at + e;
+    if (slot >= p.size) break;
+    const bool in_use = s[e] != 0;
+    int code = in_use ? (int)slot : -1;
+    if (slot < all && !in_use) p.hole[slot - rank] = (int)slot;
+    if (slot >= all && in_use) {
+      p.source[rank - front] = (int)slot;
+      code = -2 - (rank - front);
+    }
+    p.code[slot] = code;
+    if (code >= -1) p.remap[slot] = code;
+    rank += in_use;
+  }
+}
+// Workgroups that move rows (and the counts, with the first layer), those of a layer side by side, and behind them workgroups that rewrite the requests' table entries.
+constexpr int kMoveRows = 16;
+template <typename Piece, bool FIRST> __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p) {
+  const int moves = p.header[0], layer = (int)blockIdx.x / p.move_wgs;
+  if (layer < (p.layers ? p.layers : 1)) {
+    for (int m0 = ((int)blockIdx.x - layer * p.move_wgs) * kMoveRows; m0 < moves; m0 += p.move_wgs * kMoveRows) {
+      if (FIRST && layer == 0 && threadIdx.x < kMoveRows && m0 + (int)threadIdx.x < moves) {
+        const int src = p.source[m0 + threadIdx.x], dst = p.hole[m0 + threadIdx.x];
+        p.state[dst] = p.state[src];
+        p.state[src] = 0;
+        p.remap[src] = dst;
+      }
+      if (p.layers)
+        move_rows<Piece, kMoveRows>(p.r, layer, [&](int k, int& src, int& dst) {
+          if (m0 + k >= moves) return false;
+          src = p.source[m0 + k], dst = p.hole[m0 + k];
+          return true;
+        });
+    }
+    return;
+  }
+  const int x = (int)blockIdx.x - p.move_wgs * (p.layers ? p.layers : 1), i = x / p.table_blocks, pos = (x - i * p.table_blocks) * kThreads + threadIdx.x;
+  const int req = p.req[i], len = p.len[i] < p.most ? p.len[i] : p.most;
+  if (req < 0 || req >= p.num_reqs || pos >= len) return;
+  int32_t* entry = p.table + (int64_t)req * p.max_seq_len + pos;
+  const int slot = *entry;
+  if ((uint32_t)slot >= (uint32_t)p.size) return;
+  const int code = p.code[slot];
+  if (code <= -2) *entry = p.hole[-2 - code];
+}
+
+// rows of `bytes` (16-byte pieces) by lanes that are a power of two, a wave at most
+void set_rows(RowsParams& r, void* rows, int64_t layer_stride, int64_t slot_stride, int64_t pieces, int64_t num_slots) {
+  r.rows = (char*)rows, r.layer_stride = layer_stride, r.slot_stride = slot_stride, r.num_slots = (int32_t)num_slots;
+  r.pieces = (int32_t)pieces, r.lanes_shift = 0;
+  while (r.lanes_shift < 6 && (1 << r.lanes_shift) < pieces) r.lanes_shift++;
+}
+bool rows_ok(const lsattn_pool_rows* r) {
+  if (!r->rows) return r->num_layers == 0 && !r->scales;
+  if (r->num_layers < 1 || r->num_layers > 65535 || r->row_bytes < 16 || r->row_bytes % 16 || r->row_bytes > 0x7fffffff || r->slot_stride_bytes < r->row_bytes ||
+      r->slot_stride_bytes % 16 || r->layer_stride_bytes % 16 || ((uintptr_t)r->rows & 15) || r->num_slots < 1 || r->num_slots > 0x7fffffff)
+    return false;
+  return !r->scales || (r->scale_bytes >= 1 && r->scale_bytes <= 0x7fffffff && r->scale_slot_stride_bytes >= r->scale_bytes);
+}
+
+}  // namespace
+}  // namespace lsattn
+
+using namespace lsattn;
+
+extern "C" int lsattn_fork_requests(int32_t* req_to_tokens, int64_t num_reqs, int64_t max_seq_len, const int32_t* src_req_idx, const int32_t* dst_req_idx,
+                                    const int32_t* b_seq_len, int64_t n, int64_t max_len_in_batch, int32_t* mem_state, int64_t pool_size, void* stream) {
+  if (!req_to_tokens || !src_req_idx || !dst_req_idx || !b_seq_len || !mem_state || num_reqs < 0 || max_seq_len < 0 || n < 0 || max_len_in_batch < 0 || pool_size < 0 ||
+      num_reqs > 0x7fffffff || max_seq_len > 0x7fff0000 || n > 65535 || pool_size > 0x7fffffff)
+    return LSATTN_ERR_INVALID_ARG;
+  const int64_t most = max_len_in_batch < max_seq_len ? max_len_in_batch : max_seq_len;
+  if (n == 0 || most == 0) return LSATTN_OK;
+  const ForkParams p{req_to_tokens, max_seq_len, (int32_t)most, src_req_idx, dst_req_idx, b_seq_len, (int32_t)n, (int32_t)num_reqs, mem_state, (int32_t)pool_size};
+  LSATTN_LAUNCH_KERNEL(fork_share_kernel, dim3((unsigned)((most + kThreads - 1) / kThreads), (unsigned)n), dim3(kThreads), 0, (hipStream_t)stream, p);
+  return check_launch();
+}
+
+extern "C" int lsattn_copy_requests(const lsattn_copy_requests_args* a, const lsattn_pool_rows* rows, void* stream) {
+  if (!a || !rows || !a->req_to_tokens || !a->src_req_idx || !a->dst_req_idx || !a->b_seq_len || !a->b_start_loc || !a->mem_index || !rows->rows || !rows_ok(rows))
+    return LSATTN_ERR_INVALID_ARG;
+  if (a->num_reqs < 0 || a->max_seq_len < 0 || a->n < 0 || a->max_len_in_batch < 0 || a->num_index < 0 || a->num_reqs > 0x7fffffff || a->max_seq_len > 0x7fff0000 ||
+      a->n > 65535)
+    return LSATTN_ERR_INVALID_ARG;
+  const int64_t most = a->max_len_in_batch < a->max_seq_len ? a->max_len_in_batch : a->max_seq_len;
+  if (a->n == 0 || most == 0) return LSATTN_OK;
+  CopyParams p;
+  p.f = ForkParams{a->req_to_tokens, a->max_seq_len, (int32_t)most, a->src_req_idx, a->dst_req_idx, a->b_seq_len, (int32_t)a->n, (int32_t)a->num_reqs, nullptr, 0};
+  p.index = a->mem_index, p.start = a->b_start_loc, p.num_index = a->num_index, p.registers = 1;
+  const dim3 grid((unsigned)((most + kCopyRows - 1) / kCopyRows), (unsigned)a->n, (unsigned)rows->num_layers);
+  hipStream_t st = (hipStream_t)stream;
+  set_rows(p.r, rows->rows, rows->layer_stride_bytes, rows->slot_stride_bytes, rows->row_bytes / 16, rows->num_slots);
+  LSATTN_LAUNCH_KERNEL((fork_copy_kernel<u32x4>), grid, dim3(kThreads), 0, st, p);
+  if (!rows->scales || hipPeekAtLastError() != hipSuccess) return check_launch();
+  p.registers = 0;
+  set_rows(p.r, rows->scales, rows->scale_layer_stride_bytes, rows->scale_slot_stride_bytes, rows->scale_bytes, rows->num_slots);
+  LSATTN_LAUNCH_KERNEL((fork_copy_kernel<uint8_t>), grid, dim3(kThreads), 0, st, p);
+  return check_launch();
+}
+
+extern "C" size_t lsattn_release_workspace_bytes(int64_t n, int64_t max_len_in_batch) {
+  if (n <= 0 || max_len_in_batch <= 0 || n > 65535 || max_len_in_batch > 0x7fff0000 || n * max_len_in_batch <= kOneGroupTokens) return 0;
+  return (size_t)(n * ((max_len_in_batch + kThreads - 1) / kThreads) * 8);
+}
+
+extern "C" int lsattn_release_requests(const int32_t* req_to_tokens, int64_t num_reqs, int64_t max_seq_len, const int32_t* b_req_idx, const int32_t* b_seq_len, int64_t n,
+                                       int64_t max_len_in_batch, int32_t* mem_state, int64_t pool_size, int64_t* counts, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  if (!req_to_tokens || !b_req_idx || !b_seq_len || !mem_state || !counts || num_reqs < 0 || max_seq_len < 0 || n < 0 || max_len_in_batch < 0 || pool_size < 0 ||
+      num_reqs > 0x7fffffff || max_seq_len > 0x7fff0000 || n > 65535 || pool_size > 0x7fffffff || max_len_in_batch > 0x7fff0000)
+    return LSATTN_ERR_INVALID_ARG;
+  const int64_t most = max_len_in_batch < max_seq_len ? max_len_in_batch : max_seq_len;
+  const size_t need = lsattn_release_workspace_bytes(n, most);
+  if (need && (!workspace || workspace_bytes < need)) return LSATTN_ERR_WORKSPACE;
+  if (need && ((uintptr_t)workspace & 3)) return LSATTN_ERR_INVALID_ARG;
+  ReleaseParams p{req_to_tokens, max_seq_len, (int32_t)most, b_req_idx, b_seq_len, (int32_t)n, (int32_t)num_reqs, mem_state, (int32_t)pool_size, 0, (int32_t*)workspace, counts};
+  hipStream_t st = (hipStream_t)stream;
+  if (!need) {
+    LSATTN_LAUNCH_KERNEL(release_one_group_kernel, dim3(1), dim3(1024), 0, st, p, (int)most);
+    return check_launch();
+  }
+  p.blocks = (int32_t)((most + kThreads - 1) / kThreads);
+  LSATTN_LAUNCH_KERNEL(release_kernel, dim3((unsigned)p.blocks, (unsigned)n), dim3(kThreads), 0, st, p);
+  if (hipPeekAtLastError() != hipSuccess) return check_launch();
+  LSATTN_LAUNCH_KERNEL(release_sum_kernel, dim3(1), dim3(1024), 0, st, p);
+  return check_launch();
+}
+
+extern "C" size_t lsattn_compact_workspace_bytes(int64_t pool_size) {
+  if (pool_size <= 0 || pool_size > 0x7fff0000) return 0;
+  const int64_t blocks = (pool_size + kPlanSlots - 1) / kPlanSlots;
+  return (size_t)(4 * (4 + blocks + 2 * (pool_size / 2 + 1) + pool_size));
+}
+
+extern "C" int lsattn_compact_pool(const lsattn_compact_args* a, const lsattn_pool_rows* rows, void* stream) {
+  if (!a || !rows || !rows_ok(rows) || (rows->rows && rows->num_slots < a->pool_size)) return LSATTN_ERR_INVALID_ARG;
+  if (a->pool_size < 0 || a->pool_size > 0x7fff0000 || a->n < 0 || a->n > 65535 || a->max_len_in_batch < 0 || a->num_reqs < 0 || a->num_reqs > 0x7fffffff ||
+      a->max_seq_len < 0 || a->max_seq_len > 0x7fff0000)
+    return LSATTN_ERR_INVALID_ARG;
+  if (a->pool_size == 0) return LSATTN_OK;
+  if (!a->mem_state || !a->remap || (a->n && (!a->req_to_tokens || !a->b_req_idx || !a->b_seq_len))) return LSATTN_ERR_INVALID_ARG;
+  if (!a->workspace || a->workspace_bytes < lsattn_compact_workspace_bytes(a->pool_size)) return LSATTN_ERR_WORKSPACE;
+  if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
+  const int64_t most = a->max_len_in_batch < a->max_seq_len ? a->max_len_in_batch : a->max_seq_len;
+  CompactParams p = {};
+  p.state = a->mem_state, p.size = (int32_t)a->pool_size, p.blocks = (int32_t)((a->pool_size + kPlanSlots - 1) / kPlanSlots);
+  p.header = (int32_t*)a->workspace, p.used = p.header + 4, p.hole = p.used + p.blocks, p.source = p.hole + (p.size / 2 + 1), p.code = p.source + (p.size / 2 + 1);
+  p.remap = a->remap, p.table = a->req_to_tokens, p.max_seq_len = a->max_seq_len, p.req = a->b_req_idx, p.len = a->b_seq_len;
+  p.n = (int32_t)a->n, p.num_reqs = (int32_t)a->num_reqs;
+  p.table_blocks = (int32_t)((most + kThreads - 1) / kThreads), p.most = (int32_t)most;
+  if ((int64_t)p.table_blocks * p.n > kMaxUnits - 0x400000) return LSATTN_ERR_INVALID_ARG;
+  p.layers = (int32_t)rows->num_layers;
+  const int64_t moves = p.size / 2, fill = p.layers ? (16 * kCUs + p.layers - 1) / p.layers : 4 * kCUs, by_moves = (moves + kMoveRows - 1) / kMoveRows;
+  p.move_wgs = (int32_t)(by_moves < 1 ? 1 : by_moves < fill ? by_moves : fill);
+  const unsigned move_wgs = (unsigned)(p.move_wgs * (p.layers ? p.layers : 1)), table_wgs = (unsigned)(p.table_blocks * p.n);
+  hipStream_t st = (hipStream_t)stream;
+  LSATTN_LAUNCH_KERNEL(compact_count_kernel, dim3(p.blocks), dim3(kPlanThreads), 0, st, p);
+  if (hipPeekAtLastError() != hipSuccess) return check_launch();
+  LSATTN_LAUNCH_KERNEL(compact_plan_kernel, dim3(p.blocks), dim3(kPlanThreads), 0, st, p);
+  if (hipPeekAtLastError() != hipSuccess) return check_launch();
+  if (p.layers) set_rows(p.r, rows->rows, rows->layer_stride_bytes, rows->slot_stride_bytes, rows->row_bytes / 16, rows->num_slots);
+  LSATTN_LAUNCH_KERNEL((compact_move_kernel<u32x4, true>), dim3(move_wgs + table_wgs), dim3(kThreads), 0, st, p);
+  if (!rows->scales || hipPeekAtLastError() != hipSuccess) return check_launch();
+  set_rows(p.r, rows->scales, rows->scale_layer_stride_bytes, rows->scale_slot_stride_bytes, rows->scale_bytes, rows->num_slots);
+  LSATTN_LAUNCH_KERNEL((compact_move_kernel<uint8_t, false>), dim3(move_wgs), dim3(kThreads), 0, st, p);
+  return check_launch();
+}

@@ -1,0 +1,935 @@
+// Attention for requests that share the first tokens of their contexts (gfx950, wave64).
+//
+// A group of requests names the same pool slots for its first P tokens.  For its query rows (a token and a query head each) the softmax over prefix and own
+// tokens splits,
+//   o = sum_j exp(s_j) v_j / sum_j exp(s_j),   j over the prefix, then over the request's own tokens,
+// into partials with a log-sum-exp each, and the prefix's part is one product of all the group's rows with the same keys: every K/V row of the prefix is
+// read once for 128 query rows and goes through the matrix pipe, where a decode kernel reads it once per request.
+//
+// Prefix part: a workgroup of four waves owns 128 rows of one KV head (a wave 32, as rows come: token by token, the query heads of the KV head side by side,
+// whatever their number) and walks tiles of 64 keys of a share of the prefix:
+//   * the work of all groups, (row tile, block of 64 keys) pairs, is dealt in equal shares to the workgroups of a KV head, whatever the groups' sizes and prefixes
+//     are (the host does not know them); a workgroup leaves one fp32 partial per row tile it touches;
+//   * K and V rows lie where the request table says.  Direct loads to LDS take an address per lane, so gathering them costs a multiplication per load; two stages,
+//     16-byte chunks XORed with the row (prefill_small.hip says why); the slots of the tile after next are under way;
+//   * the order of the keys in a tile does not matter without a causal mask: rows lie so that a lane's slots are neighbours in the table;
+//   * entries of the table that name no slot, and positions past the prefix, are a mask of the tile; its V rows are cleared in LDS before they are used;
+//   * scores transposed, S^T = K Q^T, so that P^T goes into O^T += V^T P^T from the lane that computed it.  fp16: P as fp16, O divided by the sum of the very weights
+//     that multiplied V; bfloat16: P in two parts, high and low (8 bits alone would cost 1e-3 of O);
+//   * the running maximum is raised where a lane's eight weights pass 2^15, and then set so that the largest is 2^9.
+// Own tokens: the decode walk of pool_walk.hip.h from the prefix's end on, in the same launch (those workgroups wait for memory where the others keep the matrix
+// pipe busy), equal shares of all requests' own tokens.  A second launch joins a request's partials.
+#include <type_traits>
+
+#include "pool_walk.hip.h"
+
+namespace lsattn {
+namespace {
+
+typedef __attribute__((address_space(3))) i16x4* lds_i16x4_ptr;
+
+constexpr int kRows = 128;   // query rows of a workgroup of the prefix part
+constexpr int kKeys = 64;    // keys of a tile
+constexpr float kPrefixHead = 9.f;
+
+struct SharedParams {
+  PoolParams w;  // the pool, the table, the requests' own tokens and their shares; part_o / part_lse: the own parts
+  int64_t q_st, q_sh;  // bytes
+  const int32_t* g_start;
+  const int32_t* g_size;
+  const int32_t* g_req;
+  const int32_t* g_prefix;
+  int32_t groups, rows;  // rows of q
+  int32_t most;          // a bound of the prefixes: longer ones are cut there
+  int32_t shares, parts; // of the prefix part, per KV head; partials of 128 rows per KV head
+  int32_t wgs;           // workgroups of the prefix part
+  float* pre_o;          // [hkv, parts, 128, D]
+  float* pre_lse;        // [hkv, parts, 128], log2 domain
+  FastDiv by_hkv, by_group, by_pre_shares;
+};
+
+// s_waitcnt vmcnt(0) (expcnt / lgkmcnt fields left at their maximum)
+__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+
+// 64 groups at a time, one per lane.  Groups stand in ascending order of their rows; a row that two of them name belongs to the first, so that
+// whatever the lists hold no row is counted twice.
+struct Groups {
+  int at;                    // the group of lane 0
+  int lo, size, req, prefix; // of the lane's group: its rows, from lo on
+  int end;                   // the end of the rows up to the lane's group
+  int tiles, blocks;         // row tiles, blocks of keys
+  int tiles_to, units_to;    // sums over the 64 up to the lane's group; a unit is a row tile with a block
+  __device__ __forceinline__ void look(const SharedParams& p, int g0, int end_before) {
+    const int lane = threadIdx.x & 63, g = g0 + lane;
+    at = g0;
+    int start = 0, last = 0;
+    req = 0, prefix = 0;
+    if (g < p.groups) {
+      start = p.g_start[g], last = p.g_size[g], req = p.g_req[g], prefix = p.g_prefix[g];
+      start = start < 0 ? 0 : start < p.rows ? start : p.rows;
+      last = last < 0 ? start : last < p.rows - start ? start + last : p.rows;
+      prefix = prefix < 0 || req < 0 || req >= p.w.num_reqs ? 0 : prefix < p.most ? prefix : p.most;
+    }
+    end = last;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int below = __shfl_up(end, d, 64);
+      if (lane >= d) end = below > end ? below : end;
+    }
+    end = end > end_before ? end : end_before;
+    const int below = __shfl_up(end, 1, 64);
+    const int taken = lane ? below : end_before;
+    lo = start > taken ? start : taken;
+    size = last > lo ? last - lo : 0;
+    blocks = (prefix + kKeys - 1) / kKeys;
+    tiles = blocks ? (int)(((int64_t)size * p.w.group + kRows - 1) / kRows) : 0;
+    tiles_to = tiles, units_to = tiles * blocks;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int t = __shfl_up(tiles_to, d, 64), u = __shfl_up(units_to, d, 64);
+      if (lane >= d) tiles_to += t, units_to += u;
+    }
+  }
+  __device__ __forceinline__ int end_of_all() const { return __builtin_amdgcn_readlane(end, 63); }
+  __device__ __forceinline__ int all_tiles() const { return __builtin_amdgcn_readlane(tiles_to, 63); }
+  __device__ __forceinline__ int all_units() const { return __builtin_amdgcn_readlane(units_to, 63); }
+};
+__device__ __forceinline__ int all_units_of(const SharedParams& p, Groups& g) {  // leaves `g` at the first groups
+  g.look(p, 0, 0);
+  int total = g.all_units();
+  if (p.groups > 64) {
+    for (int g0 = 64; g0 < p.groups; g0 += 64) g.look(p, g0, g.end_of_all()), total += g.all_units();
+    g.look(p, 0, 0);
+  }
+  return total;
+}
+__device__ __forceinline__ int per_pre_share(const SharedParams& p, int total) {
+  const int per = (int)div_by((uint32_t)(total + p.shares - 1), p.by_pre_shares);
+  return per < 1 ? 1 : per;
+}
+
+// The group of row b (per lane; -1: none) and its numbers, looked up from the first groups on.
+struct Membership {
+  int lo, prefix, tile0, unit0, blocks;  // the group's first row, prefix, and the tiles and units of all groups in front of it
+  __device__ __forceinline__ void find(const SharedParams& p, Groups& g, int b) {
+    lo = prefix = tile0 = unit0 = blocks = 0;
+    int tiles = 0, units = 0;
+    for (int g0 = 0;;) {
+      int n = 0;  // groups of the 64 that end at b or in front of it
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) {
+        const int e = __shfl(g.end, n + d - 1, 64);
+        n += e <= b ? d : 0;
+      }
+      const int e63 = __shfl(g.end, 63, 64);
+      const bool here = n < 63 || e63 > b;  // (n counts up to 63)
+      const int s = __shfl(g.lo, n, 64), sz = __shfl(g.size, n, 64), pr = __shfl(g.prefix, n, 64), bl = __shfl(g.blocks, n, 64);
+      const int tt = __shfl(g.tiles_to, n, 64), t1 = __shfl(g.tiles, n, 64), ut = __shfl(g.units_to, n, 64);
+      if (here && s <= b && b < s + sz) lo = s, prefix = pr, blocks = bl, tile0 = tiles + tt - t1, unit0 = units + ut - t1 * bl;
+      tiles += g.all_tiles(), units += g.all_units();
+      g0 += 64;
+      if (g0 >= p.groups) break;
+      g.look(p, g0, g.end_of_all());
+    }
+    if (p.groups > 64) g.look(p, 0, 0);
+  }
+};
+
+// ------------------------------------------------------------------------------------------------ the prefix part
+template <typename T, int D> constexpr int kPrefixLds = 2 * 2 * kKeys * D * 2 + 2 * 8;  // two stages of K and V tiles, their masks
+
+template <typename T, int D> __device__ __forceinline__ void prefix_share(const SharedParams& p, char* lds, int kvh, int share) {
+  constexpr bool HIGH_LOW = __is_same(T, BF16);
+  constexpr int NP = HIGH_LOW ? 2 : 1;      // parts of P
+  constexpr int KS = D / 32, NDB = D / 16;  // contraction steps of Q K^T; 16-wide blocks of the head
+  constexpr int CPR = D / 8, RB = D * 2;    // 16-byte chunks and bytes of a row
+  constexpr int TB = kKeys * RB;
+  constexpr int RPI = 64 / CPR, NI = 16 / RPI;  // rows per load instruction; instructions for a wave's 16 rows of a tile
+  constexpr int RPB = 256 / RB;
+  constexpr int kMaskOff = 4 * TB;
+  auto swz_k = [](int row) { return (row / RPB) & (CPR - 1); };
+  auto swz_v = [](int row) { return ((row / RPB) & (CPR / 2 - 1)) << 1; };
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int c = lane & 15, g = lane >> 4;
+  const int lds_base = (int)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
+
+  Groups gs;
+  const int total = all_units_of(p, gs);
+  const int per = per_pre_share(p, total);
+  if ((int64_t)share * per >= total) return;
+  int at = share * per;
+  const int end = total - at < per ? total : at + per;
+  int first = 0, tiles_before = 0;  // units and tiles in front of the 64 groups
+  while (at >= first + gs.all_units()) {
+    first += gs.all_units(), tiles_before += gs.all_tiles();
+    gs.look(p, gs.at + 64, gs.end_of_all());
+  }
+  // the lane's chunk of its load instructions' rows, K and V
+  const int j_row = lane / CPR;
+  uint32_t k_chunk[NI], v_chunk[NI];
+#pragma unroll
+  for (int i = 0; i < NI; i++) {
+    k_chunk[i] = (uint32_t)(((lane % CPR) ^ swz_k(RPI * i + j_row)) * 16);
+    v_chunk[i] = (uint32_t)(((lane % CPR) ^ swz_v(RPI * i + j_row)) * 16);
+  }
+  int kaddr[KS], vaddr[NDB];
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) kaddr[ks] = lds_base + c * RB + (((4 * ks + g) & (CPR - 1)) ^ swz_k(c)) * 16;
+#pragma unroll
+  for (int db = 0; db < NDB; db++) {
+    const int row = 4 * g + (c >> 2);
+    vaddr[db] = lds_base + TB + row * RB + ((2 * db + ((c & 3) >> 1)) ^ swz_v(row)) * 16 + (c & 1) * 8;
+  }
+  const char* const kb = p.w.k + kvh * p.w.k_s1;
+  const char* const vb = p.w.v + kvh * p.w.v_s1;
+  const uint32_t k_s0 = (uint32_t)p.w.k_s0, v_s0 = (uint32_t)p.w.v_s0;
+  const float scale = p.w.scale_log2;
+
+  while (at < end) {
+    int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(first + gs.units_to > at));
+    const int blocks = __builtin_amdgcn_readlane(gs.blocks, l), tiles = __builtin_amdgcn_readlane(gs.tiles, l);
+    const int unit0 = first + __builtin_amdgcn_readlane(gs.units_to, l) - tiles * blocks;
+    const int tile = (at - unit0) / blocks, block0 = (at - unit0) - tile * blocks;
+    const int nt = blocks - block0 < end - at ? blocks - block0 : end - at;  // tiles of keys to walk
+    const int part = share + tiles_before + __builtin_amdgcn_readlane(gs.tiles_to, l) - tiles + tile;
+    const int lo = __builtin_amdgcn_readlane(gs.lo, l), prefix = __builtin_amdgcn_readlane(gs.prefix, l);
+    const int rows = __builtin_amdgcn_readlane(gs.size, l) * p.w.group;
+    const int32_t* const row_slots = p.w.table + (int64_t)__builtin_amdgcn_readlane(gs.req, l) * p.w.max_seq_len;
+    const int row0 = tile * kRows + wave * 32;
+    const bool active = row0 < rows;
+
+    u32x4 qreg[2][KS];
+    f32x4 oacc[2][NDB], l_pv[2];
+    float m_run[2], l_run[2];
+#pragma unroll
+    for (int qb = 0; qb < 2; qb++) {
+      int r = row0 + 16 * qb + c;
+      r = r < rows ? r : rows - 1;
+      const int tok = (int)div_by((uint32_t)r, p.by_group), h = kvh * p.w.group + r - tok * p.w.group;
+      const char* src = p.w.q + (int64_t)(lo + tok) * p.q_st + (int64_t)h * p.q_sh + g * 16;
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) qreg[qb][ks] = *(const u32x4*)(src + ks * 64);
+#pragma unroll
+      for (int db = 0; db < NDB; db++) oacc[qb][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+      l_pv[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_run[qb] = -INFINITY, l_run[qb] = 0.f;
+    }
+    int slot[NI];
+    // the slots of the lane's rows of tile t (positions past the prefix repeat its last one): LDS row 16 wave + RPI i + j is key 16 wave + NI j + i
+    const int pos0 = block0 * kKeys + 16 * wave + NI * j_row;
+    auto load_slots = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const int pos = pos0 + t * kKeys + i;
+        slot[i] = row_slots[pos < prefix ? pos : prefix - 1];
+      }
+    };
+    auto request = [&](int stage, int t) __attribute__((always_inline)) {
+      const int dst = __builtin_amdgcn_readfirstlane(lds_base + stage * 2 * TB + wave * 16 * RB);
+      uint32_t there = 0;  // bit per LDS row of the wave
+#pragma unroll
+      for (int i = 0; i < NI; i++) {
+        const bool ok = pos0 + t * kKeys + i < prefix && (uint32_t)slot[i] < (uint32_t)p.w.num_slots;
+        const uint64_t lanes = __builtin_amdgcn_ballot_w64(ok);
+#pragma unroll
+        for (int j = 0; j < RPI; j++) there |= (uint32_t)((lanes >> (CPR * j)) & 1u) << (RPI * i + j);
+        const uint32_t sl = ok ? (uint32_t)slot[i] : 0u;
+        const char* ka = kb + (uint64_t)sl * k_s0 + k_chunk[i];
+        const char* va = vb + (uint64_t)sl * v_s0 + v_chunk[i];
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
+                     "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, off" ::"s"(dst + i * 1024), "s"(dst + TB + i * 1024), "v"(ka), "v"(va)
+                     : "m0", "memory");
+      }
+      if (lane == 0) *(uint16_t*)(lds + kMaskOff + stage * 8 + wave * 2) = (uint16_t)there;
+    };
+    __syncthreads();  // (the tiles of the segment before are done with)
+    load_slots(0);
+    request(0, 0);
+    load_slots(1);
+    auto step = [&](auto stage_tag, int t) __attribute__((always_inline)) {
+      constexpr int S = decltype(stage_tag)::value;
+      wait_loads();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (t + 1 < nt) {
+        request(S ^ 1, t + 1);
+        load_slots(t + 2);
+      }
+      const uint64_t mask64 = *(const uint64_t*)(lds + kMaskOff + S * 8);
+      const uint32_t mask[2] = {(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)mask64), (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(mask64 >> 32))};
+      if ((mask[0] & mask[1]) != 0xffffffffu) {  // (the same for the whole workgroup)
+        // (what lies in the slot that was read in place of one that does not exist may be infinite or NaN, and 0 times that is NaN)
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+          const int r = RPI * i + j_row;
+          if (!((mask[wave >> 1] >> (16 * (wave & 1) + r)) & 1u))
+            *(u32x4*)(lds + S * 2 * TB + TB + wave * 16 * RB + i * 1024 + lane * 16) = u32x4{0u, 0u, 0u, 0u};
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      if (!active) return;
+#pragma unroll
+      for (int part32 = 0; part32 < 2; part32++) {
+        u32x4 ka[2][KS];
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+          for (int ks = 0; ks < KS; ks++)
+            ka[kk][ks] = *(const __attribute__((address_space(3))) u32x4*)(kaddr[ks] + S * 2 * TB + (32 * part32 + 16 * kk) * RB);
+        f32x4 s[2][2];
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++) s[qb][0] = s[qb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+          for (int kk = 0; kk < 2; kk++)
+#pragma unroll
+            for (int qb = 0; qb < 2; qb++) s[qb][kk] = mfma<T>(ka[kk][ks], qreg[qb][ks], s[qb][kk]);
+        if (mask[part32] != 0xffffffffu) {
+          const uint32_t mine = mask[part32] >> (4 * g);
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) s[qb][e / 4][e % 4] = (mine >> (16 * (e / 4) + e % 4)) & 1u ? s[qb][e / 4][e % 4] : -INFINITY;
+        }
+        u32x4 pk[2][NP];
+        float ps[2];
+        auto compute_p = [&](int qb, float neg_m) __attribute__((always_inline)) {
+          float pv[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][e / 4][e % 4], scale, neg_m));
+          ps[qb] = ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            pk[qb][0][e] = pack2<T>(pv[2 * e], pv[2 * e + 1]);
+            if constexpr (HIGH_LOW) {
+              float a, b;
+              unpack2<T>(pk[qb][0][e], a, b);
+              pk[qb][NP - 1][e] = pack2<T>(pv[2 * e] - a, pv[2 * e + 1] - b);
+            }
+          }
+        };
+        bool over = false;
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++) {
+          compute_p(qb, -m_run[qb]);
+          over |= !(ps[qb] < 32768.f);
+        }
+        if (__builtin_expect(__builtin_amdgcn_ballot_w64(over) != 0, 0)) {
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++) {
+            const float mx = fmaxf(fmaxf(fmaxf(s[qb][0][0], s[qb][0][1]), fmaxf(s[qb][0][2], s[qb][0][3])),
+                                   fmaxf(fmaxf(s[qb][1][0], s[qb][1][1]), fmaxf(s[qb][1][2], s[qb][1][3])));
+            const float m_new = fmaxf(m_run[qb], col_max(mx) * scale - kPrefixHead);
+            const float alpha = exp2_diff(m_run[qb], m_new);
+            l_run[qb] *= alpha;
+            l_pv[qb] *= alpha;
+#pragma unroll
+            for (int db = 0; db < NDB; db++) oacc[qb][db] *= alpha;
+            m_run[qb] = m_new;
+            compute_p(qb, m_new == -INFINITY ? 0.f : -m_new);  // (a row that has seen no key: every weight is 0)
+          }
+        }
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++) l_run[qb] += ps[qb];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int db = 0; db < NDB; db++) {
+          const int va_at = vaddr[db] + S * 2 * TB + 32 * part32 * RB;
+          const i16x4 xa = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr)va_at);
+          const i16x4 xb = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_ptr)(va_at + 16 * RB));
+          const u32x2 wa = __builtin_bit_cast(u32x2, xa), wb = __builtin_bit_cast(u32x2, xb);
+          const u32x4 va = u32x4{wa[0], wa[1], wb[0], wb[1]};
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+            for (int n = 0; n < NP; n++) oacc[qb][db] = mfma<T>(va, pk[qb][n], oacc[qb][db]);
+        }
+        if constexpr (!HIGH_LOW) {
+          constexpr uint32_t kOnes = 0x3C003C00u;
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++) l_pv[qb] = mfma<T>(u32x4{kOnes, kOnes, kOnes, kOnes}, pk[qb][0], l_pv[qb]);
+        }
+      }
+    };
+    for (int t = 0; t < nt; t += 2) {
+      step(std::integral_constant<int, 0>{}, t);
+      if (t + 1 < nt) step(std::integral_constant<int, 1>{}, t + 1);
+    }
+    if (active && part < p.parts) {
+#pragma unroll
+      for (int qb = 0; qb < 2; qb++) {
+        const float l_tot = col_sum(l_run[qb]);
+        const float l_of_v = HIGH_LOW ? l_tot : l_pv[qb][0];
+        const float inv = l_of_v == 0.f ? 0.f : 1.f / l_of_v;
+        const int r = row0 + 16 * qb + c;
+        if (r < rows) {
+          const int64_t to = ((int64_t)kvh * p.parts + part) * kRows + (r - tile * kRows);
+          float* dst = p.pre_o + to * D + 4 * g;
+#pragma unroll
+          for (int db = 0; db < NDB; db++) *(f32x4*)(dst + 16 * db) = oacc[qb][db] * inv;
+          if (g == 0) p.pre_lse[to] = l_tot > 0.f ? m_run[qb] + __builtin_amdgcn_logf(l_tot) : (l_tot == l_tot ? -INFINITY : l_tot);
+        }
+      }
+    }
+    at += nt;
+    if (at < end && at >= first + gs.all_units()) {
+      first += gs.all_units(), tiles_before += gs.all_tiles();
+      gs.look(p, gs.at + 64, gs.end_of_all());
+      while (gs.all_units() == 0) gs.look(p, gs.at + 64, gs.end_of_all());  // (at < total: a later group has some)
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the requests' own tokens
+// Blocks of own tokens of all requests, numbered request by request; 64 requests at a time, of which a lane has one each.  A request that is shorter than its group's prefix
+// shares nothing.
+struct OwnRequests {
+  int first_request, len, req, n_own, units, up_to;
+  __device__ __forceinline__ void look(const SharedParams& p, Groups& g, int b0) {
+    const int lane = threadIdx.x & 63, b = b0 + lane;
+    first_request = b0;
+    Membership m;
+    m.find(p, g, b);
+    len = req = n_own = 0;
+    if (b < p.w.batch) {
+      n_own = visible(p.w, b, len, req);
+      n_own -= m.prefix <= len ? m.prefix : 0;
+    }
+    units = (n_own + kBlock - 1) / kBlock;
+    up_to = units;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int below = __shfl_up(up_to, d, 64);
+      if (lane >= d) up_to += below;
+    }
+  }
+  __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(up_to, 63); }
+};
+__device__ __forceinline__ int per_own_share(const PoolParams& p, int total) {
+  const int per = (int)div_by((uint32_t)(total + p.shares - 1), p.by_shares);
+  return per < p.min_units ? p.min_units : per;
+}
+
+template <typename T, int D> __device__ __forceinline__ void own_share(const SharedParams& sp, char* lds, int share, int task) {
+  const PoolParams& p = sp.w;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  Groups gs;
+  gs.look(sp, 0, 0);
+  OwnRequests rs;
+  rs.look(sp, gs, 0);
+  int total = rs.all();
+  if (p.batch > 64) {
+    for (int b0 = 64; b0 < p.batch; b0 += 64) rs.look(sp, gs, b0), total += rs.all();
+    rs.look(sp, gs, 0);
+  }
+  const int per_share = per_own_share(p, total);
+  if ((int64_t)share * per_share >= total) return;
+  int at = share * per_share;
+  const int end = total - at < per_share ? total : at + per_share;
+  int first = 0;
+  while (at >= first + rs.all()) {
+    first += rs.all();
+    rs.look(sp, gs, rs.first_request + 64);
+  }
+  int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(first + rs.up_to > at));
+  first += __builtin_amdgcn_readlane(rs.up_to, l) - __builtin_amdgcn_readlane(rs.units, l);
+  Walk<T, T, D> w(p, lds + wave * kWaveLds<T, D>);
+  const int kvh = (int)div_by((uint32_t)task, p.by_sub), sg = task - kvh * p.sub_groups;
+  const int h0 = kvh * p.group + sg * kHeads;
+  const int nh = p.group - sg * kHeads < kHeads ? p.group - sg * kHeads : kHeads;
+  for (;;) {
+    const int b = rs.first_request + l, units = __builtin_amdgcn_readlane(rs.units, l), n_own = __builtin_amdgcn_readlane(rs.n_own, l);
+    const int to = end - first < units ? end : first + units;
+    if (to > at) {
+      w.start(b, __builtin_amdgcn_readlane(rs.req, l), task, __builtin_amdgcn_readlane(rs.len, l), n_own);
+      const int last = (to - first) * kBlock;
+      w.run((at - first) * kBlock, last < n_own ? last : n_own, 1);
+      w.join();
+      if (w.c < nh) {
+        const int64_t r0 = ((int64_t)(share + b) * p.hq + h0 + w.c);
+        const float inv = w.l == 0.f ? 0.f : 1.f / w.l;
+        float* dst = p.part_o + r0 * D;
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+          for (int j = 0; j < D / 16; j += 4)
+            *(f32x4*)(dst + (D / 16) * (4 * w.g + r) + j) = f32x4{w.acc[j][r], w.acc[j + 1][r], w.acc[j + 2][r], w.acc[j + 3][r]} * inv;
+        if (w.g == 0) p.part_lse[r0] = w.l > 0.f ? w.m + __builtin_amdgcn_logf(w.l) : (w.l == w.l ? -INFINITY : w.l);  // (log2 domain)
+      }
+      at = to;
+    }
+    if (at >= end) return;
+    first += units;
+    if (++l == 64) rs.look(sp, gs, rs.first_request + 64), l = 0;
+  }
+}
+
+// Workgroups of the prefix part first, then those of the own tokens, four waves with a share each.
+template <typename T, int D> constexpr int kSharedLds = kPrefixLds<T, D> > 4 * kWaveLds<T, D> ? kPrefixLds<T, D> : 4 * kWaveLds<T, D>;
+template <typename T, int D, bool OWN>
+__global__ __launch_bounds__(256, 2) void shared_prefix_kernel(SharedParams p) {
+  __shared__ __attribute__((aligned(1024))) char lds[OWN ? kSharedLds<T, D> : kPrefixLds<T, D>];
+  if (!OWN || (int)blockIdx.x < p.wgs) {
+    const int share = (int)div_by(blockIdx.x, p.by_hkv);  // (with a multiple of eight KV heads a head's workgroups run on one XCD: ids are dealt round-robin)
+    prefix_share<T, D>(p, lds, (int)blockIdx.x - share * p.w.hkv, share);
+    return;
+  }
+  if constexpr (OWN) {
+    const uint32_t n = gridDim.x - p.wgs, x = blockIdx.x - p.wgs;  // (n is a multiple of 8)
+    const uint32_t unit = ((x & 7) * (n >> 3) + (x >> 3)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int share = (int)div_by(unit, p.w.by_tasks), task = (int)(unit - (uint32_t)share * p.w.tasks);
+    if (share < p.w.shares) own_share<T, D>(p, lds, share, task);
+  }
+}
+
+// o = sum of a row's partials by their log-sum-exps: those of its group's prefix, then those of its own tokens.  First the weights of all of them, by all threads, into LDS,
+// then the rows, whose loads wait for nothing.
+constexpr int kMaxParts = 2048;
+template <int D>
+__global__ __launch_bounds__(256) void shared_decode_merge_kernel(SharedParams sp) {
+  constexpr int W = D / 4, SL = 256 / W;
+  const PoolParams& p = sp.w;
+  __shared__ __attribute__((aligned(16))) float acc[SL][W * 4];
+  __shared__ float weight[kMaxParts], red[8];
+  const int h = blockIdx.x, b = blockIdx.y;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  Groups gs;
+  const uint32_t per_pre = (uint32_t)per_pre_share(sp, all_units_of(sp, gs));
+  OwnRequests rs;
+  int total = 0, first = 0, units = 0, len = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 64) {
+    rs.look(sp, gs, b0);
+    if (b >= b0 && b < b0 + 64) {
+      units = __builtin_amdgcn_readlane(rs.units, b - b0);
+      first = total + __builtin_amdgcn_readlane(rs.up_to, b - b0) - units;
+      len = __builtin_amdgcn_readlane(rs.len, b - b0);
+    }
+    total += rs.all();
+  }
+  const uint32_t per_own = (uint32_t)per_own_share(p, total);
+  const int s0 = (int)((uint32_t)first / per_own), n_own = units ? (int)((uint32_t)(first + units - 1) / per_own) - s0 + 1 : 0;
+  Membership mb;
+  mb.find(sp, gs, b);
+  const int kvh = h / p.group;
+  const int r = (b - mb.lo) * p.group + (h - kvh * p.group), tile = r / kRows;
+  int n_pre = 0, p0 = 0;
+  if (mb.blocks && mb.prefix <= len) {
+    const uint32_t u0 = (uint32_t)(mb.unit0 + tile * mb.blocks);
+    p0 = (int)(u0 / per_pre);
+    n_pre = (int)((u0 + mb.blocks - 1) / per_pre) - p0 + 1;
+    p0 += mb.tile0 + tile;
+  }
+  const int64_t pre_row = ((int64_t)kvh * sp.parts + p0) * kRows + (r - tile * kRows), own_row = (int64_t)(s0 + b) * p.hq + h;
+  const int n = n_pre + n_own;
+  float M = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const float x = i < n_pre ? sp.pre_lse[pre_row + (int64_t)i * kRows] : p.part_lse[own_row + (int64_t)(i - n_pre) * p.hq];
+    weight[i] = x;
+    M = fmaxf(M, x);
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  if (lane == 0) red[wave] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float L = 0.f;
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const float w = exp2_diff(weight[i], M);  // (NaN stays NaN)
+    weight[i] = w;
+    L += w;
+  }
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) L += __shfl_xor(L, d, 64);
+  if (lane == 0) red[4 + wave] = L;
+  __syncthreads();
+  L = (red[4] + red[5]) + (red[6] + red[7]);
+  const int slice = threadIdx.x / W, d = (threadIdx.x & (W - 1)) * 4;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = slice; i < n; i += SL) {
+    const float* row = i < n_pre ? sp.pre_o + (pre_row + (int64_t)i * kRows) * D : p.part_o + (own_row + (int64_t)(i - n_pre) * p.hq) * D;
+    sum += *(const f32x4*)(row + d) * weight[i];
+  }
+  *(f32x4*)&acc[slice][d] = sum;
+  __syncthreads();
+  if (slice) return;
+#pragma unroll
+  for (int i = 1; i < SL; i++) sum += *(const f32x4*)&acc[i][d];
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int64_t at = (int64_t)b * p.hq + h;
+  store_elem4(p.o, p.o_dtype, at * D + d, sum * inv);
+  if (d == 0) p.lse[at] = ln_of(M, L);
+}
+
+// The prompts' step: a row's partials by their log-sum-exps, folded into the running (o, m, l) as context_attention_fwd's kernels do
+// (ring_context_flashattention_nopad.py:171-188).  D / 4 lanes have a (row, head); rows of no group, or whose prefix shows them no key, stay as they are.
+struct FoldParams {
+  char* o;
+  int64_t o_st, o_sh;  // bytes
+  float* m;
+  float* l;
+  int64_t ml_st, ml_sh;
+};
+template <typename T, int D> __global__ __launch_bounds__(256) void shared_prefix_fold_kernel(SharedParams sp, FoldParams f) {
+  constexpr int W = D / 4;
+  Groups gs;
+  const uint32_t per = (uint32_t)per_pre_share(sp, all_units_of(sp, gs));
+  const int64_t i = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
+  const int b = (int)(i / sp.w.hq), h = (int)(i - (int64_t)b * sp.w.hq);
+  Membership mb;
+  mb.find(sp, gs, b < sp.rows ? b : sp.rows - 1);
+  if (b >= sp.rows || !mb.blocks) return;
+  const int kvh = h / sp.w.group, r = (b - mb.lo) * sp.w.group + (h - kvh * sp.w.group), tile = r / kRows, x = threadIdx.x & (W - 1);
+  const uint32_t u0 = (uint32_t)(mb.unit0 + tile * mb.blocks), p0 = u0 / per;
+  const int n = (int)((u0 + mb.blocks - 1) / per - p0) + 1;
+  const int64_t row = ((int64_t)kvh * sp.parts + p0 + mb.tile0 + tile) * kRows + (r - tile * kRows);
+  float M = -INFINITY;
+  for (int j = x; j < n; j += W) M = fmaxf(M, sp.pre_lse[row + (int64_t)j * kRows]);
+#pragma unroll
+  for (int d = W / 2; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  const int64_t ml = (int64_t)b * f.ml_st + (int64_t)h * f.ml_sh;
+  const float m_old = f.m[ml], l_old = f.l[ml];
+  const float top = fmaxf(M, m_old);
+  float L = 0.f;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < n; j++) {
+    const float w = exp2_diff(sp.pre_lse[row + (int64_t)j * kRows], top);
+    L += w;
+    sum += *(const f32x4*)(sp.pre_o + (row + (int64_t)j * kRows) * D + 4 * x) * w;
+  }
+  if (L == 0.f) return;
+  const float w_old = l_old * exp2_diff(m_old, top);
+  uint16_t* o = (uint16_t*)(f.o + (int64_t)b * f.o_st + (int64_t)h * f.o_sh) + 4 * x;
+  if (w_old != 0.f) {  // (a row in its start state may hold anything)
+    const u32x2 old = *(const u32x2*)o;
+    float x0, x1, x2, x3;
+    unpack2<T>(old[0], x0, x1);
+    unpack2<T>(old[1], x2, x3);
+    sum += f32x4{x0, x1, x2, x3} * w_old;
+    L += w_old;
+  }
+  sum *= 1.f / L;
+  *(u32x2*)o = u32x2{pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3])};
+  if (x == 0) f.m[ml] = top, f.l[ml] = L;
+}
+
+// Many rows: the prefixes as contiguous K/V for the prefill kernel, group g's from row g * most on.
+struct GatherParams {
+  char* k;
+  char* v;           // [groups * most, hkv, D]; V of bfloat16 as the fp16 copy that the prefill kernel multiplies
+  int32_t* list;     // [groups, most] slots
+  int32_t* vectors;  // the six vectors of the step, [6, groups]
+  int32_t most;      // as SharedParams::most
+  FastDiv by_head_chunks;
+};
+// A group's slots in the table's order without the entries that name none, and the vectors of the step.  One workgroup per group, 4096 entries at a time.
+__global__ __launch_bounds__(1024) void shared_prefix_list_kernel(SharedParams p, GatherParams a) {
+  __shared__ int sums[2][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = blockIdx.x;
+  Groups gs;
+  for (int g0 = 0, end = 0;; g0 += 64, end = gs.end_of_all()) {
+    gs.look(p, g0, end);
+    if (g < g0 + 64) break;
+  }
+  const int l = g & 63, lo = __builtin_amdgcn_readlane(gs.lo, l), size = __builtin_amdgcn_readlane(gs.size, l);
+  const int prefix = __builtin_amdgcn_readlane(gs.prefix, l);
+  const int32_t* const slots = p.w.table + (int64_t)__builtin_amdgcn_readlane(gs.req, l) * p.w.max_seq_len;
+  int32_t* const list = a.list + (int64_t)g * a.most;
+  int count = 0, set = 0;
+  for (int at = 0; at < prefix; at += 4096, set ^= 1) {
+    int slot[4], mine = 0;
+    bool ok[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int i = at + 4 * (int)threadIdx.x + e;
+      slot[e] = i < prefix ? slots[i] : -1;
+      ok[e] = (uint32_t)slot[e] < (uint32_t)p.w.num_slots;
+      mine += ok[e];
+    }
+    int up_to = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int below = __shfl_up(up_to, d, 64);
+      if (lane >= d) up_to += below;
+    }
+    if (lane == 63) sums[set][wave] = up_to;
+    __syncthreads();
+    int rank = count + up_to - mine;
+#pragma unroll
+    for (int w = 0; w < 16; w++) {
+      rank += w < wave ? sums[set][w] : 0;
+      count += sums[set][w];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+      if (ok[e]) list[rank++] = slot[e];
+  }
+  if (threadIdx.x == 0) {
+    int32_t* v = a.vectors + g;
+    v[0] = size ? lo : 0;             // q_b_start_loc
+    v[p.groups] = size;               // q_b_seq_len
+    v[2 * p.groups] = a.most;         // the rows' position: behind every key
+    v[3 * p.groups] = g * a.most;     // kv_b_start_loc
+    v[4 * p.groups] = count;          // kv_b_seq_len
+    v[5 * p.groups] = 0;
+  }
+}
+// A thread has 16 bytes of a row.
+template <typename T> __global__ __launch_bounds__(256) void shared_prefix_gather_kernel(SharedParams p, GatherParams a, uint32_t head_chunks) {
+  const uint32_t chunks = 2 * p.w.hkv * head_chunks;  // of a token
+  const int g = blockIdx.y;
+  const int32_t* const list = a.list + (int64_t)g * a.most;
+  const int64_t total = (int64_t)a.vectors[4 * p.groups + g] * chunks;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+    const uint32_t t = (uint32_t)(i / chunks), x = (uint32_t)(i - (int64_t)t * chunks), hh = div_by(x, a.by_head_chunks), cc = x - hh * head_chunks;
+    const bool is_v = hh >= (uint32_t)p.w.hkv;
+    const uint32_t head = is_v ? hh - p.w.hkv : hh, slot = (uint32_t)list[t];
+    const char* src = is_v ? p.w.v + (uint64_t)slot * (uint32_t)p.w.v_s0 + head * p.w.v_s1 : p.w.k + (uint64_t)slot * (uint32_t)p.w.k_s0 + head * p.w.k_s1;
+    u32x4 v = *(const u32x4*)(src + cc * 16);
+    if (__is_same(T, BF16) && is_v) {  // round toward zero: exact in fp16's normal range, larger magnitudes become +-65504
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        float lo, hi;
+        unpack2<BF16>(v[e], lo, hi);
+        v[e] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+      }
+    }
+    *(u32x4*)((is_v ? a.v : a.k) + ((((int64_t)g * a.most + t) * p.w.hkv + head) * head_chunks + cc) * 16) = v;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the host's side
+constexpr int64_t kPrefixWorkgroups = 2 * kCUs;
+constexpr int64_t kOwnWaves = 4 * kCUs;
+constexpr int64_t kOwnMinUnits = 2;
+
+// a bound of the prefixes that a table can hold
+int64_t most_of(int64_t max_prefix, int64_t max_seq_len) { return max_prefix < max_seq_len ? max_prefix : max_seq_len; }
+
+struct Plan {
+  int64_t tiles, shares, parts;  // prefix part, per KV head
+  int64_t own_shares;
+  int64_t pre_floats, own_floats;  // of the workspace
+};
+// `own`: the bound of a request's own tokens (0: no own part)
+Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, int64_t max_prefix, int64_t max_own, bool decode) {
+  Plan p;
+  p.tiles = groups > 0 && max_prefix > 0 ? rows * (hq / hkv) / kRows + (groups < rows ? groups : rows) : 0;
+  const int64_t units = p.tiles * ((max_prefix + kKeys - 1) / kKeys);
+  p.shares = kPrefixWorkgroups / hkv;
+  p.shares = p.shares < 1 ? 1 : p.shares;
+  p.shares = p.shares < units ? p.shares : units < 1 ? 1 : units;
+  p.parts = p.shares + p.tiles;
+  p.pre_floats = p.tiles ? hkv * p.parts * kRows * (d + 1) : 0;
+  p.own_shares = 1, p.own_floats = 0;
+  if (decode) {
+    const int64_t tasks = hkv * ((hq / hkv + kHeads - 1) / kHeads), own_units = rows * ((max_own + kBlock - 1) / kBlock);
+    const int64_t by_waves = kOwnWaves / tasks, by_units = (own_units + kOwnMinUnits - 1) / kOwnMinUnits;
+    p.own_shares = by_waves < by_units ? by_waves : by_units;
+    p.own_shares = p.own_shares < 1 ? 1 : p.own_shares;
+    p.own_floats = (p.own_shares + rows) * hq * (d + 1);
+  }
+  return p;
+}
+
+template <typename T, int D> void launch_decode(const SharedParams& p, hipStream_t st) {
+  const int64_t own = ((int64_t)p.w.shares * p.w.tasks + 3) / 4;
+  LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<T, D, true>), dim3((unsigned)(p.wgs + (own + 7) / 8 * 8)), dim3(256), 0, st, p);
+  if (hipPeekAtLastError() != hipSuccess) return;
+  LSATTN_LAUNCH_KERNEL((shared_decode_merge_kernel<D>), dim3(p.w.hq, p.w.batch), dim3(256), 0, st, p);
+}
+
+}  // namespace
+}  // namespace lsattn
+
+using namespace lsattn;
+
+extern "C" size_t lsattn_shared_decode_workspace_bytes(int64_t batch, int64_t num_groups, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                                       int64_t max_prefix_len, int64_t max_own_len) {
+  if (batch <= 0 || num_groups < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || (head_dim != 64 && head_dim != 128) ||
+      max_prefix_len < 0 || max_own_len < 0 || batch > 65535 || num_groups > 0x7fffff00 || num_q_heads > 65535 || max_prefix_len > 0x7fffffff ||
+      max_own_len > 0x7fffffff)  // (as the launch refuses)
+    return 0;
+  const Plan pl = plan_of(batch, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, max_own_len, true);
+  return (size_t)(pl.pre_floats + pl.own_floats) * 4;
+}
+
+extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* stream) {
+  if (!a || !a->q || !a->k || !a->v || !a->o || !a->lse || !a->req_to_tokens || !a->b_req_idx || !a->b_seqlen) return LSATTN_ERR_INVALID_ARG;
+  if (a->batch < 0 || a->num_q_heads < 1 || a->num_kv_heads < 1 || a->num_slots < 1 || a->num_reqs < 0 || a->max_seq_len < 0 || a->num_groups < 0 ||
+      a->max_prefix_len < 0 || a->max_own_len < 0)
+    return LSATTN_ERR_INVALID_ARG;
+  if (a->num_groups && (!a->g_start_loc || !a->g_size || !a->g_req_idx || !a->g_prefix_len)) return LSATTN_ERR_INVALID_ARG;
+  if (a->num_q_heads % a->num_kv_heads || (a->head_dim != 128 && a->head_dim != 64)) return LSATTN_ERR_UNSUPPORTED;
+  if (a->o_dtype != LSATTN_F32 && a->o_dtype != LSATTN_F16 && a->o_dtype != LSATTN_BF16) return LSATTN_ERR_UNSUPPORTED;
+  if (a->dtype != LSATTN_F16 && a->dtype != LSATTN_BF16) return LSATTN_ERR_UNSUPPORTED;
+  if ((a->k_stride_0 * 2) % 16 || (a->k_stride_1 * 2) % 16 || (a->v_stride_0 * 2) % 16 || (a->v_stride_1 * 2) % 16 ||
+      (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->o) & 15))
+    return LSATTN_ERR_INVALID_ARG;
+  // (offsets are a slot times a stride of 32 bits)
+  auto slot_stride = [](int64_t elements) { return elements >= 0 && elements <= 0x3fffffff; };
+  if (!slot_stride(a->k_stride_0) || !slot_stride(a->v_stride_0)) return LSATTN_ERR_INVALID_ARG;
+  if (a->batch > 65535 || a->num_q_heads > 65535 || a->max_seq_len > 0x7fff0000 || a->num_slots > 0x7fffffff || a->num_reqs > 0x7fffffff ||
+      a->num_groups > 0x7fffff00 || a->max_prefix_len > 0x7fffffff || a->max_own_len > 0x7fffffff)
+    return LSATTN_ERR_INVALID_ARG;
+  if (!(a->sm_scale > 0.f)) return LSATTN_ERR_INVALID_ARG;
+  if (a->batch == 0) return LSATTN_OK;
+  const Plan pl = plan_of(a->batch, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len, a->max_own_len, true);
+  if (!a->workspace || a->workspace_bytes < (size_t)(pl.pre_floats + pl.own_floats) * 4) return LSATTN_ERR_WORKSPACE;
+  if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
+  // (units of both parts are numbered with 31 bits, and requests may be longer than the caller's bound)
+  const int64_t most = most_of(a->max_prefix_len, a->max_seq_len);
+  if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups ||
+      a->batch * ((a->max_seq_len + kBlock - 1) / kBlock) > kMaxUnits - kOwnWaves)
+    return LSATTN_ERR_INVALID_ARG;
+  SharedParams p;
+  PoolParams& w = p.w;
+  w.q = (const char*)a->q, w.k = (const char*)a->k, w.v = (const char*)a->v;
+  w.k_s0 = a->k_stride_0 * 2, w.k_s1 = a->k_stride_1 * 2, w.v_s0 = a->v_stride_0 * 2, w.v_s1 = a->v_stride_1 * 2;
+  w.ks = w.vs = nullptr, w.ks_s0 = w.ks_s1 = w.vs_s0 = w.vs_s1 = 0;
+  w.table = a->req_to_tokens, w.b_req = a->b_req_idx, w.b_len = a->b_seqlen, w.max_seq_len = a->max_seq_len;
+  w.batch = (int32_t)a->batch, w.num_reqs = (int32_t)a->num_reqs, w.num_slots = (int32_t)a->num_slots;
+  w.hq = (int32_t)a->num_q_heads, w.hkv = (int32_t)a->num_kv_heads, w.group = w.hq / w.hkv;
+  w.sub_groups = (w.group + kHeads - 1) / kHeads, w.tasks = w.hkv * w.sub_groups;
+  w.window = 0, w.sinks = 0;
+  w.scale_log2 = a->sm_scale * kLog2e;
+  w.o = (char*)a->o, w.o_dtype = a->o_dtype, w.lse = a->lse;
+  w.by_tasks = fast_div((uint32_t)w.tasks), w.by_sub = fast_div((uint32_t)w.sub_groups);
+  w.shares = (int32_t)pl.own_shares, w.by_shares = fast_div((uint32_t)pl.own_shares), w.min_units = (int32_t)kOwnMinUnits;
+  p.pre_o = (float*)a->workspace, p.pre_lse = p.pre_o + (pl.pre_floats / (a->head_dim + 1)) * a->head_dim;
+  w.part_o = p.pre_o + pl.pre_floats, w.part_lse = w.part_o + (pl.own_floats / (a->head_dim + 1)) * a->head_dim;
+  p.q_st = a->num_q_heads * a->head_dim * 2, p.q_sh = a->head_dim * 2;
+  p.g_start = a->g_start_loc, p.g_size = a->g_size, p.g_req = a->g_req_idx, p.g_prefix = a->g_prefix_len;
+  p.groups = pl.tiles ? (int32_t)a->num_groups : 0;
+  p.rows = w.batch, p.most = (int32_t)most;
+  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.wgs = pl.tiles ? (int32_t)(pl.shares * w.hkv + 7) / 8 * 8 : 0;
+  p.by_hkv = fast_div((uint32_t)w.hkv), p.by_group = fast_div((uint32_t)w.group), p.by_pre_shares = fast_div((uint32_t)pl.shares);
+  hipStream_t st = (hipStream_t)stream;
+  if (a->dtype == LSATTN_F16) {
+    if (a->head_dim == 128) launch_decode<F16, 128>(p, st);
+    else launch_decode<F16, 64>(p, st);
+  } else {
+    if (a->head_dim == 128) launch_decode<BF16, 128>(p, st);
+    else launch_decode<BF16, 64>(p, st);
+  }
+  return check_launch();
+}
+
+namespace lsattn {
+namespace {
+// The prompts' step takes its rows itself where they are few, and hands contiguous K/V to the prefill kernel where they are many.
+constexpr int64_t kGatherFromRows = 1024;  // rows of all query heads of a KV head
+bool gathers(int64_t rows, int64_t hq, int64_t hkv) { return rows * (hq / hkv) >= kGatherFromRows; }
+int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+struct PromptBytes {
+  int64_t k, list, vectors, all;
+};
+PromptBytes prompt_bytes(int64_t groups, int64_t hkv, int64_t d, int64_t most) {
+  PromptBytes b;
+  b.k = groups * most * hkv * d * 2, b.list = up16(groups * most * 4), b.vectors = up16(6 * groups * 4);
+  b.all = 2 * b.k + b.list + b.vectors;
+  return b;
+}
+}  // namespace
+}  // namespace lsattn
+
+extern "C" size_t lsattn_shared_prefill_workspace_bytes(int64_t rows, int64_t num_groups, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim,
+                                                        int64_t max_prefix_len) {
+  if (rows <= 0 || num_groups <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || (head_dim != 64 && head_dim != 128) ||
+      max_prefix_len <= 0 || rows > 0x7fffff00 || num_groups > 65535 || num_q_heads > 65535 || max_prefix_len > 0x7fff0000)  // (as the launch refuses)
+    return 0;
+  if (gathers(rows, num_q_heads, num_kv_heads)) return (size_t)prompt_bytes(num_groups, num_kv_heads, head_dim, max_prefix_len).all;
+  return (size_t)plan_of(rows, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, 0, false).pre_floats * 4;
+}
+
+extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* stream) {
+  if (!a || !a->q || !a->k || !a->v || !a->o || !a->m || !a->l || !a->req_to_tokens) return LSATTN_ERR_INVALID_ARG;
+  if (a->rows < 0 || a->num_q_heads < 1 || a->num_kv_heads < 1 || a->num_slots < 1 || a->num_reqs < 0 || a->max_seq_len < 0 || a->num_groups < 0 ||
+      a->max_prefix_len < 0 || a->max_group_rows < 0)
+    return LSATTN_ERR_INVALID_ARG;
+  if (a->num_groups && (!a->g_start_loc || !a->g_size || !a->g_req_idx || !a->g_prefix_len)) return LSATTN_ERR_INVALID_ARG;
+  if (a->num_q_heads % a->num_kv_heads || (a->head_dim != 128 && a->head_dim != 64)) return LSATTN_ERR_UNSUPPORTED;
+  if (a->dtype != LSATTN_F16 && a->dtype != LSATTN_BF16) return LSATTN_ERR_UNSUPPORTED;
+  if (((a->k_stride_0 | a->k_stride_1 | a->v_stride_0 | a->v_stride_1 | a->q_stride_t | a->q_stride_h) % 8) || ((a->o_stride_t | a->o_stride_h) % 8) ||
+      (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->o) & 15) || (((uintptr_t)a->m | (uintptr_t)a->l) & 3))
+    return LSATTN_ERR_INVALID_ARG;
+  auto slot_stride = [](int64_t elements) { return elements >= 0 && elements <= 0x3fffffff; };
+  if (!slot_stride(a->k_stride_0) || !slot_stride(a->v_stride_0)) return LSATTN_ERR_INVALID_ARG;
+  const int64_t group = a->num_q_heads / a->num_kv_heads;
+  if (a->rows * group > 0x7fffff00 || a->num_q_heads > 65535 || a->max_seq_len > 0x7fff0000 || a->num_slots > 0x7fffffff || a->num_reqs > 0x7fffffff ||
+      a->num_groups > 65535 || a->max_prefix_len > 0x7fff0000 || a->rows * a->num_q_heads > kMaxUnits)
+    return LSATTN_ERR_INVALID_ARG;
+  if (!(a->sm_scale > 0.f)) return LSATTN_ERR_INVALID_ARG;
+  const int64_t most = most_of(a->max_prefix_len, a->max_seq_len);
+  if (a->rows == 0 || a->num_groups == 0 || most == 0) return LSATTN_OK;
+  const size_t need = lsattn_shared_prefill_workspace_bytes(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len);
+  if (!a->workspace || a->workspace_bytes < need) return LSATTN_ERR_WORKSPACE;
+  if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
+  SharedParams p = {};
+  PoolParams& w = p.w;
+  w.q = (const char*)a->q, w.k = (const char*)a->k, w.v = (const char*)a->v;
+  w.k_s0 = a->k_stride_0 * 2, w.k_s1 = a->k_stride_1 * 2, w.v_s0 = a->v_stride_0 * 2, w.v_s1 = a->v_stride_1 * 2;
+  w.table = a->req_to_tokens, w.max_seq_len = a->max_seq_len;
+  w.num_reqs = (int32_t)a->num_reqs, w.num_slots = (int32_t)a->num_slots;
+  w.hq = (int32_t)a->num_q_heads, w.hkv = (int32_t)a->num_kv_heads, w.group = (int32_t)group;
+  w.scale_log2 = a->sm_scale * kLog2e;
+  p.q_st = a->q_stride_t * 2, p.q_sh = a->q_stride_h * 2;
+  p.g_start = a->g_start_loc, p.g_size = a->g_size, p.g_req = a->g_req_idx, p.g_prefix = a->g_prefix_len;
+  p.groups = (int32_t)a->num_groups, p.rows = (int32_t)a->rows, p.most = (int32_t)most;
+  p.by_hkv = fast_div((uint32_t)w.hkv), p.by_group = fast_div((uint32_t)group);
+  hipStream_t st = (hipStream_t)stream;
+  if (gathers(a->rows, a->num_q_heads, a->num_kv_heads)) {
+    if (a->num_groups * most > 0x7fffff00) return LSATTN_ERR_INVALID_ARG;  // (rows of the gathered K/V)
+    const PromptBytes pb = prompt_bytes(a->num_groups, a->num_kv_heads, a->head_dim, most);
+    GatherParams g;
+    char* at = (char*)a->workspace;
+    g.k = at, g.v = at + pb.k, g.list = (int32_t*)(at + 2 * pb.k), g.vectors = (int32_t*)(at + 2 * pb.k + pb.list);
+    g.most = (int32_t)most;
+    const uint32_t head_chunks = (uint32_t)a->head_dim / 8;
+    g.by_head_chunks = fast_div(head_chunks);
+    LSATTN_LAUNCH_KERNEL(shared_prefix_list_kernel, dim3(p.groups), dim3(1024), 0, st, p, g);
+    if (hipPeekAtLastError() != hipSuccess) return check_launch();
+    const int64_t pieces = (most * 2 * w.hkv * head_chunks + 1023) / 1024, fill = 8 * kCUs / a->num_groups + 1;
+    const dim3 grid((unsigned)(pieces < fill ? pieces : fill), (unsigned)a->num_groups);
+    if (a->dtype == LSATTN_F16) LSATTN_LAUNCH_KERNEL((shared_prefix_gather_kernel<F16>), grid, dim3(256), 0, st, p, g, head_chunks);
+    else LSATTN_LAUNCH_KERNEL((shared_prefix_gather_kernel<BF16>), grid, dim3(256), 0, st, p, g, head_chunks);
+    if (hipPeekAtLastError() != hipSuccess) return check_launch();
+    lsattn_prefill_args s = {};
+    s.q = a->q, s.k = g.k, s.v = g.v;
+    s.q_stride_t = a->q_stride_t, s.q_stride_h = a->q_stride_h;
+    s.k_stride_t = s.v_stride_t = a->num_kv_heads * a->head_dim, s.k_stride_h = s.v_stride_h = a->head_dim;
+    const int32_t* v = g.vectors;
+    s.q_b_start_loc = v, s.q_b_seq_len = v + p.groups, s.q_first_token_global_idx = v + 2 * p.groups;
+    s.kv_b_start_loc = v + 3 * p.groups, s.kv_b_seq_len = v + 4 * p.groups, s.kv_first_token_global_idx = v + 5 * p.groups;
+    s.batch = p.groups, s.num_q_heads = w.hq, s.num_kv_heads = w.hkv, s.head_dim = (int32_t)a->head_dim, s.dtype = a->dtype, s.sp_peers = 1;
+    const int64_t longest = a->max_group_rows < a->rows ? a->max_group_rows : a->rows;
+    s.max_q_len = (int32_t)longest, s.sm_scale = a->sm_scale;
+    s.o = a->o, s.o_stride_t = a->o_stride_t, s.o_stride_h = a->o_stride_h, s.o_dtype = a->dtype, s.v_is_f16 = a->dtype == LSATTN_BF16;
+    s.m = a->m, s.l = a->l, s.ml_stride_t = a->ml_stride_t, s.ml_stride_h = a->ml_stride_h;
+    s.total_q_rows = a->rows, s.total_kv_rows = a->num_groups * most, s.max_kv_len = (int32_t)most;
+    return lsattn_prefill_step_merge(&s, stream);
+  }
+  const Plan pl = plan_of(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len, 0, false);
+  if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups) return LSATTN_ERR_INVALID_ARG;  // (units are numbered with 31 bits)
+  p.pre_o = (float*)a->workspace, p.pre_lse = p.pre_o + (pl.pre_floats / (a->head_dim + 1)) * a->head_dim;
+  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.wgs = (int32_t)(pl.shares * w.hkv + 7) / 8 * 8;
+  p.by_pre_shares = fast_div((uint32_t)pl.shares);
+  FoldParams f;
+  f.o = (char*)a->o, f.o_st = a->o_stride_t * 2, f.o_sh = a->o_stride_h * 2, f.m = a->m, f.l = a->l, f.ml_st = a->ml_stride_t, f.ml_sh = a->ml_stride_h;
+  const unsigned fold_wgs = (unsigned)((a->rows * w.hq * (a->head_dim / 4) + 255) / 256);
+  auto launch = [&](auto t, auto d) {
+    constexpr int D = decltype(d)::value;
+    LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<decltype(t), D, false>), dim3(p.wgs), dim3(256), 0, st, p);
+    if (hipPeekAtLastError() != hipSuccess) return;
+    LSATTN_LAUNCH_KERNEL((shared_prefix_fold_kernel<decltype(t), D>), dim3(fold_wgs), dim3(256), 0, st, p, f);
+  };
+  constexpr std::integral_constant<int, 128> d128{};
+  constexpr std::integral_constant<int, 64> d64{};
+  if (a->dtype == LSATTN_F16) a->head_dim == 128 ? launch(F16{}, d128) : launch(F16{}, d64);
+  else a->head_dim == 128 ? launch(BF16{}, d128) : launch(BF16{}, d64);
+  return check_launch();
+}

@@ -13,9 +13,14 @@ import logging
 
 import torch
 
-from . import _lib, _native
+from . import _lib, _native, sharing
 
 logger = logging.getLogger(__name__)
+
+
+def _i32(t: torch.Tensor) -> torch.Tensor:
+    """An index vector as the kernels read it: alloc hands rows out as int64."""
+    return t.to(torch.int32) if t.dtype == torch.int64 else t
 
 
 def _stream() -> int:
@@ -142,6 +147,13 @@ class LongServeMemoryManager:
         return
 
     @torch.inference_mode()
+    def compact(self, req_to_token_indexs, b_req_idx, b_seq_len, max_len_in_batch):
+        """Moves the slots in use to the front of the pool, in all layers, and the requests' table entries with them (sharing.compact_pool; not in the
+        reference): behind it alloc_contiguous finds whatever is free.  b_req_idx / b_seq_len are all live requests; returns remap, the new
+        number of every used slot, for slot numbers that are kept elsewhere.  Rows of the idle slots stay."""
+        return sharing.compact_pool(self.mem_state, self.kv_buffer, req_to_token_indexs, _i32(b_req_idx), _i32(b_seq_len), max_len_in_batch, self.kv_scales)
+
+    @torch.inference_mode()
     def free_all(self):
         self.can_use_mem_size = len(self.mem_state)
         self.mem_state[:] = 0
@@ -192,6 +204,41 @@ class LongServeReqManager:
 
     def free_token(self, free_token_index):
         self.mem_manager.free(free_token_index)
+
+    # -------------------------------------------------------------------- requests that share tokens (not in the reference)
+    @torch.inference_mode()
+    def fork(self, b_req_idx, b_seq_len, max_len_in_batch):
+        """New requests that share the first b_seq_len[i] tokens of b_req_idx[i] (a request may be named several times): their rows, as alloc returns
+        them, or None where the table is full.  Every shared slot gets a reference per fork and is free when the last request that holds it
+        is (free_reqs); new tokens of a fork get slots of their own, as those of any request."""
+        new = self.alloc(len(b_req_idx))
+        if new is not None:
+            sharing.fork_requests(self.req_to_token_indexs, _i32(b_req_idx), _i32(new), _i32(b_seq_len), max_len_in_batch, self.mem_manager.mem_state)
+        return new
+
+    @torch.inference_mode()
+    def fork_copy(self, b_req_idx, b_seq_len, max_len_in_batch, total_len):
+        """fork with copies: total_len (the sum of b_seq_len) slots are taken from the pool, and the tokens' rows are copied in all layers.  (rows,
+        slots), or None where the table is full; a pool that is short raises, as its alloc does."""
+        if len(b_req_idx) > self.can_use_req_size:
+            return self.alloc(len(b_req_idx))  # (says so)
+        index = self.mem_manager.alloc(total_len)
+        new = self.alloc(len(b_req_idx))
+        b_seq_len = _i32(b_seq_len)
+        start = (torch.cumsum(b_seq_len, 0, dtype=torch.int32) - b_seq_len).to(torch.int32)
+        sharing.copy_requests(self.req_to_token_indexs, _i32(b_req_idx), _i32(new), b_seq_len, start, max_len_in_batch, index, self.mem_manager.kv_buffer,
+                              self.mem_manager.kv_scales)
+        return new, index
+
+    @torch.inference_mode()
+    def free_reqs(self, free_req_index, b_seq_len, max_len_in_batch):
+        """Frees requests with the tokens that their rows of the table name: every slot loses a reference per request that holds it, so that requests which
+        share tokens can go in one call (free takes a list of tokens, each once)."""
+        freed, wrong = sharing._release(self.req_to_token_indexs, _i32(free_req_index), _i32(b_seq_len), max_len_in_batch, self.mem_manager.mem_state)
+        self.mem_manager.can_use_mem_size += freed
+        self.can_use_req_size += len(free_req_index)
+        self.req_state[free_req_index] = 0
+        sharing._check_released(wrong)
 
     def free_all(self):
         self.can_use_req_size = len(self.req_state)
