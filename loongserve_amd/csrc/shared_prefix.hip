@@ -41,15 +41,22 @@ struct SharedParams {
   const int32_t* g_prefix;
   int32_t groups, rows;  // rows of q
   int32_t most;          // a bound of the prefixes: longer ones are cut there
+  int32_t near;          // whether every row lies within 2 GB of its head's first, slots and strides of 24 bits
   int32_t shares, parts; // of the prefix part, per KV head; partials of 128 rows per KV head
-  int32_t wgs;           // workgroups of the prefix part
+  int32_t own_wgs;       // workgroups of the own tokens, in front of those of the prefix part
+  int32_t* plan;         // [batch, 8] where a request's partials lie, for the second launch
   float* pre_o;          // [hkv, parts, 128, D]
   float* pre_lse;        // [hkv, parts, 128], log2 domain
   FastDiv by_hkv, by_group, by_pre_shares;
 };
 
-// s_waitcnt vmcnt(0) (expcnt / lgkmcnt fields left at their maximum)
-__device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70); }
+__device__ __forceinline__ const char* uniform_ptr(const char* ptr) {
+  const uint64_t u = (uint64_t)ptr;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
+  return (const char*)(((uint64_t)hi << 32) | lo);
+}
+// s_waitcnt vmcnt(N) (expcnt / lgkmcnt fields left at their maximum)
+template <int N> __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14)); }
 
 // 64 groups at a time, one per lane.  Groups stand in ascending order of their rows; a row that two of them name belongs to the first, so that
 // whatever the lists hold no row is counted twice.
@@ -164,14 +171,9 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
     first += gs.all_units(), tiles_before += gs.all_tiles();
     gs.look(p, gs.at + 64, gs.end_of_all());
   }
-  // the lane's chunk of its load instructions' rows, K and V
+  // the lane's row of its first load instruction, and its chunk of it, K and V (rows RPI apart differ in bits of their XOR that the lane's own row leaves free)
   const int j_row = lane / CPR;
-  uint32_t k_chunk[NI], v_chunk[NI];
-#pragma unroll
-  for (int i = 0; i < NI; i++) {
-    k_chunk[i] = (uint32_t)(((lane % CPR) ^ swz_k(RPI * i + j_row)) * 16);
-    v_chunk[i] = (uint32_t)(((lane % CPR) ^ swz_v(RPI * i + j_row)) * 16);
-  }
+  const uint32_t k_chunk = (uint32_t)(((lane % CPR) ^ swz_k(j_row)) * 16), v_chunk = (uint32_t)(((lane % CPR) ^ swz_v(j_row)) * 16);
   int kaddr[KS], vaddr[NDB];
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) kaddr[ks] = lds_base + c * RB + (((4 * ks + g) & (CPR - 1)) ^ swz_k(c)) * 16;
@@ -180,8 +182,8 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
     const int row = 4 * g + (c >> 2);
     vaddr[db] = lds_base + TB + row * RB + ((2 * db + ((c & 3) >> 1)) ^ swz_v(row)) * 16 + (c & 1) * 8;
   }
-  const char* const kb = p.w.k + kvh * p.w.k_s1;
-  const char* const vb = p.w.v + kvh * p.w.v_s1;
+  const char* const kb = uniform_ptr(p.w.k + kvh * p.w.k_s1);
+  const char* const vb = uniform_ptr(p.w.v + kvh * p.w.v_s1);
   const uint32_t k_s0 = (uint32_t)p.w.k_s0, v_s0 = (uint32_t)p.w.v_s0;
   const float scale = p.w.scale_log2;
 
@@ -194,7 +196,7 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
     const int part = share + tiles_before + __builtin_amdgcn_readlane(gs.tiles_to, l) - tiles + tile;
     const int lo = __builtin_amdgcn_readlane(gs.lo, l), prefix = __builtin_amdgcn_readlane(gs.prefix, l);
     const int rows = __builtin_amdgcn_readlane(gs.size, l) * p.w.group;
-    const int32_t* const row_slots = p.w.table + (int64_t)__builtin_amdgcn_readlane(gs.req, l) * p.w.max_seq_len;
+    const int32_t* const row_slots = (const int32_t*)uniform_ptr((const char*)(p.w.table + (int64_t)__builtin_amdgcn_readlane(gs.req, l) * p.w.max_seq_len));
     const int row0 = tile * kRows + wave * 32;
     const bool active = row0 < rows;
 
@@ -214,41 +216,70 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
       l_pv[qb] = f32x4{0.f, 0.f, 0.f, 0.f};
       m_run[qb] = -INFINITY, l_run[qb] = 0.f;
     }
+    typedef int Slots __attribute__((ext_vector_type(NI), aligned(4)));
     int slot[NI];
-    // the slots of the lane's rows of tile t (positions past the prefix repeat its last one): LDS row 16 wave + RPI i + j is key 16 wave + NI j + i
-    const int pos0 = block0 * kKeys + 16 * wave + NI * j_row;
+    // The slots of the lane's rows of tile t, neighbours in the table (LDS row 16 wave + RPI i + j is key 16 wave + NI j + i); positions past the prefix repeat its last one.
+    const uint32_t pos0 = (uint32_t)(block0 * kKeys + 16 * wave + NI * j_row);
     auto load_slots = [&](int t) __attribute__((always_inline)) {
+      const uint32_t pos = pos0 + t * kKeys;
+      if ((block0 + t + 1) * kKeys <= prefix) {  // (wave-uniform)
+        const Slots x = *(const Slots*)((const char*)row_slots + pos * 4);
 #pragma unroll
-      for (int i = 0; i < NI; i++) {
-        const int pos = pos0 + t * kKeys + i;
-        slot[i] = row_slots[pos < prefix ? pos : prefix - 1];
+        for (int i = 0; i < NI; i++) slot[i] = x[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; i++) slot[i] = *(const int*)((const char*)row_slots + (pos + i < (uint32_t)prefix ? pos + i : (uint32_t)prefix - 1) * 4);
       }
     };
+    // The rows of tile t.  What stands here is issued by every wave for every tile, so the common case, all 64 keys there, is kept short: offsets of 32 bits where the pool allows
+    // them (one full-rate multiplication each), and masks that are written only where they change.
+    uint32_t masked = 0;  // stages whose mask is not all ones
     auto request = [&](int stage, int t) __attribute__((always_inline)) {
       const int dst = __builtin_amdgcn_readfirstlane(lds_base + stage * 2 * TB + wave * 16 * RB);
-      uint32_t there = 0;  // bit per LDS row of the wave
+      bool ok = true;
 #pragma unroll
-      for (int i = 0; i < NI; i++) {
-        const bool ok = pos0 + t * kKeys + i < prefix && (uint32_t)slot[i] < (uint32_t)p.w.num_slots;
-        const uint64_t lanes = __builtin_amdgcn_ballot_w64(ok);
+      for (int i = 0; i < NI; i++) ok &= (uint32_t)slot[i] < (uint32_t)p.w.num_slots;
+      const bool whole = (block0 + t + 1) * kKeys <= prefix && __builtin_amdgcn_ballot_w64(!ok) == 0;
+      if (!whole || ((masked >> stage) & 1u)) {  // (wave-uniform)
+        uint32_t there = 0;  // bit per LDS row of the wave
 #pragma unroll
-        for (int j = 0; j < RPI; j++) there |= (uint32_t)((lanes >> (CPR * j)) & 1u) << (RPI * i + j);
-        const uint32_t sl = ok ? (uint32_t)slot[i] : 0u;
-        const char* ka = kb + (uint64_t)sl * k_s0 + k_chunk[i];
-        const char* va = vb + (uint64_t)sl * v_s0 + v_chunk[i];
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
-                     "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, off" ::"s"(dst + i * 1024), "s"(dst + TB + i * 1024), "v"(ka), "v"(va)
-                     : "m0", "memory");
+        for (int i = 0; i < NI; i++) {
+          const bool here = pos0 + t * kKeys + i < (uint32_t)prefix && (uint32_t)slot[i] < (uint32_t)p.w.num_slots;
+          const uint64_t lanes = __builtin_amdgcn_ballot_w64(here);
+#pragma unroll
+          for (int j = 0; j < RPI; j++) there |= (uint32_t)((lanes >> (CPR * j)) & 1u) << (RPI * i + j);
+          slot[i] = here ? slot[i] : 0;
+        }
+        if (lane == 0) *(uint16_t*)(lds + kMaskOff + stage * 8 + wave * 2) = (uint16_t)there;
+        masked = whole ? masked & ~(1u << stage) : masked | 1u << stage;
       }
-      if (lane == 0) *(uint16_t*)(lds + kMaskOff + stage * 8 + wave * 2) = (uint16_t)there;
+      if (p.near) {
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+          const uint32_t ko = __umul24((uint32_t)slot[i], k_s0) + (k_chunk ^ (swz_k(RPI * i) * 16)), vo = __umul24((uint32_t)slot[i], v_s0) + (v_chunk ^ (swz_v(RPI * i) * 16));
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %4\n\t"
+                       "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %5" ::"s"(dst + i * 1024), "s"(dst + TB + i * 1024), "v"(ko), "v"(vo), "s"(kb), "s"(vb)
+                       : "m0", "memory");
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+          const char* ka = kb + (uint64_t)(uint32_t)slot[i] * k_s0 + (k_chunk ^ (swz_k(RPI * i) * 16));
+          const char* va = vb + (uint64_t)(uint32_t)slot[i] * v_s0 + (v_chunk ^ (swz_v(RPI * i) * 16));
+          asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\t"
+                       "s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, off" ::"s"(dst + i * 1024), "s"(dst + TB + i * 1024), "v"(ka), "v"(va)
+                       : "m0", "memory");
+        }
+      }
     };
     __syncthreads();  // (the tiles of the segment before are done with)
+    if (lane < 2) *(uint16_t*)(lds + kMaskOff + lane * 8 + wave * 2) = 0xffff;
     load_slots(0);
     request(0, 0);
     load_slots(1);
     auto step = [&](auto stage_tag, int t) __attribute__((always_inline)) {
       constexpr int S = decltype(stage_tag)::value;
-      wait_loads();
+      wait_loads<0>();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
@@ -389,16 +420,16 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
 // shares nothing.
 struct OwnRequests {
   int first_request, len, req, n_own, units, up_to;
+  Membership group;
+  bool shares;  // whether it has its group's prefix
   __device__ __forceinline__ void look(const SharedParams& p, Groups& g, int b0) {
     const int lane = threadIdx.x & 63, b = b0 + lane;
     first_request = b0;
-    Membership m;
-    m.find(p, g, b);
     len = req = n_own = 0;
-    if (b < p.w.batch) {
-      n_own = visible(p.w, b, len, req);
-      n_own -= m.prefix <= len ? m.prefix : 0;
-    }
+    if (b < p.w.batch) n_own = visible(p.w, b, len, req);
+    group.find(p, g, b);
+    shares = group.prefix <= len;
+    n_own -= shares && b < p.w.batch ? group.prefix : 0;
     units = (n_own + kBlock - 1) / kBlock;
     up_to = units;
 #pragma unroll
@@ -427,6 +458,23 @@ template <typename T, int D> __device__ __forceinline__ void own_share(const Sha
     rs.look(sp, gs, 0);
   }
   const int per_share = per_own_share(p, total);
+  // Where every request's partials lie, for the launch that joins them: 64 requests per wave, by the first task's waves (found again by each of its workgroups, this
+  // made that launch three times as long).
+  if (task == 0) {
+    const int per_pre = per_pre_share(sp, all_units_of(sp, gs));
+    for (int b0 = 0, before = 0; b0 < p.batch; b0 += 64) {
+      if (rs.first_request != b0) rs.look(sp, gs, b0);
+      const int b = b0 + (threadIdx.x & 63);
+      if ((b0 >> 6) % p.shares == share && b < p.batch) {
+        const int u0 = before + rs.up_to - rs.units, s0 = u0 / per_share;
+        int32_t* plan = sp.plan + 8 * (int64_t)b;
+        *(u32x4*)plan = u32x4{(uint32_t)rs.group.lo, (uint32_t)rs.group.tile0, (uint32_t)rs.group.unit0, rs.shares ? (uint32_t)rs.group.blocks : 0u};
+        *(u32x4*)(plan + 4) = u32x4{(uint32_t)s0, (uint32_t)(rs.units ? (u0 + rs.units - 1) / per_share - s0 + 1 : 0), (uint32_t)per_pre, 0u};
+      }
+      before += rs.all();
+    }
+    if (rs.first_request) rs.look(sp, gs, 0);
+  }
   if ((int64_t)share * per_share >= total) return;
   int at = share * per_share;
   const int end = total - at < per_share ? total : at + per_share;
@@ -468,19 +516,20 @@ template <typename T, int D> __device__ __forceinline__ void own_share(const Sha
   }
 }
 
-// Workgroups of the prefix part first, then those of the own tokens, four waves with a share each.
+// Workgroups of the own tokens first, four waves with a share each, then those of the prefix part.
 template <typename T, int D> constexpr int kSharedLds = kPrefixLds<T, D> > 4 * kWaveLds<T, D> ? kPrefixLds<T, D> : 4 * kWaveLds<T, D>;
 template <typename T, int D, bool OWN>
 __global__ __launch_bounds__(256, 2) void shared_prefix_kernel(SharedParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[OWN ? kSharedLds<T, D> : kPrefixLds<T, D>];
-  if (!OWN || (int)blockIdx.x < p.wgs) {
-    const int share = (int)div_by(blockIdx.x, p.by_hkv);  // (with a multiple of eight KV heads a head's workgroups run on one XCD: ids are dealt round-robin)
-    prefix_share<T, D>(p, lds, (int)blockIdx.x - share * p.w.hkv, share);
+  if (!OWN || (int)blockIdx.x >= p.own_wgs) {
+    const uint32_t x = blockIdx.x - p.own_wgs;  // (a multiple of 8)
+    const int share = (int)div_by(x, p.by_hkv);  // (with a multiple of eight KV heads a head's workgroups run on one XCD: ids are dealt round-robin)
+    prefix_share<T, D>(p, lds, (int)x - share * p.w.hkv, share);
     return;
   }
   if constexpr (OWN) {
-    const uint32_t n = gridDim.x - p.wgs, x = blockIdx.x - p.wgs;  // (n is a multiple of 8)
-    const uint32_t unit = ((x & 7) * (n >> 3) + (x >> 3)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t x = blockIdx.x;
+    const uint32_t unit = ((x & 7) * (p.own_wgs >> 3) + (x >> 3)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int share = (int)div_by(unit, p.w.by_tasks), task = (int)(unit - (uint32_t)share * p.w.tasks);
     if (share < p.w.shares) own_share<T, D>(p, lds, share, task);
   }
@@ -488,7 +537,7 @@ __global__ __launch_bounds__(256, 2) void shared_prefix_kernel(SharedParams p) {
 
 // o = sum of a row's partials by their log-sum-exps: those of its group's prefix, then those of its own tokens.  First the weights of all of them, by all threads, into LDS,
 // then the rows, whose loads wait for nothing.
-constexpr int kMaxParts = 2048;
+constexpr int kMaxParts = 2048;  // (kPrefixWorkgroups + kOwnWaves)
 template <int D>
 __global__ __launch_bounds__(256) void shared_decode_merge_kernel(SharedParams sp) {
   constexpr int W = D / 4, SL = 256 / W;
@@ -497,31 +546,17 @@ __global__ __launch_bounds__(256) void shared_decode_merge_kernel(SharedParams s
   __shared__ float weight[kMaxParts], red[8];
   const int h = blockIdx.x, b = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  Groups gs;
-  const uint32_t per_pre = (uint32_t)per_pre_share(sp, all_units_of(sp, gs));
-  OwnRequests rs;
-  int total = 0, first = 0, units = 0, len = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 64) {
-    rs.look(sp, gs, b0);
-    if (b >= b0 && b < b0 + 64) {
-      units = __builtin_amdgcn_readlane(rs.units, b - b0);
-      first = total + __builtin_amdgcn_readlane(rs.up_to, b - b0) - units;
-      len = __builtin_amdgcn_readlane(rs.len, b - b0);
-    }
-    total += rs.all();
-  }
-  const uint32_t per_own = (uint32_t)per_own_share(p, total);
-  const int s0 = (int)((uint32_t)first / per_own), n_own = units ? (int)((uint32_t)(first + units - 1) / per_own) - s0 + 1 : 0;
-  Membership mb;
-  mb.find(sp, gs, b);
-  const int kvh = h / p.group;
-  const int r = (b - mb.lo) * p.group + (h - kvh * p.group), tile = r / kRows;
+  const int32_t* plan = sp.plan + 8 * (int64_t)b;
+  const int lo = plan[0], tile0 = plan[1], unit0 = plan[2], blocks = plan[3], s0 = plan[4], n_own = plan[5];
+  const uint32_t per_pre = (uint32_t)plan[6];
+  const int kvh = (int)div_by((uint32_t)h, sp.by_group);
+  const int r = (b - lo) * p.group + (h - kvh * p.group), tile = r / kRows;
   int n_pre = 0, p0 = 0;
-  if (mb.blocks && mb.prefix <= len) {
-    const uint32_t u0 = (uint32_t)(mb.unit0 + tile * mb.blocks);
+  if (blocks) {
+    const uint32_t u0 = (uint32_t)(unit0 + tile * blocks);
     p0 = (int)(u0 / per_pre);
-    n_pre = (int)((u0 + mb.blocks - 1) / per_pre) - p0 + 1;
-    p0 += mb.tile0 + tile;
+    n_pre = (int)((u0 + blocks - 1) / per_pre) - p0 + 1;
+    p0 += tile0 + tile;
   }
   const int64_t pre_row = ((int64_t)kvh * sp.parts + p0) * kRows + (r - tile * kRows), own_row = (int64_t)(s0 + b) * p.hq + h;
   const int n = n_pre + n_own;
@@ -703,42 +738,53 @@ template <typename T> __global__ __launch_bounds__(256) void shared_prefix_gathe
 }
 
 // ------------------------------------------------------------------------------------------------ the host's side
-constexpr int64_t kPrefixWorkgroups = 2 * kCUs;
+constexpr int64_t kPrefixWorkgroups = 2 * kCUs;  // at most
 constexpr int64_t kOwnWaves = 4 * kCUs;
 constexpr int64_t kOwnMinUnits = 2;
 
 // a bound of the prefixes that a table can hold
 int64_t most_of(int64_t max_prefix, int64_t max_seq_len) { return max_prefix < max_seq_len ? max_prefix : max_seq_len; }
 
+bool is_near(const PoolParams& w) {
+  const int64_t last = (int64_t)w.num_slots - 1;
+  return w.num_slots <= 1 << 24 && w.k_s0 < 1 << 24 && w.v_s0 < 1 << 24 && last * w.k_s0 < 0x7fff0000 && last * w.v_s0 < 0x7fff0000;
+}
 struct Plan {
   int64_t tiles, shares, parts;  // prefix part, per KV head
   int64_t own_shares;
-  int64_t pre_floats, own_floats;  // of the workspace
+  int64_t pre_floats, own_floats, plan_ints;  // of the workspace
+  int64_t all() const { return (pre_floats + own_floats + plan_ints) * 4; }
 };
 // `own`: the bound of a request's own tokens (0: no own part)
 Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, int64_t max_prefix, int64_t max_own, bool decode) {
   Plan p;
   p.tiles = groups > 0 && max_prefix > 0 ? rows * (hq / hkv) / kRows + (groups < rows ? groups : rows) : 0;
   const int64_t units = p.tiles * ((max_prefix + kKeys - 1) / kKeys);
-  p.shares = kPrefixWorkgroups / hkv;
+  const int64_t tasks = hkv * ((hq / hkv + kHeads - 1) / kHeads), own_units = decode ? rows * ((max_own + kBlock - 1) / kBlock) : 0;
+  // Two workgroups of the prefix part per CU, or one beside those of the own tokens, where these are as much work and the groups fill their row tiles: half the partials then, and the
+  // prefix's products beside the other part's loads.  Microseconds, two | one: 64 requests behind 16384 tokens, 32/8 heads, up to 1500 own tokens 87 | 77, 400 each 68 | 63, 100 each
+  // 51 | 52, none 44 | 47; 24 in three groups, 32/32, up to 700 own tokens (rows that fill a sixteenth of a tile: what counts is loads in flight) 105 | 113; 160 in two groups, 28/4
+  // heads of 64, up to 400 own tokens 80 | 97.
+  const bool beside = own_units * tasks >= units * hkv && rows * (hq / hkv) >= 64 * groups;
+  p.shares = (beside ? kCUs : kPrefixWorkgroups) / hkv;
   p.shares = p.shares < 1 ? 1 : p.shares;
   p.shares = p.shares < units ? p.shares : units < 1 ? 1 : units;
   p.parts = p.shares + p.tiles;
   p.pre_floats = p.tiles ? hkv * p.parts * kRows * (d + 1) : 0;
-  p.own_shares = 1, p.own_floats = 0;
+  p.own_shares = 1, p.own_floats = 0, p.plan_ints = 0;
   if (decode) {
-    const int64_t tasks = hkv * ((hq / hkv + kHeads - 1) / kHeads), own_units = rows * ((max_own + kBlock - 1) / kBlock);
     const int64_t by_waves = kOwnWaves / tasks, by_units = (own_units + kOwnMinUnits - 1) / kOwnMinUnits;
     p.own_shares = by_waves < by_units ? by_waves : by_units;
     p.own_shares = p.own_shares < 1 ? 1 : p.own_shares;
-    p.own_floats = (p.own_shares + rows) * hq * (d + 1);
+    p.own_floats = ((p.own_shares + rows) * hq * (d + 1) + 3) / 4 * 4;
+    p.plan_ints = 8 * rows;
   }
   return p;
 }
 
 template <typename T, int D> void launch_decode(const SharedParams& p, hipStream_t st) {
-  const int64_t own = ((int64_t)p.w.shares * p.w.tasks + 3) / 4;
-  LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<T, D, true>), dim3((unsigned)(p.wgs + (own + 7) / 8 * 8)), dim3(256), 0, st, p);
+  const int64_t prefix = p.groups ? (int64_t)p.shares * p.w.hkv : 0;
+  LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<T, D, true>), dim3((unsigned)(p.own_wgs + prefix)), dim3(256), 0, st, p);
   if (hipPeekAtLastError() != hipSuccess) return;
   LSATTN_LAUNCH_KERNEL((shared_decode_merge_kernel<D>), dim3(p.w.hq, p.w.batch), dim3(256), 0, st, p);
 }
@@ -755,7 +801,7 @@ extern "C" size_t lsattn_shared_decode_workspace_bytes(int64_t batch, int64_t nu
       max_own_len > 0x7fffffff)  // (as the launch refuses)
     return 0;
   const Plan pl = plan_of(batch, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, max_own_len, true);
-  return (size_t)(pl.pre_floats + pl.own_floats) * 4;
+  return (size_t)pl.all();
 }
 
 extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* stream) {
@@ -779,7 +825,7 @@ extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* st
   if (!(a->sm_scale > 0.f)) return LSATTN_ERR_INVALID_ARG;
   if (a->batch == 0) return LSATTN_OK;
   const Plan pl = plan_of(a->batch, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len, a->max_own_len, true);
-  if (!a->workspace || a->workspace_bytes < (size_t)(pl.pre_floats + pl.own_floats) * 4) return LSATTN_ERR_WORKSPACE;
+  if (!a->workspace || a->workspace_bytes < (size_t)pl.all()) return LSATTN_ERR_WORKSPACE;
   if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
   // (units of both parts are numbered with 31 bits, and requests may be longer than the caller's bound)
   const int64_t most = most_of(a->max_prefix_len, a->max_seq_len);
@@ -801,12 +847,13 @@ extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* st
   w.by_tasks = fast_div((uint32_t)w.tasks), w.by_sub = fast_div((uint32_t)w.sub_groups);
   w.shares = (int32_t)pl.own_shares, w.by_shares = fast_div((uint32_t)pl.own_shares), w.min_units = (int32_t)kOwnMinUnits;
   p.pre_o = (float*)a->workspace, p.pre_lse = p.pre_o + (pl.pre_floats / (a->head_dim + 1)) * a->head_dim;
-  w.part_o = p.pre_o + pl.pre_floats, w.part_lse = w.part_o + (pl.own_floats / (a->head_dim + 1)) * a->head_dim;
+  w.part_o = p.pre_o + pl.pre_floats, w.part_lse = w.part_o + (pl.own_shares + w.batch) * w.hq * a->head_dim;
+  p.plan = (int32_t*)(w.part_o + pl.own_floats);
   p.q_st = a->num_q_heads * a->head_dim * 2, p.q_sh = a->head_dim * 2;
   p.g_start = a->g_start_loc, p.g_size = a->g_size, p.g_req = a->g_req_idx, p.g_prefix = a->g_prefix_len;
   p.groups = pl.tiles ? (int32_t)a->num_groups : 0;
-  p.rows = w.batch, p.most = (int32_t)most;
-  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.wgs = pl.tiles ? (int32_t)(pl.shares * w.hkv + 7) / 8 * 8 : 0;
+  p.rows = w.batch, p.most = (int32_t)most, p.near = is_near(w);
+  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.own_wgs = (int32_t)(((pl.own_shares * w.tasks + 3) / 4 + 7) / 8 * 8);
   p.by_hkv = fast_div((uint32_t)w.hkv), p.by_group = fast_div((uint32_t)w.group), p.by_pre_shares = fast_div((uint32_t)pl.shares);
   hipStream_t st = (hipStream_t)stream;
   if (a->dtype == LSATTN_F16) {
@@ -821,9 +868,11 @@ extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* st
 
 namespace lsattn {
 namespace {
-// The prompts' step takes its rows itself where they are few, and hands contiguous K/V to the prefill kernel where they are many.
-constexpr int64_t kGatherFromRows = 1024;  // rows of all query heads of a KV head
-bool gathers(int64_t rows, int64_t hq, int64_t hkv) { return rows * (hq / hkv) >= kGatherFromRows; }
+// The prompts' step takes its rows itself where they are few, and hands contiguous K/V to the prefill kernel where its workgroups of 256 rows are a round and a half
+// of the CUs and more. Microseconds, own kernel | prefill kernel (f16, 32/8 heads of 128, with the fills of m and l): prefix 6001 tokens: 293 rows 70 | 120, 600 100 | 120, 1200 167 | 211, 2500
+// 314 | 341, 5000 594 | 518; 20000 tokens: 1200 484 | 564, 2500 980 | 954, 5000 1907 | 1448; five groups of 1200 rows behind 3000 435 | 331; 8/1 heads, 1200 rows behind 6001 76 | 112.
+constexpr int64_t kGatherFromRows = kCUs * 3 / 2 * 256;
+bool gathers(int64_t rows, int64_t hq) { return rows * hq >= kGatherFromRows; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 struct PromptBytes {
   int64_t k, list, vectors, all;
@@ -842,7 +891,7 @@ extern "C" size_t lsattn_shared_prefill_workspace_bytes(int64_t rows, int64_t nu
   if (rows <= 0 || num_groups <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || (head_dim != 64 && head_dim != 128) ||
       max_prefix_len <= 0 || rows > 0x7fffff00 || num_groups > 65535 || num_q_heads > 65535 || max_prefix_len > 0x7fff0000)  // (as the launch refuses)
     return 0;
-  if (gathers(rows, num_q_heads, num_kv_heads)) return (size_t)prompt_bytes(num_groups, num_kv_heads, head_dim, max_prefix_len).all;
+  if (gathers(rows, num_q_heads)) return (size_t)prompt_bytes(num_groups, num_kv_heads, head_dim, max_prefix_len).all;
   return (size_t)plan_of(rows, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, 0, false).pre_floats * 4;
 }
 
@@ -879,10 +928,10 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
   w.scale_log2 = a->sm_scale * kLog2e;
   p.q_st = a->q_stride_t * 2, p.q_sh = a->q_stride_h * 2;
   p.g_start = a->g_start_loc, p.g_size = a->g_size, p.g_req = a->g_req_idx, p.g_prefix = a->g_prefix_len;
-  p.groups = (int32_t)a->num_groups, p.rows = (int32_t)a->rows, p.most = (int32_t)most;
+  p.groups = (int32_t)a->num_groups, p.rows = (int32_t)a->rows, p.most = (int32_t)most, p.near = is_near(w);
   p.by_hkv = fast_div((uint32_t)w.hkv), p.by_group = fast_div((uint32_t)group);
   hipStream_t st = (hipStream_t)stream;
-  if (gathers(a->rows, a->num_q_heads, a->num_kv_heads)) {
+  if (gathers(a->rows, a->num_q_heads)) {
     if (a->num_groups * most > 0x7fffff00) return LSATTN_ERR_INVALID_ARG;  // (rows of the gathered K/V)
     const PromptBytes pb = prompt_bytes(a->num_groups, a->num_kv_heads, a->head_dim, most);
     GatherParams g;
@@ -916,14 +965,14 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
   const Plan pl = plan_of(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len, 0, false);
   if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups) return LSATTN_ERR_INVALID_ARG;  // (units are numbered with 31 bits)
   p.pre_o = (float*)a->workspace, p.pre_lse = p.pre_o + (pl.pre_floats / (a->head_dim + 1)) * a->head_dim;
-  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.wgs = (int32_t)(pl.shares * w.hkv + 7) / 8 * 8;
+  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts;
   p.by_pre_shares = fast_div((uint32_t)pl.shares);
   FoldParams f;
   f.o = (char*)a->o, f.o_st = a->o_stride_t * 2, f.o_sh = a->o_stride_h * 2, f.m = a->m, f.l = a->l, f.ml_st = a->ml_stride_t, f.ml_sh = a->ml_stride_h;
   const unsigned fold_wgs = (unsigned)((a->rows * w.hq * (a->head_dim / 4) + 255) / 256);
   auto launch = [&](auto t, auto d) {
     constexpr int D = decltype(d)::value;
-    LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<decltype(t), D, false>), dim3(p.wgs), dim3(256), 0, st, p);
+    LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<decltype(t), D, false>), dim3((unsigned)(pl.shares * w.hkv)), dim3(256), 0, st, p);
     if (hipPeekAtLastError() != hipSuccess) return;
     LSATTN_LAUNCH_KERNEL((shared_prefix_fold_kernel<decltype(t), D>), dim3(fold_wgs), dim3(256), 0, st, p, f);
   };

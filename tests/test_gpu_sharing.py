@@ -389,6 +389,7 @@ PROMPTS = {
     "none-in-one": [(70, 0), (129, 33), (0, 5)],
     "many": [(300, 700), (129, 500)],
     "many-one": [(1, 1500)],
+    "prefill-kernel": [(70, 9000), (65, 5100)],
 }
 
 
