@@ -58,6 +58,28 @@ __device__ __forceinline__ const char* uniform_ptr(const char* ptr) {
 // s_waitcnt vmcnt(N) (expcnt / lgkmcnt fields left at their maximum)
 template <int N> __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14)); }
 
+// Inclusive sum and maximum over the wave's lanes by DPP (through ds_bpermute each of the six steps takes a trip to LDS: a third of a small launch's start).
+template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_or(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int scan_sum(int v) {
+  v += dpp_or<0x111, 0xf>(0, v);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += dpp_or<0x112, 0xf>(0, v);
+  v += dpp_or<0x114, 0xf>(0, v);
+  v += dpp_or<0x118, 0xf>(0, v);
+  v += dpp_or<0x142, 0xa>(0, v);  // row_bcast 15 into rows 1 and 3, 31 into the upper half
+  v += dpp_or<0x143, 0xc>(0, v);
+  return v;
+}
+__device__ __forceinline__ int scan_max(int v) {
+  auto step = [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; };
+  v = step(v, dpp_or<0x111, 0xf>(v, v));
+  v = step(v, dpp_or<0x112, 0xf>(v, v));
+  v = step(v, dpp_or<0x114, 0xf>(v, v));
+  v = step(v, dpp_or<0x118, 0xf>(v, v));
+  v = step(v, dpp_or<0x142, 0xa>(v, v));
+  v = step(v, dpp_or<0x143, 0xc>(v, v));
+  return v;
+}
+
 // 64 groups at a time, one per lane.  Groups stand in ascending order of their rows; a row that two of them name belongs to the first, so that
 // whatever the lists hold no row is counted twice.
 struct Groups {
@@ -77,12 +99,7 @@ struct Groups {
       last = last < 0 ? start : last < p.rows - start ? start + last : p.rows;
       prefix = prefix < 0 || req < 0 || req >= p.w.num_reqs ? 0 : prefix < p.most ? prefix : p.most;
     }
-    end = last;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int below = __shfl_up(end, d, 64);
-      if (lane >= d) end = below > end ? below : end;
-    }
+    end = scan_max(last);
     end = end > end_before ? end : end_before;
     const int below = __shfl_up(end, 1, 64);
     const int taken = lane ? below : end_before;
@@ -90,12 +107,7 @@ struct Groups {
     size = last > lo ? last - lo : 0;
     blocks = (prefix + kKeys - 1) / kKeys;
     tiles = blocks ? (int)(((int64_t)size * p.w.group + kRows - 1) / kRows) : 0;
-    tiles_to = tiles, units_to = tiles * blocks;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int t = __shfl_up(tiles_to, d, 64), u = __shfl_up(units_to, d, 64);
-      if (lane >= d) tiles_to += t, units_to += u;
-    }
+    tiles_to = scan_sum(tiles), units_to = scan_sum(tiles * blocks);
   }
   __device__ __forceinline__ int end_of_all() const { return __builtin_amdgcn_readlane(end, 63); }
   __device__ __forceinline__ int all_tiles() const { return __builtin_amdgcn_readlane(tiles_to, 63); }
@@ -120,6 +132,15 @@ struct Membership {
   int lo, prefix, tile0, unit0, blocks;  // the group's first row, prefix, and the tiles and units of all groups in front of it
   __device__ __forceinline__ void find(const SharedParams& p, Groups& g, int b) {
     lo = prefix = tile0 = unit0 = blocks = 0;
+    if (p.groups <= 8) {  // (a trip to LDS takes as long as two of them)
+      for (int n = 0; n < p.groups; n++) {
+        const int s = __builtin_amdgcn_readlane(g.lo, n), sz = __builtin_amdgcn_readlane(g.size, n), t1 = __builtin_amdgcn_readlane(g.tiles, n);
+        const int bl = __builtin_amdgcn_readlane(g.blocks, n), pr = __builtin_amdgcn_readlane(g.prefix, n);
+        const int t0 = __builtin_amdgcn_readlane(g.tiles_to, n) - t1, u0 = __builtin_amdgcn_readlane(g.units_to, n) - t1 * bl;
+        if (s <= b && b < s + sz) lo = s, prefix = pr, blocks = bl, tile0 = t0, unit0 = u0;
+      }
+      return;
+    }
     int tiles = 0, units = 0;
     for (int g0 = 0;;) {
       int n = 0;  // groups of the 64 that end at b or in front of it
@@ -442,12 +463,7 @@ struct OwnRequests {
     shares = group.prefix <= len;
     n_own -= shares && b < p.w.batch ? group.prefix : 0;
     units = (n_own + kBlock - 1) / kBlock;
-    up_to = units;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int below = __shfl_up(up_to, d, 64);
-      if (lane >= d) up_to += below;
-    }
+    up_to = scan_sum(units);
   }
   __device__ __forceinline__ int all() const { return __builtin_amdgcn_readlane(up_to, 63); }
 };
