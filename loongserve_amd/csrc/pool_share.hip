@@ -261,18 +261,23 @@ struct CompactParams {
   const int32_t* req;
   const int32_t* len;
   int32_t n, num_reqs;
-  RowsParams r;
+  RowsParams r, scales;
   int32_t move_wgs, table_blocks, layers, most;
 };
 __device__ __forceinline__ void load_states(const CompactParams& p, int64_t at, int (&s)[4]) {  // (past the end: free)
+  if (at + 4 <= p.size) {
+    typedef int Four __attribute__((ext_vector_type(4), aligned(4)));
+    const Four x = *(const Four*)(p.state + at);
+#pragma unroll
+    for (int e = 0; e < 4; e++) s[e] = x[e];
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 4; e++) s[e] = at + e < p.size ? p.state[at + e] : 0;
 }
-__device__ __forceinline__ int count_group(int mine, int* sh) {  // over the workgroup
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) mine += __shfl_xor(mine, d, 64);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mine;
+__device__ __forceinline__ int count_group(int mine, int* sh) {  // over the workgroup; `sh`: for this count alone
+  const int wave = __builtin_amdgcn_readlane(scan_sum(mine), 63);
+  if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = wave;
   __syncthreads();
   int all = 0;
 #pragma unroll
@@ -286,44 +291,53 @@ __global__ __launch_bounds__(kPlanThreads) void compact_count_kernel(CompactPara
   const int all = count_group((s[0] != 0) + (s[1] != 0) + (s[2] != 0) + (s[3] != 0), sh);
   if (threadIdx.x == 0) p.used[blockIdx.x] = all;
 }
-__global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParams p) {
-  __shared__ int sh[kPlanThreads / 64];
+// A pool of up to kLookBlocks workgroups' slots: each of them looks through all counts itself, a bit per slot, instead of waiting for a launch that counts.
+constexpr int kLookBlocks = 16;
+template <bool LOOK> __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParams p) {
+  __shared__ int sh[4][kPlanThreads / 64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t at = (int64_t)blockIdx.x * kPlanSlots + 4 * threadIdx.x;
-  int s[4];
+  int s[4], before = 0, all = 0, front = 0;
   load_states(p, at, s);
-  int before = 0, all = 0;
-  for (int b = threadIdx.x; b < p.blocks; b += kPlanThreads) {
-    const int n = p.used[b];
-    before += b < (int)blockIdx.x ? n : 0;
-    all += n;
-  }
-  before = count_group(before, sh), all = count_group(all, sh);
-  // slots in use in front of slot `all`
-  const int border = all / kPlanSlots;
-  int front = 0;
-  for (int b = threadIdx.x; b < border; b += kPlanThreads) front += p.used[b];
-  int t[4];
-  const int64_t bat = (int64_t)border * kPlanSlots + 4 * threadIdx.x;
-  load_states(p, bat, t);
+  if (LOOK) {
+    uint64_t used = 0;  // bit 4 b + e: slot e of the thread's four in block b
+#pragma unroll 4
+    for (int b = 0; b < p.blocks; b++) {
+      int t[4];
+      load_states(p, (int64_t)b * kPlanSlots + 4 * threadIdx.x, t);
 #pragma unroll
-  for (int e = 0; e < 4; e++) front += bat + e < all && t[e] != 0;
-  front = count_group(front, sh);
+      for (int e = 0; e < 4; e++) used |= (uint64_t)(t[e] != 0) << (4 * b + e);
+    }
+    all = count_group(__builtin_popcountll(used), sh[0]);
+    before = count_group(__builtin_popcountll(used & (((uint64_t)1 << 4 * (int)blockIdx.x) - 1)), sh[1]);
+    // (all <= size: of block all / kPlanSlots the slots in front of it)
+    const int border = all / kPlanSlots, rest = all - border * kPlanSlots - 4 * (int)threadIdx.x, bits = 4 * border + (rest < 0 ? 0 : rest < 4 ? rest : 4);
+    front = count_group(__builtin_popcountll(bits < 64 ? used & (((uint64_t)1 << bits) - 1) : used), sh[2]);
+  } else {
+    for (int b = threadIdx.x; b < p.blocks; b += kPlanThreads) {
+      const int n = p.used[b];
+      before += b < (int)blockIdx.x ? n : 0;
+      all += n;
+    }
+    before = count_group(before, sh[0]), all = count_group(all, sh[1]);
+    // slots in use in front of slot `all`
+    const int border = all / kPlanSlots;
+    for (int b = threadIdx.x; b < border; b += kPlanThreads) front += p.used[b];
+    int t[4];
+    const int64_t bat = (int64_t)border * kPlanSlots + 4 * threadIdx.x;
+    load_states(p, bat, t);
+#pragma unroll
+    for (int e = 0; e < 4; e++) front += bat + e < all && t[e] != 0;
+    front = count_group(front, sh[2]);
+  }
   if (blockIdx.x == 0 && threadIdx.x == 0) p.header[0] = all - front;
   // ranks
-  const int mine = (s[0] != 0) + (s[1] != 0) + (s[2] != 0) + (s[3] != 0);
-  int up_to = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int below = __shfl_up(up_to, d, 64);
-    if (lane >= d) up_to += below;
-  }
-  __syncthreads();
-  if (lane == 63) sh[wave] = up_to;
+  const int mine = (s[0] != 0) + (s[1] != 0) + (s[2] != 0) + (s[3] != 0), up_to = scan_sum(mine);
+  if (lane == 63) sh[3][wave] = up_to;
   __syncthreads();
   int rank = before + up_to - mine;  // used slots in front of the thread's first one
 #pragma unroll
-  for (int w = 0; w < kPlanThreads / 64; w++) rank += w < wave ? sh[w] : 0;
+  for (int w = 0; w < kPlanThreads / 64; w++) rank += w < wave ? sh[3][w] : 0;
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     const int64_t slot = at + e;
@@ -342,22 +356,23 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactParam
 }
 // Workgroups that move rows (and the counts, with the first layer), those of a layer side by side, and behind them workgroups that rewrite the requests' table entries.
 constexpr int kMoveRows = 16;
-template <typename Piece, bool FIRST> __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p) {
+__global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p) {
   const int moves = p.header[0], layer = (int)blockIdx.x / p.move_wgs;
   if (layer < (p.layers ? p.layers : 1)) {
     for (int m0 = ((int)blockIdx.x - layer * p.move_wgs) * kMoveRows; m0 < moves; m0 += p.move_wgs * kMoveRows) {
-      if (FIRST && layer == 0 && threadIdx.x < kMoveRows && m0 + (int)threadIdx.x < moves) {
+      if (layer == 0 && threadIdx.x < kMoveRows && m0 + (int)threadIdx.x < moves) {
         const int src = p.source[m0 + threadIdx.x], dst = p.hole[m0 + threadIdx.x];
         p.state[dst] = p.state[src];
         p.state[src] = 0;
         p.remap[src] = dst;
       }
-      if (p.layers)
-        move_rows<Piece, kMoveRows>(p.r, layer, [&](int k, int& src, int& dst) {
-          if (m0 + k >= moves) return false;
-          src = p.source[m0 + k], dst = p.hole[m0 + k];
-          return true;
-        });
+      auto move = [&](int k, int& src, int& dst) {
+        if (m0 + k >= moves) return false;
+        src = p.source[m0 + k], dst = p.hole[m0 + k];
+        return true;
+      };
+      if (p.layers) move_rows<u32x4, kMoveRows>(p.r, layer, move);
+      if (p.scales.rows) move_rows<uint8_t, kMoveRows>(p.scales, layer, move);
     }
     return;
   }
@@ -493,14 +508,16 @@ extern "C" int lsattn_compact_pool(const lsattn_compact_args* a, const lsattn_po
   p.move_wgs = (int32_t)(by_moves < 1 ? 1 : by_moves < fill ? by_moves : fill);
   const unsigned move_wgs = (unsigned)(p.move_wgs * (p.layers ? p.layers : 1)), table_wgs = (unsigned)(p.table_blocks * p.n);
   hipStream_t st = (hipStream_t)stream;
-  LSATTN_LAUNCH_KERNEL(compact_count_kernel, dim3(p.blocks), dim3(kPlanThreads), 0, st, p);
-  if (hipPeekAtLastError() != hipSuccess) return check_launch();
-  LSATTN_LAUNCH_KERNEL(compact_plan_kernel, dim3(p.blocks), dim3(kPlanThreads), 0, st, p);
-  if (hipPeekAtLastError() != hipSuccess) return check_launch();
   if (p.layers) set_rows(p.r, rows->rows, rows->layer_stride_bytes, rows->slot_stride_bytes, rows->row_bytes / 16, rows->num_slots);
-  LSATTN_LAUNCH_KERNEL((compact_move_kernel<u32x4, true>), dim3(move_wgs + table_wgs), dim3(kThreads), 0, st, p);
-  if (!rows->scales || hipPeekAtLastError() != hipSuccess) return check_launch();
-  set_rows(p.r, rows->scales, rows->scale_layer_stride_bytes, rows->scale_slot_stride_bytes, rows->scale_bytes, rows->num_slots);
-  LSATTN_LAUNCH_KERNEL((compact_move_kernel<uint8_t, false>), dim3(move_wgs), dim3(kThreads), 0, st, p);
+  if (rows->scales) set_rows(p.scales, rows->scales, rows->scale_layer_stride_bytes, rows->scale_slot_stride_bytes, rows->scale_bytes, rows->num_slots);
+  if (p.blocks <= kLookBlocks) {
+    LSATTN_LAUNCH_KERNEL(compact_plan_kernel<true>, dim3(p.blocks), dim3(kPlanThreads), 0, st, p);
+  } else {
+    LSATTN_LAUNCH_KERNEL(compact_count_kernel, dim3(p.blocks), dim3(kPlanThreads), 0, st, p);
+    if (hipPeekAtLastError() != hipSuccess) return check_launch();
+    LSATTN_LAUNCH_KERNEL(compact_plan_kernel<false>, dim3(p.blocks), dim3(kPlanThreads), 0, st, p);
+  }
+  if (hipPeekAtLastError() != hipSuccess) return check_launch();
+  LSATTN_LAUNCH_KERNEL(compact_move_kernel, dim3(move_wgs + table_wgs), dim3(kThreads), 0, st, p);
   return check_launch();
 }

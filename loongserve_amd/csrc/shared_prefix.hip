@@ -58,28 +58,6 @@ __device__ __forceinline__ const char* uniform_ptr(const char* ptr) {
 // s_waitcnt vmcnt(N) (expcnt / lgkmcnt fields left at their maximum)
 template <int N> __device__ __forceinline__ void wait_loads() { __builtin_amdgcn_s_waitcnt(0x0F70 | (N & 15) | ((N >> 4) << 14)); }
 
-// Inclusive sum and maximum over the wave's lanes by DPP (through ds_bpermute each of the six steps takes a trip to LDS: a third of a small launch's start).
-template <int CTRL, int ROWS> __device__ __forceinline__ int dpp_or(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false); }
-__device__ __forceinline__ int scan_sum(int v) {
-  v += dpp_or<0x111, 0xf>(0, v);  // row_shr 1, 2, 4, 8: within 16 lanes
-  v += dpp_or<0x112, 0xf>(0, v);
-  v += dpp_or<0x114, 0xf>(0, v);
-  v += dpp_or<0x118, 0xf>(0, v);
-  v += dpp_or<0x142, 0xa>(0, v);  // row_bcast 15 into rows 1 and 3, 31 into the upper half
-  v += dpp_or<0x143, 0xc>(0, v);
-  return v;
-}
-__device__ __forceinline__ int scan_max(int v) {
-  auto step = [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; };
-  v = step(v, dpp_or<0x111, 0xf>(v, v));
-  v = step(v, dpp_or<0x112, 0xf>(v, v));
-  v = step(v, dpp_or<0x114, 0xf>(v, v));
-  v = step(v, dpp_or<0x118, 0xf>(v, v));
-  v = step(v, dpp_or<0x142, 0xa>(v, v));
-  v = step(v, dpp_or<0x143, 0xc>(v, v));
-  return v;
-}
-
 // 64 groups at a time, one per lane.  Groups stand in ascending order of their rows; a row that two of them name belongs to the first, so that
 // whatever the lists hold no row is counted twice.
 struct Groups {
