@@ -876,8 +876,10 @@ namespace {
 // The prompts' step takes its rows itself where they are few, and hands contiguous K/V to the prefill kernel where its workgroups of 256 rows are a round and a half
 // of the CUs and more. Microseconds, own kernel | prefill kernel (f16, 32/8 heads of 128, with the fills of m and l): prefix 6001 tokens: 293 rows 70 | 120, 600 100 | 120, 1200 167 | 211, 2500
 // 314 | 341, 5000 594 | 518; 20000 tokens: 1200 484 | 564, 2500 980 | 954, 5000 1907 | 1448; five groups of 1200 rows behind 3000 435 | 331; 8/1 heads, 1200 rows behind 6001 76 | 112.
-constexpr int64_t kGatherFromRows = kCUs * 3 / 2 * 256;
-bool gathers(int64_t rows, int64_t hq) { return rows * hq >= kGatherFromRows; }
+// Where a prefix has few rows of its own, laying it out costs more than it saves: 8192 rows behind 2000 tokens each, 32/8 heads, 32 groups 455 | 406, 64 591 | 538, 128 633 | 827;
+// 32/32 heads, 16 groups 591 | 538, 32 596 | 827.
+constexpr int64_t kGatherFromRows = kCUs * 3 / 2 * 256, kGatherFromGroupRows = 512;
+bool gathers(int64_t rows, int64_t groups, int64_t hq, int64_t hkv) { return rows * hq >= kGatherFromRows && rows * (hq / hkv) >= groups * kGatherFromGroupRows; }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 struct PromptBytes {
   int64_t k, list, vectors, all;
@@ -896,7 +898,7 @@ extern "C" size_t lsattn_shared_prefill_workspace_bytes(int64_t rows, int64_t nu
   if (rows <= 0 || num_groups <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || (head_dim != 64 && head_dim != 128) ||
       max_prefix_len <= 0 || rows > 0x7fffff00 || num_groups > 65535 || num_q_heads > 65535 || max_prefix_len > 0x7fff0000)  // (as the launch refuses)
     return 0;
-  if (gathers(rows, num_q_heads)) return (size_t)prompt_bytes(num_groups, num_kv_heads, head_dim, max_prefix_len).all;
+  if (gathers(rows, num_groups, num_q_heads, num_kv_heads)) return (size_t)prompt_bytes(num_groups, num_kv_heads, head_dim, max_prefix_len).all;
   return (size_t)plan_of(rows, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, 0, false).pre_floats * 4;
 }
 
@@ -936,7 +938,7 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
   p.groups = (int32_t)a->num_groups, p.rows = (int32_t)a->rows, p.most = (int32_t)most, p.near = is_near(w);
   p.by_hkv = fast_div((uint32_t)w.hkv), p.by_group = fast_div((uint32_t)group);
   hipStream_t st = (hipStream_t)stream;
-  if (gathers(a->rows, a->num_q_heads)) {
+  if (gathers(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads)) {
     if (a->num_groups * most > 0x7fffff00) return LSATTN_ERR_INVALID_ARG;  // (rows of the gathered K/V)
     const PromptBytes pb = prompt_bytes(a->num_groups, a->num_kv_heads, a->head_dim, most);
     GatherParams g;

@@ -391,6 +391,8 @@ PROMPTS = {
     "many-one": [(1, 1500)],
     "prefill-kernel": [(70, 9000), (65, 5100)],
 }
+# rows and heads that hand the laid-out prefix to the prefill kernel (rows x heads of 98304 and more, a row per group and head of 512 and more)
+WIDE = (128, 64, 128)
 
 
 @pytest.mark.gpu
@@ -431,11 +433,11 @@ def test_prompt_step_against_float64(lsa, name, heads, dtype):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [20, 800])
+@pytest.mark.parametrize("heads, rows", [((8, 2, 128), 20), ((8, 2, 128), 800), (WIDE, 400), ((64, 2, 64), 790)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-def test_prompt_step_entries_without_a_slot(lsa, rows, dtype):
+def test_prompt_step_entries_without_a_slot(lsa, heads, rows, dtype):
     """Holes in the prefix, prefixes cut at their bound, groups past q's rows, and NaN in every slot that is not named: both ways that the step is taken."""
-    c = _prompt_case(29, 8, 2, 128, dtype, [(200, rows), (90, rows), (80, 3)])
+    c = _prompt_case(29, *heads, dtype, [(200, rows), (90, rows), (80, 3)])
     t, (s, n, r, p) = c["table"], c["g"]
     t[r[0], :5], t[r[0], 63:66], t[r[0], 199] = PAD, -3, len(c["kv"]) + 4
     t[r[2], :80] = PAD
@@ -451,23 +453,24 @@ def test_prompt_step_entries_without_a_slot(lsa, rows, dtype):
         dead = torch.isneginf(l_ref)
         o, m, l = torch.zeros(T, Hq, D, dtype=dtype, device=DEV), torch.full((T, Hq), -math.inf, device=DEV), torch.zeros(T, Hq, device=DEV)
         _prompt_on_gpu(lsa, c, o, m, l, most=most)
-        _check((o, (torch.log2(l) + m) * math.log(2)), (o_ref, l_ref, tol_o + orc.EPS_OUT[dtype] * (o_ref.abs() + tol_o) + 2.0 ** -25, tol_l + 1e-6), (rows, most))
+        _check((o, (torch.log2(l) + m) * math.log(2)), (o_ref, l_ref, tol_o + orc.EPS_OUT[dtype] * (o_ref.abs() + tol_o) + 2.0 ** -25, tol_l + 1e-6), (heads, rows, most))
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("rows", [30, 900])
-def test_prompts_behind_a_prefix_with_their_own_chunks(lsa, rows):
+@pytest.mark.parametrize("heads, rows", [((8, 2, 128), 30), ((8, 2, 128), 900), (WIDE, 830)])
+def test_prompts_behind_a_prefix_with_their_own_chunks(lsa, heads, rows):
     """The whole of a step: own chunks by context_attention_fwd, the prefix by shared_prefix_attention_fwd, in either order, on views with wider strides; against causal
     attention over prefix and chunk."""
-    c = _prompt_case(31, 8, 2, 128, torch.float16, [(333, rows)], tail=0)
+    Hkv = heads[1]
+    c = _prompt_case(31, *heads, torch.float16, [(333, rows)], tail=0)
     lens = [rows // 3, rows - rows // 3]
     T, Hq, D = c["q"].shape
-    own = _rows((T, 4, D), c["gen"], torch.float16)
+    own = _rows((T, 2 * Hkv, D), c["gen"], torch.float16)
     slots = c["table"][c["g"][2][0], :333].long()
-    want = []
-    for b, (at, n) in enumerate(((0, lens[0]), (lens[0], lens[1]))):
-        kk, vv = torch.cat([c["kv"][slots, :2], own[at:at + n, :2]]), torch.cat([c["kv"][slots, 2:], own[at:at + n, 2:]])
-        for i in range(n):
+    want, looked_at = [], list(range(0, T, 1 if Hq < 100 else 37)) + [T - 1]
+    for at, n in ((0, lens[0]), (lens[0], lens[1])):
+        kk, vv = torch.cat([c["kv"][slots, :Hkv], own[at:at + n, :Hkv]]), torch.cat([c["kv"][slots, Hkv:], own[at:at + n, Hkv:]])
+        for i in (x - at for x in looked_at if at <= x < at + n):
             want.append(orc.attend(c["q"][at + i:at + i + 1], kk[:333 + i + 1], vv[:333 + i + 1], 2.0 ** -11))
     o_ref, l_ref, tol_o, tol_l = (torch.cat(x) for x in zip(*want))
     q_wide = torch.zeros(T, Hq + 2, D, dtype=torch.float16, device=DEV)
@@ -482,13 +485,13 @@ def test_prompts_behind_a_prefix_with_their_own_chunks(lsa, rows):
         o, m, l = o_wide[:, :Hq], ml[0, :, :Hq], ml[1, :, :Hq]
         if prefix_first:
             _prompt_on_gpu(lsa, c, o, m, l)
-        lsa.context_attention_fwd(c["q_gpu"], own_gpu[:, :2], own_gpu[:, 2:], o, starts, n, zero, starts, n, zero, 1, max(lens), m, l)
+        lsa.context_attention_fwd(c["q_gpu"], own_gpu[:, :Hkv], own_gpu[:, Hkv:], o, starts, n, zero, starts, n, zero, 1, max(lens), m, l)
         if not prefix_first:
             _prompt_on_gpu(lsa, c, o, m, l)
         assert bool((o_wide[:, Hq] == 3).all()) and bool((ml[1, :, Hq] == 0).all())
         # o is rounded twice, by half a step of a value that is at most as large as |V|
-        top = float(torch.cat([c["kv"][:, 2:].abs().amax()[None], own[:, 2:].abs().amax()[None]]).max())
-        _check((o, (torch.log2(l) + m) * math.log(2)), (o_ref, l_ref, tol_o + 2 * 2.0 ** -11 * top, tol_l + 1e-5), prefix_first)
+        top = float(torch.cat([c["kv"][:, Hkv:].abs().amax()[None], own[:, Hkv:].abs().amax()[None]]).max())
+        _check((o[looked_at], ((torch.log2(l) + m) * math.log(2))[looked_at]), (o_ref, l_ref, tol_o + 2 * 2.0 ** -11 * top, tol_l + 1e-5), prefix_first)
 
 
 @pytest.mark.gpu
