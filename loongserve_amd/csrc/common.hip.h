@@ -91,6 +91,13 @@ __device__ __forceinline__ int scan_max(int v) {
   return v;
 }
 
+// A 16-byte store that goes through to memory as it is issued (system-scope bits) instead of waiting in the L2 as a dirty
+// line until the end of the launch.  From inline assembly (the compiler has no such store that is not atomic); the
+// s_nop keeps vector instructions off the data registers for the two cycles a store of more than 64 bits needs.
+__device__ __forceinline__ void store16_through(float* addr, const f32x4 v) {
+  asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1\n\ts_nop 1" : : "v"(addr), "v"(v) : "memory");
+}
+
 // exp2 that maps (-inf) - (-inf) to 0 instead of NaN
 __device__ __forceinline__ float exp2_diff(float a, float b) {
   return (a == -INFINITY) ? 0.f : __builtin_amdgcn_exp2f(a - b);

@@ -229,13 +229,6 @@ __device__ __forceinline__ const char* uniform_ptr(const char* ptr) {
 // workgroups fit a CU, and one's start-up, finish and turn-over run beside the other's tiles.  For launches whose
 // workgroups are short (a few tiles each): there a workgroup that fills the CU spends as long starting and ending as working.
 // CUTS: a step cut along the keys (epilogue 0 only).
-// A 16-byte store that goes through to memory as it is issued (system-scope bits) instead of waiting in the L2 as a dirty
-// line until the end of the launch.  From inline assembly (the compiler has no such store that is not atomic); the
-// s_nop keeps vector instructions off the data registers for the two cycles a store of more than 64 bits needs.
-__device__ __forceinline__ void store16_through(float* addr, const f32x4 v) {
-  asm volatile("global_store_dwordx4 %0, %1, off sc0 sc1\n\ts_nop 1" : : "v"(addr), "v"(v) : "memory");
-}
-
 // WIN: a step behind a sliding window with sinks (the query at position x sees keys at positions y <= x with y > x - window or y < sinks): the workgroup walks the
 // tiles that hold sinks and those from its first row's window on; masked iterations over the sinks and the windows' starts come in front of the plain ones.  MODE 0, or
 // MODE 3: O in T's type and the LSE, from the empty state.

@@ -31,6 +31,7 @@ typedef __attribute__((address_space(3))) i16x4* lds_i16x4_ptr;
 constexpr int kRows = 128;   // query rows of a workgroup of the prefix part
 constexpr int kKeys = 64;    // keys of a tile
 constexpr float kPrefixHead = 9.f;
+constexpr int kPlanInts = 12;
 
 struct SharedParams {
   PoolParams w;  // the pool, the table, the requests' own tokens and their shares; part_o / part_lse: the own parts
@@ -43,11 +44,13 @@ struct SharedParams {
   int32_t most;          // a bound of the prefixes: longer ones are cut there
   int32_t near;          // whether every row lies within 2 GB of its head's first, slots and strides of 24 bits
   int32_t shares, parts; // of the prefix part, per KV head; partials of 128 rows per KV head
+  int32_t rounds;        // pieces that a workgroup takes at most (see Deal)
+  int32_t xcds_shift;    // log2 of the XCDs that run a KV head's workgroups
   int32_t own_wgs;       // workgroups of the own tokens, in front of those of the prefix part
-  int32_t* plan;         // [batch, 8] where a request's partials lie, for the second launch
+  int32_t* plan;         // [batch, kPlanInts] where a request's partials lie, for the second launch
   float* pre_o;          // [hkv, parts, 128, D]
   float* pre_lse;        // [hkv, parts, 128], log2 domain
-  FastDiv by_hkv, by_group, by_pre_shares;
+  FastDiv by_hkv, by_hq, by_group, by_pre_shares;
 };
 
 __device__ __forceinline__ const char* uniform_ptr(const char* ptr) {
@@ -66,6 +69,7 @@ struct Groups {
   int end;                   // the end of the rows up to the lane's group
   int tiles, blocks;         // row tiles, blocks of keys
   int tiles_to, units_to;    // sums over the 64 up to the lane's group; a unit is a row tile with a block
+  int pieces_to;             // as these, of the pieces of Deal
   __device__ __forceinline__ void look(const SharedParams& p, int g0, int end_before) {
     const int lane = threadIdx.x & 63, g = g0 + lane;
     at = g0;
@@ -91,31 +95,58 @@ struct Groups {
   __device__ __forceinline__ int all_tiles() const { return __builtin_amdgcn_readlane(tiles_to, 63); }
   __device__ __forceinline__ int all_units() const { return __builtin_amdgcn_readlane(units_to, 63); }
 };
-__device__ __forceinline__ int all_units_of(const SharedParams& p, Groups& g) {  // leaves `g` at the first groups
-  g.look(p, 0, 0);
+// How the units are dealt to the workgroups of a KV head.
+// A row tile reads all of its group's prefix, so the tiles of a group read the same rows, and where they do it at different times and the prefix is longer than an L2, each of
+// them reads it from memory again (1280 rows of 32/8 heads behind 24000 tokens: 90% of the requests missed, 160 us).  So where a group has more than one tile and it comes out even, the prefixes are cut
+// into pieces of `cut` blocks for every tile of the group, the tiles side by side, and a workgroup takes a piece (or one of each round): the tiles of a group then go
+// through a piece in step on one XCD, which reads it once.
+// Else, in order of tiles and their blocks, `per` units each.
+constexpr int kPieceCost = 4;  // blocks that a piece's start and its partials cost
+struct Deal {
+  int per, cut, pieces;
+};
+__device__ __forceinline__ Deal deal_of(const SharedParams& p, Groups& g) {  // `g`: at the first groups, and left there
   int total = g.all_units();
   if (p.groups > 64) {
     for (int g0 = 64; g0 < p.groups; g0 += 64) g.look(p, g0, g.end_of_all()), total += g.all_units();
     g.look(p, 0, 0);
   }
-  return total;
-}
-__device__ __forceinline__ int per_pre_share(const SharedParams& p, int total) {
-  const int per = (int)div_by((uint32_t)(total + p.shares - 1), p.by_pre_shares);
-  return per < 1 ? 1 : per;
+  Deal d;
+  d.per = (int)div_by((uint32_t)(total + p.shares - 1), p.by_pre_shares);
+  d.per = d.per < 1 ? 1 : d.per;
+  d.cut = 0, d.pieces = total;
+  if (!p.rounds) return d;
+  const uint32_t longest = (uint32_t)__builtin_amdgcn_readlane(scan_max(g.tiles ? g.blocks : 0), 63);
+  if (p.groups > 64 || __builtin_amdgcn_ballot_w64(g.tiles > 1) == 0 || longest >= 1u << 20) return d;
+  for (int round = 1; round <= p.rounds; round++) {
+    const uint32_t most = (uint32_t)round * p.shares;
+    const int n = (int)(most * longest / (uint32_t)total);  // pieces of the longest prefix, if they all were as long
+    for (int c = n; c > 0 && c > n - 3; c--) {
+      const int cut = (int)((longest + c - 1) / (uint32_t)c);
+      if (round * (cut + kPieceCost) * 8 > (d.per + kPieceCost) * 9) break;
+      g.pieces_to = scan_sum(g.tiles * ((g.blocks + cut - 1) / cut));
+      const int pieces = __builtin_amdgcn_readlane(g.pieces_to, 63);
+      if (pieces <= (int)most) {
+        d.cut = cut, d.pieces = pieces;
+        return d;
+      }
+    }
+  }
+  return d;
 }
 
 // The group of row b (per lane; -1: none) and its numbers, looked up from the first groups on.
 struct Membership {
   int lo, prefix, tile0, unit0, blocks;  // the group's first row, prefix, and the tiles and units of all groups in front of it
+  int g;                                 // the group, of the last 64 that were looked through
   __device__ __forceinline__ void find(const SharedParams& p, Groups& g, int b) {
-    lo = prefix = tile0 = unit0 = blocks = 0;
+    lo = prefix = tile0 = unit0 = blocks = this->g = 0;
     if (p.groups <= 8) {  // (a trip to LDS takes as long as two of them)
       for (int n = 0; n < p.groups; n++) {
         const int s = __builtin_amdgcn_readlane(g.lo, n), sz = __builtin_amdgcn_readlane(g.size, n), t1 = __builtin_amdgcn_readlane(g.tiles, n);
         const int bl = __builtin_amdgcn_readlane(g.blocks, n), pr = __builtin_amdgcn_readlane(g.prefix, n);
         const int t0 = __builtin_amdgcn_readlane(g.tiles_to, n) - t1, u0 = __builtin_amdgcn_readlane(g.units_to, n) - t1 * bl;
-        if (s <= b && b < s + sz) lo = s, prefix = pr, blocks = bl, tile0 = t0, unit0 = u0;
+        if (s <= b && b < s + sz) lo = s, prefix = pr, blocks = bl, tile0 = t0, unit0 = u0, this->g = n;
       }
       return;
     }
@@ -131,7 +162,7 @@ struct Membership {
       const bool here = n < 63 || e63 > b;  // (n counts up to 63)
       const int s = __shfl(g.lo, n, 64), sz = __shfl(g.size, n, 64), pr = __shfl(g.prefix, n, 64), bl = __shfl(g.blocks, n, 64);
       const int tt = __shfl(g.tiles_to, n, 64), t1 = __shfl(g.tiles, n, 64), ut = __shfl(g.units_to, n, 64);
-      if (here && s <= b && b < s + sz) lo = s, prefix = pr, blocks = bl, tile0 = tiles + tt - t1, unit0 = units + ut - t1 * bl;
+      if (here && s <= b && b < s + sz) lo = s, prefix = pr, blocks = bl, tile0 = tiles + tt - t1, unit0 = units + ut - t1 * bl, this->g = n;
       tiles += g.all_tiles(), units += g.all_units();
       g0 += 64;
       if (g0 >= p.groups) break;
@@ -140,6 +171,17 @@ struct Membership {
     if (p.groups > 64) g.look(p, 0, 0);
   }
 };
+
+// Where the prefix's partials of a row tile lie: n of them from `first` on, `step` apart.
+struct Partials {
+  int first, n, step;
+};
+__device__ __forceinline__ Partials partials_of(const Deal& d, int tile, int tile0, int unit0, int blocks, int tiles, int pieces0) {
+  if (!blocks) return Partials{0, 0, 1};
+  if (d.cut) return Partials{pieces0 + tile, (blocks + d.cut - 1) / d.cut, tiles};
+  const uint32_t u0 = (uint32_t)(unit0 + tile * blocks), first = u0 / (uint32_t)d.per;
+  return Partials{(int)first + tile0 + tile, (int)((u0 + blocks - 1) / (uint32_t)d.per - first) + 1, 1};
+}
 
 // ------------------------------------------------------------------------------------------------ the prefix part
 template <typename T, int D> constexpr int kPrefixLds = 2 * 2 * kKeys * D * 2 + 2 * 8;  // two stages of K and V tiles, their masks
@@ -160,16 +202,12 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
   const int lds_base = (int)(uintptr_t)(__attribute__((address_space(3))) char*)lds;
 
   Groups gs;
-  const int total = all_units_of(p, gs);
-  const int per = per_pre_share(p, total);
-  if ((int64_t)share * per >= total) return;
-  int at = share * per;
-  const int end = total - at < per ? total : at + per;
+  gs.look(p, 0, 0);
+  const Deal deal = deal_of(p, gs);
+  // units, or pieces, in the order in which they are dealt: from `at` on, up to `end`
+  int at = deal.cut ? share : (int)((int64_t)share * deal.per < deal.pieces ? share * deal.per : deal.pieces);
+  const int end = deal.cut || deal.pieces - at < deal.per ? deal.pieces : at + deal.per;
   int first = 0, tiles_before = 0;  // units and tiles in front of the 64 groups
-  while (at >= first + gs.all_units()) {
-    first += gs.all_units(), tiles_before += gs.all_tiles();
-    gs.look(p, gs.at + 64, gs.end_of_all());
-  }
   // the lane's row of its first load instruction, and its chunk of it, K and V (rows RPI apart differ in bits of their XOR that the lane's own row leaves free)
   const int j_row = lane / CPR;
   const uint32_t k_chunk = (uint32_t)(((lane % CPR) ^ swz_k(j_row)) * 16), v_chunk = (uint32_t)(((lane % CPR) ^ swz_v(j_row)) * 16);
@@ -187,12 +225,22 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
   const float scale = p.w.scale_log2;
 
   while (at < end) {
-    int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64(first + gs.units_to > at));
+    while (!deal.cut && at >= first + gs.all_units()) {  // (at < deal.pieces: a later group has some)
+      first += gs.all_units(), tiles_before += gs.all_tiles();
+      gs.look(p, gs.at + 64, gs.end_of_all());
+    }
+    const int l = __builtin_ctzll(__builtin_amdgcn_ballot_w64((deal.cut ? gs.pieces_to : first + gs.units_to) > at));
     const int blocks = __builtin_amdgcn_readlane(gs.blocks, l), tiles = __builtin_amdgcn_readlane(gs.tiles, l);
-    const int unit0 = first + __builtin_amdgcn_readlane(gs.units_to, l) - tiles * blocks;
-    const int tile = (at - unit0) / blocks, block0 = (at - unit0) - tile * blocks;
-    const int nt = blocks - block0 < end - at ? blocks - block0 : end - at;  // tiles of keys to walk
-    const int part = share + tiles_before + __builtin_amdgcn_readlane(gs.tiles_to, l) - tiles + tile;
+    int tile, block0, nt, part;  // tiles of keys to walk
+    if (deal.cut) {
+      const int i = at - (__builtin_amdgcn_readlane(gs.pieces_to, l) - tiles * ((blocks + deal.cut - 1) / deal.cut)), chunk = i / tiles;
+      tile = i - chunk * tiles, block0 = chunk * deal.cut, nt = blocks - block0 < deal.cut ? blocks - block0 : deal.cut, part = at;
+    } else {
+      const int unit0 = first + __builtin_amdgcn_readlane(gs.units_to, l) - tiles * blocks;
+      tile = (at - unit0) / blocks, block0 = (at - unit0) - tile * blocks;
+      nt = blocks - block0 < end - at ? blocks - block0 : end - at;
+      part = share + tiles_before + __builtin_amdgcn_readlane(gs.tiles_to, l) - tiles + tile;
+    }
     const int lo = __builtin_amdgcn_readlane(gs.lo, l), prefix = __builtin_amdgcn_readlane(gs.prefix, l);
     const int rows = __builtin_amdgcn_readlane(gs.size, l) * p.w.group;
     const int32_t* const row_slots = (const int32_t*)uniform_ptr((const char*)(p.w.table + (int64_t)__builtin_amdgcn_readlane(gs.req, l) * p.w.max_seq_len));
@@ -338,27 +386,52 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
         }
         u32x4 pk[2][NP];
         float ps[2];
-        auto compute_p = [&](int qb, float neg_m) __attribute__((always_inline)) {
-          float pv[8];
+        // (independent operations of one kind at a time: beside another wave's products, which hold the SIMD's matrix pipe, vector work goes on only without short dependent chains)
+        auto compute_p = [&](float neg0, float neg1) __attribute__((always_inline)) {
+          float pv[2][8], sum[2][4];
 #pragma unroll
-          for (int e = 0; e < 8; e++) pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][e / 4][e % 4], scale, neg_m));
-          ps[qb] = ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
+          for (int qb = 0; qb < 2; qb++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            pk[qb][0][e] = pack2<T>(pv[2 * e], pv[2 * e + 1]);
-            if constexpr (HIGH_LOW) {
-              float a, b;
-              unpack2<T>(pk[qb][0][e], a, b);
-              pk[qb][NP - 1][e] = pack2<T>(pv[2 * e] - a, pv[2 * e + 1] - b);
+            for (int e = 0; e < 8; e++) pv[qb][e] = __builtin_fmaf(s[qb][e / 4][e % 4], scale, qb ? neg1 : neg0);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) pv[qb][e] = __builtin_amdgcn_exp2f(pv[qb][e]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              sum[qb][e] = pv[qb][2 * e] + pv[qb][2 * e + 1];
+              pk[qb][0][e] = pack2<T>(pv[qb][2 * e], pv[qb][2 * e + 1]);
             }
-          }
-        };
-        bool over = false;
+          __builtin_amdgcn_sched_barrier(0);
+          if constexpr (HIGH_LOW) {
+            float high[2][8];
 #pragma unroll
-        for (int qb = 0; qb < 2; qb++) {
-          compute_p(qb, -m_run[qb]);
-          over |= !(ps[qb] < 32768.f);
-        }
+            for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) unpack2<T>(pk[qb][0][e], high[qb][2 * e], high[qb][2 * e + 1]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+              for (int e = 0; e < 8; e++) pv[qb][e] -= high[qb][e];
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int qb = 0; qb < 2; qb++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) pk[qb][NP - 1][e] = pack2<T>(pv[qb][2 * e], pv[qb][2 * e + 1]);
+          }
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++) sum[qb][0] += sum[qb][1], sum[qb][2] += sum[qb][3];
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int qb = 0; qb < 2; qb++) ps[qb] = sum[qb][0] + sum[qb][2];
+        };
+        compute_p(-m_run[0], -m_run[1]);
+        const bool over = !(ps[0] < 32768.f) || !(ps[1] < 32768.f);
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(over) != 0, 0)) {
 #pragma unroll
           for (int qb = 0; qb < 2; qb++) {
@@ -371,8 +444,8 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
 #pragma unroll
             for (int db = 0; db < NDB; db++) oacc[qb][db] *= alpha;
             m_run[qb] = m_new;
-            compute_p(qb, m_new == -INFINITY ? 0.f : -m_new);  // (a row that has seen no key: every weight is 0)
           }
+          compute_p(m_run[0] == -INFINITY ? 0.f : -m_run[0], m_run[1] == -INFINITY ? 0.f : -m_run[1]);  // (a row that has seen no key: every weight is 0)
         }
 #pragma unroll
         for (int qb = 0; qb < 2; qb++) l_run[qb] += ps[qb];
@@ -411,17 +484,12 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
           const int64_t to = ((int64_t)kvh * p.parts + part) * kRows + (r - tile * kRows);
           float* dst = p.pre_o + to * D + 4 * g;
 #pragma unroll
-          for (int db = 0; db < NDB; db++) *(f32x4*)(dst + 16 * db) = oacc[qb][db] * inv;
+          for (int db = 0; db < NDB; db++) store16_through(dst + 16 * db, oacc[qb][db] * inv);
           if (g == 0) p.pre_lse[to] = l_tot > 0.f ? m_run[qb] + __builtin_amdgcn_logf(l_tot) : (l_tot == l_tot ? -INFINITY : l_tot);
         }
       }
     }
-    at += nt;
-    if (at < end && at >= first + gs.all_units()) {
-      first += gs.all_units(), tiles_before += gs.all_tiles();
-      gs.look(p, gs.at + 64, gs.end_of_all());
-      while (gs.all_units() == 0) gs.look(p, gs.at + 64, gs.end_of_all());  // (at < total: a later group has some)
-    }
+    at += deal.cut ? p.shares : nt;
   }
 }
 
@@ -466,15 +534,17 @@ template <typename T, int D> __device__ __forceinline__ void own_share(const Sha
   // Where every request's partials lie, for the launch that joins them: 64 requests per wave, by the first task's waves (found again by each of its workgroups, this
   // made that launch three times as long).
   if (task == 0) {
-    const int per_pre = per_pre_share(sp, all_units_of(sp, gs));
+    const Deal deal = deal_of(sp, gs);
     for (int b0 = 0, before = 0; b0 < p.batch; b0 += 64) {
       if (rs.first_request != b0) rs.look(sp, gs, b0);
       const int b = b0 + (threadIdx.x & 63);
+      const int tiles = __shfl(gs.tiles, rs.group.g, 64), pieces0 = deal.cut ? __shfl(gs.pieces_to - gs.tiles * ((gs.blocks + deal.cut - 1) / deal.cut), rs.group.g, 64) : 0;
       if ((b0 >> 6) % p.shares == share && b < p.batch) {
         const int u0 = before + rs.up_to - rs.units, s0 = u0 / per_share;
-        int32_t* plan = sp.plan + 8 * (int64_t)b;
+        int32_t* plan = sp.plan + kPlanInts * (int64_t)b;
         *(u32x4*)plan = u32x4{(uint32_t)rs.group.lo, (uint32_t)rs.group.tile0, (uint32_t)rs.group.unit0, rs.shares ? (uint32_t)rs.group.blocks : 0u};
-        *(u32x4*)(plan + 4) = u32x4{(uint32_t)s0, (uint32_t)(rs.units ? (u0 + rs.units - 1) / per_share - s0 + 1 : 0), (uint32_t)per_pre, 0u};
+        *(u32x4*)(plan + 4) = u32x4{(uint32_t)s0, (uint32_t)(rs.units ? (u0 + rs.units - 1) / per_share - s0 + 1 : 0), (uint32_t)deal.per, (uint32_t)deal.cut};
+        *(u32x4*)(plan + 8) = u32x4{(uint32_t)tiles, (uint32_t)pieces0, 0u, 0u};
       }
       before += rs.all();
     }
@@ -528,8 +598,9 @@ __global__ __launch_bounds__(256, 2) void shared_prefix_kernel(SharedParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[OWN ? kSharedLds<T, D> : kPrefixLds<T, D>];
   if (!OWN || (int)blockIdx.x >= p.own_wgs) {
     const uint32_t x = blockIdx.x - p.own_wgs;  // (a multiple of 8)
-    const int share = (int)div_by(x, p.by_hkv);  // (with a multiple of eight KV heads a head's workgroups run on one XCD: ids are dealt round-robin)
-    prefix_share<T, D>(p, lds, (int)x - share * p.w.hkv, share);
+    // ids are dealt to the XCDs round-robin; the workgroups of a KV head that run on one XCD take neighbouring shares
+    const int i = (int)div_by(x, p.by_hkv), share = (i & ((1 << p.xcds_shift) - 1)) * (p.shares >> p.xcds_shift) + (i >> p.xcds_shift);
+    prefix_share<T, D>(p, lds, (int)x - i * p.w.hkv, share);
     return;
   }
   if constexpr (OWN) {
@@ -540,9 +611,28 @@ __global__ __launch_bounds__(256, 2) void shared_prefix_kernel(SharedParams p) {
   }
 }
 
-// o = sum of a row's partials by their log-sum-exps: those of its group's prefix, then those of its own tokens.  First the weights of all of them, by all threads, into LDS,
+// The partials of a request's row: those of its group's prefix, then those of its own tokens.
+struct MergeRow {
+  int n, n_pre, pre_step;
+  int64_t pre_row, own_row;
+  __device__ __forceinline__ MergeRow(const SharedParams& sp, int b, int h) {
+    const int32_t* const plan = sp.plan + kPlanInts * (int64_t)b;
+    const int kvh = (int)div_by((uint32_t)h, sp.by_group);
+    const int r = (b - plan[0]) * sp.w.group + (h - kvh * sp.w.group), tile = r / kRows;
+    const Partials pre = partials_of(Deal{plan[6], plan[7], 0}, tile, plan[1], plan[2], plan[3], plan[8], plan[9]);
+    n_pre = pre.n, n = pre.n + plan[5], pre_step = pre.step * kRows;
+    pre_row = ((int64_t)kvh * sp.parts + pre.first) * kRows + (r - tile * kRows), own_row = (int64_t)(plan[4] + b) * sp.w.hq + h;
+  }
+  __device__ __forceinline__ float lse(const SharedParams& sp, int i) const {
+    return i < n_pre ? sp.pre_lse[pre_row + (int64_t)i * pre_step] : sp.w.part_lse[own_row + (int64_t)(i - n_pre) * sp.w.hq];
+  }
+  __device__ __forceinline__ const float* row(const SharedParams& sp, int i, int d) const {
+    return i < n_pre ? sp.pre_o + (pre_row + (int64_t)i * pre_step) * d : sp.w.part_o + (own_row + (int64_t)(i - n_pre) * sp.w.hq) * d;
+  }
+};
+// o = sum of a row's partials by their log-sum-exps.  First the weights of all of them, by all threads, into LDS,
 // then the rows, whose loads wait for nothing.
-constexpr int kMaxParts = 2048;  // (kPrefixWorkgroups + kOwnWaves)
+constexpr int kMaxParts = 2600;  // of a row: see where the launches are planned
 template <int D>
 __global__ __launch_bounds__(256) void shared_decode_merge_kernel(SharedParams sp) {
   constexpr int W = D / 4, SL = 256 / W;
@@ -551,23 +641,11 @@ __global__ __launch_bounds__(256) void shared_decode_merge_kernel(SharedParams s
   __shared__ float weight[kMaxParts], red[8];
   const int h = blockIdx.x, b = blockIdx.y;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int32_t* plan = sp.plan + 8 * (int64_t)b;
-  const int lo = plan[0], tile0 = plan[1], unit0 = plan[2], blocks = plan[3], s0 = plan[4], n_own = plan[5];
-  const uint32_t per_pre = (uint32_t)plan[6];
-  const int kvh = (int)div_by((uint32_t)h, sp.by_group);
-  const int r = (b - lo) * p.group + (h - kvh * p.group), tile = r / kRows;
-  int n_pre = 0, p0 = 0;
-  if (blocks) {
-    const uint32_t u0 = (uint32_t)(unit0 + tile * blocks);
-    p0 = (int)(u0 / per_pre);
-    n_pre = (int)((u0 + blocks - 1) / per_pre) - p0 + 1;
-    p0 += tile0 + tile;
-  }
-  const int64_t pre_row = ((int64_t)kvh * sp.parts + p0) * kRows + (r - tile * kRows), own_row = (int64_t)(s0 + b) * p.hq + h;
-  const int n = n_pre + n_own;
+  const MergeRow m(sp, b, h);
+  const int n = m.n;
   float M = -INFINITY;
   for (int i = threadIdx.x; i < n; i += 256) {
-    const float x = i < n_pre ? sp.pre_lse[pre_row + (int64_t)i * kRows] : p.part_lse[own_row + (int64_t)(i - n_pre) * p.hq];
+    const float x = m.lse(sp, i);
     weight[i] = x;
     M = fmaxf(M, x);
   }
@@ -590,15 +668,50 @@ __global__ __launch_bounds__(256) void shared_decode_merge_kernel(SharedParams s
   const int slice = threadIdx.x / W, d = (threadIdx.x & (W - 1)) * 4;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = slice; i < n; i += SL) {
-    const float* row = i < n_pre ? sp.pre_o + (pre_row + (int64_t)i * kRows) * D : p.part_o + (own_row + (int64_t)(i - n_pre) * p.hq) * D;
-    sum += *(const f32x4*)(row + d) * weight[i];
-  }
+  for (int i = slice; i < n; i += SL) sum += *(const f32x4*)(m.row(sp, i, D) + d) * weight[i];
   *(f32x4*)&acc[slice][d] = sum;
   __syncthreads();
   if (slice) return;
 #pragma unroll
   for (int i = 1; i < SL; i++) sum += *(const f32x4*)&acc[i][d];
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const int64_t at = (int64_t)b * p.hq + h;
+  store_elem4(p.o, p.o_dtype, at * D + d, sum * inv);
+  if (d == 0) p.lse[at] = ln_of(M, L);
+}
+
+// As above with a wave per row, where there are enough of them: no barriers, 64 weights at a time in the wave's lanes.
+template <int D>
+__global__ __launch_bounds__(256) void shared_decode_merge_rows_kernel(SharedParams sp) {
+  constexpr int W = D / 4, SL = 64 / W;
+  const PoolParams& p = sp.w;
+  const int lane = threadIdx.x & 63, i0 = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = (int)div_by((uint32_t)i0, sp.by_hq), h = i0 - b * p.hq;
+  if (b >= p.batch) return;
+  const MergeRow m(sp, b, h);
+  float M = -INFINITY;
+  for (int i = lane; i < m.n; i += 64) M = fmaxf(M, m.lse(sp, i));
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  float L = 0.f;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  const int slice = lane / W, d = (lane & (W - 1)) * 4;
+  for (int i1 = 0; i1 < m.n; i1 += 64) {
+    const float weight = i1 + lane < m.n ? exp2_diff(m.lse(sp, i1 + lane), M) : 0.f;  // (NaN stays NaN)
+    L += weight;
+    const int n = m.n - i1 < 64 ? m.n - i1 : 64;
+#pragma unroll 4
+    for (int i = slice; i < n; i += SL) sum += *(const f32x4*)(m.row(sp, i1 + i, D) + d) * __shfl(weight, i, 64);
+  }
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) {
+    L += __shfl_xor(L, x, 64);
+    if (x >= W) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum[e] += __shfl_xor(sum[e], x, 64);
+    }
+  }
+  if (slice) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int64_t at = (int64_t)b * p.hq + h;
   store_elem4(p.o, p.o_dtype, at * D + d, sum * inv);
@@ -617,18 +730,20 @@ struct FoldParams {
 template <typename T, int D> __global__ __launch_bounds__(256) void shared_prefix_fold_kernel(SharedParams sp, FoldParams f) {
   constexpr int W = D / 4;
   Groups gs;
-  const uint32_t per = (uint32_t)per_pre_share(sp, all_units_of(sp, gs));
+  gs.look(sp, 0, 0);
+  const Deal deal = deal_of(sp, gs);
   const int64_t i = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
   const int b = (int)(i / sp.w.hq), h = (int)(i - (int64_t)b * sp.w.hq);
   Membership mb;
   mb.find(sp, gs, b < sp.rows ? b : sp.rows - 1);
+  const int tiles = __shfl(gs.tiles, mb.g, 64), pieces0 = deal.cut ? __shfl(gs.pieces_to - gs.tiles * ((gs.blocks + deal.cut - 1) / deal.cut), mb.g, 64) : 0;
   if (b >= sp.rows || !mb.blocks) return;
   const int kvh = h / sp.w.group, r = (b - mb.lo) * sp.w.group + (h - kvh * sp.w.group), tile = r / kRows, x = threadIdx.x & (W - 1);
-  const uint32_t u0 = (uint32_t)(mb.unit0 + tile * mb.blocks), p0 = u0 / per;
-  const int n = (int)((u0 + mb.blocks - 1) / per - p0) + 1;
-  const int64_t row = ((int64_t)kvh * sp.parts + p0 + mb.tile0 + tile) * kRows + (r - tile * kRows);
+  const Partials pre = partials_of(deal, tile, mb.tile0, mb.unit0, mb.blocks, tiles, pieces0);
+  const int n = pre.n;
+  const int64_t row = ((int64_t)kvh * sp.parts + pre.first) * kRows + (r - tile * kRows), step = (int64_t)pre.step * kRows;
   float M = -INFINITY;
-  for (int j = x; j < n; j += W) M = fmaxf(M, sp.pre_lse[row + (int64_t)j * kRows]);
+  for (int j = x; j < n; j += W) M = fmaxf(M, sp.pre_lse[row + j * step]);
 #pragma unroll
   for (int d = W / 2; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
   const int64_t ml = (int64_t)b * f.ml_st + (int64_t)h * f.ml_sh;
@@ -637,9 +752,9 @@ template <typename T, int D> __global__ __launch_bounds__(256) void shared_prefi
   float L = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   for (int j = 0; j < n; j++) {
-    const float w = exp2_diff(sp.pre_lse[row + (int64_t)j * kRows], top);
+    const float w = exp2_diff(sp.pre_lse[row + j * step], top);
     L += w;
-    sum += *(const f32x4*)(sp.pre_o + (row + (int64_t)j * kRows) * D + 4 * x) * w;
+    sum += *(const f32x4*)(sp.pre_o + (row + j * step) * D + 4 * x) * w;
   }
   if (L == 0.f) return;
   const float w_old = l_old * exp2_diff(m_old, top);
@@ -744,7 +859,9 @@ template <typename T> __global__ __launch_bounds__(256) void shared_prefix_gathe
 
 // ------------------------------------------------------------------------------------------------ the host's side
 constexpr int64_t kPrefixWorkgroups = 2 * kCUs;  // at most
+constexpr int64_t kRounds = 3;  // pieces per workgroup, at most
 constexpr int64_t kOwnWaves = 4 * kCUs;
+static_assert(kRounds * kPrefixWorkgroups + kOwnWaves + 2 <= kMaxParts, "a row's partials have their weights in LDS");
 constexpr int64_t kOwnMinUnits = 2;
 
 // a bound of the prefixes that a table can hold
@@ -755,7 +872,7 @@ bool is_near(const PoolParams& w) {
   return w.num_slots <= 1 << 24 && w.k_s0 < 1 << 24 && w.v_s0 < 1 << 24 && last * w.k_s0 < 0x7fff0000 && last * w.v_s0 < 0x7fff0000;
 }
 struct Plan {
-  int64_t tiles, shares, parts;  // prefix part, per KV head
+  int64_t tiles, shares, parts, rounds, xcds_shift;  // prefix part, per KV head
   int64_t own_shares;
   int64_t pre_floats, own_floats, plan_ints;  // of the workspace
   int64_t all() const { return (pre_floats + own_floats + plan_ints) * 4; }
@@ -774,7 +891,12 @@ Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, i
   p.shares = (beside ? kCUs : kPrefixWorkgroups) / hkv;
   p.shares = p.shares < 1 ? 1 : p.shares;
   p.shares = p.shares < units ? p.shares : units < 1 ? 1 : units;
-  p.parts = p.shares + p.tiles;
+  p.xcds_shift = hkv % 8 == 0 ? 0 : hkv % 4 == 0 ? 1 : hkv % 2 == 0 ? 2 : 3;
+  if (p.shares >> p.xcds_shift) p.shares = p.shares >> p.xcds_shift << p.xcds_shift;
+  else p.xcds_shift = 0;
+  // (no group has more rows than there are; code that is not run is not fetched: a small launch is 1.5 us shorter)
+  p.rounds = rows * (hq / hkv) <= kRows ? 0 : p.tiles * 6 <= p.shares ? 1 : kRounds;
+  p.parts = p.shares + p.tiles > p.rounds * p.shares ? p.shares + p.tiles : p.rounds * p.shares;
   p.pre_floats = p.tiles ? hkv * p.parts * kRows * (d + 1) : 0;
   p.own_shares = 1, p.own_floats = 0, p.plan_ints = 0;
   if (decode) {
@@ -782,16 +904,21 @@ Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, i
     p.own_shares = by_waves < by_units ? by_waves : by_units;
     p.own_shares = p.own_shares < 1 ? 1 : p.own_shares;
     p.own_floats = ((p.own_shares + rows) * hq * (d + 1) + 3) / 4 * 4;
-    p.plan_ints = 8 * rows;
+    p.plan_ints = kPlanInts * rows;
   }
   return p;
 }
 
+// Rows of a launch from which the one that joins them has a wave per row instead of a workgroup (us, workgroup | wave): 32 heads of 128, 32 requests 6.2 | 10.3, 64 6.5 | 7.5, 160 10.0 | 7.3;
+// 28 heads of 64, 64 requests 5.6 | 7.2, 160 9.6 | 6.5.
+constexpr int64_t kMergeByWaves = 4096;
 template <typename T, int D> void launch_decode(const SharedParams& p, hipStream_t st) {
   const int64_t prefix = p.groups ? (int64_t)p.shares * p.w.hkv : 0;
   LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<T, D, true>), dim3((unsigned)(p.own_wgs + prefix)), dim3(256), 0, st, p);
   if (hipPeekAtLastError() != hipSuccess) return;
-  LSATTN_LAUNCH_KERNEL((shared_decode_merge_kernel<D>), dim3(p.w.hq, p.w.batch), dim3(256), 0, st, p);
+  const int64_t rows = (int64_t)p.w.batch * p.w.hq;
+  if (rows >= kMergeByWaves) LSATTN_LAUNCH_KERNEL((shared_decode_merge_rows_kernel<D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
+  else LSATTN_LAUNCH_KERNEL((shared_decode_merge_kernel<D>), dim3(p.w.hq, p.w.batch), dim3(256), 0, st, p);
 }
 
 }  // namespace
@@ -858,8 +985,8 @@ extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* st
   p.g_start = a->g_start_loc, p.g_size = a->g_size, p.g_req = a->g_req_idx, p.g_prefix = a->g_prefix_len;
   p.groups = pl.tiles ? (int32_t)a->num_groups : 0;
   p.rows = w.batch, p.most = (int32_t)most, p.near = is_near(w);
-  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.own_wgs = (int32_t)(((pl.own_shares * w.tasks + 3) / 4 + 7) / 8 * 8);
-  p.by_hkv = fast_div((uint32_t)w.hkv), p.by_group = fast_div((uint32_t)w.group), p.by_pre_shares = fast_div((uint32_t)pl.shares);
+  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.rounds = (int32_t)pl.rounds, p.xcds_shift = (int32_t)pl.xcds_shift, p.own_wgs = (int32_t)(((pl.own_shares * w.tasks + 3) / 4 + 7) / 8 * 8);
+  p.by_hkv = fast_div((uint32_t)w.hkv), p.by_hq = fast_div((uint32_t)w.hq), p.by_group = fast_div((uint32_t)w.group), p.by_pre_shares = fast_div((uint32_t)pl.shares);
   hipStream_t st = (hipStream_t)stream;
   if (a->dtype == LSATTN_F16) {
     if (a->head_dim == 128) launch_decode<F16, 128>(p, st);
@@ -972,7 +1099,7 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
   const Plan pl = plan_of(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len, 0, false);
   if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups) return LSATTN_ERR_INVALID_ARG;  // (units are numbered with 31 bits)
   p.pre_o = (float*)a->workspace, p.pre_lse = p.pre_o + (pl.pre_floats / (a->head_dim + 1)) * a->head_dim;
-  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts;
+  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.rounds = (int32_t)pl.rounds, p.xcds_shift = (int32_t)pl.xcds_shift;
   p.by_pre_shares = fast_div((uint32_t)pl.shares);
   FoldParams f;
   f.o = (char*)a->o, f.o_st = a->o_stride_t * 2, f.o_sh = a->o_stride_h * 2, f.m = a->m, f.l = a->l, f.ml_st = a->ml_stride_t, f.ml_sh = a->ml_stride_h;

@@ -495,6 +495,22 @@ def test_prompts_behind_a_prefix_with_their_own_chunks(lsa, heads, rows):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads, prefix", [(64, 10253), (256, 2711), (8, 9000)])
+def test_prompt_step_pieces_of_a_long_prefix(lsa, heads, prefix):
+    """Row tiles that go through a long prefix side by side, in pieces: two and three of them per workgroup with few workgroups per head, one with many; every 29th row."""
+    c = _prompt_case(33, heads, heads, 64, torch.float16, [(prefix, 300), (70, 2)], tail=0)
+    T, Hq, D = c["q"].shape
+    c["table"][c["g"][2][0], 100] = PAD
+    rows = list(range(0, T, 29)) + [T - 1]
+    of = [int(i >= 300) for i in rows]
+    want = [_prompt_ref(dict(c, q=c["q"][i:i + 1], g=([0], [1], [c["g"][2][n]], [c["g"][3][n]]))) for i, n in zip(rows, of)]
+    o_ref, l_ref, tol_o, tol_l = (torch.cat(x) for x in zip(*want))
+    o, m, l = torch.zeros(T, Hq, D, dtype=torch.float16, device=DEV), torch.full((T, Hq), -math.inf, device=DEV), torch.zeros(T, Hq, device=DEV)
+    _prompt_on_gpu(lsa, c, o, m, l)
+    _check((o[rows], ((torch.log2(l) + m) * math.log(2))[rows]), (o_ref, l_ref, tol_o + 2.0 ** -11 * (o_ref.abs() + tol_o) + 2.0 ** -25, tol_l + 1e-6), (heads, prefix))
+
+
+@pytest.mark.gpu
 def test_prompt_step_refusals(lsa):
     c = _prompt_case(37, 8, 2, 128, torch.float16, [(20, 4)])
     T, Hq, D = c["q"].shape
