@@ -186,7 +186,9 @@ __device__ __forceinline__ Partials partials_of(const Deal& d, int tile, int til
 // ------------------------------------------------------------------------------------------------ the prefix part
 template <typename T, int D> constexpr int kPrefixLds = 2 * 2 * kKeys * D * 2 + 2 * 8;  // two stages of K and V tiles, their masks
 
-template <typename T, int D> __device__ __forceinline__ void prefix_share(const SharedParams& p, char* lds, int kvh, int share) {
+// THROUGH: partials go through to memory as they are stored.  Of many rows the launch's end waits for less then (prompts of 293 rows behind 6001 tokens 67 -> 65 us); beside workgroups that
+// still read, or of few rows, it waits for more (24 requests 96 -> 97.5 us).
+template <typename T, int D, bool THROUGH> __device__ __forceinline__ void prefix_share(const SharedParams& p, char* lds, int kvh, int share) {
   constexpr bool HIGH_LOW = __is_same(T, BF16);
   constexpr int NP = HIGH_LOW ? 2 : 1;      // parts of P
   constexpr int KS = D / 32, NDB = D / 16;  // contraction steps of Q K^T; 16-wide blocks of the head
@@ -386,52 +388,27 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
         }
         u32x4 pk[2][NP];
         float ps[2];
-        // (independent operations of one kind at a time: beside another wave's products, which hold the SIMD's matrix pipe, vector work goes on only without short dependent chains)
-        auto compute_p = [&](float neg0, float neg1) __attribute__((always_inline)) {
-          float pv[2][8], sum[2][4];
+        auto compute_p = [&](int qb, float neg_m) __attribute__((always_inline)) {
+          float pv[8];
 #pragma unroll
-          for (int qb = 0; qb < 2; qb++)
+          for (int e = 0; e < 8; e++) pv[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[qb][e / 4][e % 4], scale, neg_m));
+          ps[qb] = ((pv[0] + pv[1]) + (pv[2] + pv[3])) + ((pv[4] + pv[5]) + (pv[6] + pv[7]));
 #pragma unroll
-            for (int e = 0; e < 8; e++) pv[qb][e] = __builtin_fmaf(s[qb][e / 4][e % 4], scale, qb ? neg1 : neg0);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int qb = 0; qb < 2; qb++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) pv[qb][e] = __builtin_amdgcn_exp2f(pv[qb][e]);
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int qb = 0; qb < 2; qb++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              sum[qb][e] = pv[qb][2 * e] + pv[qb][2 * e + 1];
-              pk[qb][0][e] = pack2<T>(pv[qb][2 * e], pv[qb][2 * e + 1]);
+          for (int e = 0; e < 4; e++) {
+            pk[qb][0][e] = pack2<T>(pv[2 * e], pv[2 * e + 1]);
+            if constexpr (HIGH_LOW) {
+              float a, b;
+              unpack2<T>(pk[qb][0][e], a, b);
+              pk[qb][NP - 1][e] = pack2<T>(pv[2 * e] - a, pv[2 * e + 1] - b);
             }
-          __builtin_amdgcn_sched_barrier(0);
-          if constexpr (HIGH_LOW) {
-            float high[2][8];
-#pragma unroll
-            for (int qb = 0; qb < 2; qb++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) unpack2<T>(pk[qb][0][e], high[qb][2 * e], high[qb][2 * e + 1]);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int qb = 0; qb < 2; qb++)
-#pragma unroll
-              for (int e = 0; e < 8; e++) pv[qb][e] -= high[qb][e];
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int qb = 0; qb < 2; qb++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) pk[qb][NP - 1][e] = pack2<T>(pv[qb][2 * e], pv[qb][2 * e + 1]);
           }
-#pragma unroll
-          for (int qb = 0; qb < 2; qb++) sum[qb][0] += sum[qb][1], sum[qb][2] += sum[qb][3];
-          __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-          for (int qb = 0; qb < 2; qb++) ps[qb] = sum[qb][0] + sum[qb][2];
         };
-        compute_p(-m_run[0], -m_run[1]);
-        const bool over = !(ps[0] < 32768.f) || !(ps[1] < 32768.f);
+        bool over = false;
+#pragma unroll
+        for (int qb = 0; qb < 2; qb++) {
+          compute_p(qb, -m_run[qb]);
+          over |= !(ps[qb] < 32768.f);
+        }
         if (__builtin_expect(__builtin_amdgcn_ballot_w64(over) != 0, 0)) {
 #pragma unroll
           for (int qb = 0; qb < 2; qb++) {
@@ -444,8 +421,8 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
 #pragma unroll
             for (int db = 0; db < NDB; db++) oacc[qb][db] *= alpha;
             m_run[qb] = m_new;
+            compute_p(qb, m_new == -INFINITY ? 0.f : -m_new);  // (a row that has seen no key: every weight is 0)
           }
-          compute_p(m_run[0] == -INFINITY ? 0.f : -m_run[0], m_run[1] == -INFINITY ? 0.f : -m_run[1]);  // (a row that has seen no key: every weight is 0)
         }
 #pragma unroll
         for (int qb = 0; qb < 2; qb++) l_run[qb] += ps[qb];
@@ -484,7 +461,10 @@ template <typename T, int D> __device__ __forceinline__ void prefix_share(const 
           const int64_t to = ((int64_t)kvh * p.parts + part) * kRows + (r - tile * kRows);
           float* dst = p.pre_o + to * D + 4 * g;
 #pragma unroll
-          for (int db = 0; db < NDB; db++) store16_through(dst + 16 * db, oacc[qb][db] * inv);
+          for (int db = 0; db < NDB; db++) {
+            if constexpr (THROUGH) store16_through(dst + 16 * db, oacc[qb][db] * inv);
+            else *(f32x4*)(dst + 16 * db) = oacc[qb][db] * inv;
+          }
           if (g == 0) p.pre_lse[to] = l_tot > 0.f ? m_run[qb] + __builtin_amdgcn_logf(l_tot) : (l_tot == l_tot ? -INFINITY : l_tot);
         }
       }
@@ -600,7 +580,7 @@ __global__ __launch_bounds__(256, 2) void shared_prefix_kernel(SharedParams p) {
     const uint32_t x = blockIdx.x - p.own_wgs;  // (a multiple of 8)
     // ids are dealt to the XCDs round-robin; the workgroups of a KV head that run on one XCD take neighbouring shares
     const int i = (int)div_by(x, p.by_hkv), share = (i & ((1 << p.xcds_shift) - 1)) * (p.shares >> p.xcds_shift) + (i >> p.xcds_shift);
-    prefix_share<T, D>(p, lds, (int)x - i * p.w.hkv, share);
+    prefix_share<T, D, !OWN>(p, lds, (int)x - i * p.w.hkv, share);
     return;
   }
   if constexpr (OWN) {
