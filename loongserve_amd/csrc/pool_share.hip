@@ -79,15 +79,14 @@ template <typename Piece, int ROWS, typename F> __device__ __forceinline__ void 
 
 struct CopyParams {
   ForkParams f;
-  RowsParams r;
+  RowsParams r, scales;
   const int64_t* index;
   const int32_t* start;
   int64_t num_index;
-  int32_t registers;  // whether this launch writes the table
 };
 constexpr int kCopyRows = 16;
 // grid (positions, forks, layers)
-template <typename Piece> __global__ __launch_bounds__(kThreads) void fork_copy_kernel(CopyParams p) {
+__global__ __launch_bounds__(kThreads) void fork_copy_kernel(CopyParams p) {
   const int i = blockIdx.y, pos0 = (int)blockIdx.x * kCopyRows, len = fork_len(p.f, i);
   if (pos0 >= len) return;
   const int32_t* const src_row = p.f.table + (int64_t)p.f.src[i] * p.f.max_seq_len;
@@ -97,16 +96,18 @@ template <typename Piece> __global__ __launch_bounds__(kThreads) void fork_copy_
     const int64_t d = pos < len && at >= 0 && at < p.num_index ? p.index[at] : -1;
     return d >= 0 && d < p.r.num_slots ? (int)d : -1;
   };
-  if (p.registers && blockIdx.z == 0 && threadIdx.x < kCopyRows) {
+  if (blockIdx.z == 0 && threadIdx.x < kCopyRows) {
     const int d = target(pos0 + threadIdx.x);
     if (d >= 0) p.f.table[(int64_t)p.f.dst[i] * p.f.max_seq_len + pos0 + threadIdx.x] = d;
   }
-  move_rows<Piece, kCopyRows>(p.r, blockIdx.z, [&](int k, int& src, int& dst) {
+  auto copy = [&](int k, int& src, int& dst) {
     if (pos0 + k >= len) return false;
     src = src_row[pos0 + k];
     dst = target(pos0 + k);
     return dst >= 0 && (uint32_t)src < (uint32_t)p.r.num_slots;
-  });
+  };
+  move_rows<u32x4, kCopyRows>(p.r, blockIdx.z, copy);
+  if (p.scales.rows) move_rows<uint8_t, kCopyRows>(p.scales, blockIdx.z, copy);
 }
 
 // ------------------------------------------------------------------------------------------------ release
@@ -127,20 +128,23 @@ struct ReleaseParams {
 __device__ __forceinline__ int release_len(const ReleaseParams& p, int i) { return p.len[i] < p.most ? p.len[i] : p.most; }
 // `refs` references less on a slot.  A count does not fall below zero: what is too much is given back and counts as wrong.  (Of any number of threads one sees the count end: what is given back
 // was below zero.)
-__device__ __forceinline__ void release_seen(const ReleaseParams& p, int slot, int refs, int old, int& freed, int& wrong) {
+template <int SCOPE> __device__ __forceinline__ int release_refs(const ReleaseParams& p, int slot, int refs) {
+  return __hip_atomic_fetch_sub(p.state + slot, refs, __ATOMIC_RELAXED, SCOPE);
+}
+template <int SCOPE> __device__ __forceinline__ void release_seen(const ReleaseParams& p, int slot, int refs, int old, int& freed, int& wrong) {
   const int had = old > 0 ? old : 0;
   if (had && had <= refs) freed++;
   if (had < refs) {
-    atomicAdd(p.state + slot, refs - had);
+    __hip_atomic_fetch_add(p.state + slot, refs - had, __ATOMIC_RELAXED, SCOPE);
     wrong += refs - had;
   }
 }
-__device__ __forceinline__ void release_one(const ReleaseParams& p, int i, int pos, int& freed, int& wrong) {
+template <int SCOPE> __device__ __forceinline__ void release_one(const ReleaseParams& p, int i, int pos, int& freed, int& wrong) {
   const int req = p.req[i];
   if (pos >= release_len(p, i)) return;
   const int slot = req >= 0 && req < p.num_reqs ? p.table[(int64_t)req * p.max_seq_len + pos] : -1;
   if ((uint32_t)slot >= (uint32_t)p.size) wrong++;
-  else release_seen(p, slot, 1, atomicSub(p.state + slot, 1), freed, wrong);
+  else release_seen<SCOPE>(p, slot, 1, release_refs<SCOPE>(p, slot, 1), freed, wrong);
 }
 template <int THREADS> __device__ __forceinline__ void sum_group(int& a, int& b) {
   __shared__ int sh[2][THREADS / 64];
@@ -152,14 +156,14 @@ template <int THREADS> __device__ __forceinline__ void sum_group(int& a, int& b)
 #pragma unroll
   for (int w = 0; w < THREADS / 64; w++) a += sh[0][w], b += sh[1][w];
 }
-// (the cells may lie in host memory; every atomic of the call has returned what it found by now)
+// (the cells may lie in host memory)
 __device__ __forceinline__ void tell(int64_t* cells, int64_t freed, int64_t wrong) {
   __hip_atomic_store(cells, freed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
   __hip_atomic_store(cells + 1, wrong, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
 }
 __global__ __launch_bounds__(kThreads) void release_kernel(ReleaseParams p) {
   int freed = 0, wrong = 0;
-  release_one(p, blockIdx.y, (int)(blockIdx.x * kThreads + threadIdx.x), freed, wrong);
+  release_one<__HIP_MEMORY_SCOPE_AGENT>(p, blockIdx.y, (int)(blockIdx.x * kThreads + threadIdx.x), freed, wrong);
   sum_group<kThreads>(freed, wrong);
   if (threadIdx.x == 0) {
     int32_t* s = p.sums + 2 * ((int64_t)blockIdx.y * p.blocks + blockIdx.x);
@@ -212,11 +216,11 @@ __global__ __launch_bounds__(kThreads) void release_columns_kernel(ReleaseParams
 #pragma unroll
   for (int k = 0; k < kRun; k++) {
     old[k] = 0;
-    if (refs[k]) old[k] = atomicSub(p.state + slot[k], refs[k]);
+    if (refs[k]) old[k] = release_refs<__HIP_MEMORY_SCOPE_AGENT>(p, slot[k], refs[k]);
   }
 #pragma unroll
   for (int k = 0; k < kRun; k++)
-    if (refs[k]) release_seen(p, slot[k], refs[k], old[k], freed, wrong);
+    if (refs[k]) release_seen<__HIP_MEMORY_SCOPE_AGENT>(p, slot[k], refs[k], old[k], freed, wrong);
   sum_group<kThreads>(freed, wrong);
   if (threadIdx.x == 0) {
     int32_t* s = p.sums + 2 * ((int64_t)blockIdx.y * p.blocks + blockIdx.x);
@@ -235,11 +239,13 @@ __global__ __launch_bounds__(1024) void release_sum_kernel(ReleaseParams p, int6
   for (int w = 1; w < 16; w++) a += sh[0][w], b += sh[1][w];
   tell(p.cells, a, b);
 }
-// Few tokens: one workgroup takes all of them and tells the counts itself.
+// Few tokens: one workgroup takes all of them and tells the counts itself.  Whoever sees those (the host, which may go on to another stream) finds the states changed: the atomics are the
+// system's and have arrived in front of the barrier.
 constexpr int64_t kOneGroupTokens = 4096;
 __global__ __launch_bounds__(1024) void release_one_group_kernel(ReleaseParams p, int max_len) {
   int freed = 0, wrong = 0;
-  for (int i = threadIdx.x; i < p.n * max_len; i += 1024) release_one(p, i / max_len, i % max_len, freed, wrong);
+  for (int i = threadIdx.x; i < p.n * max_len; i += 1024) release_one<__HIP_MEMORY_SCOPE_SYSTEM>(p, i / max_len, i % max_len, freed, wrong);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   sum_group<1024>(freed, wrong);
   if (threadIdx.x == 0) tell(p.cells, freed, wrong);
 }
@@ -435,17 +441,14 @@ extern "C" int lsattn_copy_requests(const lsattn_copy_requests_args* a, const ls
     return LSATTN_ERR_INVALID_ARG;
   const int64_t most = a->max_len_in_batch < a->max_seq_len ? a->max_len_in_batch : a->max_seq_len;
   if (a->n == 0 || most == 0) return LSATTN_OK;
-  CopyParams p;
+  CopyParams p = {};
   p.f = ForkParams{a->req_to_tokens, a->max_seq_len, (int32_t)most, a->src_req_idx, a->dst_req_idx, a->b_seq_len, (int32_t)a->n, (int32_t)a->num_reqs, nullptr, 0};
-  p.index = a->mem_index, p.start = a->b_start_loc, p.num_index = a->num_index, p.registers = 1;
+  p.index = a->mem_index, p.start = a->b_start_loc, p.num_index = a->num_index;
   const dim3 grid((unsigned)((most + kCopyRows - 1) / kCopyRows), (unsigned)a->n, (unsigned)rows->num_layers);
   hipStream_t st = (hipStream_t)stream;
   set_rows(p.r, rows->rows, rows->layer_stride_bytes, rows->slot_stride_bytes, rows->row_bytes / 16, rows->num_slots);
-  LSATTN_LAUNCH_KERNEL((fork_copy_kernel<u32x4>), grid, dim3(kThreads), 0, st, p);
-  if (!rows->scales || hipPeekAtLastError() != hipSuccess) return check_launch();
-  p.registers = 0;
-  set_rows(p.r, rows->scales, rows->scale_layer_stride_bytes, rows->scale_slot_stride_bytes, rows->scale_bytes, rows->num_slots);
-  LSATTN_LAUNCH_KERNEL((fork_copy_kernel<uint8_t>), grid, dim3(kThreads), 0, st, p);
+  if (rows->scales) set_rows(p.scales, rows->scales, rows->scale_layer_stride_bytes, rows->scale_slot_stride_bytes, rows->scale_bytes, rows->num_slots);
+  LSATTN_LAUNCH_KERNEL(fork_copy_kernel, grid, dim3(kThreads), 0, st, p);
   return check_launch();
 }
 

@@ -872,10 +872,10 @@ Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, i
   p.shares = p.shares < 1 ? 1 : p.shares;
   p.shares = p.shares < units ? p.shares : units < 1 ? 1 : units;
   p.xcds_shift = hkv % 8 == 0 ? 0 : hkv % 4 == 0 ? 1 : hkv % 2 == 0 ? 2 : 3;
-  if (p.shares >> p.xcds_shift) p.shares = p.shares >> p.xcds_shift << p.xcds_shift;
+  if (p.shares >> p.xcds_shift >= 8) p.shares = p.shares >> p.xcds_shift << p.xcds_shift;  // (as many on each of the XCDs, and not many fewer for it)
   else p.xcds_shift = 0;
-  // (no group has more rows than there are; code that is not run is not fetched: a small launch is 1.5 us shorter)
-  p.rounds = rows * (hq / hkv) <= kRows ? 0 : p.tiles * 6 <= p.shares ? 1 : kRounds;
+  // (no group has more rows than there are; code that is not run is not fetched: a small launch is 1 us shorter)
+  p.rounds = rows * (hq / hkv) <= kRows ? 0 : p.tiles * 6 <= kPrefixWorkgroups / hkv ? 1 : kRounds;
   p.parts = p.shares + p.tiles > p.rounds * p.shares ? p.shares + p.tiles : p.rounds * p.shares;
   p.pre_floats = p.tiles ? hkv * p.parts * kRows * (d + 1) : 0;
   p.own_shares = 1, p.own_floats = 0, p.plan_ints = 0;
@@ -942,7 +942,7 @@ extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* st
   // (units of both parts are numbered with 31 bits, and requests may be longer than the caller's bound)
   const int64_t most = most_of(a->max_prefix_len, a->max_seq_len);
   if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups ||
-      a->batch * ((a->max_seq_len + kBlock - 1) / kBlock) > kMaxUnits - kOwnWaves)
+      a->batch * ((a->max_seq_len + kBlock - 1) / kBlock) > kMaxUnits - kOwnWaves || a->batch * a->num_q_heads > kMaxUnits)
     return LSATTN_ERR_INVALID_ARG;
   SharedParams p;
   PoolParams& w = p.w;
