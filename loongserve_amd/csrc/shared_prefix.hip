@@ -46,7 +46,7 @@ struct SharedParams {
   int32_t shares, parts; // of the prefix part, per KV head; partials of 128 rows per KV head
   int32_t rounds;        // pieces that a workgroup takes at most (see Deal)
   int32_t xcds_shift;    // log2 of the XCDs that run a KV head's workgroups
-  int32_t own_wgs;       // workgroups of the own tokens, in front of those of the prefix part
+  int32_t own_wgs;       // workgroups of the own tokens (prompts: of the plan), in front of those of the prefix part; a multiple of 8
   int32_t* plan;         // [batch, kPlanInts] where a request's partials lie, for the second launch
   float* pre_o;          // [hkv, parts, 128, D]
   float* pre_lse;        // [hkv, parts, 128], log2 domain
@@ -182,6 +182,23 @@ __device__ __forceinline__ Partials partials_of(const Deal& d, int tile, int til
   const uint32_t u0 = (uint32_t)(unit0 + tile * blocks), first = u0 / (uint32_t)d.per;
   return Partials{(int)first + tile0 + tile, (int)((u0 + blocks - 1) / (uint32_t)d.per - first) + 1, 1};
 }
+
+// What the launch that joins the partials has to know of a row of q (found again by each of its workgroups, this made that launch two to three times as long).
+struct PlanRow {
+  const Membership& m;
+  const Deal& d;
+  int tiles, pieces0;
+  __device__ __forceinline__ PlanRow(const Membership& m, const Groups& g, const Deal& d) : m(m), d(d) {  // (by whole waves)
+    tiles = __shfl(g.tiles, m.g, 64);
+    pieces0 = d.cut ? __shfl(g.pieces_to - g.tiles * ((g.blocks + d.cut - 1) / d.cut), m.g, 64) : 0;
+  }
+  __device__ __forceinline__ void put(const SharedParams& p, int b, bool shares, int own0, int n_own) const {
+    int32_t* const plan = p.plan + kPlanInts * (int64_t)b;
+    *(u32x4*)plan = u32x4{(uint32_t)m.lo, (uint32_t)m.tile0, (uint32_t)m.unit0, shares ? (uint32_t)m.blocks : 0u};
+    *(u32x4*)(plan + 4) = u32x4{(uint32_t)own0, (uint32_t)n_own, (uint32_t)d.per, (uint32_t)d.cut};
+    *(u32x4*)(plan + 8) = u32x4{(uint32_t)tiles, (uint32_t)pieces0, 0u, 0u};
+  }
+};
 
 // ------------------------------------------------------------------------------------------------ the prefix part
 template <typename T, int D> constexpr int kPrefixLds = 2 * 2 * kKeys * D * 2 + 2 * 8;  // two stages of K and V tiles, their masks
@@ -511,20 +528,16 @@ template <typename T, int D> __device__ __forceinline__ void own_share(const Sha
     rs.look(sp, gs, 0);
   }
   const int per_share = per_own_share(p, total);
-  // Where every request's partials lie, for the launch that joins them: 64 requests per wave, by the first task's waves (found again by each of its workgroups, this
-  // made that launch three times as long).
+  // Where every request's partials lie, for the launch that joins them: 64 requests per wave, by the first task's waves.
   if (task == 0) {
     const Deal deal = deal_of(sp, gs);
     for (int b0 = 0, before = 0; b0 < p.batch; b0 += 64) {
       if (rs.first_request != b0) rs.look(sp, gs, b0);
       const int b = b0 + (threadIdx.x & 63);
-      const int tiles = __shfl(gs.tiles, rs.group.g, 64), pieces0 = deal.cut ? __shfl(gs.pieces_to - gs.tiles * ((gs.blocks + deal.cut - 1) / deal.cut), rs.group.g, 64) : 0;
+      const PlanRow row(rs.group, gs, deal);
       if ((b0 >> 6) % p.shares == share && b < p.batch) {
         const int u0 = before + rs.up_to - rs.units, s0 = u0 / per_share;
-        int32_t* plan = sp.plan + kPlanInts * (int64_t)b;
-        *(u32x4*)plan = u32x4{(uint32_t)rs.group.lo, (uint32_t)rs.group.tile0, (uint32_t)rs.group.unit0, rs.shares ? (uint32_t)rs.group.blocks : 0u};
-        *(u32x4*)(plan + 4) = u32x4{(uint32_t)s0, (uint32_t)(rs.units ? (u0 + rs.units - 1) / per_share - s0 + 1 : 0), (uint32_t)deal.per, (uint32_t)deal.cut};
-        *(u32x4*)(plan + 8) = u32x4{(uint32_t)tiles, (uint32_t)pieces0, 0u, 0u};
+        row.put(sp, b, rs.shares, s0, rs.units ? (u0 + rs.units - 1) / per_share - s0 + 1 : 0);
       }
       before += rs.all();
     }
@@ -571,12 +584,12 @@ template <typename T, int D> __device__ __forceinline__ void own_share(const Sha
   }
 }
 
-// Workgroups of the own tokens first, four waves with a share each, then those of the prefix part.
+// Workgroups of the own tokens first, four waves with a share each, then those of the prefix part.  Prompts (!OWN) have no such tokens here.
 template <typename T, int D> constexpr int kSharedLds = kPrefixLds<T, D> > 4 * kWaveLds<T, D> ? kPrefixLds<T, D> : 4 * kWaveLds<T, D>;
 template <typename T, int D, bool OWN>
 __global__ __launch_bounds__(256, 2) void shared_prefix_kernel(SharedParams p) {
   __shared__ __attribute__((aligned(1024))) char lds[OWN ? kSharedLds<T, D> : kPrefixLds<T, D>];
-  if (!OWN || (int)blockIdx.x >= p.own_wgs) {
+  if ((int)blockIdx.x >= p.own_wgs) {
     const uint32_t x = blockIdx.x - p.own_wgs;  // (a multiple of 8)
     // ids are dealt to the XCDs round-robin; the workgroups of a KV head that run on one XCD take neighbouring shares
     const int i = (int)div_by(x, p.by_hkv), share = (i & ((1 << p.xcds_shift) - 1)) * (p.shares >> p.xcds_shift) + (i >> p.xcds_shift);
@@ -588,6 +601,17 @@ __global__ __launch_bounds__(256, 2) void shared_prefix_kernel(SharedParams p) {
     const uint32_t unit = ((x & 7) * (p.own_wgs >> 3) + (x >> 3)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int share = (int)div_by(unit, p.w.by_tasks), task = (int)(unit - (uint32_t)share * p.w.tasks);
     if (share < p.w.shares) own_share<T, D>(p, lds, share, task);
+  } else {  // (prompts: these workgroups write the plan)
+    Groups gs;
+    gs.look(p, 0, 0);
+    const Deal deal = deal_of(p, gs);
+    for (int b0 = (int)blockIdx.x * 256; b0 < p.rows; b0 += p.own_wgs * 256) {
+      const int b = b0 + threadIdx.x;
+      Membership m;
+      m.find(p, gs, b < p.rows ? b : p.rows - 1);
+      const PlanRow row(m, gs, deal);
+      if (b < p.rows) row.put(p, b, true, 0, 0);
+    }
   }
 }
 
@@ -709,21 +733,13 @@ struct FoldParams {
 };
 template <typename T, int D> __global__ __launch_bounds__(256) void shared_prefix_fold_kernel(SharedParams sp, FoldParams f) {
   constexpr int W = D / 4;
-  Groups gs;
-  gs.look(sp, 0, 0);
-  const Deal deal = deal_of(sp, gs);
-  const int64_t i = (int64_t)blockIdx.x * (256 / W) + threadIdx.x / W;
-  const int b = (int)(i / sp.w.hq), h = (int)(i - (int64_t)b * sp.w.hq);
-  Membership mb;
-  mb.find(sp, gs, b < sp.rows ? b : sp.rows - 1);
-  const int tiles = __shfl(gs.tiles, mb.g, 64), pieces0 = deal.cut ? __shfl(gs.pieces_to - gs.tiles * ((gs.blocks + deal.cut - 1) / deal.cut), mb.g, 64) : 0;
-  if (b >= sp.rows || !mb.blocks) return;
-  const int kvh = h / sp.w.group, r = (b - mb.lo) * sp.w.group + (h - kvh * sp.w.group), tile = r / kRows, x = threadIdx.x & (W - 1);
-  const Partials pre = partials_of(deal, tile, mb.tile0, mb.unit0, mb.blocks, tiles, pieces0);
-  const int n = pre.n;
-  const int64_t row = ((int64_t)kvh * sp.parts + pre.first) * kRows + (r - tile * kRows), step = (int64_t)pre.step * kRows;
+  const int i = (int)blockIdx.x * (256 / W) + threadIdx.x / W, x = threadIdx.x & (W - 1);
+  const int b = (int)div_by((uint32_t)i, sp.by_hq), h = i - b * sp.w.hq;
+  if (b >= sp.rows) return;
+  const MergeRow r(sp, b, h);
+  if (!r.n) return;
   float M = -INFINITY;
-  for (int j = x; j < n; j += W) M = fmaxf(M, sp.pre_lse[row + j * step]);
+  for (int j = x; j < r.n; j += W) M = fmaxf(M, r.lse(sp, j));
 #pragma unroll
   for (int d = W / 2; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
   const int64_t ml = (int64_t)b * f.ml_st + (int64_t)h * f.ml_sh;
@@ -731,10 +747,11 @@ template <typename T, int D> __global__ __launch_bounds__(256) void shared_prefi
   const float top = fmaxf(M, m_old);
   float L = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < n; j++) {
-    const float w = exp2_diff(sp.pre_lse[row + j * step], top);
+#pragma unroll 4
+  for (int j = 0; j < r.n; j++) {
+    const float w = exp2_diff(r.lse(sp, j), top);
     L += w;
-    sum += *(const f32x4*)(sp.pre_o + (row + j * step) * D + 4 * x) * w;
+    sum += *(const f32x4*)(r.row(sp, j, D) + 4 * x) * w;
   }
   if (L == 0.f) return;
   const float w_old = l_old * exp2_diff(m_old, top);
@@ -839,6 +856,7 @@ template <typename T> __global__ __launch_bounds__(256) void shared_prefix_gathe
 
 // ------------------------------------------------------------------------------------------------ the host's side
 constexpr int64_t kPrefixWorkgroups = 2 * kCUs;  // at most
+constexpr int kPlanWorkgroups = 8;  // in front of a prompts' step (a multiple of the XCDs)
 constexpr int64_t kRounds = 3;  // pieces per workgroup, at most
 constexpr int64_t kOwnWaves = 4 * kCUs;
 static_assert(kRounds * kPrefixWorkgroups + kOwnWaves + 2 <= kMaxParts, "a row's partials have their weights in LDS");
@@ -878,13 +896,12 @@ Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, i
   p.rounds = rows * (hq / hkv) <= kRows ? 0 : p.tiles * 6 <= kPrefixWorkgroups / hkv ? 1 : kRounds;
   p.parts = p.shares + p.tiles > p.rounds * p.shares ? p.shares + p.tiles : p.rounds * p.shares;
   p.pre_floats = p.tiles ? hkv * p.parts * kRows * (d + 1) : 0;
-  p.own_shares = 1, p.own_floats = 0, p.plan_ints = 0;
+  p.own_shares = 1, p.own_floats = 0, p.plan_ints = kPlanInts * rows;
   if (decode) {
     const int64_t by_waves = kOwnWaves / tasks, by_units = (own_units + kOwnMinUnits - 1) / kOwnMinUnits;
     p.own_shares = by_waves < by_units ? by_waves : by_units;
     p.own_shares = p.own_shares < 1 ? 1 : p.own_shares;
     p.own_floats = ((p.own_shares + rows) * hq * (d + 1) + 3) / 4 * 4;
-    p.plan_ints = kPlanInts * rows;
   }
   return p;
 }
@@ -1006,7 +1023,7 @@ extern "C" size_t lsattn_shared_prefill_workspace_bytes(int64_t rows, int64_t nu
       max_prefix_len <= 0 || rows > 0x7fffff00 || num_groups > 65535 || num_q_heads > 65535 || max_prefix_len > 0x7fff0000)  // (as the launch refuses)
     return 0;
   if (gathers(rows, num_groups, num_q_heads, num_kv_heads)) return (size_t)prompt_bytes(num_groups, num_kv_heads, head_dim, max_prefix_len).all;
-  return (size_t)plan_of(rows, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, 0, false).pre_floats * 4;
+  return (size_t)plan_of(rows, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, 0, false).all();
 }
 
 extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* stream) {
@@ -1080,13 +1097,14 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
   if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups) return LSATTN_ERR_INVALID_ARG;  // (units are numbered with 31 bits)
   p.pre_o = (float*)a->workspace, p.pre_lse = p.pre_o + (pl.pre_floats / (a->head_dim + 1)) * a->head_dim;
   p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.rounds = (int32_t)pl.rounds, p.xcds_shift = (int32_t)pl.xcds_shift;
-  p.by_pre_shares = fast_div((uint32_t)pl.shares);
+  p.by_pre_shares = fast_div((uint32_t)pl.shares), p.by_hq = fast_div((uint32_t)w.hq);
+  p.plan = (int32_t*)(p.pre_o + pl.pre_floats), p.own_wgs = kPlanWorkgroups;
   FoldParams f;
   f.o = (char*)a->o, f.o_st = a->o_stride_t * 2, f.o_sh = a->o_stride_h * 2, f.m = a->m, f.l = a->l, f.ml_st = a->ml_stride_t, f.ml_sh = a->ml_stride_h;
   const unsigned fold_wgs = (unsigned)((a->rows * w.hq * (a->head_dim / 4) + 255) / 256);
   auto launch = [&](auto t, auto d) {
     constexpr int D = decltype(d)::value;
-    LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<decltype(t), D, false>), dim3((unsigned)(pl.shares * w.hkv)), dim3(256), 0, st, p);
+    LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<decltype(t), D, false>), dim3((unsigned)(p.own_wgs + pl.shares * w.hkv)), dim3(256), 0, st, p);
     if (hipPeekAtLastError() != hipSuccess) return;
     LSATTN_LAUNCH_KERNEL((shared_prefix_fold_kernel<decltype(t), D>), dim3(fold_wgs), dim3(256), 0, st, p, f);
   };
