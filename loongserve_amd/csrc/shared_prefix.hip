@@ -44,6 +44,7 @@ struct SharedParams {
   int32_t most;          // a bound of the prefixes: longer ones are cut there
   int32_t near;          // whether every row lies within 2 GB of its head's first, slots and strides of 24 bits
   int32_t shares, parts; // of the prefix part, per KV head; partials of 128 rows per KV head
+  int32_t ahead;         // whether the prefix part's waves come before those of the own tokens
   int32_t rounds;        // pieces that a workgroup takes at most (see Deal)
   int32_t xcds_shift;    // log2 of the XCDs that run a KV head's workgroups
   int32_t own_wgs;       // workgroups of the own tokens (prompts: of the plan), in front of those of the prefix part; a multiple of 8
@@ -243,6 +244,7 @@ template <typename T, int D, bool THROUGH> __device__ __forceinline__ void prefi
   const uint32_t k_s0 = (uint32_t)p.w.k_s0, v_s0 = (uint32_t)p.w.v_s0;
   const float scale = p.w.scale_log2;
 
+  if (p.ahead) __builtin_amdgcn_s_setprio(3);
   while (at < end) {
     while (!deal.cut && at >= first + gs.all_units()) {  // (at < deal.pieces: a later group has some)
       first += gs.all_units(), tiles_before += gs.all_tiles();
@@ -871,6 +873,7 @@ bool is_near(const PoolParams& w) {
 }
 struct Plan {
   int64_t tiles, shares, parts, rounds, xcds_shift;  // prefix part, per KV head
+  bool ahead;
   int64_t own_shares;
   int64_t pre_floats, own_floats, plan_ints;  // of the workspace
   int64_t all() const { return (pre_floats + own_floats + plan_ints) * 4; }
@@ -881,11 +884,16 @@ Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, i
   p.tiles = groups > 0 && max_prefix > 0 ? rows * (hq / hkv) / kRows + (groups < rows ? groups : rows) : 0;
   const int64_t units = p.tiles * ((max_prefix + kKeys - 1) / kKeys);
   const int64_t tasks = hkv * ((hq / hkv + kHeads - 1) / kHeads), own_units = decode ? rows * ((max_own + kBlock - 1) / kBlock) : 0;
-  // Two workgroups of the prefix part per CU, or one beside those of the own tokens, where these are as much work and the groups fill their row tiles: half the partials then, and the
-  // prefix's products beside the other part's loads.  Microseconds, two | one: 64 requests behind 16384 tokens, 32/8 heads, up to 1500 own tokens 87 | 77, 400 each 68 | 63, 100 each
-  // 51 | 52, none 44 | 47; 24 in three groups, 32/32, up to 700 own tokens (rows that fill a sixteenth of a tile: what counts is loads in flight) 105 | 113; 160 in two groups, 28/4
-  // heads of 64, up to 400 own tokens 80 | 97.
-  const bool beside = own_units * tasks >= units * hkv && rows * (hq / hkv) >= 64 * groups;
+  // The two parts of a decode step beside each other, where the groups fill their row tiles.  Blocks of own tokens and units of the prefix cost about the same, so their ratio says
+  // which part is the longer one (us; 32/8 heads of 128 if not said):
+  // * of 128-wide heads a SIMD holds two waves: one workgroup of each part per CU, not two of the prefix part, unless that has nearly all the work: 64 requests behind 16384 tokens, up to
+  //   1500 own tokens 79 | 68, 200 54 | 52; behind 24000, 200 own 64 | 66.  Of 64-wide ones it holds three: always two (160 in two groups, 28/4 heads, up to 800 own tokens 76 | 96).
+  //   Rows that do not fill a tile: what counts is loads in flight (24 in three groups, 32/32 heads, 105 | 113; 64 in four groups, up to 400 own tokens 80 | 94).
+  // * the prefix part's waves come first, as long as it is not much the shorter one: each of its matrix instructions waits for a turn among the other part's vector work, which waits for memory
+  //   all the same: 64 behind 16384 tokens, up to 1500 own 77 | 68; 160 in two groups, 28/4 of 64, up to 3000 own 95 | 89; but 64 behind 8192, up to 3000 own 88 | 93.
+  const bool full = decode && rows * (hq / hkv) >= kRows * groups;
+  const bool beside = full && d == 128 && own_units * tasks * 2 >= units * hkv;
+  p.ahead = full && own_units * tasks <= units * hkv * 6;
   p.shares = (beside ? kCUs : kPrefixWorkgroups) / hkv;
   p.shares = p.shares < 1 ? 1 : p.shares;
   p.shares = p.shares < units ? p.shares : units < 1 ? 1 : units;
@@ -982,7 +990,7 @@ extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* st
   p.g_start = a->g_start_loc, p.g_size = a->g_size, p.g_req = a->g_req_idx, p.g_prefix = a->g_prefix_len;
   p.groups = pl.tiles ? (int32_t)a->num_groups : 0;
   p.rows = w.batch, p.most = (int32_t)most, p.near = is_near(w);
-  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.rounds = (int32_t)pl.rounds, p.xcds_shift = (int32_t)pl.xcds_shift, p.own_wgs = (int32_t)(((pl.own_shares * w.tasks + 3) / 4 + 7) / 8 * 8);
+  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.rounds = (int32_t)pl.rounds, p.ahead = pl.ahead, p.xcds_shift = (int32_t)pl.xcds_shift, p.own_wgs = (int32_t)(((pl.own_shares * w.tasks + 3) / 4 + 7) / 8 * 8);
   p.by_hkv = fast_div((uint32_t)w.hkv), p.by_hq = fast_div((uint32_t)w.hq), p.by_group = fast_div((uint32_t)w.group), p.by_pre_shares = fast_div((uint32_t)pl.shares);
   hipStream_t st = (hipStream_t)stream;
   if (a->dtype == LSATTN_F16) {
@@ -1096,7 +1104,7 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
   const Plan pl = plan_of(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len, 0, false);
   if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups) return LSATTN_ERR_INVALID_ARG;  // (units are numbered with 31 bits)
   p.pre_o = (float*)a->workspace, p.pre_lse = p.pre_o + (pl.pre_floats / (a->head_dim + 1)) * a->head_dim;
-  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.rounds = (int32_t)pl.rounds, p.xcds_shift = (int32_t)pl.xcds_shift;
+  p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.rounds = (int32_t)pl.rounds, p.ahead = pl.ahead, p.xcds_shift = (int32_t)pl.xcds_shift;
   p.by_pre_shares = fast_div((uint32_t)pl.shares), p.by_hq = fast_div((uint32_t)w.hq);
   p.plan = (int32_t*)(p.pre_o + pl.pre_floats), p.own_wgs = kPlanWorkgroups;
   FoldParams f;
