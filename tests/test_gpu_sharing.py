@@ -245,6 +245,15 @@ def test_decode_many_groups_and_a_large_batch(lsa, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads, groups", [((64, 32, 64), [(2000, [1] * 150), (700, [0, 3] * 40)]), ((16, 2, 128), [(70, [9] * 17), (1300, [0, 40] * 20), (300, [2])]),
+                                           ((128, 64, 64), [(4500, [0] * 130)])])
+def test_decode_groups_of_several_row_tiles(lsa, heads, groups, dtype):
+    """Row tiles that go through their group's prefix side by side, groups of one and of several; few workgroups per KV head and many."""
+    _decode_check(lsa, _case(6, *heads, dtype, groups, [5, 900]), heads)
+
+
+@pytest.mark.gpu
 def test_decode_lists_that_say_strange_things(lsa):
     """Overlapping groups, groups past the batch, unknown rows, negative numbers, a prefix past its bound: each as documented, none reads out of range."""
     c = _case(5, 8, 2, 128, torch.float16, [(100, [3, 4, 5]), (70, [1, 2])], [6, 2])
