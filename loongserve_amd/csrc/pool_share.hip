@@ -63,17 +63,21 @@ struct RowsParams {
   int32_t pieces, lanes_shift;        // pieces of a row; log2 of the lanes that take one
   int32_t num_slots;
 };
-// `row_of(i, src, dst)`: the slots of the workgroup's row i, false if it has none.
-template <typename Piece, int ROWS, typename F> __device__ __forceinline__ void move_rows(const RowsParams& p, int layer, F row_of) {
+// `row_of(i, src, dst)`: the slots of the workgroup's row i (dst: -1 where a target has none), false if it has none.
+template <typename Piece, int ROWS, int TARGETS, typename F> __device__ __forceinline__ void move_rows(const RowsParams& p, int layer, F row_of) {
   const int lanes = 1 << p.lanes_shift, sub = threadIdx.x & (lanes - 1);
   char* const base = p.rows + layer * p.layer_stride;
   for (int i = threadIdx.x >> p.lanes_shift; i < ROWS; i += kThreads >> p.lanes_shift) {
-    int src, dst;
+    int src, dst[TARGETS];
     if (!row_of(i, src, dst)) continue;
     const Piece* from = (const Piece*)(base + (int64_t)src * p.slot_stride);
-    Piece* to = (Piece*)(base + (int64_t)dst * p.slot_stride);
 #pragma unroll 4
-    for (int x = sub; x < p.pieces; x += lanes) to[x] = from[x];
+    for (int x = sub; x < p.pieces; x += lanes) {
+      const Piece v = from[x];
+#pragma unroll
+      for (int t = 0; t < TARGETS; t++)
+        if (dst[t] >= 0) ((Piece*)(base + (int64_t)dst[t] * p.slot_stride))[x] = v;
+    }
   }
 }
 
@@ -85,29 +89,60 @@ struct CopyParams {
   int64_t num_index;
 };
 constexpr int kCopyRows = 16;
-// grid (positions, forks, layers)
-__global__ __launch_bounds__(kThreads) void fork_copy_kernel(CopyParams p) {
-  const int i = blockIdx.y, pos0 = (int)blockIdx.x * kCopyRows, len = fork_len(p.f, i);
-  if (pos0 >= len) return;
-  const int32_t* const src_row = p.f.table + (int64_t)p.f.src[i] * p.f.max_seq_len;
-  const int64_t start = p.start[i];
-  auto target = [&](int pos) -> int {  // the slot of a position, -1 if there is none
-    const int64_t at = start + pos;
-    const int64_t d = pos < len && at >= 0 && at < p.num_index ? p.index[at] : -1;
+// grid (positions, forks, layers).  FORKS of one source that stand next to each other read it together where there are more than a few (us, alone | four together, 32 layers of 8 heads: 8 copies of 2000 tokens
+// 677 | 502, of 300 114 | 92, 4 of 2000 336 | 281; but 4 of 300 61 | 65, 8 of 20 11 | 23, where a workgroup's chain of loads and stores counts, and 2 of 6500 526 | 535).
+constexpr int kCopyTogether = 4;
+constexpr int64_t kTogetherFromTokens = 2048;
+template <int FORKS> __global__ __launch_bounds__(kThreads) void fork_copy_kernel(CopyParams p) {
+  const int i = blockIdx.y, pos0 = (int)blockIdx.x * kCopyRows;
+  [[maybe_unused]] const int lane = threadIdx.x & 63;
+  const int req = p.f.src[i];
+  if constexpr (FORKS > 1) {
+    int in_run = 0;  // the forks of the source right in front of this one
+    for (int k1 = i; k1 > 0; k1 -= 64) {
+      const int k = k1 - 1 - lane;
+      const uint64_t ends = __builtin_amdgcn_ballot_w64(k < 0 || p.f.src[k] != req);
+      in_run += ends ? __builtin_ctzll(ends) : 64;
+      if (ends) break;
+    }
+    if (in_run % FORKS) return;
+  }
+  int len[FORKS], most = 0;
+  int64_t start[FORKS];
+#pragma unroll
+  for (int f = 0; f < FORKS; f++) {
+    const bool with = i + f < p.f.n && (f == 0 || (len[f - 1] >= 0 && p.f.src[i + f] == req));
+    len[f] = with ? fork_len(p.f, i + f) : -1;
+    len[f] = with && len[f] < 0 ? 0 : len[f];
+    start[f] = with ? p.start[i + f] : 0;
+    most = len[f] > most ? len[f] : most;
+  }
+  if (pos0 >= most) return;
+  const int32_t* const src_row = p.f.table + (int64_t)req * p.f.max_seq_len;
+  auto target = [&](int64_t first, int n, int pos) -> int {  // the slot of a position, -1 if there is none
+    const int64_t at = first + pos;
+    const int64_t d = pos < n && at >= 0 && at < p.num_index ? p.index[at] : -1;
     return d >= 0 && d < p.r.num_slots ? (int)d : -1;
   };
   if (blockIdx.z == 0 && threadIdx.x < kCopyRows) {
-    const int d = target(pos0 + threadIdx.x);
-    if (d >= 0) p.f.table[(int64_t)p.f.dst[i] * p.f.max_seq_len + pos0 + threadIdx.x] = d;
+    const int pos = pos0 + threadIdx.x;
+#pragma unroll
+    for (int f = 0; f < FORKS; f++) {
+      const int d = target(start[f], len[f], pos);
+      if (d >= 0) p.f.table[(int64_t)p.f.dst[i + f] * p.f.max_seq_len + pos] = d;
+    }
   }
-  auto copy = [&](int k, int& src, int& dst) {
-    if (pos0 + k >= len) return false;
-    src = src_row[pos0 + k];
-    dst = target(pos0 + k);
-    return dst >= 0 && (uint32_t)src < (uint32_t)p.r.num_slots;
+  auto row_of = [&](int k, int& src, int (&dst)[FORKS]) {
+    const int pos = pos0 + k;
+    if (pos >= most) return false;
+    src = src_row[pos];
+    if ((uint32_t)src >= (uint32_t)p.r.num_slots) return false;
+#pragma unroll
+    for (int f = 0; f < FORKS; f++) dst[f] = target(start[f], len[f], pos);
+    return true;
   };
-  move_rows<u32x4, kCopyRows>(p.r, blockIdx.z, copy);
-  if (p.scales.rows) move_rows<uint8_t, kCopyRows>(p.scales, blockIdx.z, copy);
+  move_rows<u32x4, kCopyRows, FORKS>(p.r, blockIdx.z, row_of);
+  if (p.scales.rows) move_rows<uint8_t, kCopyRows, FORKS>(p.scales, blockIdx.z, row_of);
 }
 
 // ------------------------------------------------------------------------------------------------ release
@@ -372,13 +407,13 @@ __global__ __launch_bounds__(kThreads) void compact_move_kernel(CompactParams p)
         p.state[src] = 0;
         p.remap[src] = dst;
       }
-      auto move = [&](int k, int& src, int& dst) {
+      auto move = [&](int k, int& src, int (&dst)[1]) {
         if (m0 + k >= moves) return false;
-        src = p.source[m0 + k], dst = p.hole[m0 + k];
+        src = p.source[m0 + k], dst[0] = p.hole[m0 + k];
         return true;
       };
-      if (p.layers) move_rows<u32x4, kMoveRows>(p.r, layer, move);
-      if (p.scales.rows) move_rows<uint8_t, kMoveRows>(p.scales, layer, move);
+      if (p.layers) move_rows<u32x4, kMoveRows, 1>(p.r, layer, move);
+      if (p.scales.rows) move_rows<uint8_t, kMoveRows, 1>(p.scales, layer, move);
     }
     return;
   }
@@ -448,7 +483,8 @@ extern "C" int lsattn_copy_requests(const lsattn_copy_requests_args* a, const ls
   hipStream_t st = (hipStream_t)stream;
   set_rows(p.r, rows->rows, rows->layer_stride_bytes, rows->slot_stride_bytes, rows->row_bytes / 16, rows->num_slots);
   if (rows->scales) set_rows(p.scales, rows->scales, rows->scale_layer_stride_bytes, rows->scale_slot_stride_bytes, rows->scale_bytes, rows->num_slots);
-  LSATTN_LAUNCH_KERNEL(fork_copy_kernel, grid, dim3(kThreads), 0, st, p);
+  if (a->n >= kCopyTogether && a->n * most >= kTogetherFromTokens) LSATTN_LAUNCH_KERNEL(fork_copy_kernel<kCopyTogether>, grid, dim3(kThreads), 0, st, p);
+  else LSATTN_LAUNCH_KERNEL(fork_copy_kernel<1>, grid, dim3(kThreads), 0, st, p);
   return check_launch();
 }
 

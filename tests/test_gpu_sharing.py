@@ -659,6 +659,42 @@ def test_copies_bit_for_bit(lsa, layers, heads, D, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, F8])
+def test_copies_of_a_source_side_by_side(lsa, dtype):
+    """Runs of forks of one source, one of more than 64, with lengths that rise and fall in them, sources and destinations that do not exist between them."""
+    g = torch.Generator().manual_seed(9)
+    layers, slots, width, n = 2, 9000, 130, 93
+    pool = _raw_pool(g, layers, slots, 2, 32, dtype)
+    scales = torch.randint(0, 256, (layers, slots, 2), dtype=torch.uint8, generator=g) if dtype == F8 else None
+    src = [3] * 7 + [1] + [3] * 3 + [-1, 200] + [5] * 71 + [1] * 8 + [3]
+    assert len(src) == n
+    dst = list(range(10, 10 + n))
+    dst[2], dst[40] = -7, 10 ** 6
+    lens = torch.randint(0, width + 20, (n,), generator=g).tolist()
+    lens[1], lens[50] = 0, -3
+    table = torch.full((10 + n, width), PAD, dtype=torch.int32)
+    table[:10] = torch.randint(0, 500, (10, width), generator=g).to(torch.int32)
+    table[5, 7], table[3, 129] = -2, slots
+    start = torch.tensor([0] + [max(0, min(x, width)) for x in lens]).cumsum(0)[:-1].tolist()
+    index = torch.randperm(slots - 500, generator=g)[:start[-1] + width] + 500
+    index[start[20]] = slots + 1
+    want, want_t, want_sc = pool.view(torch.uint8).clone(), table.clone(), None if scales is None else scales.clone()
+    for a, b, m, s in zip(src, dst, lens, start):
+        if 0 <= a < 10 + n and 0 <= b < 10 + n:
+            for i in range(min(m, width)):
+                old, new = int(table[a, i]), int(index[s + i])
+                if new < slots:
+                    want_t[b, i] = new
+                    if 0 <= old < slots:
+                        want[:, new] = pool.view(torch.uint8)[:, old]
+                        if scales is not None:
+                            want_sc[:, new] = scales[:, old]
+    p, t, sc = pool.to(DEV), table.to(DEV), None if scales is None else scales.to(DEV)
+    lsa.copy_requests(t, _i32(src), _i32(dst), _i32(lens), _i32(start), width, index.to(DEV), p, sc)
+    assert torch.equal(p.view(torch.uint8).cpu(), want) and torch.equal(t.cpu(), want_t) and (sc is None or torch.equal(sc.cpu(), want_sc))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("size", [1, 5, 300, 4096, 4097, 20000])
 @pytest.mark.parametrize("share", [0.0, 0.03, 0.5, 0.97, 1.0])
 @pytest.mark.parametrize("layers, heads, D, dtype", POOLS[:3])
