@@ -707,7 +707,10 @@ __global__ __launch_bounds__(256) void shared_decode_merge_rows_kernel(SharedPar
     L += weight;
     const int n = m.n - i1 < 64 ? m.n - i1 : 64;
 #pragma unroll 4
-    for (int i = slice; i < n; i += SL) sum += *(const f32x4*)(m.row(sp, i1 + i, D) + d) * __shfl(weight, i, 64);
+    for (int i0 = 0; i0 < n; i0 += SL) {  // (by the whole wave: a lane that has left the loop would hand out no weight)
+      const float w = __shfl(weight, i0 + slice, 64);
+      if (i0 + slice < n) sum += *(const f32x4*)(m.row(sp, i1 + i0 + slice, D) + d) * w;
+    }
   }
 #pragma unroll
   for (int x = 32; x > 0; x >>= 1) {

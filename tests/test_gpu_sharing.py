@@ -247,10 +247,20 @@ def test_decode_many_groups_and_a_large_batch(lsa, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("heads, groups", [((64, 32, 64), [(2000, [1] * 150), (700, [0, 3] * 40)]), ((16, 2, 128), [(70, [9] * 17), (1300, [0, 40] * 20), (300, [2])]),
-                                           ((128, 64, 64), [(4500, [0] * 130)])])
+                                           ((128, 64, 64), [(1000, [0] * 130)])])
 def test_decode_groups_of_several_row_tiles(lsa, heads, groups, dtype):
     """Row tiles that go through their group's prefix side by side, groups of one and of several; few workgroups per KV head and many."""
     _decode_check(lsa, _case(6, *heads, dtype, groups, [5, 900]), heads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(32, 4, 64), (32, 8, 128), (128, 128, 128)])
+def test_decode_large_batches(lsa, heads):
+    """Rows enough to be joined by a wave each: from one partial to more than a wave has lanes, none among them."""
+    groups = [(5, [0] * 3), (900, [3, 200, 0] * 8), (64, [33] * 50), (2500, [1] * 40)] if heads[0] < 100 else [(70, [1, 0, 500]), (1100, [2] * 20), (1, [0] * 12)]
+    c = _case(8, *heads, torch.float16, groups, [0, 2100, 1] + [9] * 9)
+    assert len(c["q"]) * heads[0] >= 4096
+    _decode_check(lsa, c, heads)
 
 
 @pytest.mark.gpu
