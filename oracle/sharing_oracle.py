@@ -111,16 +111,17 @@ def release(table, req, lens, most, state):
 def compact(state, table, req, lens, most):
     """(state, table, remap, sources, holes)"""
     state, table = state.clone(), table.clone()
-    used = [i for i in range(len(state)) if state[i] != 0]
+    values = state.tolist()
+    used = [i for i, n in enumerate(values) if n != 0]
     U = len(used)
     source = [i for i in used if i >= U]
-    hole = [i for i in range(U) if state[i] == 0]
+    hole = [i for i in range(U) if values[i] == 0]
     remap = torch.full((len(state),), -1, dtype=torch.int32)
-    for i in used:
-        remap[i] = i
+    remap[used] = torch.tensor(used, dtype=torch.int32)
     for a, b in zip(source, hole):
-        remap[a] = b
-        state[b], state[a] = state[a].clone(), 0
+        values[b], values[a] = values[a], 0
+    remap[source] = torch.tensor(hole, dtype=torch.int32)[:len(source)]
+    state = torch.tensor(values, dtype=torch.int32)
     for r, n in zip(req, lens):
         for i in range(min(n, most, table.shape[1])):
             s = int(table[r, i])

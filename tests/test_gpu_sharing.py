@@ -247,7 +247,7 @@ def test_decode_many_groups_and_a_large_batch(lsa, dtype):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("heads, groups", [((64, 32, 64), [(2000, [1] * 150), (700, [0, 3] * 40)]), ((16, 2, 128), [(70, [9] * 17), (1300, [0, 40] * 20), (300, [2])]),
-                                           ((128, 64, 64), [(1000, [0] * 130)])])
+                                           ((128, 64, 64), [(1000, [0] * 130)]), ((32, 4, 64), [(60 + 37 * i, [i % 3] * (15 + i)) for i in range(12)])])
 def test_decode_groups_of_several_row_tiles(lsa, heads, groups, dtype):
     """Row tiles that go through their group's prefix side by side, groups of one and of several; few workgroups per KV head and many."""
     _decode_check(lsa, _case(6, *heads, dtype, groups, [5, 900]), heads)
@@ -408,6 +408,7 @@ PROMPTS = {
     "none-in-one": [(70, 0), (129, 33), (0, 5)],
     "many": [(300, 700), (129, 500)],
     "many-one": [(1, 1500)],
+    "twelve": [(40 + 61 * i, 5 + 29 * i) for i in range(12)],
     "prefill-kernel": [(70, 9000), (65, 5100)],
 }
 # rows and heads that hand the laid-out prefix to the prefill kernel (rows x heads of 98304 and more, a row per group and head of 512 and more)
@@ -740,6 +741,14 @@ def test_compaction_against_lists(lsa, size, share, layers, heads, D, dtype):
     n = int((state != 0).sum())
     assert torch.equal(again.cpu()[:n], torch.arange(n, dtype=torch.int32)) and bool((again.cpu()[n:] == -1).all())
     assert torch.equal(st.cpu(), want_s) and torch.equal(p.view(torch.uint8).cpu(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [65536, 65537, 200001])
+@pytest.mark.parametrize("share", [0.002, 0.6, 1.0])
+def test_compaction_of_a_large_pool(lsa, size, share):
+    """Pools whose counts come from a launch of their own, and the largest whose do not."""
+    test_compaction_against_lists(lsa, size, share, 1, 2, 64, F8)
 
 
 @pytest.mark.gpu
