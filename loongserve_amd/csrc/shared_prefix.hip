@@ -8,8 +8,8 @@
 //
 // Prefix part: a workgroup of four waves owns 128 rows of one KV head (a wave 32, as rows come: token by token, the query heads of the KV head side by side,
 // whatever their number) and walks tiles of 64 keys of a share of the prefix:
-//   * the work of all groups, (row tile, block of 64 keys) pairs, is dealt in equal shares to the workgroups of a KV head, whatever the groups' sizes and prefixes
-//     are (the host does not know them); a workgroup leaves one fp32 partial per row tile it touches;
+//   * the work of all groups, (row tile, block of 64 keys) pairs, is dealt to the workgroups of a KV head on the device, whatever the groups' sizes and prefixes are (the host
+//     does not know them): in equal shares, or in pieces that the row tiles of a group go through side by side (Deal); a workgroup leaves one fp32 partial per row tile it touches;
 //   * K and V rows lie where the request table says.  Direct loads to LDS take an address per lane, so gathering them costs a multiplication per load; two stages,
 //     16-byte chunks XORed with the row (prefill_small.hip says why); the slots of the tile after next are under way;
 //   * the order of the keys in a tile does not matter without a causal mask: rows lie so that a lane's slots are neighbours in the table;
@@ -19,6 +19,17 @@
 //   * the running maximum is raised where a lane's eight weights pass 2^15, and then set so that the largest is 2^9.
 // Own tokens: the decode walk of pool_walk.hip.h from the prefix's end on, in the same launch (those workgroups wait for memory where the others keep the matrix
 // pipe busy), equal shares of all requests' own tokens.  A second launch joins a request's partials.
+//
+// What bounds it, with the case that shows it (launches alone, without the one that joins):
+//   * few rows per group: HBM reads.  24 requests in three groups and alone, 32/32 heads, 449 MB: 92 us, 4.9 TB/s;
+//   * prefix and own tokens together: 64 requests behind 16384 tokens, 32/8 heads, up to 1500 own: 60 us (284 MB, 4.8 TB/s; the parts alone 35 and 42 us);
+//   * many rows, 64-wide bfloat16: vector work, then the matrix pipe, which runs beside it only in part (busy 54% and 30%): 160 requests in two groups, 28/4 heads: 67 us, 0.4 PFLOP/s of the
+//     formula, a half more with the second part of P;
+//   * many rows, 128-wide fp16: the products (0.9 PFLOP/s of whole row tiles as the prefix grows, 1.14 where nothing has to be loaded, 1.17 a large library product), and 17 us of start and end: prompts of
+//     293 rows behind 6001 tokens 50 us, of which 6 are 28 MB of partials that all workgroups store at once.
+// Tried and left out (128-wide heads, all 0.70 to 0.75 PFLOP/s before the tiles went side by side, as this form): four stages of 32 keys; operands read a step ahead, or all at once (decode 5 to
+// 8% slower); eight waves of 256 rows in alternating phases (no room beside it for the own tokens); lines fetched into the L2 ahead (5%, few rows 30% slower); three and four waves per SIMD of
+// the 64-wide form (equal, and slower for spills); sums and exponentials in independent batches (equal).
 #include <type_traits>
 
 #include "pool_walk.hip.h"
@@ -98,9 +109,10 @@ struct Groups {
 };
 // How the units are dealt to the workgroups of a KV head.
 // A row tile reads all of its group's prefix, so the tiles of a group read the same rows, and where they do it at different times and the prefix is longer than an L2, each of
-// them reads it from memory again (1280 rows of 32/8 heads behind 24000 tokens: 90% of the requests missed, 160 us).  So where a group has more than one tile and it comes out even, the prefixes are cut
-// into pieces of `cut` blocks for every tile of the group, the tiles side by side, and a workgroup takes a piece (or one of each round): the tiles of a group then go
-// through a piece in step on one XCD, which reads it once.
+// them reads it from memory again (293 rows of 32/8 heads behind 24000 tokens: 90% of the L2's requests missed).  So where a group has more than one tile and it comes out even,
+// the prefixes are cut into pieces of `cut` blocks for every tile of the group, the tiles of a piece side by side, and a workgroup takes a piece (or one of each round): the tiles go
+// through it in step on one XCD, which reads it once (12% missed; us, without | with, both launches: 293 rows behind 1000 tokens 45 | 41, 6001 70 | 63, 20000 147 | 139; 150 behind 6001 54 | 46).
+// "Even": no more than an eighth longer than equal shares, a piece's start and end counted (600 rows behind 6001 in three rounds of short pieces: 97 | 114).
 // Else, in order of tiles and their blocks, `per` units each.
 constexpr int kPieceCost = 4;  // blocks that a piece's start and its partials cost
 struct Deal {
@@ -346,8 +358,8 @@ template <typename T, int D, bool THROUGH> __device__ __forceinline__ void prefi
           }
         }
       };
-      // (rows that one row tile reads are read once: nontemporal, 24 requests of 32/32 heads 105 -> 99 us; of a group of several tiles they come from the L2 for the others, and so 64 requests behind
-      // 32768 tokens take 77 us instead of 70)
+      // (rows that one row tile reads are read once: nontemporal, 24 requests of 32/32 heads 105 -> 97 us; of a group of several tiles they come from the L2 for the others: 64 requests behind 32768
+      // tokens 70 us, 77 with nontemporal loads)
       if (tiles == 1) send(std::true_type{});
       else send(std::false_type{});
     };
@@ -1009,8 +1021,8 @@ extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* st
 namespace lsattn {
 namespace {
 // The prompts' step takes its rows itself where they are few, and hands contiguous K/V to the prefill kernel where its workgroups of 256 rows are a round and a half
-// of the CUs and more. Microseconds, own kernel | prefill kernel (f16, 32/8 heads of 128, with the fills of m and l): prefix 6001 tokens: 293 rows 70 | 120, 600 100 | 120, 1200 167 | 211, 2500
-// 314 | 341, 5000 594 | 518; 20000 tokens: 1200 484 | 564, 2500 980 | 954, 5000 1907 | 1448; five groups of 1200 rows behind 3000 435 | 331; 8/1 heads, 1200 rows behind 6001 76 | 112.
+// of the CUs and more. Microseconds, own kernel | prefill kernel (f16, 32/8 heads of 128, with the fills of m and l): prefix 6001 tokens: 293 rows 62 | 120, 600 97 | 120, 1200 161 | 211, 2500
+// 301 | 341, 5000 594 | 518; 20000 tokens: 1200 455 | 564, 2500 965 | 954, 5000 1907 | 1448; five groups of 1200 rows behind 3000 435 | 331; 8/1 heads, 1200 rows behind 6001 76 | 112.
 // Where a prefix has few rows of its own, laying it out costs more than it saves: 8192 rows behind 2000 tokens each, 32/8 heads, 32 groups 455 | 406, 64 591 | 538, 128 633 | 827;
 // 32/32 heads, 16 groups 591 | 538, 32 596 | 827.
 constexpr int64_t kGatherFromRows = kCUs * 3 / 2 * 256, kGatherFromGroupRows = 512;
