@@ -209,9 +209,10 @@ __global__ __launch_bounds__(kThreads) void release_kernel(ReleaseParams p) {
 // Many requests: a lane has a request, a wave 64 of them and kRun positions.  Requests that share tokens share them at the same positions, so lanes that name one slot there are counted and the
 // first of them makes one change: an atomic on a slot that lies anywhere costs a transaction of its own, and a search's branches name most slots many times (128 requests, 560000 tokens
 // on 69000 slots: 20.5 us with an atomic each, 11.4 so; a wave of sixteen positions, one atomic behind the other, 26).  Two lanes in a row that are alone with their slots end the counting:
-// behind the shared part everybody is.  With 23 requests of one parent's 3000 tokens a thread per token takes 18.6 us a call, with 24 a lane per request 20.5: about equal, and from there on it gains.
+// behind the shared part everybody is.  A call, a thread per token | a lane per request, us: forks of one parent's 3000 tokens, 24 21.0 | 21.2, 32 21.2 | 20.6, 64 25 | 21, 256 46 | 30; of eight
+// parents of 300 to 8000, 24 22.2 | 23.1, 128 37 | 26; requests that share nothing (1000 tokens each) 64 20.0 | 21.1, 256 28.0 | 28.3.
 constexpr int kRun = 4;
-constexpr int64_t kColumnsFromRequests = 24;
+constexpr int64_t kColumnsFromRequests = 32;
 __global__ __launch_bounds__(kThreads) void release_columns_kernel(ReleaseParams p) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = blockIdx.y * 64 + lane;
   const int pos0 = ((int)blockIdx.x * (kThreads / 64) + wave) * kRun;
