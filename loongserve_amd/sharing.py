@@ -70,7 +70,7 @@ def longserve_shared_prefix_decode_attention(q: torch.Tensor, req_to_token_index
 
     out: q's type unless given (float16, bfloat16 or float32).  Over the prefixes a request's weights are rounded to V's type, for bfloat16 in two
     parts, and o is divided by the sum of the rounded ones; the log-sum-exp is float32's.  max_len_in_batch, or max_own_len (a bound of the
-    tokens behind the prefix) where given, only sizes the launch.  workspace: the caller's scratch
+    tokens behind the prefix) where given, only sizes the launch and weighs its two parts (a close bound helps).  workspace: the caller's scratch
     (shared_prefix_decode_workspace_bytes; else torch allocates it), one for each call that may run at the same time, graphs' replays among them."""
     own = max_len_in_batch if max_own_len is None else max_own_len
     done = _native.shared_decode(q, req_to_token_indexs, b_req_idx, b_seq_len, cache_k, cache_v, g_start_loc, g_size, g_req_idx, g_prefix_len,
