@@ -494,7 +494,9 @@ extern "C" int lsattn_copy_requests(const lsattn_copy_requests_args* a, const ls
 
 extern "C" size_t lsattn_release_workspace_bytes(int64_t n, int64_t max_len_in_batch) {
   if (n <= 0 || max_len_in_batch <= 0 || n > 65535 || max_len_in_batch > 0x7fff0000 || n * max_len_in_batch <= kOneGroupTokens) return 0;
-  return (size_t)(release_groups(n, max_len_in_batch).all() * 8);
+  // (enough for fewer requests, too, which may be more workgroups)
+  const int64_t all = release_groups(n, max_len_in_batch).all(), fewer = n < kColumnsFromRequests ? 0 : release_groups(kColumnsFromRequests - 1, max_len_in_batch).all();
+  return (size_t)((all > fewer ? all : fewer) * 8);
 }
 
 extern "C" int lsattn_release_requests(const int32_t* req_to_tokens, int64_t num_reqs, int64_t max_seq_len, const int32_t* b_req_idx, const int32_t* b_seq_len, int64_t n,
