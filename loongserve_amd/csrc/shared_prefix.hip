@@ -649,69 +649,31 @@ struct MergeRow {
     return i < n_pre ? sp.pre_o + (pre_row + (int64_t)i * pre_step) * d : sp.w.part_o + (own_row + (int64_t)(i - n_pre) * sp.w.hq) * d;
   }
 };
-// o = sum of a row's partials by their log-sum-exps.  First the weights of all of them, by all threads, into LDS,
-// then the rows, whose loads wait for nothing.
-constexpr int kMaxParts = 2600;  // of a row: see where the launches are planned
-template <int D>
-__global__ __launch_bounds__(256) void shared_decode_merge_kernel(SharedParams sp) {
-  constexpr int W = D / 4, SL = 256 / W;
-  const PoolParams& p = sp.w;
-  __shared__ __attribute__((aligned(16))) float acc[SL][W * 4];
-  __shared__ float weight[kMaxParts], red[8];
-  const int h = blockIdx.x, b = blockIdx.y;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const MergeRow m(sp, b, h);
-  const int n = m.n;
-  float M = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const float x = m.lse(sp, i);
-    weight[i] = x;
-    M = fmaxf(M, x);
-  }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
-  if (lane == 0) red[wave] = M;
-  __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  float L = 0.f;
-  for (int i = threadIdx.x; i < n; i += 256) {
-    const float w = exp2_diff(weight[i], M);  // (NaN stays NaN)
-    weight[i] = w;
-    L += w;
-  }
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) L += __shfl_xor(L, d, 64);
-  if (lane == 0) red[4 + wave] = L;
-  __syncthreads();
-  L = (red[4] + red[5]) + (red[6] + red[7]);
-  const int slice = threadIdx.x / W, d = (threadIdx.x & (W - 1)) * 4;
-  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-  for (int i = slice; i < n; i += SL) sum += *(const f32x4*)(m.row(sp, i, D) + d) * weight[i];
-  *(f32x4*)&acc[slice][d] = sum;
-  __syncthreads();
-  if (slice) return;
-#pragma unroll
-  for (int i = 1; i < SL; i++) sum += *(const f32x4*)&acc[i][d];
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  const int64_t at = (int64_t)b * p.hq + h;
-  store_elem4(p.o, p.o_dtype, at * D + d, sum * inv);
-  if (d == 0) p.lse[at] = ln_of(M, L);
+// Maximum and sum over the wave, in every lane: within rows of 16 lanes by DPP, then of the four rows.
+__device__ __forceinline__ float of_row(float v, int row) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 16 * row)); }
+__device__ __forceinline__ float wave_max(float v) {
+  v = fmaxf(v, dpp_mov<0xB1>(v)), v = fmaxf(v, dpp_mov<0x4E>(v)), v = fmaxf(v, dpp_mov<0x141>(v)), v = fmaxf(v, dpp_mov<0x140>(v));
+  return fmaxf(fmaxf(of_row(v, 0), of_row(v, 1)), fmaxf(of_row(v, 2), of_row(v, 3)));
 }
-
-// As above with a wave per row, where there are enough of them: no barriers, 64 weights at a time in the wave's lanes.
-template <int D>
-__global__ __launch_bounds__(256) void shared_decode_merge_rows_kernel(SharedParams sp) {
-  constexpr int W = D / 4, SL = 64 / W;
+__device__ __forceinline__ float wave_sum(float v) {
+  v = sum_row16(v);
+  return (of_row(v, 0) + of_row(v, 1)) + (of_row(v, 2) + of_row(v, 3));
+}
+// o = sum of a row's partials by their log-sum-exps, by WAVES waves a row: each of them finds all weights for itself, 64 at a time in its lanes, so that its rows' loads wait for no other, and
+// takes every WAVES-th of the partials.
+template <int D, int WAVES>
+__global__ __launch_bounds__(256) void shared_decode_merge_kernel(SharedParams sp) {
+  constexpr int W = D / 4, SL = 64 / W, kLoads = WAVES > 1 ? 4 : 8;
   const PoolParams& p = sp.w;
-  const int lane = threadIdx.x & 63, i0 = (int)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ __attribute__((aligned(16))) float acc[WAVES > 1 ? WAVES - 1 : 1][D];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave & (WAVES - 1);
+  const int i0 = (int)blockIdx.x * (4 / WAVES) + wave / WAVES;
   const int b = (int)div_by((uint32_t)i0, sp.by_hq), h = i0 - b * p.hq;
-  if (b >= p.batch) return;
+  if (b >= p.batch) return;  // (WAVES of 4: every workgroup has a row)
   const MergeRow m(sp, b, h);
   float M = -INFINITY;
   for (int i = lane; i < m.n; i += 64) M = fmaxf(M, m.lse(sp, i));
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
+  M = wave_max(M);
   float L = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
   const int slice = lane / W, d = (lane & (W - 1)) * 4;
@@ -719,19 +681,32 @@ __global__ __launch_bounds__(256) void shared_decode_merge_rows_kernel(SharedPar
     const float weight = i1 + lane < m.n ? exp2_diff(m.lse(sp, i1 + lane), M) : 0.f;  // (NaN stays NaN)
     L += weight;
     const int n = m.n - i1 < 64 ? m.n - i1 : 64;
-#pragma unroll 4
-    for (int i0 = 0; i0 < n; i0 += SL) {  // (by the whole wave: a lane that has left the loop would hand out no weight)
-      const float w = __shfl(weight, i0 + slice, 64);
-      if (i0 + slice < n) sum += *(const f32x4*)(m.row(sp, i1 + i0 + slice, D) + d) * w;
+    for (int k0 = part * SL; k0 < n; k0 += kLoads * WAVES * SL) {  // (by the whole wave: a lane that has left the loop would hand out no weight)
+      f32x4 x[kLoads];
+#pragma unroll
+      for (int u = 0; u < kLoads; u++) {
+        const int k = k0 + u * WAVES * SL + slice;
+        x[u] = *(const f32x4*)(m.row(sp, i1 + (k < n ? k : n - 1), D) + d);
+      }
+#pragma unroll
+      for (int u = 0; u < kLoads; u++) {
+        const int k = k0 + u * WAVES * SL + slice;
+        const float w = __shfl(weight, k & 63, 64);
+        if (k < n) sum += x[u] * w;
+      }
     }
   }
+  L = wave_sum(L);
 #pragma unroll
-  for (int x = 32; x > 0; x >>= 1) {
-    L += __shfl_xor(L, x, 64);
-    if (x >= W) {
+  for (int x = 32; x >= W; x >>= 1)
 #pragma unroll
-      for (int e = 0; e < 4; e++) sum[e] += __shfl_xor(sum[e], x, 64);
-    }
+    for (int e = 0; e < 4; e++) sum[e] += __shfl_xor(sum[e], x, 64);
+  if constexpr (WAVES > 1) {
+    if (part && slice == 0) *(f32x4*)&acc[part - 1][d] = sum;
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int k = 0; k < WAVES - 1; k++) sum += *(const f32x4*)&acc[k][d];
   }
   if (slice) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
@@ -877,7 +852,6 @@ constexpr int64_t kPrefixWorkgroups = 2 * kCUs;  // at most
 constexpr int kPlanWorkgroups = 8;  // in front of a prompts' step (a multiple of the XCDs)
 constexpr int64_t kRounds = 3;  // pieces per workgroup, at most
 constexpr int64_t kOwnWaves = 4 * kCUs;
-static_assert(kRounds * kPrefixWorkgroups + kOwnWaves + 2 <= kMaxParts, "a row's partials have their weights in LDS");
 constexpr int64_t kOwnMinUnits = 2;
 
 // a bound of the prefixes that a table can hold
@@ -930,16 +904,16 @@ Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, i
   return p;
 }
 
-// Rows of a launch from which the one that joins them has a wave per row instead of a workgroup (us, workgroup | wave): 32 heads of 128, 32 requests 6.2 | 10.3, 64 6.5 | 7.5, 160 10.0 | 7.3;
-// 28 heads of 64, 64 requests 5.6 | 7.2, 160 9.6 | 6.5.
+// Rows from which the launch that joins them has a wave per row instead of four (us, four | one): 32 heads of 128, 4 requests 3.9 | 5.4, 32 6.5 | 5.8, 64 6.5 | 6.7, 160 12.5 | 7.0; 28 heads of
+// 64, 16 requests 4.9 | 6.1, 64 5.8 | 5.8, 160 10.7 | 6.6.
 constexpr int64_t kMergeByWaves = 4096;
 template <typename T, int D> void launch_decode(const SharedParams& p, hipStream_t st) {
   const int64_t prefix = p.groups ? (int64_t)p.shares * p.w.hkv : 0;
   LSATTN_LAUNCH_KERNEL((shared_prefix_kernel<T, D, true>), dim3((unsigned)(p.own_wgs + prefix)), dim3(256), 0, st, p);
   if (hipPeekAtLastError() != hipSuccess) return;
   const int64_t rows = (int64_t)p.w.batch * p.w.hq;
-  if (rows >= kMergeByWaves) LSATTN_LAUNCH_KERNEL((shared_decode_merge_rows_kernel<D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
-  else LSATTN_LAUNCH_KERNEL((shared_decode_merge_kernel<D>), dim3(p.w.hq, p.w.batch), dim3(256), 0, st, p);
+  if (rows >= kMergeByWaves) LSATTN_LAUNCH_KERNEL((shared_decode_merge_kernel<D, 1>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, p);
+  else LSATTN_LAUNCH_KERNEL((shared_decode_merge_kernel<D, 4>), dim3((unsigned)rows), dim3(256), 0, st, p);
 }
 
 }  // namespace
