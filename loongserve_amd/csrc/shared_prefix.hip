@@ -28,7 +28,8 @@
 //   * many rows, 128-wide fp16: the products (0.9 PFLOP/s of whole row tiles as the prefix grows, 1.14 where nothing has to be loaded, 1.17 a large library product), and 17 us of start and end: prompts of
 //     293 rows behind 6001 tokens 50 us, of which 6 are 28 MB of partials that all workgroups store at once.
 // Tried and left out (128-wide heads, all 0.70 to 0.75 PFLOP/s before the tiles went side by side, as this form): four stages of 32 keys; operands read a step ahead, or all at once (decode 5 to
-// 8% slower); eight waves of 256 rows in alternating phases (no room beside it for the own tokens); lines fetched into the L2 ahead (5%, few rows 30% slower); three and four waves per SIMD of
+// 8% slower); eight waves of 256 rows, in alternating phases or not (no room beside it for the own tokens; prompts of
+// 150 to 400 rows 0 to 8% slower, of 1200 2 to 4% faster, of 2500 behind 20000 tokens 10%); lines fetched into the L2 ahead (5%, few rows 30% slower); three and four waves per SIMD of
 // the 64-wide form (equal, and slower for spills); sums and exponentials in independent batches, products of 32 x 32 for bfloat16 (equal).  Of 64-wide bfloat16 rows 16 exponentials take an eighth of
 // a tile's time, the low parts of P a ninth, the reads from LDS nothing.
 #include <type_traits>
