@@ -671,7 +671,8 @@ int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* stream);
  * and rows outside [0, num_reqs).  P is held in the type of V (bfloat16: in two parts) and O divided by the sum of the weights so rounded.
  * max_prefix_len bounds g_prefix_len: of a longer prefix the first max_prefix_len positions are shared.  max_own_len (a bound of the positions behind the prefix) only
  * steers the launch.
- * Workspace: lsattn_shared_decode_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant before and after; calls that overlap in time need one each.
+ * Workspace: lsattn_shared_decode_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant before and after; calls that overlap in time need one each.  For given heads
+ * the bytes fall with none of the other sizes: a workspace for the largest ones does for all calls.
  * No counterpart in the reference.
  */
 typedef struct lsattn_shared_decode_args {

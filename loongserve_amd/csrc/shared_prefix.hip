@@ -893,8 +893,13 @@ Plan plan_of(int64_t rows, int64_t groups, int64_t hq, int64_t hkv, int64_t d, i
   else p.xcds_shift = 0;
   // (no group has more rows than there are; code that is not run is not fetched: a small launch is 1 us shorter)
   p.rounds = rows * (hq / hkv) <= kRows ? 0 : p.tiles * 6 <= kPrefixWorkgroups / hkv ? 1 : kRounds;
-  p.parts = p.shares + p.tiles > p.rounds * p.shares ? p.shares + p.tiles : p.rounds * p.shares;
-  p.pre_floats = p.tiles ? hkv * p.parts * kRows * (d + 1) : 0;
+  auto parts = [&](int64_t shares) { return shares + p.tiles > p.rounds * shares ? shares + p.tiles : p.rounds * shares; };
+  p.parts = parts(p.shares);
+  // (room for the partials of the most workgroups that a launch of these sizes or smaller ones takes, so that a workspace for the largest sizes does for all)
+  int64_t most_shares = kPrefixWorkgroups / hkv;
+  most_shares = most_shares < 1 ? 1 : most_shares;
+  most_shares = most_shares < units ? most_shares : units < 1 ? 1 : units;
+  p.pre_floats = p.tiles ? hkv * parts(most_shares) * kRows * (d + 1) : 0;
   p.own_shares = 1, p.own_floats = 0, p.plan_ints = kPlanInts * rows;
   if (decode) {
     const int64_t by_waves = kOwnWaves / tasks, by_units = (own_units + kOwnMinUnits - 1) / kOwnMinUnits;
@@ -952,11 +957,11 @@ extern "C" int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* st
     return LSATTN_ERR_INVALID_ARG;
   if (!(a->sm_scale > 0.f)) return LSATTN_ERR_INVALID_ARG;
   if (a->batch == 0) return LSATTN_OK;
-  const Plan pl = plan_of(a->batch, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len, a->max_own_len, true);
+  const int64_t most = most_of(a->max_prefix_len, a->max_seq_len);
+  const Plan pl = plan_of(a->batch, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, most, a->max_own_len, true);
   if (!a->workspace || a->workspace_bytes < (size_t)pl.all()) return LSATTN_ERR_WORKSPACE;
   if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
   // (units of both parts are numbered with 31 bits, and requests may be longer than the caller's bound)
-  const int64_t most = most_of(a->max_prefix_len, a->max_seq_len);
   if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups ||
       a->batch * ((a->max_seq_len + kBlock - 1) / kBlock) > kMaxUnits - kOwnWaves || a->batch * a->num_q_heads > kMaxUnits)
     return LSATTN_ERR_INVALID_ARG;

@@ -48,7 +48,8 @@ def _workspace(workspace, need: int, what: str) -> None:
 
 def shared_prefix_decode_workspace_bytes(batch_size: int, groups: int, q_head_num: int, kv_head_num: int, head_dim: int, max_prefix_len: int,
                                          max_own_len: int) -> int:
-    """Bytes of device memory that longserve_shared_prefix_decode_attention needs for the partials of such a call."""
+    """Bytes of device memory that longserve_shared_prefix_decode_attention needs for the partials of such a call, and of every call with the same heads in
+    which no other size is larger."""
     return int(_lib.load().lsattn_shared_decode_workspace_bytes(int(batch_size), int(groups), int(q_head_num), int(kv_head_num), int(head_dim),
                                                                 int(max_prefix_len), int(max_own_len)))
 
