@@ -709,7 +709,8 @@ int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* stream);
  * group, and rows that see no key, stay as they are.  Groups and table entries as in lsattn_shared_decode; prefixes longer than max_prefix_len are cut there.
  * max_group_rows bounds g_size (rows past it may stay uncomputed).  Few rows are taken against the pool's rows where they lie; for many the prefix is laid out once
  * in the workspace for the prefill kernel (a bfloat16 V as fp16, values beyond its range as +-65504).  Workspace as above, by
- * lsattn_shared_prefill_workspace_bytes.
+ * lsattn_shared_prefill_workspace_bytes: enough for all calls with the same heads and no larger sizes.  (Fewer groups than it was asked for may be laid out where more are not: if
+ * there is no room for that, the pool's rows are taken where they lie.)
  */
 typedef struct lsattn_shared_prefill_args {
   const void* q;                /* [rows, num_q_heads, head_dim], strides in elements, multiples of 8 */

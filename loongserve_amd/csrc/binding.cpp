@@ -962,7 +962,7 @@ PyObject* shared_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// (q, k, v, o, g_start, g_size, table, g_req, g_prefix, max_rows, max_prefix, m, l, rows, workspace or None) -> True or None
+// (q, k, v, o, g_start, g_size, table, g_req, g_prefix, max_rows, max_prefix, m, l, workspace or None) -> True or None
 PyObject* shared_prefill(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   NEED_ARGS(14);
@@ -982,10 +982,10 @@ PyObject* shared_prefill(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   lsattn_shared_prefill_args a;
   std::memset(&a, 0, sizeof a);
   a.num_groups = G;
-  a.workspace_bytes = lib.shared_prefill_workspace_bytes(T, G, Hq, Hkv, D, max_prefix);
-  OR_NONE(!ws_in || (ws_in->is_contiguous() && ws_in->nbytes() >= a.workspace_bytes));
-  const at::Tensor ws = ws_in ? *ws_in : empty({(int64_t)a.workspace_bytes}, q, at::kByte);
-  a.workspace = ws.data_ptr();
+  // (no prefix is longer than the table is wide; whether the caller's room is enough, the launch says)
+  OR_NONE(!ws_in || ws_in->is_contiguous());
+  const at::Tensor ws = ws_in ? *ws_in : empty({(int64_t)lib.shared_prefill_workspace_bytes(T, G, Hq, Hkv, D, std::min(max_prefix, table.size(1)))}, q, at::kByte);
+  a.workspace = ws.data_ptr(), a.workspace_bytes = ws.nbytes();
   a.q = q.data_ptr(), a.q_stride_t = q.stride(0), a.q_stride_h = q.stride(1);
   a.k = k.data_ptr(), a.v = v.data_ptr();
   a.k_stride_0 = k.stride(0), a.k_stride_1 = k.stride(1), a.v_stride_0 = v.stride(0), a.v_stride_1 = v.stride(1);
@@ -995,7 +995,10 @@ PyObject* shared_prefill(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   a.dtype = dtype_of(q), a.sm_scale = (float)(1.0 / std::sqrt((double)D));
   a.o = o.data_ptr(), a.o_stride_t = o.stride(0), a.o_stride_h = o.stride(1);
   a.m = (float*)m.data_ptr(), a.l = (float*)l.data_ptr(), a.ml_stride_t = m.stride(0), a.ml_stride_h = m.stride(1);
-  if (const int rc = call(lib.shared_prefill, &a, stream())) return failed(rc, "lsattn_shared_prefill");
+  if (const int rc = call(lib.shared_prefill, &a, stream())) {
+    OR_NONE(rc != LSATTN_ERR_WORKSPACE || !ws_in);
+    return failed(rc, "lsattn_shared_prefill");
+  }
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }

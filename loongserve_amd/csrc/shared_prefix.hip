@@ -1008,6 +1008,11 @@ namespace {
 // 32/32 heads, 16 groups 591 | 538, 32 596 | 827.
 constexpr int64_t kGatherFromRows = kCUs * 3 / 2 * 256, kGatherFromGroupRows = 512;
 bool gathers(int64_t rows, int64_t groups, int64_t hq, int64_t hkv) { return rows * hq >= kGatherFromRows && rows * (hq / hkv) >= groups * kGatherFromGroupRows; }
+// the most rows that do not gather, 1 at least
+int64_t most_direct_rows(int64_t groups, int64_t hq, int64_t hkv) {
+  const int64_t group = hq / hkv, by_all = (kGatherFromRows + hq - 1) / hq, by_group = (groups * kGatherFromGroupRows + group - 1) / group;
+  return (by_all > by_group ? by_all : by_group) - 1;
+}
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 struct PromptBytes {
   int64_t k, list, vectors, all;
@@ -1026,8 +1031,11 @@ extern "C" size_t lsattn_shared_prefill_workspace_bytes(int64_t rows, int64_t nu
   if (rows <= 0 || num_groups <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || (head_dim != 64 && head_dim != 128) ||
       max_prefix_len <= 0 || rows > 0x7fffff00 || num_groups > 65535 || num_q_heads > 65535 || max_prefix_len > 0x7fff0000)  // (as the launch refuses)
     return 0;
-  if (gathers(rows, num_groups, num_q_heads, num_kv_heads)) return (size_t)prompt_bytes(num_groups, num_kv_heads, head_dim, max_prefix_len).all;
-  return (size_t)plan_of(rows, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, 0, false).all();
+  // (fewer rows of as many groups may be taken the other way, whose room does not follow from this one's)
+  const int64_t direct_most = most_direct_rows(num_groups, num_q_heads, num_kv_heads), direct_rows = rows < direct_most ? rows : direct_most;
+  const int64_t direct = plan_of(direct_rows, num_groups, num_q_heads, num_kv_heads, head_dim, max_prefix_len, 0, false).all();
+  const int64_t laid_out = gathers(rows, num_groups, num_q_heads, num_kv_heads) ? prompt_bytes(num_groups, num_kv_heads, head_dim, max_prefix_len).all : 0;
+  return (size_t)(direct > laid_out ? direct : laid_out);
 }
 
 extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* stream) {
@@ -1050,8 +1058,11 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
   if (!(a->sm_scale > 0.f)) return LSATTN_ERR_INVALID_ARG;
   const int64_t most = most_of(a->max_prefix_len, a->max_seq_len);
   if (a->rows == 0 || a->num_groups == 0 || most == 0) return LSATTN_OK;
-  const size_t need = lsattn_shared_prefill_workspace_bytes(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len);
-  if (!a->workspace || a->workspace_bytes < need) return LSATTN_ERR_WORKSPACE;
+  // A workspace for more groups, which are not laid out, may be too small to lay out these: then they are taken as those would be.
+  const PromptBytes pb = prompt_bytes(a->num_groups, a->num_kv_heads, a->head_dim, most);
+  const bool lay_out = gathers(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads) && a->workspace_bytes >= (size_t)pb.all;
+  const Plan pl = plan_of(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, most, 0, false);
+  if (!a->workspace || (!lay_out && a->workspace_bytes < (size_t)pl.all())) return LSATTN_ERR_WORKSPACE;
   if ((uintptr_t)a->workspace & 15) return LSATTN_ERR_INVALID_ARG;
   SharedParams p = {};
   PoolParams& w = p.w;
@@ -1066,9 +1077,8 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
   p.groups = (int32_t)a->num_groups, p.rows = (int32_t)a->rows, p.most = (int32_t)most, p.near = is_near(w);
   p.by_hkv = fast_div((uint32_t)w.hkv), p.by_group = fast_div((uint32_t)group);
   hipStream_t st = (hipStream_t)stream;
-  if (gathers(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads)) {
+  if (lay_out) {
     if (a->num_groups * most > 0x7fffff00) return LSATTN_ERR_INVALID_ARG;  // (rows of the gathered K/V)
-    const PromptBytes pb = prompt_bytes(a->num_groups, a->num_kv_heads, a->head_dim, most);
     GatherParams g;
     char* at = (char*)a->workspace;
     g.k = at, g.v = at + pb.k, g.list = (int32_t*)(at + 2 * pb.k), g.vectors = (int32_t*)(at + 2 * pb.k + pb.list);
@@ -1097,7 +1107,6 @@ extern "C" int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* 
     s.total_q_rows = a->rows, s.total_kv_rows = a->num_groups * most, s.max_kv_len = (int32_t)most;
     return lsattn_prefill_step_merge(&s, stream);
   }
-  const Plan pl = plan_of(a->rows, a->num_groups, a->num_q_heads, a->num_kv_heads, a->head_dim, a->max_prefix_len, 0, false);
   if (pl.tiles * ((most + kKeys - 1) / kKeys) > kMaxUnits - kPrefixWorkgroups) return LSATTN_ERR_INVALID_ARG;  // (units are numbered with 31 bits)
   p.pre_o = (float*)a->workspace, p.pre_lse = p.pre_o + (pl.pre_floats / (a->head_dim + 1)) * a->head_dim;
   p.shares = (int32_t)pl.shares, p.parts = (int32_t)pl.parts, p.rounds = (int32_t)pl.rounds, p.ahead = pl.ahead, p.xcds_shift = (int32_t)pl.xcds_shift;

@@ -110,7 +110,8 @@ def longserve_shared_prefix_decode_attention(q: torch.Tensor, req_to_token_index
 
 
 def shared_prefix_attention_workspace_bytes(rows: int, groups: int, q_head_num: int, kv_head_num: int, head_dim: int, max_prefix_len: int) -> int:
-    """Bytes of device memory that shared_prefix_attention_fwd needs for such a call."""
+    """Bytes of device memory that shared_prefix_attention_fwd needs for such a call.  They are enough for calls with the same heads and fewer rows, groups and
+    shorter prefixes, too; calls with fewer groups may need more to have a prefix laid out and are taken without that where it is not there."""
     return int(_lib.load().lsattn_shared_prefill_workspace_bytes(int(rows), int(groups), int(q_head_num), int(kv_head_num), int(head_dim), int(max_prefix_len)))
 
 
@@ -151,8 +152,8 @@ def shared_prefix_attention_fwd(q: torch.Tensor, cache_k: torch.Tensor, cache_v:
         raise ValueError("m and l must be float32 [tokens, q_heads] with the same strides")
     if max_g_size < 0 or max_prefix_len < 0:
         raise ValueError("max_g_size and max_prefix_len must be >= 0")
-    _workspace(workspace, shared_prefix_attention_workspace_bytes(q.shape[0], g_start_loc.shape[0], q.shape[1], cache_k.shape[1], q.shape[2], max_prefix_len),
-               "shared_prefix_attention_workspace_bytes")
+    _workspace(workspace, shared_prefix_attention_workspace_bytes(q.shape[0], g_start_loc.shape[0], q.shape[1], cache_k.shape[1], q.shape[2],
+                                                                  min(max_prefix_len, req_to_token_indexs.shape[1])), "shared_prefix_attention_workspace_bytes")
     if q.numel() == 0 or g_start_loc.shape[0] == 0 or max_g_size == 0 or max_prefix_len == 0:
         return
     raise ValueError("shared_prefix_attention_fwd: arguments that no kernel takes (an empty pool?)")

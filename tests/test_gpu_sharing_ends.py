@@ -29,6 +29,18 @@ def test_a_decode_workspace_for_the_largest_sizes_does_for_all(heads):
                 assert need(more[0], more[1], *heads, *more[2:]) >= least > 0, (sizes, more)
 
 
+@pytest.mark.parametrize("heads", HEADS)
+def test_a_prompt_workspace_for_the_most_rows_does_for_fewer(heads):
+    """More rows or longer prefixes never need less room, whichever way either is taken."""
+    from loongserve_amd import shared_prefix_attention_workspace_bytes as need
+    prefixes = [1, 64, 65, 100, 6001, 131072]
+    edges = sorted({1, 2, 3, 5, 100, 293, 5000, 65536} | {max(1, 98304 // heads[0] + d) for d in (-1, 0, 1)} | {g * 512 * heads[1] // heads[0] + d for g in (2, 12, 64) for d in (0, 1)})
+    for groups in (1, 2, 12, 64, 500):
+        for p, longer in zip(prefixes, prefixes[1:] + [200000]):
+            for n, more in zip(edges, edges[1:] + [70000]):
+                assert 0 < need(n, groups, *heads, p) <= min(need(more, groups, *heads, p), need(n, groups, *heads, longer)), (groups, p, n)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("own", [1, 100, 200, 2000])
 def test_decode_steps_in_one_workspace(lsa, own):
@@ -37,3 +49,55 @@ def test_decode_steps_in_one_workspace(lsa, own):
     c = _case(51, 32, 8, 128, torch.float16, [(4000, [own] * 40)], [])
     got, want = _decode_on_gpu(lsa, c, workspace=ws), _decode_on_gpu(lsa, c)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ------------------------------------------------------------------------------------------------ the prompts' step
+def _prompt_some_rows(lsa, c, rows, what, eps_p=2.0 ** -11, **kw):
+    """The step from the empty state against float64 at some of its rows; the outputs."""
+    T, Hq, D = c["q"].shape
+    kv, (start, size, req, pre) = c["kv"], c["g"]
+    of = [max(g for g in range(len(start)) if start[g] <= i) for i in rows]
+    want = [orc.prompt(c["q"][i:i + 1], kv[:, :c["Hkv"]], kv[:, c["Hkv"]:], c["table"], [0], [1], [req[g]], [pre[g]], c["most"], eps_p) for i, g in zip(rows, of)]
+    o_ref, l_ref, tol_o, tol_l = (torch.cat(x) for x in zip(*want))
+    o, m, l = torch.zeros(T, Hq, D, dtype=c["q"].dtype, device=DEV), torch.full((T, Hq), -math.inf, device=DEV), torch.zeros(T, Hq, device=DEV)
+    _prompt_on_gpu(lsa, c, o, m, l, **kw)
+    _check((o[rows], ((torch.log2(l) + m) * math.log(2))[rows]), (o_ref, l_ref, tol_o + orc.EPS_OUT[o.dtype] * (o_ref.abs() + tol_o) + 2.0 ** -25, tol_l + 1e-6), what)
+    return o, m, l
+
+
+@pytest.mark.gpu
+def test_prompt_steps_in_one_workspace(lsa):
+    """The workspace of the longest chunk for shorter ones, on either side of the rows from which a prefix is laid out."""
+    heads = (128, 64, 128)
+    ws = torch.empty(lsa.shared_prefix_attention_workspace_bytes(1500, 1, *heads, 300), dtype=torch.uint8, device=DEV)
+    for rows in (1500, 768, 767, 100, 1):
+        c = _prompt_case(53, *heads, torch.float16, [(300, rows)], tail=0)
+        _prompt_some_rows(lsa, c, sorted({0, rows // 2, rows - 1}), rows, workspace=ws)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prompt_step_without_the_room_to_lay_out(lsa, dtype):
+    """A workspace for four groups, which are taken where they lie, and a call with one, which would be laid out if there were room."""
+    heads, prefix, rows = (128, 64, 128), 4000, 800
+    need = lsa.shared_prefix_attention_workspace_bytes
+    small = torch.empty(need(rows, 4, *heads, prefix), dtype=torch.uint8, device=DEV)
+    assert small.numel() < prefix * heads[1] * heads[2] * 4 <= need(rows, 1, *heads, prefix)
+    c = _prompt_case(57, *heads, dtype, [(prefix, rows)], tail=0)
+    looked_at = list(range(0, rows, 97)) + [rows - 1]
+    guard = torch.full((small.numel() + 64,), 77, dtype=torch.uint8, device=DEV)
+    _prompt_some_rows(lsa, c, looked_at, "where they lie", eps_p=orc.EPS_P[dtype], workspace=guard[:small.numel()])
+    assert bool((guard[small.numel():] == 77).all())
+    _prompt_some_rows(lsa, c, looked_at, "laid out")
+
+
+@pytest.mark.gpu
+def test_prompt_step_behind_a_loose_bound(lsa):
+    """A bound far past the table's width costs no memory."""
+    c = _prompt_case(59, 32, 8, 128, torch.float16, [(300, 3100)], tail=0)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    c["most"] = 1 << 22
+    _prompt_some_rows(lsa, c, [0, 1700, 3099], "loose")
+    assert torch.cuda.max_memory_allocated() - before < 1 << 30
