@@ -230,10 +230,21 @@ class LongServeReqManager:
                               self.mem_manager.kv_scales)
         return new, index
 
+    def _check_in_use(self, req_index):
+        if req_index.dim() != 1:
+            return  # (the release says what is wrong)
+        rows, state = req_index.cpu().long(), self.req_state.cpu()
+        known = (rows >= 0) & (rows < len(state))
+        bad = rows[~known | (state[rows.clamp(0, len(state) - 1)] == 0)]
+        if len(bad) or len(rows.unique()) < len(rows):
+            raise IndexError("request rows that are not in use, or named twice: %s" % (bad if len(bad) else rows).tolist())
+
     @torch.inference_mode()
     def free_reqs(self, free_req_index, b_seq_len, max_len_in_batch):
         """Frees requests with the tokens that their rows of the table name: every slot loses a reference per request that holds it, so that requests which
-        share tokens can go in one call (free takes a list of tokens, each once)."""
+        share tokens can go in one call (free takes a list of tokens, each once).  Rows that are not in use, or named twice, are an IndexError before anything
+        is freed: what they name may be others' tokens by now.  Tokens that were free already are one once everything else is freed."""
+        self._check_in_use(free_req_index)
         freed, wrong = sharing._release(self.req_to_token_indexs, _i32(free_req_index), _i32(b_seq_len), max_len_in_batch, self.mem_manager.mem_state)
         self.mem_manager.can_use_mem_size += freed
         self.can_use_req_size += len(free_req_index)

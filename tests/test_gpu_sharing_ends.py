@@ -101,3 +101,75 @@ def test_prompt_step_behind_a_loose_bound(lsa):
     c["most"] = 1 << 22
     _prompt_some_rows(lsa, c, [0, 1700, 3099], "loose")
     assert torch.cuda.max_memory_allocated() - before < 1 << 30
+
+
+# ------------------------------------------------------------------------------------------------ the managers
+def _managers(lsa, slots=100, rows=6, width=40, dtype=torch.float16):
+    mem = lsa.LongServeMemoryManager(slots, dtype, 2, 64, 3)
+    return mem, lsa.LongServeReqManager(rows, width, mem)
+
+
+def _request(lsa, mem, reqs, tokens):
+    row, slots = reqs.alloc(1), mem.alloc(tokens)
+    lsa.init_req_to_token_indexes(reqs.req_to_token_indexs, row.int(), _i32([tokens]), slots)
+    return row, slots
+
+
+def _as_counted(mem, reqs):
+    assert mem.can_use_mem_size == int((mem.mem_state == 0).sum()) and reqs.can_use_req_size == int((reqs.req_state == 0).sum())
+
+
+def _everything(mem, reqs):
+    return [t.clone() for t in (mem.mem_state, reqs.req_state, reqs.req_to_token_indexs)] + [mem.can_use_mem_size, reqs.can_use_req_size]
+
+
+def _same(a, b):
+    return all(torch.equal(x, y) if isinstance(x, torch.Tensor) else x == y for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+def test_requests_freed_twice_change_nothing(lsa):
+    """A row that is free still names its old slots, which a fork may hold: freeing it again is refused, so is a row twice in a call, a row never taken."""
+    mem, reqs = _managers(lsa)
+    parent, slots = _request(lsa, mem, reqs, 20)
+    other, _ = _request(lsa, mem, reqs, 7)
+    fork = reqs.fork(parent, _i32([20]), 20)
+    reqs.free_reqs(parent, _i32([20]), 20)
+    assert mem.mem_state[slots].unique().tolist() == [1]
+    before = _everything(mem, reqs)
+    unused = torch.tensor([4], device=DEV)
+    for rows, lens in ((parent, [20]), (torch.cat([other, parent]), [7, 20]), (other.repeat(2), [7, 7]), (unused, [0]), (torch.cat([fork, other, fork]), [20, 7, 0])):
+        with pytest.raises(IndexError, match="request"):
+            reqs.free_reqs(rows, _i32(lens), 20)
+        assert _same(before, _everything(mem, reqs))
+    for rows, lens in ((fork, _i32([20, 1])), (fork, _i32([20]).float())):
+        with pytest.raises(ValueError):
+            reqs.free_reqs(rows, lens, 20)
+        assert _same(before, _everything(mem, reqs))
+    reqs.free_reqs(torch.cat([other, fork]).int(), _i32([7, 20]), 20)
+    _as_counted(mem, reqs)
+    assert mem.can_use_mem_size == 100 and reqs.can_use_req_size == 6
+    reqs.free_reqs(fork[:0], _i32([]), 20)
+
+
+@pytest.mark.gpu
+def test_requests_outside_the_table_are_refused(lsa):
+    mem, reqs = _managers(lsa)
+    row, _ = _request(lsa, mem, reqs, 5)
+    before = _everything(mem, reqs)
+    for bad in (-1, 6, 1 << 20, 1 << 40):
+        with pytest.raises(IndexError, match="request"):
+            reqs.free_reqs(torch.cat([row, torch.tensor([bad], device=DEV)]), _i32([5, 0]), 20)
+        assert _same(before, _everything(mem, reqs))
+
+
+@pytest.mark.gpu
+def test_tokens_that_were_gone_leave_the_counts_right(lsa):
+    """A live request some of whose tokens were freed one by one: an IndexError, everything else is freed, the counts fit."""
+    mem, reqs = _managers(lsa)
+    row, slots = _request(lsa, mem, reqs, 20)
+    mem.free(slots[15:])
+    with pytest.raises(IndexError, match="5 tokens"):
+        reqs.free_reqs(row, _i32([20]), 20)
+    _as_counted(mem, reqs)
+    assert mem.can_use_mem_size == 100 and reqs.can_use_req_size == 6
