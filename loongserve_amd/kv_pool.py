@@ -213,7 +213,11 @@ class LongServeReqManager:
         is (free_reqs); new tokens of a fork get slots of their own, as those of any request."""
         new = self.alloc(len(b_req_idx))
         if new is not None:
-            sharing.fork_requests(self.req_to_token_indexs, _i32(b_req_idx), _i32(new), _i32(b_seq_len), max_len_in_batch, self.mem_manager.mem_state)
+            try:
+                sharing.fork_requests(self.req_to_token_indexs, _i32(b_req_idx), _i32(new), _i32(b_seq_len), max_len_in_batch, self.mem_manager.mem_state)
+            except BaseException:
+                self.free(new, None)
+                raise
         return new
 
     @torch.inference_mode()
@@ -224,10 +228,14 @@ class LongServeReqManager:
             return self.alloc(len(b_req_idx))  # (says so)
         index = self.mem_manager.alloc(total_len)
         new = self.alloc(len(b_req_idx))
-        b_seq_len = _i32(b_seq_len)
-        start = (torch.cumsum(b_seq_len, 0, dtype=torch.int32) - b_seq_len).to(torch.int32)
-        sharing.copy_requests(self.req_to_token_indexs, _i32(b_req_idx), _i32(new), b_seq_len, start, max_len_in_batch, index, self.mem_manager.kv_buffer,
-                              self.mem_manager.kv_scales)
+        try:
+            b_seq_len = _i32(b_seq_len)
+            start = (torch.cumsum(b_seq_len, 0, dtype=torch.int32) - b_seq_len).to(torch.int32)
+            sharing.copy_requests(self.req_to_token_indexs, _i32(b_req_idx), _i32(new), b_seq_len, start, max_len_in_batch, index, self.mem_manager.kv_buffer,
+                                  self.mem_manager.kv_scales)
+        except BaseException:
+            self.free(new, index)
+            raise
         return new, index
 
     def _check_in_use(self, req_index):

@@ -173,3 +173,21 @@ def test_tokens_that_were_gone_leave_the_counts_right(lsa):
         reqs.free_reqs(row, _i32([20]), 20)
     _as_counted(mem, reqs)
     assert mem.can_use_mem_size == 100 and reqs.can_use_req_size == 6
+
+
+@pytest.mark.gpu
+def test_forks_that_are_refused_take_nothing(lsa):
+    mem, reqs = _managers(lsa)
+    row, _ = _request(lsa, mem, reqs, 20)
+    before = _everything(mem, reqs)
+    two = row.repeat(2)
+    for lens, most in ((_i32([20]), 20), (_i32([20, 20]).float(), 20), (_i32([20, 20]).cpu(), 20), (_i32([20, 20]), -1), (_i32([[20, 20]]), 20)):
+        with pytest.raises(ValueError):
+            reqs.fork(two, lens, most)
+        assert _same(before, _everything(mem, reqs))
+        with pytest.raises(ValueError):
+            reqs.fork_copy(two, lens, most, 40)
+        assert _same(before, _everything(mem, reqs))
+    with pytest.raises(AssertionError):
+        reqs.fork_copy(two, _i32([20, 20]), 20, 81)  # more than the pool has
+    assert _same(before, _everything(mem, reqs))
