@@ -741,8 +741,8 @@ int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* stream);
 
 /*
  * New requests over another's tokens, the same slots: for i < n and pos < b_seq_len[i]
- *   req_to_tokens[dst_req_idx[i], pos] = slot = req_to_tokens[src_req_idx[i], pos],   mem_state[slot] += 1   (a slot outside the pool is not counted).
- * Destination rows are distinct and no source of the call.  Forks of one request cost one addition per token where they stand next to each other.
+ *   req_to_tokens[dst_req_idx[i], pos] = slot = req_to_tokens[src_req_idx[i], pos],   mem_state[slot] += 1   (a slot outside the pool is not counted;
+ * positions of a source outside [0, num_reqs) name no slot, 2147483647).  Destination rows are distinct and no source of the call.  Forks of one request cost one addition per token where they stand next to each other.
  * max_len_in_batch bounds b_seq_len: positions past it are left out.  No counterpart in the reference, nor have the four entry points below.
  */
 int lsattn_fork_requests(int32_t* req_to_tokens, int64_t num_reqs, int64_t max_seq_len, const int32_t* src_req_idx, const int32_t* dst_req_idx,
@@ -760,7 +760,8 @@ typedef struct lsattn_pool_rows {
 /*
  * New requests over copies of another's tokens: for i < n and pos < b_seq_len[i], in every layer
  *   row[slot] = row[req_to_tokens[src_req_idx[i], pos]],   req_to_tokens[dst_req_idx[i], pos] = slot = mem_index[b_start_loc[i] + pos].
- * The slots come from the allocator: distinct, and none of a source's.  Slots outside the pool and places past num_index are left out.
+ * The slots come from the allocator: distinct, and none of a source's.  Where mem_index gives no slot of the pool (a number outside, a place past num_index) or the source is no row
+ * of the table, the copy's entry names no slot (2147483647).  Where the source's entry names none, the copy's slot keeps the row that it has: the caller's to write.
  */
 typedef struct lsattn_copy_requests_args {
   int32_t* req_to_tokens;       /* [num_reqs, max_seq_len] contiguous */

@@ -27,10 +27,11 @@ struct ForkParams {
 };
 __device__ __forceinline__ int fork_len(const ForkParams& p, int i) {
   const int n = p.len[i];
-  return p.src[i] < 0 || p.src[i] >= p.num_reqs || p.dst[i] < 0 || p.dst[i] >= p.num_reqs ? 0 : n < p.most ? n : p.most;
+  return p.dst[i] < 0 || p.dst[i] >= p.num_reqs ? 0 : n < p.most ? n : p.most;
 }
+constexpr int kNoSlot = 0x7fffffff;  // as the table's unused entries
 // A thread has a position of a fork.  Forks of one request that stand next to each other count as one addition per token, made by the first of them: many samples of one
-// question would otherwise queue at the same words.
+// question would otherwise queue at the same words.  Positions of a source that is no row of the table name no slot: what the fork's row held before may be others' tokens by now.
 __global__ __launch_bounds__(kThreads) void fork_share_kernel(ForkParams p) {
   const int i = blockIdx.y, pos = (int)(blockIdx.x * kThreads + threadIdx.x), lane = threadIdx.x & 63;
   const int src = p.src[i], mine = fork_len(p, i);
@@ -38,7 +39,7 @@ __global__ __launch_bounds__(kThreads) void fork_share_kernel(ForkParams p) {
   const bool valid_src = src >= 0 && src < p.num_reqs;
   const bool leads = i == 0 || p.src[i - 1] != src;
   if (pos < mine) {
-    slot = p.table[(int64_t)src * p.max_seq_len + pos];
+    slot = valid_src ? p.table[(int64_t)src * p.max_seq_len + pos] : kNoSlot;
     p.table[(int64_t)p.dst[i] * p.max_seq_len + pos] = slot;
   }
   if (!leads || !valid_src) return;
@@ -119,6 +120,7 @@ template <int FORKS> __global__ __launch_bounds__(kThreads) void fork_copy_kerne
     most = len[f] > most ? len[f] : most;
   }
   if (pos0 >= most) return;
+  const bool known = req >= 0 && req < p.f.num_reqs;
   const int32_t* const src_row = p.f.table + (int64_t)req * p.f.max_seq_len;
   auto target = [&](int64_t first, int n, int pos) -> int {  // the slot of a position, -1 if there is none
     const int64_t at = first + pos;
@@ -130,9 +132,10 @@ template <int FORKS> __global__ __launch_bounds__(kThreads) void fork_copy_kerne
 #pragma unroll
     for (int f = 0; f < FORKS; f++) {
       const int d = target(start[f], len[f], pos);
-      if (d >= 0) p.f.table[(int64_t)p.f.dst[i + f] * p.f.max_seq_len + pos] = d;
+      if (pos < len[f]) p.f.table[(int64_t)p.f.dst[i + f] * p.f.max_seq_len + pos] = known && d >= 0 ? d : kNoSlot;
     }
   }
+  if (!known) return;
   auto row_of = [&](int k, int& src, int (&dst)[FORKS]) {
     const int pos = pos0 + k;
     if (pos >= most) return false;

@@ -165,8 +165,8 @@ def fork_requests(req_to_token_indexs: torch.Tensor, src_req_idx: torch.Tensor, 
     more reference in mem_state.  LongServeReqManager.fork does this with rows of its own.
 
     The index vectors and lengths are int32 on the GPU.  A source may be named any number of times (forks of one source next to each other cost one addition per
-    token); destination rows are distinct and no source of the call.  Entries that name no slot are copied and not counted.  max_len_in_batch bounds b_seq_len:
-    positions past it are left out."""
+    token); destination rows are distinct and no source of the call.  Entries that name no slot are copied and not counted, positions of a source that is no row of the
+    table name none.  max_len_in_batch bounds b_seq_len: positions past it are left out."""
     if _native.fork_requests(req_to_token_indexs, src_req_idx, dst_req_idx, b_seq_len, max_len_in_batch, mem_state):
         return
     if _other_ints(max_len_in_batch):
@@ -201,8 +201,10 @@ def copy_requests(req_to_token_indexs: torch.Tensor, src_req_idx: torch.Tensor, 
     then.  mem_index is what LongServeMemoryManager.alloc returns (int64), the index vectors and lengths are int32 on the GPU.  LongServeReqManager.fork_copy does
     this with rows and slots of its own.
 
-    A source may be named any number of times; destination rows are distinct and no source of the call, slots of mem_index likewise.  Entries of a source that name no slot
-    leave the copy's row as it was.  max_len_in_batch bounds b_seq_len: positions past it are left out."""
+    A source may be named any number of times; destination rows are distinct and no source of the call, slots of mem_index likewise.  A position whose entry in the source names
+    no slot has its slot of mem_index like any other, whose K/V stay as they were: the caller's to write before the copy is attended to (fork_copy refuses such sources).  Positions
+    for which mem_index has no slot of the pool (its end, a number outside) name none (2147483647), nor do those of a source that is no row of the table.
+    max_len_in_batch bounds b_seq_len: positions past it are left out."""
     if _native.copy_requests(req_to_token_indexs, src_req_idx, dst_req_idx, b_seq_len, b_start_loc, max_len_in_batch, mem_index, kv_buffer, kv_scales):
         return
     if _other_ints(max_len_in_batch):

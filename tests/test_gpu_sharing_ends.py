@@ -191,3 +191,37 @@ def test_forks_that_are_refused_take_nothing(lsa):
     with pytest.raises(AssertionError):
         reqs.fork_copy(two, _i32([20, 20]), 20, 81)  # more than the pool has
     assert _same(before, _everything(mem, reqs))
+
+
+@pytest.mark.gpu
+def test_forks_and_copies_of_no_request(lsa):
+    """Positions that get no slot name none: a row's entries from before are other requests' by now."""
+    for copies in (False, True):
+        table = torch.arange(80, dtype=torch.int32, device=DEV).reshape(8, 10).contiguous()
+        state = torch.ones(100, dtype=torch.int32, device=DEV)
+        src, dst, lens = _i32([-1, 8, 1, 1, 1, 1, 1]), _i32([2, 3, 4, 5, 6, 7, 99]), _i32([4, 10, 3, 10, 0, 25, 5])
+        want = table.cpu().clone()
+        want[2, :4] = PAD
+        want[3, :] = PAD
+        if copies:
+            pool = torch.arange(2 * 100 * 2 * 64, device=DEV).reshape(2, 100, 2, 64).half()
+            rows = pool.cpu().clone()
+            index = torch.arange(80, 100, device=DEV)
+            start = [0, 4, 0, 3, 0, 13, 0]  # 20 slots: the last request of 10 has 7 of them
+            index[5] = 100  # and one that does not exist, of the second one's
+            lsa.copy_requests(table, src, dst, lens, _i32(start), 10, index, pool)
+            for s, n, at in ((4, 3, 0), (5, 10, 3), (7, 10, 13)):
+                for i in range(n):
+                    new = int(index[at + i]) if at + i < 20 else 100
+                    want[s, i] = new if new < 100 else PAD
+                    if new < 100:
+                        rows[:, new] = rows[:, 10 + i]
+            assert torch.equal(pool.cpu(), rows)
+        else:
+            lsa.fork_requests(table, src, dst, lens, 10, state)
+            want[4, :3], want[5], want[7] = want[1, :3].clone(), want[1].clone(), want[1].clone()
+            held = torch.ones(100, dtype=torch.int32)
+            held[10:20] += 2
+            held[10:13] += 1
+            assert torch.equal(state.cpu(), held)
+        assert torch.equal(table.cpu(), want), copies
