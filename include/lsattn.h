@@ -742,7 +742,8 @@ int lsattn_shared_prefill(const lsattn_shared_prefill_args* a, void* stream);
 /*
  * New requests over another's tokens, the same slots: for i < n and pos < b_seq_len[i]
  *   req_to_tokens[dst_req_idx[i], pos] = slot = req_to_tokens[src_req_idx[i], pos],   mem_state[slot] += 1   (a slot outside the pool is not counted;
- * positions of a source outside [0, num_reqs) name no slot, 2147483647).  Destination rows are distinct and no source of the call.  Forks of one request cost one addition per token where they stand next to each other.
+ * positions of a source outside [0, num_reqs), and those whose slot is free (mem_state 0), name no slot, 2147483647).  Destination rows are distinct and no source of the
+ * call.  Forks of one request cost one addition per token where they stand next to each other.
  * max_len_in_batch bounds b_seq_len: positions past it are left out.  No counterpart in the reference, nor have the four entry points below.
  */
 int lsattn_fork_requests(int32_t* req_to_tokens, int64_t num_reqs, int64_t max_seq_len, const int32_t* src_req_idx, const int32_t* dst_req_idx,

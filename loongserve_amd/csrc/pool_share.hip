@@ -32,6 +32,8 @@ __device__ __forceinline__ int fork_len(const ForkParams& p, int i) {
 constexpr int kNoSlot = 0x7fffffff;  // as the table's unused entries
 // A thread has a position of a fork.  Forks of one request that stand next to each other count as one addition per token, made by the first of them: many samples of one
 // question would otherwise queue at the same words.  Positions of a source that is no row of the table name no slot: what the fork's row held before may be others' tokens by now.
+// Nor do those whose slot is free: nobody holds it, and a count that began here would be one that the allocator's number of free slots has not seen.  (Counts that are not zero stay so within the
+// call, and zeros stay zeros, so that it does not matter when a thread looks.)
 __global__ __launch_bounds__(kThreads) void fork_share_kernel(ForkParams p) {
   const int i = blockIdx.y, pos = (int)(blockIdx.x * kThreads + threadIdx.x), lane = threadIdx.x & 63;
   const int src = p.src[i], mine = fork_len(p, i);
@@ -40,6 +42,7 @@ __global__ __launch_bounds__(kThreads) void fork_share_kernel(ForkParams p) {
   const bool leads = i == 0 || p.src[i - 1] != src;
   if (pos < mine) {
     slot = valid_src ? p.table[(int64_t)src * p.max_seq_len + pos] : kNoSlot;
+    if ((uint32_t)slot < (uint32_t)p.size && p.state[slot] == 0) slot = kNoSlot;
     p.table[(int64_t)p.dst[i] * p.max_seq_len + pos] = slot;
   }
   if (!leads || !valid_src) return;
@@ -54,7 +57,10 @@ __global__ __launch_bounds__(kThreads) void fork_share_kernel(ForkParams p) {
     if (run < 64) break;
   }
   if (refs == 0) return;
-  if (slot < 0 && pos >= mine && pos < p.most) slot = p.table[(int64_t)src * p.max_seq_len + pos];  // (a longer fork behind the first)
+  if (pos >= mine) {  // (a longer fork behind the first)
+    slot = p.table[(int64_t)src * p.max_seq_len + pos];
+    if ((uint32_t)slot < (uint32_t)p.size && p.state[slot] == 0) slot = kNoSlot;
+  }
   if ((uint32_t)slot < (uint32_t)p.size) atomicAdd(p.state + slot, refs);
 }
 

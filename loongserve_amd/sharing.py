@@ -165,8 +165,8 @@ def fork_requests(req_to_token_indexs: torch.Tensor, src_req_idx: torch.Tensor, 
     more reference in mem_state.  LongServeReqManager.fork does this with rows of its own.
 
     The index vectors and lengths are int32 on the GPU.  A source may be named any number of times (forks of one source next to each other cost one addition per
-    token); destination rows are distinct and no source of the call.  Entries that name no slot are copied and not counted, positions of a source that is no row of the
-    table name none.  max_len_in_batch bounds b_seq_len: positions past it are left out."""
+    token); destination rows are distinct and no source of the call.  Entries that name no slot are copied and not counted; positions of a source that is no row of the
+    table, and those whose slot is free, name none in the new row (2147483647).  max_len_in_batch bounds b_seq_len: positions past it are left out."""
     if _native.fork_requests(req_to_token_indexs, src_req_idx, dst_req_idx, b_seq_len, max_len_in_batch, mem_state):
         return
     if _other_ints(max_len_in_batch):

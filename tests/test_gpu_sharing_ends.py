@@ -194,6 +194,23 @@ def test_forks_that_are_refused_take_nothing(lsa):
 
 
 @pytest.mark.gpu
+def test_forks_do_not_take_up_slots_that_are_free(lsa):
+    """Entries behind a request's tokens may name slots that are free: nobody holds them, and a fork does not either."""
+    mem, reqs = _managers(lsa)
+    row, slots = _request(lsa, mem, reqs, 20)
+    mem.free(slots[12:18].contiguous())
+    forks = reqs.fork(row.repeat(3), _i32([20, 14, 12]), 20)
+    _as_counted(mem, reqs)
+    table = reqs.req_to_token_indexs.cpu()
+    held = slots.int().tolist()
+    held[12:18] = [PAD] * 6
+    for f, n in zip(forks.tolist(), (20, 14, 12)):
+        assert table[f, :n].tolist() == held[:n]
+    assert table[int(row), :20].tolist() == slots.tolist()  # the source's own entries stay
+    assert mem.mem_state[slots].tolist() == [4] * 12 + [0] * 6 + [2] * 2
+
+
+@pytest.mark.gpu
 def test_forks_and_copies_of_no_request(lsa):
     """Positions that get no slot name none: a row's entries from before are other requests' by now."""
     for copies in (False, True):
