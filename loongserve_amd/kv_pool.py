@@ -223,13 +223,19 @@ class LongServeReqManager:
     @torch.inference_mode()
     def fork_copy(self, b_req_idx, b_seq_len, max_len_in_batch, total_len):
         """fork with copies: total_len (the sum of b_seq_len) slots are taken from the pool, and the tokens' rows are copied in all layers.  (rows,
-        slots), or None where the table is full; a pool that is short raises, as its alloc does."""
+        slots), or None where the table is full; a pool that is short raises, as its alloc does.  Copies are whole: a total that is less than the tokens, or a source
+        with positions that have no slot (or one that is free), is a ValueError before anything is taken (so the call waits for the device)."""
         if len(b_req_idx) > self.can_use_req_size:
             return self.alloc(len(b_req_idx))  # (says so)
+        b_seq_len, tokens, missing = sharing._sources_of_copies(self.req_to_token_indexs, _i32(b_req_idx), _i32(b_seq_len), max_len_in_batch,
+                                                                self.mem_manager.mem_state)
+        if tokens > total_len:
+            raise ValueError("total_len is %d, the requests to be copied have %d tokens" % (total_len, tokens))
+        if missing:
+            raise ValueError("%d positions of the requests to be copied have no slot, or one that is free" % missing)
         index = self.mem_manager.alloc(total_len)
         new = self.alloc(len(b_req_idx))
         try:
-            b_seq_len = _i32(b_seq_len)
             start = (torch.cumsum(b_seq_len, 0, dtype=torch.int32) - b_seq_len).to(torch.int32)
             sharing.copy_requests(self.req_to_token_indexs, _i32(b_req_idx), _i32(new), b_seq_len, start, max_len_in_batch, index, self.mem_manager.kv_buffer,
                                   self.mem_manager.kv_scales)

@@ -225,6 +225,26 @@ def copy_requests(req_to_token_indexs: torch.Tensor, src_req_idx: torch.Tensor, 
     raise ValueError("copy_requests: arguments that no kernel takes")
 
 
+def _sources_of_copies(req_to_token_indexs, src_req_idx, b_seq_len, max_len_in_batch, mem_state) -> Tuple[torch.Tensor, int, int]:
+    """(the lengths as a copy takes them, their sum, how many of the positions have no slot, or one that is free).  Waits for the device."""
+    _on_current_device(((req_to_token_indexs, "req_to_token_indexs"), (src_req_idx, "src_req_idx"), (b_seq_len, "b_seq_len")))
+    _table(req_to_token_indexs)
+    for t, name in ((src_req_idx, "src_req_idx"), (b_seq_len, "b_seq_len")):
+        _i32vec(t, name, len(src_req_idx))
+    if max_len_in_batch < 0:
+        raise ValueError("max_len_in_batch must be >= 0")
+    rows, width = req_to_token_indexs.shape
+    most = min(as_int(max_len_in_batch), width)
+    lens = b_seq_len.clamp(0, most)
+    size = len(mem_state)
+    if not len(src_req_idx) or not most or not rows or not size:
+        return lens, 0, 0
+    slots = req_to_token_indexs[src_req_idx.clamp(0, rows - 1), :most]
+    there = (slots >= 0) & (slots < size) & (mem_state[slots.clamp(0, size - 1)] != 0) & ((src_req_idx >= 0) & (src_req_idx < rows))[:, None]
+    missing = ~there & (torch.arange(most, device=slots.device) < lens[:, None])
+    return lens, *torch.stack([lens.sum(), missing.sum()]).tolist()
+
+
 def _release(req_to_token_indexs, b_req_idx, b_seq_len, max_len_in_batch, mem_state) -> Tuple[int, int]:
     counts = _native.release_requests(req_to_token_indexs, b_req_idx, b_seq_len, max_len_in_batch, mem_state)
     if counts is not None:

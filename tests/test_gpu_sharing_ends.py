@@ -242,3 +242,32 @@ def test_forks_and_copies_of_no_request(lsa):
             held[10:13] += 1
             assert torch.equal(state.cpu(), held)
         assert torch.equal(table.cpu(), want), copies
+
+
+@pytest.mark.gpu
+def test_copies_are_whole_or_refused(lsa):
+    """fork_copy refuses a source with positions that have no slot, and a total that is less than the tokens: nothing is taken."""
+    mem, reqs = _managers(lsa)
+    row, slots = _request(lsa, mem, reqs, 20)
+    before = _everything(mem, reqs)
+    for total in (0, 39):
+        with pytest.raises(ValueError, match="total_len"):
+            reqs.fork_copy(row.repeat(2), _i32([20, 20]), 20, total)
+        assert _same(before, _everything(mem, reqs))
+    for lens in ([21], [400]):
+        with pytest.raises(ValueError, match="no slot"):
+            reqs.fork_copy(row, _i32(lens), 400, 41)
+        assert _same(before, _everything(mem, reqs))
+    with pytest.raises(ValueError, match="no slot"):
+        reqs.fork_copy(torch.tensor([6], device=DEV), _i32([3]), 20, 3)
+    assert _same(before, _everything(mem, reqs))
+    mem.free(slots[7:8])
+    before = _everything(mem, reqs)
+    with pytest.raises(ValueError, match="1 positions"):
+        reqs.fork_copy(row, _i32([20]), 20, 20)
+    assert _same(before, _everything(mem, reqs))
+    mem.add_refs(slots[7:8])
+    new, own = reqs.fork_copy(row.repeat(3), _i32([20, -5, 400]), 20, 41)  # (cut at 20 positions; a slot to spare)
+    assert len(own) == 41 and torch.equal(reqs.req_to_token_indexs[new[0], :20].long(), own[:20]) and torch.equal(reqs.req_to_token_indexs[new[2], :20].long(), own[20:40])
+    assert torch.equal(mem.kv_buffer[:, own[20:40]].view(torch.int16), mem.kv_buffer[:, slots].view(torch.int16))
+    _as_counted(mem, reqs)
