@@ -301,16 +301,18 @@ template <typename T, int D, bool THROUGH> __device__ __forceinline__ void prefi
     typedef int Slots __attribute__((ext_vector_type(NI), aligned(4)));
     int slot[NI];
     // The slots of the lane's rows of tile t, neighbours in the table (LDS row 16 wave + RPI i + j is key 16 wave + NI j + i); positions past the prefix repeat its last one.
-    const uint32_t pos0 = (uint32_t)(block0 * kKeys + 16 * wave + NI * j_row);
+    // (the tile's place in the row is the wave's, with 64 bits: a row may be longer than 2^30 entries)
+    const int of_tile = 16 * wave + NI * j_row;
+    const uint32_t pos0 = (uint32_t)(block0 * kKeys + of_tile);
     auto load_slots = [&](int t) __attribute__((always_inline)) {
-      const uint32_t pos = pos0 + t * kKeys;
-      if ((block0 + t + 1) * kKeys <= prefix) {  // (wave-uniform)
-        const Slots x = *(const Slots*)((const char*)row_slots + pos * 4);
+      const int start = (block0 + t) * kKeys;
+      if (start + kKeys <= prefix) {  // (wave-uniform)
+        const Slots x = *(const Slots*)(row_slots + start + of_tile);
 #pragma unroll
         for (int i = 0; i < NI; i++) slot[i] = x[i];
       } else {
 #pragma unroll
-        for (int i = 0; i < NI; i++) slot[i] = *(const int*)((const char*)row_slots + (pos + i < (uint32_t)prefix ? pos + i : (uint32_t)prefix - 1) * 4);
+        for (int i = 0; i < NI; i++) slot[i] = row_slots[start + of_tile + i < prefix ? start + of_tile + i : prefix - 1];
       }
     };
     // The rows of tile t.  What stands here is issued by every wave for every tile, so the common case, all 64 keys there, is kept short: offsets of 32 bits where the pool allows

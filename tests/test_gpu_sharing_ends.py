@@ -271,3 +271,31 @@ def test_copies_are_whole_or_refused(lsa):
     assert len(own) == 41 and torch.equal(reqs.req_to_token_indexs[new[0], :20].long(), own[:20]) and torch.equal(reqs.req_to_token_indexs[new[2], :20].long(), own[20:40])
     assert torch.equal(mem.kv_buffer[:, own[20:40]].view(torch.int16), mem.kv_buffer[:, slots].view(torch.int16))
     _as_counted(mem, reqs)
+
+
+# ------------------------------------------------------------------------------------------------ far positions
+@pytest.mark.gpu
+def test_positions_past_a_billion(lsa):
+    """Byte offsets in a table's row that pass 32 bits: a prefix of 2^30 positions and more, of which a few exist, in both attention operators."""
+    far, D = 1 << 30, 64
+    P = far + 70
+    g = torch.Generator().manual_seed(61)
+    kv, q = _rows((60, 2, D), g, torch.float16), _rows((3, 8, D), g, torch.float16)
+    table = torch.full((3, P + 5), -1, dtype=torch.int32, device=DEV)
+    near = {7: 1, far // 2 + 3: 2}
+    there = {**near, **{far + i: 3 + i for i in range(40)}, P - 1: 50}
+    for pos, slot in there.items():
+        table[1, pos] = slot
+    table[0, P:P + 5], table[2, P:P + 2] = _i32([51, 52, 53, 54, 55]), _i32([56, 57])
+    kv_gpu = kv.to(DEV)
+    o, lse = lsa.longserve_shared_prefix_decode_attention(q[:2].to(DEV), table, _i32([0, 2]), _i32([P + 5, P + 2]), 5, kv_gpu[:, :1], kv_gpu[:, 1:], _i32([0]), _i32([2]), _i32([1]),
+                                                          _i32([P]), P, max_own_len=5)
+    small = torch.full((3, len(there) + 5), PAD, dtype=torch.int32)
+    n = len(there)
+    small[1, :n] = torch.tensor(list(there.values()))
+    small[0, n:n + 5], small[2, n:n + 2] = torch.arange(51, 56), torch.arange(56, 58)
+    _check((o, lse), orc.decode(q[:2], kv[:, :1], kv[:, 1:], small, torch.tensor([0, 2]), torch.tensor([n + 5, n + 2]), [0], [2], [1], [n], n, torch.float16), "decode")
+    o, m, l = torch.zeros(3, 8, D, dtype=torch.float16, device=DEV), torch.full((3, 8), -math.inf, device=DEV), torch.zeros(3, 8, device=DEV)
+    lsa.shared_prefix_attention_fwd(q.to(DEV), kv_gpu[:, :1], kv_gpu[:, 1:], o, _i32([0]), _i32([3]), table, _i32([1]), _i32([P]), 3, P, m, l)
+    o_ref, l_ref, tol_o, tol_l = orc.prompt(q, kv[:, :1], kv[:, 1:], small, [0], [3], [1], [n], n, 2.0 ** -11)
+    _check((o, (torch.log2(l) + m) * math.log(2)), (o_ref, l_ref, tol_o + 2.0 ** -11 * (o_ref.abs() + tol_o) + 2.0 ** -25, tol_l + 1e-6), "prompt")
