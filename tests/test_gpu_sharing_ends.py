@@ -299,3 +299,216 @@ def test_positions_past_a_billion(lsa):
     lsa.shared_prefix_attention_fwd(q.to(DEV), kv_gpu[:, :1], kv_gpu[:, 1:], o, _i32([0]), _i32([3]), table, _i32([1]), _i32([P]), 3, P, m, l)
     o_ref, l_ref, tol_o, tol_l = orc.prompt(q, kv[:, :1], kv[:, 1:], small, [0], [3], [1], [n], n, 2.0 ** -11)
     _check((o, (torch.log2(l) + m) * math.log(2)), (o_ref, l_ref, tol_o + 2.0 ** -11 * (o_ref.abs() + tol_o) + 2.0 ** -25, tol_l + 1e-6), "prompt")
+
+
+# ------------------------------------------------------------------------------------------------ the weights' bits
+BITS = {"one": ([(200, [1, 33, 64, 7])], []), "long": ([(1000, [100] * 5), (513, [0] * 3)], []), "rows-past-a-tile": ([(130, [2] * 37)], [9, 1]),
+        "tile-ends": ([(63, [3]), (64, [0, 5]), (65, [32, 31, 1]), (128, [1])], [1, 40])}
+
+
+def _even(c):
+    """The same case with small scores and V of one size: what a sum of products may be off by grows with them, and would hide the weights' bits."""
+    c["q"] = (c["q"].float() / 64).to(c["q"].dtype)
+    c["kv"][:, c["Hkv"]:] = c["kv"][:, c["Hkv"]:].clamp(-1, 1)
+    return c
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("heads", [(8, 2, 128), (16, 1, 128), (20, 2, 64)])
+@pytest.mark.parametrize("name", list(BITS))
+def test_decode_weights_in_float32_outputs(lsa, name, heads, dtype):
+    """What the weights over a prefix are off by, where the output's rounding does not hide it: 2^-11 (fp16), 2^-16 (two parts of bfloat16)."""
+    groups, alone = BITS[name]
+    c = _even(_case(71, *heads, dtype, groups, alone))
+    _decode_check(lsa, c, (name, heads, dtype), out_dtype=torch.float32, out=torch.empty(c["q"].shape, device=DEV))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads", [(8, 2, 128), (7, 1, 128), (4, 4, 64)])
+@pytest.mark.parametrize("groups", [[(500, 40), (3, 90)], [(2000, 300)], [(90, 5)] * 3])
+def test_prompt_weights_of_bfloat16_rows(lsa, heads, groups):
+    """Rows that are taken where they lie: P in two parts.  (O is the mean of hundreds of values of either sign: where it is small, its rounding does not hide the weights'.)"""
+    c = _even(_prompt_case(73, *heads, torch.bfloat16, groups, tail=0))
+    rows = len(c["q"])
+    assert rows * heads[0] < 98304
+    _prompt_some_rows(lsa, c, sorted(set(range(0, rows, 7)) | {rows - 1}), (heads, groups), eps_p=orc.EPS_P[torch.bfloat16])
+
+
+def test_the_weights_bits_would_be_missed():
+    """The two tests above see a kernel that keeps one part of a bfloat16 weight: planted in the oracle's weights, it is past their tolerances."""
+    one_part = lambda p: (p * 512).bfloat16().double() / 512  # noqa: E731  (the largest is 2^9 there)
+
+    def off(q, k, v, out_dtype):
+        o, lse, tol, _ = orc.attend(q, k, v, orc.EPS_P[torch.bfloat16])
+        s = torch.einsum("mhd,nhd->mhn", q.double(), k.double().repeat_interleave(q.shape[1] // k.shape[1], 1)) / math.sqrt(q.shape[2])
+        p = torch.exp(s - s.amax(-1, keepdim=True))
+        planted = torch.einsum("mhn,nhd->mhd", one_part(p), v.double().repeat_interleave(q.shape[1] // v.shape[1], 1)) / p.sum(-1, keepdim=True)
+        tol = tol + orc.EPS_OUT[out_dtype] * (o.abs() + tol) + 2.0 ** -25
+        return float(((planted.to(out_dtype).double() - o).abs() / tol).max())
+    c = _even(_case(71, 8, 2, 128, torch.bfloat16, *BITS["rows-past-a-tile"]))
+    slots = c["table"][c["g"][2][0], :130].long()
+    assert off(c["q"][:37], c["kv"][slots, :2], c["kv"][slots, 2:], torch.float32) > 2
+    c = _even(_prompt_case(73, 8, 2, 128, torch.bfloat16, [(500, 40), (3, 90)], tail=0))
+    slots = c["table"][c["g"][2][0], :500].long()
+    assert off(c["q"][:40], c["kv"][slots, :2], c["kv"][slots, 2:], torch.bfloat16) > 2
+
+
+# ------------------------------------------------------------------------------------------------ pools of other sizes and types, other streams
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, slots", [(40, 700_000), (800, 700_000), (800, 2_200_000)])
+def test_prompts_of_slots_past_two_gigabytes(lsa, rows, slots):
+    """Offsets of slots that pass 31 and 32 bits, prefixes where they lie and laid out."""
+    Hq, Hkv, D = (128, 16, 128) if rows > 100 else (32, 16, 128)
+    pool = torch.empty(slots, 2 * Hkv, D, dtype=torch.float16, device=DEV)
+    assert pool.numel() * 2 > (1 << 32) and slots * 2 * Hkv * D * 2 > 2 ** 31
+    c = _prompt_case(79, Hq, Hkv, D, torch.float16, [(300, rows)], tail=0)
+    far = torch.randperm(slots, generator=c["gen"])[:len(c["kv"])].sort().values
+    far[-5:] = torch.arange(slots - 5, slots)
+    assert len(far.unique()) == len(far)
+    pool[far.to(DEV)] = c["kv"].to(DEV)
+    t = c["table"]
+    table = torch.where((t >= 0) & (t < len(far)), far[t.clamp(0, len(far) - 1).long()].int(), t)
+    o, m, l = torch.zeros(rows, Hq, D, dtype=torch.float16, device=DEV), torch.full((rows, Hq), -math.inf, device=DEV), torch.zeros(rows, Hq, device=DEV)
+    s, n, r, p = (_i32(x) for x in c["g"])
+    lsa.shared_prefix_attention_fwd(c["q"].to(DEV), pool[:, :Hkv], pool[:, Hkv:], o, s, n, table.to(DEV), r, p, rows, 300, m, l)
+    i = sorted({0, rows // 3, rows - 1})
+    o_ref, l_ref, tol_o, tol_l = orc.prompt(c["q"][i], c["kv"][:, :Hkv], c["kv"][:, Hkv:], t, [0], [len(i)], c["g"][2], c["g"][3], 300, 2.0 ** -11)
+    _check((o[i], (torch.log2(l[i]) + m[i]) * math.log(2)), (o_ref, l_ref, tol_o + 2.0 ** -11 * (o_ref.abs() + tol_o) + 2.0 ** -25, tol_l + 1e-6), (rows, slots))
+
+
+@pytest.mark.gpu
+def test_all_of_it_on_another_stream(lsa):
+    """Prompts both ways, forks, copies, releases and compaction behind work that is queued on their stream."""
+    side = torch.cuda.Stream()
+    for heads, rows in (((8, 2, 128), 30), ((128, 64, 128), 800)):
+        c = _prompt_case(83, *heads, torch.float16, [(200, rows)], tail=0)
+        T, Hq, D = c["q"].shape
+        kv, q, s = c["kv"].to(DEV), c["q"].to(DEV), [_i32(x) for x in c["g"]]
+        table, late = c["table"].to(DEV), torch.zeros_like(kv)
+        out = []
+        for stream, pool in ((torch.cuda.current_stream(), kv), (side, late)):
+            o, m, l = torch.zeros_like(q), torch.full((T, Hq), -math.inf, device=DEV), torch.zeros(T, Hq, device=DEV)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                if pool is late:
+                    torch.cuda._sleep(20_000_000)
+                    late.copy_(kv)
+                lsa.shared_prefix_attention_fwd(q, pool[:, :c["Hkv"]], pool[:, c["Hkv"]:], o, s[0], s[1], table, s[2], s[3], rows, 200, m, l)
+            stream.synchronize()
+            out.append((o, m, l))
+        assert all(torch.equal(a, b) for a, b in zip(*out))
+    table0 = torch.full((6, 30), PAD, dtype=torch.int32)
+    table0[0] = torch.randperm(200, generator=torch.Generator().manual_seed(4))[:30].int() + 100
+    rows0 = torch.randn(2, 300, 4, 64).half()
+    state0 = torch.zeros(300, dtype=torch.int32)
+    state0[table0[0].long()] = 1
+    free = torch.arange(0, 30)
+    out = []
+    for stream in (torch.cuda.current_stream(), side):
+        table, pool, state = torch.zeros(6, 30, dtype=torch.int32, device=DEV), torch.zeros(2, 300, 4, 64, dtype=torch.float16, device=DEV), torch.zeros(300, dtype=torch.int32, device=DEV)
+        now = [x.to(DEV) for x in (table0, rows0, state0, free)]
+        zero, one, two, n = _i32([0]), _i32([1]), _i32([2]), _i32([30])
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            torch.cuda._sleep(20_000_000)
+            for x, y in zip((table, pool, state), now):
+                x.copy_(y)
+            lsa.fork_requests(table, zero, one, n, 30, state)
+            state[now[3]] += 1
+            lsa.copy_requests(table, zero, two, n, zero, 30, now[3], pool)
+            freed = lsa.release_requests(table, _i32([0, 1]), _i32([30, 12]), 30, state)
+            remap = lsa.compact_pool(state, pool, table, _i32([1, 2]), _i32([30, 30]), 30)
+        stream.synchronize()
+        out.append((table, pool, state, remap, freed))
+    assert out[0][4] == out[1][4] == 12 and all(torch.equal(a, b) for a, b in zip(out[0][:4], out[1][:4]))
+    table, pool, state = out[1][0].cpu(), out[1][1].cpu(), out[1][2].cpu()
+    held = table0[0].long()
+    assert torch.equal(pool[:, table[2].long()], rows0[:, held]) and torch.equal(pool[:, table[1, 12:].long()], rows0[:, held[12:]])
+    assert state[:48].tolist() == [1] * 48 and not bool(state[48:].any())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [300, 70000])
+def test_compaction_without_rows(lsa, size):
+    """The entry point of the library with no rows to move: counts, table and remap alone."""
+    import ctypes as C
+    from loongserve_amd import _lib
+    lib, g = _lib.load(), torch.Generator().manual_seed(size)
+    state = (torch.rand(size, generator=g) < 0.4).int() * 3
+    used = state.nonzero().squeeze(1)
+    table = used[torch.randint(0, len(used), (3, 50), generator=g)].int()
+    table[1, 3] = PAD
+    want_s, want_t, want_r, _, _ = orc.compact(state, table, [2, 0], [50, 20], 50)
+    st, t, remap = state.to(DEV), table.to(DEV), torch.empty(size, dtype=torch.int32, device=DEV)
+    req, lens, ws = _i32([2, 0]), _i32([50, 20]), torch.empty(lib.lsattn_compact_workspace_bytes(size), dtype=torch.uint8, device=DEV)
+    a = _lib.CompactArgs(mem_state=st.data_ptr(), pool_size=size, remap=remap.data_ptr(), req_to_tokens=t.data_ptr(), num_reqs=3, max_seq_len=50, b_req_idx=req.data_ptr(),
+                         b_seq_len=lens.data_ptr(), n=2, max_len_in_batch=50, workspace=ws.data_ptr(), workspace_bytes=ws.numel())
+    assert lib.lsattn_compact_pool(C.byref(a), C.byref(_lib.PoolRows()), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert torch.equal(st.cpu(), want_s) and torch.equal(t.cpu(), want_t) and torch.equal(remap.cpu(), want_r)
+
+
+@pytest.mark.gpu
+def test_managers_of_an_8_bit_pool(lsa):
+    """Forks, copies and compaction of a pool in 8 bits: rows and exponents together, read back bit for bit; decode over the copies."""
+    mem, reqs = _managers(lsa, slots=200, dtype=F8)
+    g = torch.Generator().manual_seed(89)
+    gap = mem.alloc(30)
+    row, slots = _request(lsa, mem, reqs, 33)
+    src = torch.randn(33, 4, 64, generator=g).half().to(DEV)
+    for layer in range(3):
+        lsa.kv_scatter_fp8(src * 2.0 ** layer, slots, mem.kv_buffer[layer], mem.kv_scales[layer])
+
+    def read(r):
+        out = torch.zeros(3, 33, 4, 64, dtype=torch.float16, device=DEV)
+        for layer in range(3):
+            lsa.kv_gather_fp8(mem.kv_buffer[layer], mem.kv_scales[layer], reqs.req_to_token_indexs, r.int(), _i32([33]), _i32([0]), 33, out[layer])
+        return out
+    want = read(row)
+    assert float((want[2] - src * 4).abs().max()) <= 2.0 ** -4 * float((src * 4).abs().max())
+    fork = reqs.fork(row, _i32([33]), 33)
+    copy, own = reqs.fork_copy(fork, _i32([33]), 33, 33)
+    mem.free(gap)
+    reqs.free_reqs(row, _i32([33]), 33)
+    remap = mem.compact(reqs.req_to_token_indexs, torch.cat([fork, copy]), _i32([33, 33]), 33)
+    assert torch.equal(read(fork), want) and torch.equal(read(copy), want)
+    assert reqs.req_to_token_indexs[copy[0], :33].tolist() == remap[own].tolist() and bool((mem.mem_state[:66] == 1).all())
+    q = torch.randn(2, 4, 64, generator=g).half().to(DEV)
+    o, lse = lsa.longserve_fp8_decode_attention(q[:1].repeat(2, 1, 1), reqs.req_to_token_indexs, torch.cat([fork, copy]).int(), _i32([33, 33]), 33, mem.kv_buffer[1][:, :2],
+                                                mem.kv_buffer[1][:, 2:], mem.kv_scales[1][:, :2], mem.kv_scales[1][:, 2:])
+    assert torch.equal(o[0], o[1]) and torch.equal(lse[0], lse[1])
+    reqs.free_reqs(torch.cat([fork, copy]), _i32([33, 33]), 33)
+    _as_counted(mem, reqs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_a_prefix_over_two_instances(lsa, dtype):
+    """The prefix's first tokens in one pool, its last ones and the own tokens in another: float32 partials of both, joined by lse_merge."""
+    c = _case(97, 8, 2, 128, dtype, [(400, [3, 40, 0])], [])
+    kv, t, r = c["kv"], c["table"], c["g"][2][0]
+    want = orc.decode(c["q"], kv[:, :2], kv[:, 2:], t, c["req"], c["len"], *c["g"], 400, dtype)
+    first = dict(c, table=t.clone(), len=torch.full((3,), 150, dtype=torch.int32), g=(*c["g"][:3], [150]), most=150, own=0)
+    second = dict(c, table=torch.full_like(t, PAD), len=c["len"] - 150, g=(*c["g"][:3], [250]), most=250)
+    second["table"][:, :-150] = t[:, 150:]
+    parts = [_decode_on_gpu(lsa, x, out=torch.empty(c["q"].shape, device=DEV)) for x in (first, second)]
+    o, lse = lsa.lse_merge(parts, out_dtype=dtype)
+    # (each part is off by what the whole may be off by, relative to the same sums; joining adds less than the 64 eps that are counted for that)
+    _check((o, lse), (want[0], want[1], 2 * want[2], 2 * want[3]), dtype)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_the_same_call_gives_the_same_bits(lsa, dtype):
+    """Work is dealt by the sizes alone and joined in one order: repeated calls, in workspaces that hold anything, agree bit for bit."""
+    c = _case(101, 32, 8, 128, dtype, [(1500, [100, 3, 700] * 6), (700, [0, 9])], [400])
+    p = _prompt_case(103, 32, 8, 128, dtype, [(1200, 150), (300, 40)], tail=0)
+    runs = []
+    for fill in (0, 77, 255):
+        ws = torch.full((lsa.shared_prefix_decode_workspace_bytes(len(c["q"]), 2, 32, 8, 128, c["most"], c["own"]),), fill, dtype=torch.uint8, device=DEV)
+        pws = torch.full((lsa.shared_prefix_attention_workspace_bytes(len(p["q"]), 2, 32, 8, 128, p["most"]),), fill, dtype=torch.uint8, device=DEV)
+        o, m, l = torch.zeros(p["q"].shape, dtype=dtype, device=DEV), torch.full(p["q"].shape[:2], -math.inf, device=DEV), torch.zeros(p["q"].shape[:2], device=DEV)
+        _prompt_on_gpu(lsa, p, o, m, l, workspace=pws)
+        runs.append((*_decode_on_gpu(lsa, c, workspace=ws), o, m, l))
+    assert all(torch.equal(a, b) for run in runs[1:] for a, b in zip(runs[0], run))
