@@ -245,12 +245,13 @@ class LongServeReqManager:
         return new, index
 
     def _check_in_use(self, req_index):
-        if req_index.dim() != 1:
+        if req_index.dim() != 1 or req_index.dtype not in (torch.int32, torch.int64) or req_index.device != self.req_state.device:
             return  # (the release says what is wrong)
-        rows, state = req_index.cpu().long(), self.req_state.cpu()
+        both, n = torch.cat((req_index, self.req_state)).cpu().numpy(), len(req_index)  # (one copy: each waits for the device)
+        rows, state = both[:n], both[n:]
         known = (rows >= 0) & (rows < len(state))
-        bad = rows[~known | (state[rows.clamp(0, len(state) - 1)] == 0)]
-        if len(bad) or len(rows.unique()) < len(rows):
+        bad = rows[~known | (state[rows * known] == 0)]
+        if len(bad) or len(set(rows.tolist())) < n:
             raise IndexError("request rows that are not in use, or named twice: %s" % (bad if len(bad) else rows).tolist())
 
     @torch.inference_mode()
