@@ -667,8 +667,9 @@ int lsattn_pool_attention(const lsattn_pool_attention_args* a, void* stream);
  *   o[b, h] = sum_j softmax_j(sm_scale * q[b, h] . k_j) v_j  over the b_seqlen[b] positions j,   lse[b, h] = natural log-sum-exp of the scores
  * (o = 0, lse = -inf where there is none).  A prefix's rows are read once for 128 query rows of the group.  Groups stand in ascending order of their requests; a
  * request that two groups name belongs to the first of them, one that no group names, or that is shorter than its group's prefix, shares nothing: its
- * own row of the table has all its positions.  Table entries outside [0, num_slots) count as positions that do not exist, so do positions past max_seq_len
- * and rows outside [0, num_reqs).  P is held in the type of V (bfloat16: in two parts) and O divided by the sum of the weights so rounded.
+ * own row of the table has all its positions.  Table entries outside [0, num_slots) count as positions that do not exist, so do positions past max_seq_len;
+ * a request whose own row lies outside [0, num_reqs) has none at all, a group whose row does has no prefix.  Over a prefix P is held in the type of V, fp16 in one part (off by 2^-11 of a
+ * weight, in fp32 outputs too), bfloat16 in two (2^-16), and O divided by the sum of the weights so rounded (bfloat16: of the weights).
  * max_prefix_len bounds g_prefix_len: of a longer prefix the first max_prefix_len positions are shared.  max_own_len (a bound of the positions behind the prefix) only
  * steers the launch.
  * Workspace: lsattn_shared_decode_workspace_bytes(...) bytes, 16-byte aligned, contents irrelevant before and after; calls that overlap in time need one each.  For given heads
@@ -708,7 +709,7 @@ int lsattn_shared_decode(const lsattn_shared_decode_args* a, void* stream);
  * lsattn_prefill_step_merge folds a step (ring_context_flashattention_nopad.py:171-188); the requests' own chunks are further steps of that kind, in any order.  Rows of no
  * group, and rows that see no key, stay as they are.  Groups and table entries as in lsattn_shared_decode; prefixes longer than max_prefix_len are cut there.
  * max_group_rows bounds g_size (rows past it may stay uncomputed).  Few rows are taken against the pool's rows where they lie; for many the prefix is laid out once
- * in the workspace for the prefill kernel (a bfloat16 V as fp16, values beyond its range as +-65504).  Workspace as above, by
+ * in the workspace for the prefill kernel (a bfloat16 V as fp16: magnitudes past 65504 as 65504, below 2^-14 cut to multiples of 2^-24; P in fp16).  Workspace as above, by
  * lsattn_shared_prefill_workspace_bytes: enough for all calls with the same heads and no larger sizes.  (Fewer groups than it was asked for may be laid out where more are not: if
  * there is no room for that, the pool's rows are taken where they lie.)
  */

@@ -1085,7 +1085,7 @@ PyObject* release_requests(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
-// (state, kv or None, table, req, len, max_len, scales or None, remap) -> True or None
+// (state, kv, table, req, len, max_len, scales or None, remap, workspace or None) -> True or None
 PyObject* compact_pool(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
   NEED_ARGS(9);

@@ -2,9 +2,9 @@
 // requests' tokens, and compaction.  No counterpart in the reference, whose slots have reference counts too (loongserve/common/longserve_mem_manager.py:61-88) but whose
 // lists count a slot that is named twice once, so that requests that share tokens cannot be freed together.
 //
-// All of it is whole numbers and rows as bytes.  What bounds it: rows, HBM (two copies of 6500 tokens in 32 layers of 8 heads of 128, 3.3 GB there and back, 525 us, 6.2 TB/s; half of 60000
-// slots in use, 12 layers, compacted: 1.43 GB, 303 us, 4.7 TB/s, a large copy's rate); the rest, launch latency and a few MB of tables and counts (eight forks of 2999 tokens 3.6 us, a
-// release of 100 tokens 2.5 and of 128 requests 11.4 + 3.8, the plan of a compaction 5.2 for 5000 slots and 10.4 for 60000).  Counts change by integer atomics, whose order does not change a result.
+// All of it is whole numbers and rows as bytes.  What bounds it: rows, HBM (two copies of 6500 tokens in 32 layers of 8 heads of 128, 3.3 GB there and back, 533 us, 6.2 TB/s, in 8 bits
+// with their exponents 302, 5.7; half of 60000 slots in use, 12 layers, compacted: 1.43 GB, 306 us, 4.7 TB/s, a large copy's rate); the rest, launch latency and a few MB of tables and counts
+// (eight forks of 2999 tokens 3.7 us, a release of 100 tokens 2.4 and of 128 requests 11.4 + 3.8, the plan of a compaction 5.3 for 5000 slots and 10.4 for 60000).  Counts change by integer atomics, whose order does not change a result.
 #include "common.hip.h"
 
 namespace lsattn {

@@ -14,20 +14,24 @@
 //     16-byte chunks XORed with the row (prefill_small.hip says why); the slots of the tile after next are under way;
 //   * the order of the keys in a tile does not matter without a causal mask: rows lie so that a lane's slots are neighbours in the table;
 //   * entries of the table that name no slot, and positions past the prefix, are a mask of the tile; its V rows are cleared in LDS before they are used;
-//   * scores transposed, S^T = K Q^T, so that P^T goes into O^T += V^T P^T from the lane that computed it.  fp16: P as fp16, O divided by the sum of the very weights
-//     that multiplied V; bfloat16: P in two parts, high and low (8 bits alone would cost 1e-3 of O);
+//   * scores transposed, S^T = K Q^T, so that P^T goes into O^T += V^T P^T from the lane that computed it.  fp16: P as fp16, 2^-11, which a 16-bit output rounds away for the most part
+//     (2.9e-4 against 2.1e-4 with fp32 weights; a second part would be half as many products again), O divided by the sum of the very weights
+//     that multiplied V; bfloat16: P in two parts, high and low, 2^-16 (8 bits alone would cost 1e-3 of O);
 //   * the running maximum is raised where a lane's eight weights pass 2^15, and then set so that the largest is 2^9.
 // Own tokens: the decode walk of pool_walk.hip.h from the prefix's end on, in the same launch (those workgroups wait for memory where the others keep the matrix
 // pipe busy), equal shares of all requests' own tokens.  A second launch joins a request's partials.
 //
-// What bounds it, with the case that shows it (launches alone, without the one that joins):
-//   * few rows per group: HBM reads.  24 requests in three groups and alone, 32/32 heads, 449 MB: 92 us, 4.9 TB/s;
-//   * prefix and own tokens together: 64 requests behind 16384 tokens, 32/8 heads, up to 1500 own: 60 us (284 MB, 4.8 TB/s; the parts alone 35 and 42 us);
-//   * many rows, 64-wide bfloat16: vector work, then the matrix pipe, which runs beside it only in part (busy 54% and 30%): 160 requests in two groups, 28/4 heads: 67 us, 0.4 PFLOP/s of the
+// What bounds it, with the case that shows it (launches alone, without the one that joins, of a GPU that was idle before; hundreds of passes in a row raise the clock, and those that compute
+// get 6 to 10% faster):
+//   * few rows per group: reads, of which too few are under way.  24 requests in three groups and alone, 32/32 heads, 449 MB: 92 us, 4.9 TB/s (a streaming read: 7.0).  A group of 8 has 8 rows of
+//     a tile's 128, which one wave of four multiplies while the tile's loads have been waited for;
+//   * prefix and own tokens together, reads too: 64 requests behind 16384 tokens, 32/8 heads, up to 1500 own: 59 us (284 MB, 4.8 TB/s; the parts alone 35 and 42 us; 64 us, 4.4 TB/s, where
+//     nothing of it is in the last-level cache);
+//   * many rows, 64-wide bfloat16: vector work, then the matrix pipe, which runs beside it only in part (busy 54% and 30%): 160 requests in two groups, 28/4 heads: 66 us, 0.4 PFLOP/s of the
 //     formula, a half more with the second part of P;
 //   * many rows, 128-wide fp16: the products (0.9 PFLOP/s of whole row tiles as the prefix grows, 1.14 where nothing has to be loaded, 1.17 a large library product), and 17 us of start and end: prompts of
 //     293 rows behind 6001 tokens 50 us, of which 6 are 28 MB of partials that all workgroups store at once.
-// Tried and left out (128-wide heads, all 0.70 to 0.75 PFLOP/s before the tiles went side by side, as this form): four stages of 32 keys; operands read a step ahead, or all at once (decode 5 to
+// Tried and left out (timed while this was built; 128-wide heads, all 0.70 to 0.75 PFLOP/s before the tiles went side by side, as this form): four stages of 32 keys; operands read a step ahead, or all at once (decode 5 to
 // 8% slower); eight waves of 256 rows, in alternating phases or not (no room beside it for the own tokens; prompts of
 // 150 to 400 rows 0 to 8% slower, of 1200 2 to 4% faster, of 2500 behind 20000 tokens 10%); lines fetched into the L2 ahead (5%, few rows 30% slower); three and four waves per SIMD of
 // the 64-wide form (equal, and slower for spills); sums and exponentials in independent batches, products of 32 x 32 for bfloat16 (equal).  Of 64-wide bfloat16 rows 16 exponentials take an eighth of

@@ -67,10 +67,10 @@ def longserve_shared_prefix_decode_attention(q: torch.Tensor, req_to_token_index
     g_start_loc[g] .. + g_size[g] - 1 of the batch, in ascending order; its first g_prefix_len[g] tokens are the slots that row g_req_idx[g] of the table
     names.  A request of no group, or shorter than its group's prefix, attends by its own row of the table alone (a length of 0: o = 0,
     -inf), one that two groups name belongs to the first.  max_prefix_len bounds g_prefix_len: what a group has beyond it is read by each
-    request for itself.  Entries of the table that name no slot count as positions that do not exist.
+    request for itself.  Entries of the table that name no slot count as positions that do not exist; a request whose own row is not in the table has none at all.
 
-    out: q's type unless given (float16, bfloat16 or float32).  Over the prefixes a request's weights are rounded to V's type, for bfloat16 in two
-    parts, and o is divided by the sum of the rounded ones; the log-sum-exp is float32's.  max_len_in_batch, or max_own_len (a bound of the
+    out: q's type unless given (float16, bfloat16 or float32).  Over the prefixes a request's weights are rounded: to float16, 2^-11 of a weight, and o is divided by the sum
+    of the rounded ones; or to two parts of bfloat16, 2^-16.  A float32 out, which lse_merge joins with another instance's, carries that.  The log-sum-exp is float32's.  max_len_in_batch, or max_own_len (a bound of the
     tokens behind the prefix) where given, only sizes the launch and weighs its two parts (a close bound helps).  workspace: the caller's scratch
     (shared_prefix_decode_workspace_bytes; else torch allocates it), one for each call that may run at the same time, graphs' replays among them."""
     own = max_len_in_batch if max_own_len is None else max_own_len
@@ -129,8 +129,9 @@ def shared_prefix_attention_fwd(q: torch.Tensor, cache_k: torch.Tensor, cache_v:
     g_prefix_len (rows past the one may stay uncomputed, prefixes are cut at the other).  Entries of the table that name no slot count as positions that
     do not exist.
 
-    Few rows are multiplied with the pool's rows where they lie, their partials folded by a second launch; for many the prefix is laid out once
-    (a bfloat16 V as float16: magnitudes past 65504 count as 65504) for the kernel behind context_attention_fwd.  workspace: the caller's scratch
+    Few rows are multiplied with the pool's rows where they lie, their partials folded by a second launch; for many (98304 rows x heads, 512 rows x heads of a KV head per
+    group) the prefix is laid out once for the kernel behind context_attention_fwd, with its precision: a bfloat16 V counts as float16 there (magnitudes past 65504 as 65504,
+    below 2^-14 cut to multiples of 2^-24), the weights as float16.  Rows that come together in fewer calls or more may differ by so much.  workspace: the caller's scratch
     (shared_prefix_attention_workspace_bytes for q's rows; else torch allocates it), one for each call that may run at the same time."""
     if _native.shared_prefill(q, cache_k, cache_v, o, g_start_loc, g_size, req_to_token_indexs, g_req_idx, g_prefix_len, max_g_size, max_prefix_len, m, l,
                               workspace):
