@@ -83,14 +83,21 @@ def prompt(q, k, v, table, g_start, g_size, g_req, g_prefix, max_prefix, eps_p):
 
 
 def fork(table, src, dst, lens, most, state=None):
+    """(table, state): entries as they are and a reference on each slot; no slot (2147483647) where the source is no row of the table, or the slot is free."""
     table, state = table.clone(), None if state is None else state.clone()
-    old = table.clone()
+    old, held = table.clone(), None if state is None else state.clone()
     for a, b, n in zip(src, dst, lens):
         n = min(n, most, table.shape[1])
-        table[b, :n] = old[a, :n]
-        for s in old[a, :n].tolist() if state is not None else ():
-            if 0 <= s < len(state):
-                state[s] += 1
+        if not 0 <= b < len(table) or n <= 0:
+            continue
+        row = old[a, :n].clone() if 0 <= a < len(table) else torch.full((n,), 2147483647, dtype=table.dtype)
+        if state is not None:
+            inside = (row >= 0) & (row < len(state))
+            row[inside & (held[row.clamp(0, len(state) - 1).long()] == 0)] = 2147483647
+            for s in row.tolist():
+                if 0 <= s < len(state):
+                    state[s] += 1
+        table[b, :n] = row
     return table, state
 
 

@@ -512,3 +512,22 @@ def test_the_same_call_gives_the_same_bits(lsa, dtype):
         _prompt_on_gpu(lsa, p, o, m, l, workspace=pws)
         runs.append((*_decode_on_gpu(lsa, c, workspace=ws), o, m, l))
     assert all(torch.equal(a, b) for run in runs[1:] for a, b in zip(runs[0], run))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("run", [1, 5, 90])
+def test_forks_against_lists_where_slots_are_free(lsa, run):
+    """Runs of forks of one source, rising and falling lengths, sources and destinations that do not exist, a quarter of the slots free."""
+    g = torch.Generator().manual_seed(run)
+    rows, width, size = 120, 300, 5000
+    table = torch.randint(-2, size + 2, (rows, width), generator=g).int()
+    state = torch.randint(0, 4, (size,), generator=g).int()
+    dst = torch.randperm(100, generator=g).tolist()
+    src = [100 + (i // run) % 20 for i in range(100)]
+    src[7], src[50], dst[20], dst[70] = -1, rows, -3, rows + 5
+    lens = torch.randint(-2, width + 20, (100,), generator=g).tolist()
+    for most in (width, 170):
+        want_t, want_s = orc.fork(table, src, dst, lens, most, state)
+        t, st = table.to(DEV), state.to(DEV)
+        lsa.fork_requests(t, _i32(src), _i32(dst), _i32(lens), most, st)
+        assert torch.equal(t.cpu(), want_t) and torch.equal(st.cpu(), want_s)
